@@ -57,6 +57,16 @@ SIGNATURES = {
     "flk_w8a8_qk_prep_pair": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i64,
                                    _p, _p, _p, _p, _p, _p, _p, _p, _i, _i64,
                                    _i, _i64, _i, _f, _i, _i, _i, _p, _p, _p, _i64, _p]),
+    "flk_layer_norm": (_i, [_p, _i64, _i64, _i, _p, _p, _i, _i64, _i, _f, _i, _i, _i, _p, _i64, _i64, _p]),
+    "flk_layer_norm_backward_plan": (_i, [_i, _i, _i, _i, ctypes.POINTER(ctypes.c_int64)]),
+    "flk_layer_norm_backward": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i, _p, _i, _i64, _i, _f, _i, _i, _i, _p, _i64, _i64,
+                                     _p, _p, _p, _i64, _p]),
+    "flk_swiglu": (_i, [_p, _i64, _i64, _i, _i, _i, _i, _p, _i64, _i64, _p]),
+    "flk_swiglu_backward": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _i, _p, _i64, _i64, _p]),
+    "flk_mlp_plan": (_i, [_i, _i, _i, _i, ctypes.POINTER(ctypes.c_int64)]),
+    "flk_mlp_gate": (_i, [_p, _i64, _p, _i64, _i, _i, _i, _i, _p, _i64, _p, _p, _i64, _p]),
+    "flk_mlp_gate_backward": (_i, [_p, _i64, _p, _i64, _p, _i, _i, _i, _i, _p, _i64, _p, _i64, _p]),
+    "flk_mlp_matmul": (_i, [_p, _i64, _i, _p, _i64, _i, _i, _i, _i, _i, _p, _i64, _p, _i64, _p]),
 }
 
 ABI_VERSION = 1

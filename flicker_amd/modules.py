@@ -132,8 +132,18 @@ def double_attention_int8(txt_x, img_x, txt_qw, img_qw, txt_scales, img_scales, 
 def single_attention(linear1_out, q_scale, k_scale, freqs: Freqs | PositionIds, num_heads: int,
                      hidden: int, *, pe=None):
     """modules.py:185-191 + 198 -- the qkv part of the fused linear1 output (a strided view,
-    consumed without a copy) -> qk prep -> attention -> merge; returns (attn, mlp).  ``pe``
+    consumed without a copy) -> qk prep -> attention -> merge; returns (attn, mlp), mlp the view of
+    both MLP halves that ``mlp.swiglu`` gates in place (modules.py:199).  ``pe``
     is the joint sequence's rope table, read only by the gate's plain branch (no row tile)."""
     qkv, mlp = linear1_out[..., : 3 * hidden], linear1_out[..., 3 * hidden:]
     q, k, v = qkv_prep(qkv, q_scale, k_scale, pe, freqs, num_heads)
     return attend_merged(q, k, v), mlp
+
+
+def mlp_section(x, shift, scale, w_in, w_out):
+    """modules.py:157-167 (per stream) -- a double block's MLP: the gated MLP of modulate(x, shift, scale), before
+    the block's gate and residual.  x (B, L, hidden) bf16 or fp16, shift and scale (B, hidden) or (B, 1, hidden),
+    w_in (hidden, 2 * mlp), w_out (mlp, hidden).  Its gradients are those of ``norm.modulate`` and
+    ``mlp.gated_mlp``, or ``autograd``'s."""
+    from . import mlp, norm
+    return mlp.gated_mlp(norm.modulate(x, shift, scale), w_in, w_out)

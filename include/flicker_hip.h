@@ -39,6 +39,11 @@ extern "C" {
 #define FLK_ABI_VERSION 1
 int flk_abi_version(void);
 
+/* Element types of the norm and MLP entry points. */
+#define FLK_BF16 0
+#define FLK_F16 1
+#define FLK_F32 2
+
 /* Static, human-readable text for a return code of any entry point. */
 const char* flk_status_string(int status);
 
@@ -398,6 +403,82 @@ int flk_w8a8_qk_prep_pair(const int8_t* xq0, const int8_t* wq_t0, const float* a
                           int k, int64_t table_row_stride, int scale_is_f32, float q_gain, int batch,
                           int num_heads, int head_dim, void* q_out, void* k_out, void* v_out,
                           int64_t out_length, void* stream);
+
+/* Layer norm over the last axis with a per-channel factor and offset:
+ *   y = (x - mean) / sqrt(var + eps) * a + c,  a = factor (+ 1 with add_one), c = offset
+ * in float32, rounded once.  Replaces layer_norm (src/flicker/nn.py:17-21) and, with add_one and
+ * one row per batch entry, modulate (modules.py:38-40).
+ *   x, y     (batch, length, width) of type dtype (FLK_BF16, FLK_F16, FLK_F32); element (b, t, j) at
+ *            b*batch_stride + t*row_stride + j, strides in elements, any of them
+ *   factor, offset  (width,) rows of type params_dtype (dtype itself or FLK_F32), one per batch
+ *            entry at b*param_batch_stride, or one for all (stride 0); NULL: a = 1, c = 0
+ * y may be x.  Any alignment of whole elements; width at most 32768. */
+int flk_layer_norm(const void* x, int64_t x_batch_stride, int64_t x_row_stride, int dtype, const void* factor,
+                   const void* offset, int params_dtype, int64_t param_batch_stride, int add_one, float eps, int batch,
+                   int length, int width, void* y, int64_t y_batch_stride, int64_t y_row_stride, void* stream);
+
+/* Gradients of flk_layer_norm for the incoming gradient dy (laid out as x):
+ *   dx       of x; dx may be dy or x
+ *   dfactor, doffset  of the parameter rows, (batch, width) or, with param_batch_stride 0, (width,)
+ *            of type params_dtype, dense; either may be NULL.  They are not written when batch or
+ *            length is 0.
+ * The column sums go through `workspace` (16-byte aligned; the plan's bytes, given whether the
+ * parameters are shared by all batch entries; not needed when dfactor and doffset are NULL) and
+ * are added in a fixed order. */
+int flk_layer_norm_backward_plan(int batch, int length, int width, int shared_params, int64_t* workspace_bytes);
+int flk_layer_norm_backward(const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride, const void* x,
+                            int64_t x_batch_stride, int64_t x_row_stride, int dtype, const void* factor,
+                            int params_dtype, int64_t param_batch_stride, int add_one, float eps, int batch, int length,
+                            int width, void* dx, int64_t dx_batch_stride, int64_t dx_row_stride, void* dfactor,
+                            void* doffset, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* h = silu(g) * u of gu = [g | u], silu(z) = z / (1 + exp(-z)), in float32, rounded once: the gate of
+ * the blocks' MLP (modules.py:157-167, 185-200).
+ *   gu  (batch, length, 2*hidden), h (batch, length, hidden) of type dtype, laid out as in
+ *       flk_layer_norm: gu may be columns of a wider projection, h columns of a wider buffer. */
+int flk_swiglu(const void* gu, int64_t gu_batch_stride, int64_t gu_row_stride, int dtype, int batch, int length,
+               int hidden, void* h, int64_t h_batch_stride, int64_t h_row_stride, void* stream);
+
+/* dgu = [dg | du] for the incoming gradient dh, with s = 1 / (1 + exp(-g)):
+ *   dg = dh u s (1 + g (1 - s)),  du = dh g s.   dgu may be gu. */
+int flk_swiglu_backward(const void* dh, int64_t dh_batch_stride, int64_t dh_row_stride, const void* gu,
+                        int64_t gu_batch_stride, int64_t gu_row_stride, int dtype, int batch, int length, int hidden,
+                        void* dgu, int64_t dgu_batch_stride, int64_t dgu_row_stride, void* stream);
+
+/* The matrix products of the gated MLP y = (silu(x Wg) * (x Wu)) Wout and of its gradients, on bf16 or
+ * fp16 operands (dtype) with float32 sums.  Strides are in elements between rows; every pointer
+ * is 16-byte aligned, and widths (all sizes but the token count) and strides are multiples of 8.
+ * Every output row is dense in its last axis; outputs overlap no input.  Products that would leave
+ * most of the GPU idle are cut along their inner axis: their partial sums go through `workspace`
+ * (16-byte aligned; flk_mlp_plan's bytes for the same product and sizes) and are added in a fixed
+ * order.
+ *
+ * flk_mlp_gate: h (m, hidden) = silu(g) * u of [g | u] = x (m, width) w_in (width, 2*hidden); gu, if
+ * not NULL, receives [g | u] as float32 (m, 2*hidden), dense, which the backward pass needs.
+ *
+ * flk_mlp_gate_backward: dgu (m, 2*hidden) = [dg | du] (flk_swiglu_backward's formulas) of
+ * dh = dy (m, width) w_out^T, w_out (hidden, width), and of flk_mlp_gate's gu.
+ *
+ * flk_mlp_matmul: d (rows, cols) = A B with `inner` terms, where A is a (rows, inner) or, with
+ * a_transposed, a's transpose, a (inner, rows); and B is b (inner, cols) or, with b_transposed, the
+ * transpose of b (cols, inner).  Not both A and B^T may lie across their rows' memory: a_transposed
+ * with b_transposed is FLK_E_UNSUPPORTED.  With a_transposed the inner axis is the tokens' and may
+ * have any length; otherwise `rows` may. */
+#define FLK_MLP_GATE 0           /* rows = tokens, cols = hidden, inner = width          */
+#define FLK_MLP_GATE_BACKWARD 1  /* rows = tokens, cols = hidden, inner = width          */
+#define FLK_MLP_MATMUL 2         /* rows, cols, inner of a product with neither transposed */
+#define FLK_MLP_MATMUL_BT 3      /* ... with b_transposed                               */
+#define FLK_MLP_MATMUL_AT 4      /* ... with a_transposed                               */
+int flk_mlp_plan(int product, int rows, int cols, int inner, int64_t* workspace_bytes);
+int flk_mlp_gate(const void* x, int64_t x_row_stride, const void* w_in, int64_t w_in_row_stride, int dtype, int m,
+                 int width, int hidden, void* h, int64_t h_row_stride, float* gu, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+int flk_mlp_gate_backward(const void* dy, int64_t dy_row_stride, const void* w_out, int64_t w_out_row_stride,
+                          const float* gu, int dtype, int m, int width, int hidden, void* dgu, int64_t dgu_row_stride,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+int flk_mlp_matmul(const void* a, int64_t a_row_stride, int a_transposed, const void* b, int64_t b_row_stride,
+                   int b_transposed, int dtype, int rows, int cols, int inner, void* d, int64_t d_row_stride,
+                   void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

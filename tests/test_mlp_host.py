@@ -1,0 +1,161 @@
+"""The norm and gated MLP without a GPU: the oracle against differences of its own forward pass, the C entry
+points' checks of arguments, and the Python layer's refusals."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from flicker_amd import _lib, autograd, mlp, norm
+from oracle import mlp as M
+
+BF16, F16, F32 = 0, 1, 2
+OK, INVALID, ALIGN, UNSUPPORTED, SCRATCH = 0, -1, -2, -3, -4
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _lib.LIB_PATH.exists():
+        pytest.fail("libflicker_hip.so is not built (python -m flicker_amd.build)")
+    return _lib.lib()
+
+
+def _difference(f, at, along, h=1e-5):
+    """Central difference of f at `at` along `along`: off by O(h^2) and by 1e-16 |f| / h."""
+    return (f(at + h * along) - f(at - h * along)) / (2 * h)
+
+
+@pytest.mark.parametrize("seed", [0, 1])
+def test_oracle_gradients_are_the_forward_pass_differences(seed):
+    r = np.random.RandomState(seed)
+    x, dy, d = r.randn(3, 7, 10) + 0.4, r.randn(3, 7, 10), r.randn(3, 7, 10)
+    factor, offset = 1 + 0.3 * r.randn(3, 1, 10), r.randn(3, 1, 10)
+    dx, dn, db = M.layer_norm_grads(dy, x, factor)
+    loss = lambda x, f, o: float((M.layer_norm(x, f, o) * dy).sum())  # noqa: E731
+    df, do = r.randn(3, 1, 10), r.randn(3, 1, 10)
+    # second and third derivatives are of order ten here: h^2 of them, 1e-9
+    assert abs((dx * d).sum() - _difference(lambda v: loss(v, factor, offset), x, d)) < 1e-6
+    assert abs((dn.sum(1, keepdims=True) * df).sum() - _difference(lambda v: loss(x, v, offset), factor, df)) < 1e-6
+    assert abs((db.sum(1, keepdims=True) * do).sum() - _difference(lambda v: loss(x, factor, v), offset, do)) < 1e-6
+    gu, dh, e = 2 * r.randn(5, 12), r.randn(5, 6), r.randn(5, 12)
+    assert abs((M.swiglu_grads(dh, gu) * e).sum() - _difference(lambda v: float((M.swiglu(v) * dh).sum()), gu, e)) < 1e-6
+    ops = [r.randn(4, 6), r.randn(6, 16), r.randn(8, 6)]
+    dy = r.randn(4, 6)
+    for i, grad in enumerate(M.gated_mlp_grads(dy, *ops)):
+        along = r.randn(*ops[i].shape)
+        got = _difference(lambda v: float((M.gated_mlp(*ops[:i], v, *ops[i + 1:]) * dy).sum()), ops[i], along)
+        assert abs((grad * along).sum() - got) < 1e-5
+
+
+def test_oracle_sigmoid_at_the_ends():
+    gu = np.array([[-1e4, -800.0, 0.0, 800.0, 1e4, 1.0, 2.0, 3.0, 4.0, 5.0]])
+    with np.errstate(all="raise", under="ignore"):
+        assert np.array_equal(M.swiglu(gu), [[-0.0, -0.0, 0.0, 3200.0, 5e4]])
+        assert np.array_equal(M.swiglu_grads(np.ones((1, 5)), gu)[0, 5:], [0.0, 0.0, 0.0, 800.0, 1e4])
+
+
+P16 = 4096   # any address: the checks come before the launch
+
+
+def _norm(lib, **k):
+    a = dict(x=P16, xb=0, xr=64, dtype=BF16, factor=P16, offset=P16, params=BF16, pstride=64, add=1, eps=1e-6, batch=0,
+             length=4, width=64, y=P16, yb=0, yr=64)
+    a.update(k)
+    return lib.flk_layer_norm(*a.values(), None)
+
+
+def test_layer_norm_checks(lib):
+    assert _norm(lib) == OK and _norm(lib, batch=2, length=0, x=None, y=None) == OK
+    assert _norm(lib, dtype=3) == INVALID and _norm(lib, dtype=-1) == INVALID and _norm(lib, params=5) == INVALID
+    assert _norm(lib, width=0) == INVALID and _norm(lib, batch=-1) == INVALID and _norm(lib, length=-1) == INVALID
+    assert _norm(lib, eps=-1.0) == INVALID and _norm(lib, eps=float("nan")) == INVALID
+    assert _norm(lib, pstride=32) == INVALID
+    assert _norm(lib, batch=65536, length=65536) == INVALID
+    assert _norm(lib, width=32769, pstride=0) == UNSUPPORTED
+    assert _norm(lib, batch=1, x=None) == INVALID and _norm(lib, batch=1, y=None) == INVALID
+    assert _norm(lib, batch=1, x=P16 + 1) == ALIGN and _norm(lib, batch=1, dtype=F32, params=F32, y=P16 + 2) == ALIGN
+    assert _norm(lib, batch=1, params=F32, factor=P16 + 2) == ALIGN
+    assert _norm(lib, batch=1, dtype=F32, params=BF16) == UNSUPPORTED
+    assert _norm(lib, batch=1, dtype=BF16, params=F16) == UNSUPPORTED
+
+
+def _norm_backward(lib, **k):
+    a = dict(dy=P16, gb=0, gr=64, x=P16, xb=0, xr=64, dtype=BF16, factor=P16, params=BF16, pstride=64, add=1, eps=1e-6,
+             batch=0, length=4, width=64, dx=P16, ob=0, orow=64, dfactor=P16, doffset=P16, ws=P16, nbytes=1 << 30)
+    a.update(k)
+    return lib.flk_layer_norm_backward(*a.values(), None)
+
+
+def test_layer_norm_backward_checks(lib):
+    assert _norm_backward(lib) == OK
+    assert _norm_backward(lib, batch=1, dy=None) == INVALID
+    assert _norm_backward(lib, batch=1, dy=P16 + 1) == ALIGN and _norm_backward(lib, batch=1, doffset=P16 + 1) == ALIGN
+    size = ctypes.c_int64(-1)
+    assert lib.flk_layer_norm_backward_plan(2, 4, 64, 0, ctypes.byref(size)) == OK and size.value >= 2 * 2 * 64 * 4
+    need = size.value
+    assert _norm_backward(lib, batch=2, nbytes=need - 1) == SCRATCH and _norm_backward(lib, batch=2, ws=None) == SCRATCH
+    assert _norm_backward(lib, batch=2, ws=P16 + 4) == ALIGN
+    assert _norm_backward(lib, batch=1 << 23, length=1) == INVALID   # more groups than one launch takes
+    assert lib.flk_layer_norm_backward_plan(0, 4, 64, 0, ctypes.byref(size)) == OK and size.value == 0
+    assert lib.flk_layer_norm_backward_plan(1, 4, 0, 0, ctypes.byref(size)) == INVALID
+    assert lib.flk_layer_norm_backward_plan(1, 4, 8, 0, None) == INVALID
+
+
+def test_swiglu_checks(lib):
+    def call(dtype=BF16, batch=0, length=3, hidden=5, gu=P16, h=P16):
+        return lib.flk_swiglu(gu, 0, 10, dtype, batch, length, hidden, h, 0, 5, None)
+
+    def back(dtype=BF16, batch=0, length=3, hidden=5, dh=P16, gu=P16, dgu=P16):
+        return lib.flk_swiglu_backward(dh, 0, 5, gu, 0, 10, dtype, batch, length, hidden, dgu, 0, 10, None)
+
+    for f in (call, back):
+        assert f() == OK and f(dtype=3) == INVALID and f(hidden=0) == INVALID and f(batch=-1) == INVALID
+        assert f(length=-1) == INVALID and f(hidden=2 ** 31 - 1) == INVALID
+        assert f(batch=1, gu=None) == INVALID and f(batch=1, gu=P16 + 1) == ALIGN and f(batch=1, dtype=F32, gu=P16 + 2) == ALIGN
+    assert call(batch=1, h=None) == INVALID and back(batch=1, dh=None) == INVALID and back(batch=1, dgu=P16 + 1) == ALIGN
+
+
+def test_mlp_checks(lib):
+    def gate(x=P16, xr=64, w=P16, wr=256, dtype=BF16, m=0, width=64, hidden=128, h=P16, hr=128, gu=P16, ws=P16):
+        return lib.flk_mlp_gate(x, xr, w, wr, dtype, m, width, hidden, h, hr, gu, ws, 1 << 40, None)
+
+    def back(x=P16, xr=64, w=P16, wr=64, gu=P16, dtype=BF16, m=0, width=64, hidden=128, h=P16, hr=256, ws=P16):
+        return lib.flk_mlp_gate_backward(x, xr, w, wr, gu, dtype, m, width, hidden, h, hr, ws, 1 << 40, None)
+
+    def mm(x=P16, xr=64, at=0, w=P16, wr=128, bt=0, dtype=BF16, rows=0, cols=128, inner=64, h=P16, hr=128):
+        return lib.flk_mlp_matmul(x, xr, at, w, wr, bt, dtype, rows, cols, inner, h, hr, P16, 1 << 40, None)
+
+    for f in (gate, back):
+        assert f() == OK and f(dtype=F32) == INVALID and f(m=-1) == INVALID and f(width=-8) == INVALID
+        assert f(xr=56) == INVALID and f(wr=56) == INVALID and f(hr=120) == INVALID
+        assert f(m=1, x=None) == INVALID and f(m=1, w=None) == INVALID and f(m=1, h=None) == INVALID
+        assert f(m=1, width=0) == INVALID and f(m=2 ** 31 - 1) == INVALID
+        assert f(m=1, width=60) == UNSUPPORTED and f(m=1, hidden=100) == UNSUPPORTED
+        assert f(m=1, xr=68) == ALIGN and f(m=1, wr=260) == ALIGN and f(m=1, hr=260) == ALIGN
+        assert f(m=1, x=P16 + 8) == ALIGN and f(m=1, w=P16 + 8) == ALIGN and f(m=1, h=P16 + 8) == ALIGN
+        assert f(m=1, gu=P16 + 8) == ALIGN
+    assert back(m=1, gu=None) == INVALID
+    assert mm() == OK and mm(rows=-1) == INVALID and mm(dtype=F32) == INVALID and mm(at=1, bt=1, wr=64) == UNSUPPORTED
+    assert mm(xr=56) == INVALID and mm(wr=120) == INVALID and mm(hr=120) == INVALID
+    assert mm(rows=1, inner=0) == INVALID and mm(rows=1, x=None) == INVALID
+    assert mm(rows=1, inner=60) == UNSUPPORTED and mm(rows=1, cols=124) == UNSUPPORTED
+    assert mm(at=1, rows=60, xr=64) == UNSUPPORTED
+    assert mm(rows=1, xr=68) == ALIGN and mm(rows=1, w=P16 + 8) == ALIGN
+    size = ctypes.c_int64(-1)
+    for product in range(5):
+        assert lib.flk_mlp_plan(product, 1, 4096, 1024, ctypes.byref(size)) == OK and size.value >= 0
+    assert lib.flk_mlp_plan(5, 1, 8, 8, ctypes.byref(size)) == INVALID
+    assert lib.flk_mlp_plan(0, -1, 8, 8, ctypes.byref(size)) == INVALID and lib.flk_mlp_plan(0, 1, 8, 8, None) == INVALID
+
+
+def test_python_refuses_host_tensors_and_bad_calls():
+    x = torch.zeros(2, 3, 16, dtype=torch.bfloat16)
+    for call in (lambda: norm.layer_norm(x), lambda: norm.modulate(x, x[:, 0], x[:, 0]), lambda: mlp.swiglu(x),
+                 lambda: norm.layer_norm_backward(x, x), lambda: mlp.swiglu_backward(x[..., :8], x),
+                 lambda: mlp.gated_mlp(x, torch.zeros(16, 32), torch.zeros(16, 16)),
+                 lambda: autograd.layer_norm(x), lambda: autograd.swiglu(x)):
+        with pytest.raises(ValueError, match="GPU only"):
+            call()
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        norm.layer_norm([1.0, 2.0])
