@@ -16,13 +16,16 @@ namespace {
 using flk::f32x4;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kThreads = 256;
-constexpr int kT = 64, kK = 32;       // tile edge, inner terms a step
-constexpr int kPitch = kK + 8;        // an LDS row, padded
+constexpr int kWaves = 8, kWN = 2, kWM = 4;   // waves of a block: across columns x across rows of D
+constexpr int kThreads = kWaves * 64;
+constexpr int kK = 64;                // inner terms a stage
+constexpr int kKBytes = kK * 2;       // of one operand row: a 128-byte line
+constexpr int kXcds = 8;
+constexpr int kGroup = 4;             // row tiles that sweep the column tiles together
 
 enum Epilogue { kPlain, kGate, kGateBackward };
 
-struct Operand {      // rows x inner: element (r, k) at r * stride + k, or with kAcross k * stride + r
+struct Operand {      // rows x inner: element (r, k) at r * stride + k, or, across its memory, k * stride + r
   const void* p;
   int64_t stride;
   int rows;
@@ -55,112 +58,383 @@ struct Mfma<_Float16> {
   }
 };
 
-// Row of the operand that tile row r holds: with kPair, 16 rows of the first half, then the same 16 of
-// the second (hidden further), for each 32 of the tile; -1 past the end.
-template <bool kPair>
-__device__ __forceinline__ int source_row(int tile, int r, int rows, int hidden) {
-  if constexpr (!kPair) return tile * kT + r < rows ? tile * kT + r : -1;
-  const int col = tile * (kT / 2) + r / 32 * 16 + r % 16;
-  return col >= hidden ? -1 : r % 32 < 16 ? col : hidden + col;
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  typedef T pair __attribute__((ext_vector_type(2)));
+  const pair p = {(T)lo, (T)hi};
+  return __builtin_bit_cast(uint32_t, p);
 }
 
-template <typename T, bool kAcross, bool kPair>
-__device__ __forceinline__ void stage(T (*lds)[kPitch], const Operand& o, int tile, int k0, int inner, int hidden) {
+// The 8-term chunk of an inner step's 32 that lane group h4 holds.  The LDS serves a b128 read's lanes l
+// and l + 32 together: groups 0 and 2 take neighbouring chunks.
+__device__ __forceinline__ int slot_chunk(int h4) { return ((h4 & 1) << 1) | (h4 >> 1); }
+
+// One operand's half of a stage: kT rows x 64 inner terms of 16 bits, in 16-byte chunks.
+//
+// Along its memory (a row's inner terms are contiguous) the half holds kT lines of 128 bytes, whose 8
+// chunks are XOR-swizzled by the row: an operand read takes one chunk each of 16 rows
+// (ds_read_b128) and lanes l, l + 32 take neighbouring chunks of the same 8 rows.
+//
+// Across its memory (neighbouring rows are contiguous) it holds 64 lines of kT elements, one per
+// inner term, and an operand read is two ds_read_b64_tr_b16: in each 16 lanes, source lane s points at
+// term s / 4 and columns 4 (s % 4) .. +3, and lane i receives column i of the four terms.  32 lanes
+// read 8 lines (four terms and the same + 16) x 2 chunks, which the swizzle puts on the 16
+// chunk positions of the 256-byte bank line: lines of whole 256 bytes need three bits of the
+// term, lines of odd multiples of 128 alternate between the halves and need two.
+//
+// Copies go from global memory straight into LDS (dma16_at), a wave instruction filling 64 chunks in
+// order, so the swizzle chooses what a lane fetches.  Both forms give the same k slots: lane groups
+// 0, 1, 2, 3 of an MFMA operand hold terms 0-7, 16-23, 8-15, 24-31 (slot_chunk).
+template <typename T, bool kAcross, int kT>
+struct Half {
   typedef typename Mfma<T>::vec vec;
-  const T* p = static_cast<const T*>(o.p);
-  vec v{};
-  if constexpr (!kAcross) {
-    const int r = threadIdx.x / 4, k = k0 + threadIdx.x % 4 * 8;
-    const int row = source_row<kPair>(tile, r, o.rows, hidden);
-    if (row >= 0 && k < inner) v = *reinterpret_cast<const vec*>(p + row * o.stride + k);
-    *reinterpret_cast<vec*>(&lds[r][threadIdx.x % 4 * 8]) = v;
-  } else {
-    const int k = k0 + threadIdx.x / 8, r = threadIdx.x % 8 * 8;
-    const int row = source_row<kPair>(tile, r, o.rows, hidden);
-    if (row >= 0 && k < inner) v = *reinterpret_cast<const vec*>(p + k * o.stride + row);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) lds[r + i][threadIdx.x / 8] = v[i];
+  static constexpr int kBytes = kT * kKBytes;
+  static constexpr int kCopies = kBytes / 1024 / kWaves;   // copy instructions per wave
+  static constexpr int kLine = kAcross ? kT * 2 : kKBytes;
+  static constexpr int kLineChunks = kLine / 16;
+  static_assert(kBytes % (1024 * kWaves) == 0, "whole copies per wave");
+
+  static __device__ __forceinline__ int swizzle(int line) {
+    if constexpr (!kAcross) return (line & 7) ^ ((line >> 3) & 1);
+    if constexpr (kLine % 256 == 0) return 2 * ((line & 3) | ((line >> 2) & 4));
+    return 2 * (((line >> 1) & 1) | ((line >> 3) & 2));
   }
-}
 
-template <typename T, bool kAAcross, bool kBAcross, Epilogue kE>
-__global__ __launch_bounds__(kThreads) void mlp_kernel(const Product P) {
-  typedef typename Mfma<T>::vec vec;
-  __shared__ __attribute__((aligned(16))) T la[kT][kPitch], lb[kT][kPitch];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wb = wave >> 1, wa = wave & 1, l16 = lane & 15, h4 = lane >> 4;
-  const int ta = blockIdx.x % P.tiles_a, tb = blockIdx.x / P.tiles_a;
-  f32x4 acc[2][2] = {};
-  for (int k0 = 0; k0 < P.inner; k0 += kK) {
-    stage<T, kAAcross, false>(la, P.a, ta, k0, P.inner, 0);
-    stage<T, kBAcross, kE == kGate>(lb, P.b, tb, k0, P.inner, P.hidden);
-    __syncthreads();
-    vec fa[2], fb[2];
+  const uint8_t* base;          // the tile's first row / column
+  int64_t step;                 // bytes from one stage to the next
+  uint32_t from[kCopies];       // what this lane fetches, from base
+
+  // rows / terms beyond the operand repeat its last one; results of repeated rows are never stored, and
+  // repeated terms are never fetched (tail).  kPair: see pair_column.
+  template <typename Column>
+  __device__ __forceinline__ void init(const Operand& o, int64_t first, int wave, int lane, Column column) {
+    const int64_t pitch = o.stride * 2;
+    base = static_cast<const uint8_t*>(o.p) + (kAcross ? 0 : first * pitch);
+    step = kAcross ? kK * pitch : kKBytes;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      fa[i] = *reinterpret_cast<const vec*>(&la[wa * 32 + i * 16 + l16][h4 * 8]);
-      fb[i] = *reinterpret_cast<const vec*>(&lb[wb * 32 + i * 16 + l16][h4 * 8]);
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = (wave * kCopies + i) * 64 + lane, line = at / kLineChunks, chunk = (at % kLineChunks) ^ swizzle(line);
+      if constexpr (kAcross)
+        from[i] = (uint32_t)(line * (uint32_t)pitch) + 2u * (uint32_t)column(chunk * 8);
+      else
+        from[i] = (uint32_t)column(line) * (uint32_t)pitch + chunk * 16;
     }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int m = 0; m < 2; ++m) acc[n][m] = Mfma<T>::run(fb[n], fa[m], acc[n][m]);
-    __syncthreads();
   }
-  T* d = static_cast<T*>(P.d);
+  __device__ __forceinline__ void copy(int i, int stage, uint8_t* lds, int wave) const {
+    flk::dma16_at(base + stage * step, from[i], lds + (wave * kCopies + i) * 1024);
+  }
+  // The last stage where `left` < 64 terms are left: zeros in place of the terms that are not there.
+  __device__ __forceinline__ void tail(int stage, int left, uint8_t* lds, int wave, int lane) const {
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const int64_t row = (int64_t)ta * kT + wa * 32 + m * 16 + l16;
-    if (row >= P.a.rows) continue;
-    if constexpr (kE == kGate) {
-      const int col = tb * (kT / 2) + wb * 16 + h4 * 4;
-      if (col >= P.hidden) continue;
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = (wave * kCopies + i) * 64 + lane, line = at / kLineChunks;
+      const int term = kAcross ? line : ((at % kLineChunks) ^ swizzle(line)) * 8;
+      uint4 v = {0, 0, 0, 0};
+      if (term < left) v = *reinterpret_cast<const uint4*>(base + stage * step + from[i]);
+      *reinterpret_cast<uint4*>(lds + at * 16) = v;
+    }
+  }
+};
+
+// A wave's fragments of 16 rows x 32 terms of a half: fragment f, inner step ks.
+template <typename T, bool kAcross, int kT, int kFrags>
+struct Frags {
+  typedef typename Mfma<T>::vec vec;
+  typedef Half<T, kAcross, kT> H;
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef short s16x8 __attribute__((ext_vector_type(8)));
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  int off[kAcross ? kFrags : 2];   // along: of inner steps 0, 1; across: of fragment f
+  __device__ __forceinline__ void init(int first, int lane) {   // first: the wave's first row in the tile
+    const int l16 = lane & 15, c4 = slot_chunk(lane >> 4);
+    if constexpr (!kAcross) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float g = acc[0][m][i], u = acc[1][m][i];
-        d[row * P.d_stride + col + i] = (T)flk::gate(g, u);
-        if (P.gu) {
-          P.gu[row * 2 * P.hidden + col + i] = g;
-          P.gu[row * 2 * P.hidden + P.hidden + col + i] = u;
-        }
-      }
+      for (int ks = 0; ks < 2; ++ks) off[ks] = (first + l16) * kKBytes + (((4 * ks + c4) ^ H::swizzle(l16)) * 16);
     } else {
+      const int line = 8 * c4 + (l16 >> 2);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int col = tb * kT + wb * 32 + n * 16 + h4 * 4;
-        if (col >= P.b.rows) continue;
+      for (int f = 0; f < kFrags; ++f) {
+        const int chunk = (first + f * 16) / 8 + ((l16 >> 1) & 1);
+        off[f] = line * H::kLine + ((chunk ^ H::swizzle(line)) * 16) + (l16 & 1) * 8;
+      }
+    }
+  }
+  __device__ __forceinline__ vec read(const uint8_t* half, int f, int ks) const {
+    if constexpr (!kAcross) {
+      return *reinterpret_cast<const vec*>(half + off[ks] + f * 16 * kKBytes);
+    } else {
+      const uint8_t* p = half + off[f] + ks * 32 * H::kLine;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * H::kLine));
+      const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(vec, both);
+    }
+  }
+};
+
+// Column tiles of the gate's product: a wave's kCols columns are kCols / 2 of g, then the same of u.
+template <int kCols>
+__device__ __forceinline__ int pair_column(int tile, int c, int hidden) {
+  const int wave = c / kCols, i = c % kCols, half = kCols / 2;
+  const int col = min(tile * (kWN * half) + wave * half + i % half, hidden - 8 + i % 8);
+  return i < half ? col : hidden + col;
+}
+
+// Finished values leave through the wave's part of the LDS as rows of kChunks 16-byte chunks, written
+// four columns a lane and read back a chunk a lane, so that every store is 16 bytes of a
+// contiguous row.
+template <int kChunks>
+__device__ __forceinline__ int out_swizzle(int row) {
+  constexpr int mask = kChunks % 16 == 0 ? 15 : kChunks % 8 == 0 ? 7 : kChunks % 4 == 0 ? 3 : 1;
+  return row & mask;
+}
+
+template <typename T, int kChunks, int kRows>
+__device__ __forceinline__ void store_rows(const uint8_t* lds, T* d, int64_t stride, int64_t row0, int64_t rows,
+                                           int col0, int cols, int lane) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = acc[n][m][i];
-          if constexpr (kE == kPlain) {
-            d[row * P.d_stride + col + i] = (T)x;
-          } else {
-            const float g = P.gu[row * 2 * P.hidden + col + i], u = P.gu[row * 2 * P.hidden + P.hidden + col + i];
-            float dg, du;
-            flk::gate_backward(x, g, u, dg, du);
-            d[row * P.d_stride + col + i] = (T)dg;
-            d[row * P.d_stride + P.hidden + col + i] = (T)du;
+  for (int it = 0; it < (kRows * kChunks + 63) / 64; ++it) {
+    const int at = it * 64 + lane, r = at / kChunks, c = at % kChunks;
+    if (kRows * kChunks % 64 && r >= kRows) break;
+    const uint4 v = *reinterpret_cast<const uint4*>(lds + (r * kChunks + (c ^ out_swizzle<kChunks>(r))) * 16);
+    if (row0 + r < rows && col0 + c * 8 < cols) *reinterpret_cast<uint4*>(d + (row0 + r) * stride + col0 + c * 8) = v;
+  }
+}
+
+template <typename T, int kChunks>
+__device__ __forceinline__ void put4(uint8_t* lds, int row, int col, const float (&x)[4]) {
+  *reinterpret_cast<uint2*>(lds + (row * kChunks + ((col >> 3) ^ out_swizzle<kChunks>(row))) * 16 + (col & 4) * 2) =
+      uint2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+}
+
+// Logical tile u -> its row and column tiles: kGroup row tiles sweep the column tiles together.
+__device__ __forceinline__ void tile_of(int u, int tiles_a, int tiles_b, int& ta, int& tb) {
+  const int group_tiles = kGroup * tiles_b, group = u / group_tiles, first = group * kGroup;
+  const int rows = min(kGroup, tiles_a - first), in_group = u - group * group_tiles;
+  ta = first + in_group % rows;
+  tb = in_group / rows;
+}
+
+// One tile of D: 32 kNF columns x 64 kMF rows, a wave 16 kNF x 16 kMF of them.
+template <typename T, bool kAAcross, bool kBAcross, Epilogue kE, int kNF, int kMF>
+__global__ __launch_bounds__(kThreads, 2) void mlp_kernel(const Product P) {
+  constexpr int kTB = 16 * kNF * kWN, kTA = 16 * kMF * kWM;
+  typedef Half<T, kBAcross, kTB> HB;
+  typedef Half<T, kAAcross, kTA> HA;
+  constexpr int kStage = HB::kBytes + HA::kBytes;
+  constexpr int kRing = kNF % 4 == 0 ? 4 : 3, kLead = kRing - 1;   // column fragments in flight, and read ahead
+  static_assert(kNF % kRing == 0, "the fragment ring must divide the groups of a step");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wb = wave / kWM, wa = wave % kWM, l16 = lane & 15, h4 = lane >> 4;
+
+  // Blocks are dealt round-robin over the XCDs; each XCD runs a contiguous range of logical tiles.
+  const int xcd = blockIdx.x % kXcds, per = gridDim.x / kXcds, extra = gridDim.x % kXcds;
+  int ta, tb;
+  tile_of(xcd * per + min(xcd, extra) + blockIdx.x / kXcds, P.tiles_a, P.tiles_b, ta, tb);
+
+  HB hb;
+  HA ha;
+  const int64_t row0 = (int64_t)ta * kTA, col0 = (int64_t)tb * kTB;
+  if constexpr (kE == kGate)
+    hb.init(P.b, 0, wave, lane, [&](int c) { return pair_column<16 * kNF>(tb, c, P.hidden); });
+  else if constexpr (kBAcross)
+    hb.init(P.b, 0, wave, lane, [&](int c) { return min((int)col0 + c, P.b.rows - 8); });
+  else
+    hb.init(P.b, col0, wave, lane, [&](int r) { return min(r, P.b.rows - 1 - (int)col0); });
+  if constexpr (kAAcross)
+    ha.init(P.a, 0, wave, lane, [&](int c) { return min((int)row0 + c, P.a.rows - 8); });
+  else
+    ha.init(P.a, row0, wave, lane, [&](int r) { return min(r, P.a.rows - 1 - (int)row0); });
+
+  const int stages = (P.inner + kK - 1) / kK, left = P.inner - (stages - 1) * kK;   // terms of the last stage
+  auto copy_stage = [&](int s) {
+    uint8_t* lds = smem + (s & 1) * kStage;
+    if (left < kK && s == stages - 1) {
+      hb.tail(s, left, lds, wave, lane);
+      ha.tail(s, left, lds + HB::kBytes, wave, lane);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < HB::kCopies || i < HA::kCopies; ++i) {
+      if (i < HB::kCopies) hb.copy(i, s, lds, wave);
+      if (i < HA::kCopies) ha.copy(i, s, lds + HB::kBytes, wave);
+    }
+  };
+  Frags<T, kBAcross, kTB, kNF> fb;
+  Frags<T, kAAcross, kTA, kMF> fa;
+  fb.init(wb * 16 * kNF, lane);
+  fa.init(wa * 16 * kMF, lane);
+
+  f32x4 acc[kNF][kMF];
+#pragma unroll
+  for (int n = 0; n < kNF; ++n)
+#pragma unroll
+    for (int m = 0; m < kMF; ++m) acc[n][m] = f32x4{};
+
+  // Two stages of two inner steps each.  Step 0 reads step 1's fragments as it goes; step 1 reads its own
+  // last column fragments, then -- every wave done reading the stage, the next one landed everywhere
+  // (the barrier) -- refills the stage's buffer with the stage after next and reads the next
+  // stage's first fragments.  After the last stage those reads take what is there; nothing uses it.
+  copy_stage(0);
+  if (stages > 1) copy_stage(1);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+  typedef typename Mfma<T>::vec vec;
+  vec ring[kRing], a0[kMF], a1[kMF];
+#pragma unroll
+  for (int m = 0; m < kMF; ++m) a0[m] = fa.read(smem + HB::kBytes, m, 0);
+#pragma unroll
+  for (int n = 0; n < kLead; ++n) ring[n] = fb.read(smem, n, 0);
+  auto group = [&](int n, const vec (&a)[kMF]) {
+#pragma unroll
+    for (int m = 0; m < kMF; ++m) acc[n][m] = Mfma<T>::run(ring[n % kRing], a[m], acc[n][m]);
+  };
+  for (int s = 0; s < stages; ++s) {
+    const uint8_t* cs = smem + (s & 1) * kStage;
+    const uint8_t* ns = smem + ((s + 1) & 1) * kStage;
+#pragma unroll
+    for (int n = 0; n < kNF; ++n) {
+      group(n, a0);
+      const int next = n + kLead;
+      ring[next % kRing] = next < kNF ? fb.read(cs, next, 0) : fb.read(cs, next - kNF, 1);
+      if (n < kMF) a1[n] = fa.read(cs + HB::kBytes, n, 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int n = 0; n < kNF - kLead; ++n) {
+      group(n, a1);
+      ring[(n + kLead) % kRing] = fb.read(cs, n + kLead, 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + 2 < stages) copy_stage(s + 2);
+#pragma unroll
+    for (int n = kNF - kLead; n < kNF; ++n) {
+      group(n, a1);
+      ring[(n + kLead) % kRing] = fb.read(ns, n + kLead - kNF, 0);
+      const int j = n - (kNF - kLead);
+#pragma unroll
+      for (int m = 0; m < kMF; ++m)
+        if (m * kLead / kMF == j) a0[m] = fa.read(ns + HB::kBytes, m, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();   // every wave is done reading the stages
+
+  // The lane owns row l16 and columns 4 h4 .. +3 of each 16 x 16 fragment.
+  constexpr int kRows = 16 * kMF;
+  T* d = static_cast<T*>(P.d);
+  const int64_t wrow = row0 + wa * kRows;
+  if constexpr (kE == kPlain) {
+    constexpr int kChunks = 2 * kNF;
+    uint8_t* out = smem + wave * (kRows * kChunks * 16);
+#pragma unroll
+    for (int n = 0; n < kNF; ++n)
+#pragma unroll
+      for (int m = 0; m < kMF; ++m) {
+        const float x[4] = {acc[n][m][0], acc[n][m][1], acc[n][m][2], acc[n][m][3]};
+        put4<T, kChunks>(out, m * 16 + l16, n * 16 + h4 * 4, x);
+      }
+    store_rows<T, kChunks, kRows>(out, d, P.d_stride, wrow, P.a.rows, (int)col0 + wb * 16 * kNF, P.b.rows, lane);
+  } else if constexpr (kE == kGateBackward) {
+    // dh leaves as float32 rows of half the wave's columns at a time; a lane takes 8 columns of a row
+    // back, so that g and u are read, and dg and du written, in whole lines.
+    constexpr int kPass = kNF / 2, kChunks = kPass * 4, kParts = kPass * 2;   // chunks of 4, parts of 8 columns
+    constexpr int kTurns = (kRows * kParts + 63) / 64, kBatch = kTurns % 4 == 0 ? 4 : 3;
+    uint8_t* out = smem + wave * (kRows * kChunks * 16);
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+      for (int n = 0; n < kPass; ++n)
+#pragma unroll
+        for (int m = 0; m < kMF; ++m) {
+          const int r = m * 16 + l16;
+          *reinterpret_cast<f32x4*>(out + (r * kChunks + ((n * 4 + h4) ^ out_swizzle<kChunks>(r))) * 16) =
+              acc[pass * kPass + n][m];
+        }
+      const int wcol = (int)col0 + wb * 16 * kNF + pass * kPass * 16;
+#pragma unroll
+      for (int first = 0; first < kTurns; first += kBatch) {
+        f32x4 g[kBatch][2], u[kBatch][2];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int at = (first + i) * 64 + lane, r = at / kParts, col = wcol + at % kParts * 8;
+          if (r >= kRows || wrow + r >= P.a.rows || col >= P.hidden) continue;
+          const f32x4* src = reinterpret_cast<const f32x4*>(P.gu + (wrow + r) * 2 * P.hidden + col);
+          const f32x4* usrc = reinterpret_cast<const f32x4*>(P.gu + (wrow + r) * 2 * P.hidden + P.hidden + col);
+          g[i][0] = src[0];
+          g[i][1] = src[1];
+          u[i][0] = usrc[0];
+          u[i][1] = usrc[1];
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int at = (first + i) * 64 + lane, r = at / kParts, part = at % kParts, col = wcol + part * 8;
+          if (r >= kRows || wrow + r >= P.a.rows || col >= P.hidden) continue;
+          float dg[8], du[8];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const f32x4 dh = *reinterpret_cast<const f32x4*>(
+                out + (r * kChunks + ((part * 2 + c) ^ out_swizzle<kChunks>(r))) * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) flk::gate_backward(dh[j], g[i][c][j], u[i][c][j], dg[c * 4 + j], du[c * 4 + j]);
           }
+          T* dst = d + (wrow + r) * P.d_stride + col;
+          *reinterpret_cast<uint4*>(dst) = uint4{pack2<T>(dg[0], dg[1]), pack2<T>(dg[2], dg[3]), pack2<T>(dg[4], dg[5]),
+                                                 pack2<T>(dg[6], dg[7])};
+          *reinterpret_cast<uint4*>(dst + P.hidden) = uint4{pack2<T>(du[0], du[1]), pack2<T>(du[2], du[3]),
+                                                            pack2<T>(du[4], du[5]), pack2<T>(du[6], du[7])};
         }
       }
     }
+  } else {
+    constexpr int kHalf = kNF / 2, kChunks = kNF;
+    uint8_t* out = smem + wave * (kRows * kChunks * 16);
+    const int wcol = tb * (kTB / 2) + wb * 16 * kHalf;
+#pragma unroll
+    for (int n = 0; n < kHalf; ++n)
+#pragma unroll
+      for (int m = 0; m < kMF; ++m) {
+        const f32x4 g = acc[n][m], u = acc[n + kHalf][m];
+        const int64_t row = wrow + m * 16 + l16;
+        const int col = wcol + n * 16 + h4 * 4;
+        if (P.gu && row < P.a.rows && col < P.hidden) {
+          float* dst = P.gu + row * 2 * P.hidden + col;
+          *reinterpret_cast<f32x4*>(dst) = g;
+          *reinterpret_cast<f32x4*>(dst + P.hidden) = u;
+        }
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = flk::gate(g[i], u[i]);
+        put4<T, kChunks>(out, m * 16 + l16, n * 16 + h4 * 4, x);
+      }
+    store_rows<T, kChunks, kRows>(out, d, P.d_stride, wrow, P.a.rows, wcol, P.hidden, lane);
   }
 }
 
 constexpr int kMaxDim = INT32_MAX - 256;
+constexpr int64_t kMaxStride = 1 << 22;   // 256 rows of one operand are addressed in 32 bits
+
+template <typename T, bool kAAcross, bool kBAcross, Epilogue kE, int kNF, int kMF>
+int launch_tiles(Product& p, void* stream) {
+  constexpr int kTB = 16 * kNF * kWN, kTA = 16 * kMF * kWM;
+  p.tiles_a = (p.a.rows + kTA - 1) / kTA;
+  p.tiles_b = kE == kGate ? (p.hidden + kTB / 2 - 1) / (kTB / 2) : (p.b.rows + kTB - 1) / kTB;
+  const int64_t blocks = (int64_t)p.tiles_a * p.tiles_b;
+  if (blocks > (1 << 22)) return FLK_E_INVALID;   // work-items of a launch are counted in 32 bits
+  mlp_kernel<T, kAAcross, kBAcross, kE, kNF, kMF>
+      <<<dim3((unsigned)blocks), kThreads, 0, static_cast<hipStream_t>(stream)>>>(p);
+  return flk_launch_status();
+}
 
 template <bool kAAcross, bool kBAcross, Epilogue kE>
 int launch(Product& p, int dtype, void* stream) {
-  p.tiles_a = (p.a.rows + kT - 1) / kT;
-  p.tiles_b = kE == kGate ? (p.hidden + kT / 2 - 1) / (kT / 2) : (p.b.rows + kT - 1) / kT;
-  const int64_t blocks = (int64_t)p.tiles_a * p.tiles_b;
-  if (blocks > (1 << 23)) return FLK_E_INVALID;   // work-items of a launch are counted in 32 bits
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == FLK_BF16)
-    mlp_kernel<__bf16, kAAcross, kBAcross, kE><<<dim3((unsigned)blocks), kThreads, 0, s>>>(p);
-  else
-    mlp_kernel<_Float16, kAAcross, kBAcross, kE><<<dim3((unsigned)blocks), kThreads, 0, s>>>(p);
-  return flk_launch_status();
+  if (p.a.stride > kMaxStride || p.b.stride > kMaxStride) return FLK_E_INVALID;
+  if (dtype == FLK_BF16) return launch_tiles<__bf16, kAAcross, kBAcross, kE, 8, 4>(p, stream);
+  return launch_tiles<_Float16, kAAcross, kBAcross, kE, 8, 4>(p, stream);
 }
 
 bool odd8(int64_t v) { return v % 8 != 0; }
