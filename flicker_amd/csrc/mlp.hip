@@ -9,6 +9,8 @@
 // columns of one row.  The gate's product takes g's and u's columns into one tile: a lane that holds
 // g of a column holds u of the same column, and h leaves the registers as the only output.
 
+#include <algorithm>
+
 #include "elems.h"
 
 namespace {
@@ -16,14 +18,28 @@ namespace {
 using flk::f32x4;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kWaves = 8, kWN = 2, kWM = 4;   // waves of a block: across columns x across rows of D
-constexpr int kThreads = kWaves * 64;
+// A block's tile: WN x WM waves across the columns and rows of D, each NF x MF fragments of 16 x 16.
+template <int WN, int WM, int NF, int MF, int BUFFERS, int PER_CU, int RING, int LEAD, int BAR>
+struct Geometry {
+  static constexpr int kWN = WN, kWM = WM, kNF = NF, kMF = MF;
+  static constexpr int kRing = RING, kLead = LEAD, kBar = BAR;
+  static constexpr int kBuffers = BUFFERS;   // stages in LDS
+  static constexpr int kPerCU = PER_CU;      // blocks a CU holds
+  static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
+  static constexpr int kTB = 16 * NF * WN, kTA = 16 * MF * WM;
+};
+typedef Geometry<2, 4, 8, 4, 2, 1, 4, 3, 3> Large;    // 256 columns x 256 rows
+typedef Geometry<2, 4, 6, 4, 2, 1, 3, 2, 2> Medium;   // 192 x 256
+typedef Geometry<2, 2, 4, 4, 2, 2, 4, 3, 3> Small;    // 128 x 128, two blocks a CU
+typedef Geometry<2, 2, 4, 4, 4, 1, 4, 3, 3> Deep;     // 128 x 128, one block a CU with more stages in flight
+typedef Geometry<4, 1, 2, 2, 4, 2, 4, 2, 1> Few;      // 128 x 32: few rows, the columns' operand streams through
+
 constexpr int kK = 64;                // inner terms a stage
 constexpr int kKBytes = kK * 2;       // of one operand row: a 128-byte line
 constexpr int kXcds = 8;
 constexpr int kGroup = 4;             // row tiles that sweep the column tiles together
 
-enum Epilogue { kPlain, kGate, kGateBackward };
+enum Epilogue { kPlain, kGate, kGateBackward, kPartial };
 
 struct Operand {      // rows x inner: element (r, k) at r * stride + k, or, across its memory, k * stride + r
   const void* p;
@@ -39,6 +55,8 @@ struct Product {
   float* gu;          // kGate: out, may be NULL; kGateBackward: in
   int hidden;         // kGate, kGateBackward
   int tiles_a, tiles_b;
+  float* partial;     // kPartial: (splits, rows, cols) sums over `stages` stages each
+  int splits, stages;
 };
 
 template <typename T>
@@ -85,7 +103,7 @@ __device__ __forceinline__ int slot_chunk(int h4) { return ((h4 & 1) << 1) | (h4
 // Copies go from global memory straight into LDS (dma16_at), a wave instruction filling 64 chunks in
 // order, so the swizzle chooses what a lane fetches.  Both forms give the same k slots: lane groups
 // 0, 1, 2, 3 of an MFMA operand hold terms 0-7, 16-23, 8-15, 24-31 (slot_chunk).
-template <typename T, bool kAcross, int kT>
+template <typename T, bool kAcross, int kT, int kWaves>
 struct Half {
   typedef typename Mfma<T>::vec vec;
   static constexpr int kBytes = kT * kKBytes;
@@ -137,10 +155,9 @@ struct Half {
 };
 
 // A wave's fragments of 16 rows x 32 terms of a half: fragment f, inner step ks.
-template <typename T, bool kAcross, int kT, int kFrags>
+template <typename T, typename H, bool kAcross, int kFrags>
 struct Frags {
   typedef typename Mfma<T>::vec vec;
-  typedef Half<T, kAcross, kT> H;
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   typedef short s16x8 __attribute__((ext_vector_type(8)));
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -173,7 +190,7 @@ struct Frags {
 };
 
 // Column tiles of the gate's product: a wave's kCols columns are kCols / 2 of g, then the same of u.
-template <int kCols>
+template <int kCols, int kWN>
 __device__ __forceinline__ int pair_column(int tile, int c, int hidden) {
   const int wave = c / kCols, i = c % kCols, half = kCols / 2;
   const int col = min(tile * (kWN * half) + wave * half + i % half, hidden - 8 + i % 8);
@@ -215,30 +232,37 @@ __device__ __forceinline__ void tile_of(int u, int tiles_a, int tiles_b, int& ta
   tb = in_group / rows;
 }
 
-// One tile of D: 32 kNF columns x 64 kMF rows, a wave 16 kNF x 16 kMF of them.
-template <typename T, bool kAAcross, bool kBAcross, Epilogue kE, int kNF, int kMF>
-__global__ __launch_bounds__(kThreads, 2) void mlp_kernel(const Product P) {
-  constexpr int kTB = 16 * kNF * kWN, kTA = 16 * kMF * kWM;
-  typedef Half<T, kBAcross, kTB> HB;
-  typedef Half<T, kAAcross, kTA> HA;
-  constexpr int kStage = HB::kBytes + HA::kBytes;
-  constexpr int kRing = kNF % 4 == 0 ? 4 : 3, kLead = kRing - 1;   // column fragments in flight, and read ahead
-  static_assert(kNF % kRing == 0, "the fragment ring must divide the groups of a step");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
+// One tile of D; kPartial: its sum over one range of the inner axis.
+template <typename T, bool kAAcross, bool kBAcross, Epilogue kE, typename G>
+__global__ __launch_bounds__(G::kThreads, G::kThreads * G::kPerCU / 256) void mlp_kernel(const Product P) {
+  constexpr int kNF = G::kNF, kMF = G::kMF, kWM = G::kWM, kTB = G::kTB, kTA = G::kTA, kBuffers = G::kBuffers;
+  typedef Half<T, kBAcross, kTB, G::kWaves> HB;
+  typedef Half<T, kAAcross, kTA, G::kWaves> HA;
+  constexpr int kStage = HB::kBytes + HA::kBytes, kCopies = HB::kCopies + HA::kCopies;
+  // A stage is kGroups groups of kMF MFMAs, inner step by inner step, each on one column fragment.  Fragments
+  // are read kLead groups ahead into a ring; kBar groups of a stage follow its barrier.
+  constexpr int kGroups = 2 * kNF, kRing = G::kRing, kLead = G::kLead, kBar = G::kBar;
+  static_assert(kGroups % kRing == 0 && kLead < kRing && kBar <= kLead && kMF <= kNF, "the fragment ring divides a stage");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kBuffers * kStage];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wb = wave / kWM, wa = wave % kWM, l16 = lane & 15, h4 = lane >> 4;
 
-  // Blocks are dealt round-robin over the XCDs; each XCD runs a contiguous range of logical tiles.
+  // Blocks are dealt round-robin over the XCDs; each XCD runs a contiguous range of logical tiles, the
+  // ranges of a split tile's inner axis one after the other.
   const int xcd = blockIdx.x % kXcds, per = gridDim.x / kXcds, extra = gridDim.x % kXcds;
-  int ta, tb;
-  tile_of(xcd * per + min(xcd, extra) + blockIdx.x / kXcds, P.tiles_a, P.tiles_b, ta, tb);
+  int unit = xcd * per + min(xcd, extra) + blockIdx.x / kXcds, ta, tb, range = 0;
+  if constexpr (kE == kPartial) {
+    range = unit / (P.tiles_a * P.tiles_b);
+    unit -= range * (P.tiles_a * P.tiles_b);
+  }
+  tile_of(unit, P.tiles_a, P.tiles_b, ta, tb);
 
   HB hb;
   HA ha;
   const int64_t row0 = (int64_t)ta * kTA, col0 = (int64_t)tb * kTB;
   if constexpr (kE == kGate)
-    hb.init(P.b, 0, wave, lane, [&](int c) { return pair_column<16 * kNF>(tb, c, P.hidden); });
+    hb.init(P.b, 0, wave, lane, [&](int c) { return pair_column<16 * kNF, G::kWN>(tb, c, P.hidden); });
   else if constexpr (kBAcross)
     hb.init(P.b, 0, wave, lane, [&](int c) { return min((int)col0 + c, P.b.rows - 8); });
   else
@@ -248,22 +272,32 @@ __global__ __launch_bounds__(kThreads, 2) void mlp_kernel(const Product P) {
   else
     ha.init(P.a, row0, wave, lane, [&](int r) { return min(r, P.a.rows - 1 - (int)row0); });
 
-  const int stages = (P.inner + kK - 1) / kK, left = P.inner - (stages - 1) * kK;   // terms of the last stage
-  auto copy_stage = [&](int s) {
-    uint8_t* lds = smem + (s & 1) * kStage;
-    if (left < kK && s == stages - 1) {
-      hb.tail(s, left, lds, wave, lane);
-      ha.tail(s, left, lds + HB::kBytes, wave, lane);
-      return;
-    }
+  // Stages first .. first + stages - 1 of the inner axis; the axis' last may have fewer terms (left).
+  const int all = (P.inner + kK - 1) / kK, left = P.inner - (all - 1) * kK;
+  const int first = kE == kPartial ? range * P.stages : 0;
+  const int stages = kE == kPartial ? min(P.stages, all - first) : all;
+  const int whole = first + stages == all && left < kK ? stages - 1 : stages;   // stages that are copied by DMA
+  auto copy_some = [&](int s, int from, int to) {   // copy instructions [from, to) of a whole stage
+    uint8_t* lds = smem + s % kBuffers * kStage;
 #pragma unroll
-    for (int i = 0; i < HB::kCopies || i < HA::kCopies; ++i) {
-      if (i < HB::kCopies) hb.copy(i, s, lds, wave);
-      if (i < HA::kCopies) ha.copy(i, s, lds + HB::kBytes, wave);
+    for (int i = 0; i < kCopies; ++i) {
+      if (i < from || i >= to) continue;
+      constexpr int kBoth = 2 * (HB::kCopies < HA::kCopies ? HB::kCopies : HA::kCopies);   // alternating, then the rest
+      const bool b = i < kBoth ? i % 2 == 0 : HB::kCopies > HA::kCopies;
+      const int k = i < kBoth ? i / 2 : i - kBoth / 2;
+      if (b)
+        hb.copy(k, first + s, lds, wave);
+      else
+        ha.copy(k, first + s, lds + HB::kBytes, wave);
     }
   };
-  Frags<T, kBAcross, kTB, kNF> fb;
-  Frags<T, kAAcross, kTA, kMF> fa;
+  auto tail_stage = [&](int s) {
+    uint8_t* lds = smem + s % kBuffers * kStage;
+    hb.tail(first + s, left, lds, wave, lane);
+    ha.tail(first + s, left, lds + HB::kBytes, wave, lane);
+  };
+  Frags<T, HB, kBAcross, kNF> fb;
+  Frags<T, HA, kAAcross, kMF> fa;
   fb.init(wb * 16 * kNF, lane);
   fa.init(wa * 16 * kMF, lane);
 
@@ -273,51 +307,63 @@ __global__ __launch_bounds__(kThreads, 2) void mlp_kernel(const Product P) {
 #pragma unroll
     for (int m = 0; m < kMF; ++m) acc[n][m] = f32x4{};
 
-  // Two stages of two inner steps each.  Step 0 reads step 1's fragments as it goes; step 1 reads its own
-  // last column fragments, then -- every wave done reading the stage, the next one landed everywhere
-  // (the barrier) -- refills the stage's buffer with the stage after next and reads the next
-  // stage's first fragments.  After the last stage those reads take what is there; nothing uses it.
-  copy_stage(0);
-  if (stages > 1) copy_stage(1);
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  // kBuffers stages of two inner steps each.  Step 0 reads step 1's fragments as it goes; step 1 reads its
+  // own last column fragments, then -- every wave done reading the stage, the next one landed
+  // everywhere (the barrier) -- refills the stage's buffer with the stage kBuffers on and reads the
+  // next stage's first fragments.  After the last stage those reads take what is there; nothing uses it.
+  // Copies return in order: while `later` whole stages follow the awaited one, theirs may be in flight.
+  constexpr int kLater = kBuffers - 2;
+  constexpr int kSpread = (kCopies + kBar + kNF - 1) / (kBar + kNF);   // copy instructions a group
+#pragma unroll
+  for (int s = 0; s < kBuffers; ++s) {
+    if (s < whole)
+      copy_some(s, 0, kCopies);
+    else if (s < stages)
+      tail_stage(s);
+  }
+  if (kLater > 0 && kBuffers <= whole)
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((kLater + 1) * kCopies) : "memory");
+  else
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
   typedef typename Mfma<T>::vec vec;
-  vec ring[kRing], a0[kMF], a1[kMF];
+  vec ring[kRing], a[2][kMF];
+  auto read_b = [&](const uint8_t* stage, int g) { return fb.read(stage, g % kNF, g / kNF); };
 #pragma unroll
-  for (int m = 0; m < kMF; ++m) a0[m] = fa.read(smem + HB::kBytes, m, 0);
+  for (int m = 0; m < kMF; ++m) a[0][m] = fa.read(smem + HB::kBytes, m, 0);
 #pragma unroll
-  for (int n = 0; n < kLead; ++n) ring[n] = fb.read(smem, n, 0);
-  auto group = [&](int n, const vec (&a)[kMF]) {
-#pragma unroll
-    for (int m = 0; m < kMF; ++m) acc[n][m] = Mfma<T>::run(ring[n % kRing], a[m], acc[n][m]);
-  };
+  for (int g = 0; g < kLead; ++g) ring[g] = read_b(smem, g);
   for (int s = 0; s < stages; ++s) {
-    const uint8_t* cs = smem + (s & 1) * kStage;
-    const uint8_t* ns = smem + ((s + 1) & 1) * kStage;
+    const uint8_t* cs = smem + s % kBuffers * kStage;
+    const uint8_t* ns = smem + (s + 1) % kBuffers * kStage;
 #pragma unroll
-    for (int n = 0; n < kNF; ++n) {
-      group(n, a0);
-      const int next = n + kLead;
-      ring[next % kRing] = next < kNF ? fb.read(cs, next, 0) : fb.read(cs, next - kNF, 1);
-      if (n < kMF) a1[n] = fa.read(cs + HB::kBytes, n, 1);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    for (int g = 0; g < kGroups; ++g) {
+      const int after = g - (kGroups - kBar);   // groups since the barrier
+      if (after == 0) {
+        if (kLater > 0 && s + kBuffers <= whole)
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kLater * kCopies) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s + kBuffers >= whole && s + kBuffers < stages) tail_stage(s + kBuffers);
+      }
+      if (after >= 0) {
+        if (s + kBuffers < whole) copy_some(s + kBuffers, after * kSpread, (after + 1) * kSpread);
+      } else if ((kBar + g) * kSpread < kCopies) {
+        if (s > 0 && s + kBuffers - 1 < whole) copy_some(s + kBuffers - 1, (kBar + g) * kSpread, (kBar + g + 1) * kSpread);
+      }
 #pragma unroll
-    for (int n = 0; n < kNF - kLead; ++n) {
-      group(n, a1);
-      ring[(n + kLead) % kRing] = fb.read(cs, n + kLead, 1);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + 2 < stages) copy_stage(s + 2);
+      for (int m = 0; m < kMF; ++m) acc[g % kNF][m] = Mfma<T>::run(ring[g % kRing], a[g / kNF][m], acc[g % kNF][m]);
+      if (after < 0) {
+        if (g + kLead < kGroups) ring[(g + kLead) % kRing] = read_b(cs, g + kLead);
+        if (g < kMF) a[1][g] = fa.read(cs + HB::kBytes, g, 1);
+      } else {
 #pragma unroll
-    for (int n = kNF - kLead; n < kNF; ++n) {
-      group(n, a1);
-      ring[(n + kLead) % kRing] = fb.read(ns, n + kLead - kNF, 0);
-      const int j = n - (kNF - kLead);
+        for (int i = 0; i < kLead; ++i)
+          if (i * kBar / kLead == after) ring[i % kRing] = read_b(ns, i);
 #pragma unroll
-      for (int m = 0; m < kMF; ++m)
-        if (m * kLead / kMF == j) a0[m] = fa.read(ns + HB::kBytes, m, 0);
+        for (int m = 0; m < kMF; ++m)
+          if (m * kBar / kMF == after) a[0][m] = fa.read(ns + HB::kBytes, m, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -328,7 +374,19 @@ __global__ __launch_bounds__(kThreads, 2) void mlp_kernel(const Product P) {
   constexpr int kRows = 16 * kMF;
   T* d = static_cast<T*>(P.d);
   const int64_t wrow = row0 + wa * kRows;
-  if constexpr (kE == kPlain) {
+  if constexpr (kE == kPartial) {
+    float* out = P.partial + (int64_t)range * P.a.rows * P.b.rows;
+#pragma unroll
+    for (int m = 0; m < kMF; ++m) {
+      const int64_t row = wrow + m * 16 + l16;
+      if (row >= P.a.rows) continue;
+#pragma unroll
+      for (int n = 0; n < kNF; ++n) {
+        const int col = (int)col0 + wb * 16 * kNF + n * 16 + h4 * 4;
+        if (col < P.b.rows) *reinterpret_cast<f32x4*>(out + row * P.b.rows + col) = acc[n][m];
+      }
+    }
+  } else if constexpr (kE == kPlain) {
     constexpr int kChunks = 2 * kNF;
     uint8_t* out = smem + wave * (kRows * kChunks * 16);
 #pragma unroll
@@ -415,26 +473,154 @@ __global__ __launch_bounds__(kThreads, 2) void mlp_kernel(const Product P) {
   }
 }
 
+// Adds the ranges' partial sums in order and finishes as kE says, four columns a lane: of one row of D,
+// or for the gate's product four of g and the same four of u.
+template <typename T, Epilogue kE>
+__global__ __launch_bounds__(256) void mlp_join_kernel(const Product P) {
+  const int cols = kE == kGate ? P.hidden : P.b.rows, quads = cols / 4;
+  const int64_t range = (int64_t)P.a.rows * P.b.rows, total = (int64_t)P.a.rows * quads;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+    const int64_t row = at / quads;
+    const int col = (int)(at - row * quads) * 4;
+    const float* src = P.partial + row * P.b.rows + col;
+    f32x4 x{}, y{};
+#pragma unroll 4
+    for (int r = 0; r < P.splits; ++r) {
+      x += *reinterpret_cast<const f32x4*>(src + r * range);
+      if constexpr (kE == kGate) y += *reinterpret_cast<const f32x4*>(src + r * range + P.hidden);
+    }
+    T* d = static_cast<T*>(P.d) + row * P.d_stride + col;
+    float a[4], b[4];
+    if constexpr (kE == kGate) {
+      if (P.gu) {
+        float* gu = P.gu + row * 2 * P.hidden + col;
+        *reinterpret_cast<f32x4*>(gu) = x;
+        *reinterpret_cast<f32x4*>(gu + P.hidden) = y;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = flk::gate(x[i], y[i]);
+    } else if constexpr (kE == kGateBackward) {
+      const float* gu = P.gu + row * 2 * P.hidden + col;
+      const f32x4 g = *reinterpret_cast<const f32x4*>(gu), u = *reinterpret_cast<const f32x4*>(gu + P.hidden);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) flk::gate_backward(x[i], g[i], u[i], a[i], b[i]);
+      *reinterpret_cast<uint2*>(d + P.hidden) = uint2{pack2<T>(b[0], b[1]), pack2<T>(b[2], b[3])};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = x[i];
+    }
+    *reinterpret_cast<uint2*>(d) = uint2{pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3])};
+  }
+}
+
 constexpr int kMaxDim = INT32_MAX - 256;
 constexpr int64_t kMaxStride = 1 << 22;   // 256 rows of one operand are addressed in 32 bits
+constexpr int64_t kMaxBlocks = 1 << 22;   // work-items of a launch are counted in 32 bits
+constexpr int kCUs = 256;
 
-template <typename T, bool kAAcross, bool kBAcross, Epilogue kE, int kNF, int kMF>
-int launch_tiles(Product& p, void* stream) {
-  constexpr int kTB = 16 * kNF * kWN, kTA = 16 * kMF * kWM;
-  p.tiles_a = (p.a.rows + kTA - 1) / kTA;
-  p.tiles_b = kE == kGate ? (p.hidden + kTB / 2 - 1) / (kTB / 2) : (p.b.rows + kTB - 1) / kTB;
-  const int64_t blocks = (int64_t)p.tiles_a * p.tiles_b;
-  if (blocks > (1 << 22)) return FLK_E_INVALID;   // work-items of a launch are counted in 32 bits
-  mlp_kernel<T, kAAcross, kBAcross, kE, kNF, kMF>
-      <<<dim3((unsigned)blocks), kThreads, 0, static_cast<hipStream_t>(stream)>>>(p);
+enum Tile { kLarge, kMedium, kSmall, kDeep, kFew, kTiles };
+
+struct Choice {
+  Tile tile;
+  int splits;       // ranges of the inner axis; 1: no partial sums
+  int stages;       // of each range
+};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The tile and the split of a product of `rows` x `cols` (all columns, both of the gate's halves): the least
+// estimated time over tiles and numbers of ranges.  A tile's blocks run in rounds of what the GPU
+// holds; a stage takes the measured time below with one or two blocks on a CU, a round some more to
+// fill its first stages and to write its tiles, and split products pay a second launch and write
+// and read their partial sums (6 TB/s, mostly from the caches).
+Choice choose(int64_t rows, int64_t cols, int64_t inner, bool a_across) {
+  struct Cost {
+    int rows, cols, per_cu;
+    double stage[2], round;   // microseconds: a stage with one / two blocks on the CU, a round
+    bool whole, split;
+  };
+  static constexpr Cost kCost[kTiles] = {
+      {Large::kTA, Large::kTB, Large::kPerCU, {1.42, 0}, 4.0, true, false},
+      {Medium::kTA, Medium::kTB, Medium::kPerCU, {1.14, 0}, 3.5, true, false},
+      {Small::kTA, Small::kTB, Small::kPerCU, {0.66, 0.92}, 3.0, true, true},
+      {Deep::kTA, Deep::kTB, Deep::kPerCU, {0.56, 0}, 3.0, true, true},
+      {Few::kTA, Few::kTB, Few::kPerCU, {0.55, 0.95}, 2.0, false, true},
+  };
+  static constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48};
+  const int64_t all = ceil_div(inner, kK);
+  Choice best{kLarge, 1, (int)all};
+  double least = 1e300;
+  for (int tile = 0; tile < kTiles; ++tile) {
+    const Cost& c = kCost[tile];
+    if (tile == kFew && a_across) continue;
+    const int64_t tiles = ceil_div(rows, c.rows) * ceil_div(cols, c.cols), slots = (int64_t)kCUs * c.per_cu;
+    for (const int want : kSplits) {
+      if (want == 1 ? !c.whole : !c.split || want > all) continue;
+      const int64_t stages = ceil_div(all, want), splits = ceil_div(all, stages);
+      const int64_t blocks = tiles * splits, rounds = blocks / slots, rest = blocks - rounds * slots;
+      double us = rounds * (c.stage[c.per_cu - 1] * stages + c.round);
+      if (rest) us += c.stage[rest > kCUs] * stages + c.round;
+      if (splits > 1) us += 3.0 + 8.0 * splits * rows * cols / 6e6;
+      if (us < least) {
+        least = us;
+        best = Choice{(Tile)tile, (int)splits, (int)stages};
+      }
+    }
+  }
+  return best;
+}
+
+int64_t partial_bytes(const Choice& c, int64_t rows, int64_t cols) { return c.splits > 1 ? 4 * c.splits * rows * cols : 0; }
+
+template <typename T, bool kAAcross, bool kBAcross, Epilogue kE, typename G>
+int launch_tiles(Product& p, hipStream_t s) {
+  p.tiles_a = (int)ceil_div(p.a.rows, G::kTA);
+  p.tiles_b = (int)(kE == kGate ? ceil_div(p.hidden, G::kTB / 2) : ceil_div(p.b.rows, G::kTB));
+  const int64_t blocks = (int64_t)p.tiles_a * p.tiles_b * p.splits;
+  if (blocks > kMaxBlocks) return FLK_E_INVALID;
+  mlp_kernel<T, kAAcross, kBAcross, kE, G><<<dim3((unsigned)blocks), G::kThreads, 0, s>>>(p);
+  return flk_launch_status();
+}
+
+template <typename T, bool kAAcross, bool kBAcross, Epilogue kE>
+int launch_typed(Product& p, const Choice& c, hipStream_t s) {
+  p.splits = c.splits;
+  p.stages = c.stages;
+  if (c.splits == 1) {
+    switch (c.tile) {
+      case kLarge: return launch_tiles<T, kAAcross, kBAcross, kE, Large>(p, s);
+      case kMedium: return launch_tiles<T, kAAcross, kBAcross, kE, Medium>(p, s);
+      case kSmall: return launch_tiles<T, kAAcross, kBAcross, kE, Small>(p, s);
+      default: return launch_tiles<T, kAAcross, kBAcross, kE, Deep>(p, s);
+    }
+  }
+  int st = FLK_OK;
+  if (c.tile == kSmall) {
+    st = launch_tiles<T, kAAcross, kBAcross, kPartial, Small>(p, s);
+  } else if (c.tile == kDeep) {
+    st = launch_tiles<T, kAAcross, kBAcross, kPartial, Deep>(p, s);
+  } else if constexpr (!kAAcross) {
+    st = launch_tiles<T, kAAcross, kBAcross, kPartial, Few>(p, s);
+  }
+  if (st) return st;
+  const int64_t quads = (int64_t)p.a.rows * ((kE == kGate ? p.hidden : p.b.rows) / 4);
+  mlp_join_kernel<T, kE><<<dim3((unsigned)std::min(ceil_div(quads, 256), kMaxBlocks)), 256, 0, s>>>(p);
   return flk_launch_status();
 }
 
 template <bool kAAcross, bool kBAcross, Epilogue kE>
-int launch(Product& p, int dtype, void* stream) {
+int launch(Product& p, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (p.a.stride > kMaxStride || p.b.stride > kMaxStride) return FLK_E_INVALID;
-  if (dtype == FLK_BF16) return launch_tiles<__bf16, kAAcross, kBAcross, kE, 8, 4>(p, stream);
-  return launch_tiles<_Float16, kAAcross, kBAcross, kE, 8, 4>(p, stream);
+  const Choice c = choose(p.a.rows, p.b.rows, p.inner, kAAcross);
+  const int64_t need = partial_bytes(c, p.a.rows, p.b.rows);
+  if (need) {
+    if (!workspace || workspace_bytes < need) return FLK_E_SCRATCH;
+    if (!flk_host_aligned(workspace, 16)) return FLK_E_ALIGN;
+    p.partial = static_cast<float*>(workspace);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == FLK_BF16) return launch_typed<__bf16, kAAcross, kBAcross, kE>(p, c, s);
+  return launch_typed<_Float16, kAAcross, kBAcross, kE>(p, c, s);
 }
 
 bool odd8(int64_t v) { return v % 8 != 0; }
@@ -444,7 +630,10 @@ bool odd8(int64_t v) { return v % 8 != 0; }
 extern "C" int flk_mlp_plan(int product, int rows, int cols, int inner, int64_t* workspace_bytes) {
   if (product < FLK_MLP_GATE || product > FLK_MLP_MATMUL_AT || rows < 0 || cols < 0 || inner < 0 || !workspace_bytes)
     return FLK_E_INVALID;
+  const int64_t columns = product == FLK_MLP_GATE ? 2LL * cols : cols;
+  if (rows > kMaxDim || columns > kMaxDim || inner > kMaxDim) return FLK_E_INVALID;
   *workspace_bytes = 0;
+  if (rows && cols && inner) *workspace_bytes = partial_bytes(choose(rows, columns, inner, product == FLK_MLP_MATMUL_AT), rows, columns);
   return FLK_OK;
 }
 
@@ -470,7 +659,7 @@ extern "C" int flk_mlp_gate(const void* x, int64_t x_row_stride, const void* w_i
   p.d_stride = h_row_stride;
   p.gu = gu;
   p.hidden = hidden;
-  return launch<false, true, kGate>(p, dtype, stream);
+  return launch<false, true, kGate>(p, dtype, workspace, workspace_bytes, stream);
 }
 
 extern "C" int flk_mlp_gate_backward(const void* dy, int64_t dy_row_stride, const void* w_out, int64_t w_out_row_stride,
@@ -495,7 +684,7 @@ extern "C" int flk_mlp_gate_backward(const void* dy, int64_t dy_row_stride, cons
   p.d_stride = dgu_row_stride;
   p.gu = const_cast<float*>(gu);
   p.hidden = hidden;
-  return launch<false, false, kGateBackward>(p, dtype, stream);
+  return launch<false, false, kGateBackward>(p, dtype, workspace, workspace_bytes, stream);
 }
 
 extern "C" int flk_mlp_matmul(const void* a, int64_t a_row_stride, int a_transposed, const void* b,
@@ -519,7 +708,7 @@ extern "C" int flk_mlp_matmul(const void* a, int64_t a_row_stride, int a_transpo
   p.inner = inner;
   p.d = d;
   p.d_stride = d_row_stride;
-  if (a_transposed) return launch<true, true, kPlain>(p, dtype, stream);
-  if (b_transposed) return launch<false, false, kPlain>(p, dtype, stream);
-  return launch<false, true, kPlain>(p, dtype, stream);
+  if (a_transposed) return launch<true, true, kPlain>(p, dtype, workspace, workspace_bytes, stream);
+  if (b_transposed) return launch<false, false, kPlain>(p, dtype, workspace, workspace_bytes, stream);
+  return launch<false, true, kPlain>(p, dtype, workspace, workspace_bytes, stream);
 }
