@@ -541,7 +541,7 @@ Choice choose(int64_t rows, int64_t cols, int64_t inner, bool a_across) {
   };
   static constexpr Cost kCost[kTiles] = {
       {Large::kTA, Large::kTB, Large::kPerCU, {1.42, 0}, 4.0, true, false},
-      {Medium::kTA, Medium::kTB, Medium::kPerCU, {1.14, 0}, 3.5, true, false},
+      {Medium::kTA, Medium::kTB, Medium::kPerCU, {1.26, 0}, 3.5, true, false},
       {Small::kTA, Small::kTB, Small::kPerCU, {0.66, 0.92}, 3.0, true, true},
       {Deep::kTA, Deep::kTB, Deep::kPerCU, {0.56, 0}, 3.0, true, true},
       {Few::kTA, Few::kTB, Few::kPerCU, {0.55, 0.95}, 2.0, false, true},

@@ -8,15 +8,22 @@
 //   dx_j = q (t_j - mean(t) - n_j mean(t n))
 //   dfactor_j = sum over the rows that share it of dy_j n_j,  doffset_j = sum of dy_j
 //
-// All arithmetic is float32 and every output is rounded once.  The variance is summed from the
-// centred row (two passes over registers): sums of squares of an uncentred residual stream,
-// whose tokens sit off zero, would cancel.
+// All arithmetic is float32 and every output is rounded once.  Sums of squares of an uncentred residual
+// stream, whose tokens sit off zero, would cancel, so each wave centres its part of the row on its own
+// mean, and the waves' (mean, centred squares) are joined by the parallel form of the variance:
+//   m = sum_w k_w m_w / K,   K v = sum_w s_w + k_w (m_w - m)^2
+// and likewise sum t (x - m) = sum_w [sum t (x - m_w) + (m_w - m) sum t]: one exchange through LDS and
+// one barrier a row, forwards and backwards.
 //
-// HBM bounds both directions: a row is read once and kept in registers, kW lanes of it at a
-// time, kV chunks of 8 elements a lane.  The backward pass recomputes m and q from the row it has
-// to read anyway, so the forward pass keeps nothing.  Its column sums stay in the lanes that own
-// the columns while a block walks its rows; blocks write them as partial rows, which a second
-// kernel adds in a fixed order: the gradients do not depend on timing.
+// HBM bounds both directions: a row is read once and held in registers, one 8-element chunk a lane
+// (two past 8192 columns), so a lane owns few columns and a CU has many rows in flight.  The
+// backward pass recomputes m and q from the row it has to read anyway, so the forward pass
+// keeps nothing.  Its column sums stay in the lanes that own the columns while a block walks its
+// rows; blocks write them as partial rows, which a second kernel adds in a fixed order: the
+// gradients do not depend on timing.
+//
+// A row's last chunk starts 8 columns before its end, so that every load is a whole one; the columns that
+// it shares with the lane before are left out of its sums and stores.
 
 #include <algorithm>
 
@@ -24,7 +31,9 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+using flk::f32x4;
+
+constexpr int kMaxWaves = 16;   // of a row: kV chunks of 8 x 64 columns each
 
 struct Rows {            // row t of batch entry b at p + b * batch_stride + t * row_stride
   const void* p;
@@ -39,233 +48,279 @@ struct NormArgs {
   float add;             // a = factor + add
   float eps, inv_width;
   int length, width;
-  int64_t rows;          // batch * length
-  // backward: blocks of `per_block` rows of one group; partial sums (block, 2, width)
-  float* partial;
+  // Blocks walk `per_block` rows of one group: of one batch entry's, or, where all share the parameters, of all.
   int64_t group_rows;
   int per_block, blocks_per_group;
+  float* partial;        // backward: column sums (block, 2, width), or NULL
 };
 
-template <typename T>
-__device__ __forceinline__ const T* row_at(const Rows& r, int64_t b, int64_t t) {
-  return static_cast<const T*>(r.p) + b * r.batch_stride + t * r.row_stride;
-}
-
-// Sum over 64 lanes; every lane ends with the same value.
+// Sum over 64 lanes without leaving the registers; every lane ends with the same value.
 __device__ __forceinline__ float wave_sum(float v) {
   v = flk::row16_sum(v);
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Sums of a and b over the kW lanes of a row.  With more than one wave a row, the waves exchange
-// their sums through `scratch`; the halves alternate (turn), so one barrier a call is enough.
-template <int kW>
-__device__ __forceinline__ void row_sums(float& a, float& b, float (*scratch)[2][kW / 64], int& turn) {
-  a = wave_sum(a);
-  b = wave_sum(b);
-  if constexpr (kW > 64) {
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
-      scratch[turn][0][wave] = a;
-      scratch[turn][1][wave] = b;
-    }
-    __syncthreads();
-    a = b = 0.0f;
+// A lane's chunks of a row of `width` >= 8 columns (kNarrow: of fewer, one lane's), kV of them a block's lanes apart.
+template <int kV, bool kNarrow>
+struct Chunks {
+  int at[kV];      // first column; past the end: the row's last 8 columns
+  int skip[kV];    // leading columns that another lane has too (8: all)
+  bool live[kV];
+  __device__ __forceinline__ Chunks(int width, int lane, int lanes) {
 #pragma unroll
-    for (int w = 0; w < kW / 64; ++w) {
-      a += scratch[turn][0][w];
-      b += scratch[turn][1][w];
+    for (int c = 0; c < kV; ++c) {
+      const int first = (lane + lanes * c) * 8;
+      live[c] = first < width;
+      at[c] = kNarrow ? first : min(first, width - 8);
+      skip[c] = kNarrow ? 0 : min(first - at[c], 8);
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ flk::Raw8<T> load(const T* row, int c, int width) const {
+    if constexpr (kNarrow) return flk::load8(row + at[c], width - at[c]);
+    return flk::load8(row + at[c], 8);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, int c, int width, const float (&x)[8]) const {
+    if (!live[c]) return;
+    if constexpr (kNarrow) {
+      flk::store8(row + at[c], width - at[c], x);
+    } else if (skip[c] == 0) {
+      flk::store8(row + at[c], 8, x);
+    } else {
+#pragma unroll
+      for (int i = 1; i < 8; ++i)
+        if (i >= skip[c]) row[at[c] + i] = (T)x[i];
+    }
+  }
+  // Whether element i of chunk c counts in the row's sums.
+  __device__ __forceinline__ bool counts(int c, int i, int width) const {
+    return kNarrow ? at[c] + i < width : i >= skip[c];
+  }
+};
+
+// What a row's waves exchange, in turns of two: a wave's turn ends for all at the next row's barrier.
+struct Exchange {
+  f32x4 values[2][kMaxWaves];   // of the waves there are; zeros in the other places
+};
+
+// The row's mean and 1 / sqrt(v + eps), and with kGrads the sums of t and of t (x - mean).  own: this wave's
+// mean, centred squares, sum of t, sum of t (x - own mean).
+struct Stats {
+  float mean, rstd, t, tx;
+};
+
+// columns: of wave lane % 16.
+template <bool kOne, bool kGrads>
+__device__ __forceinline__ Stats join(const f32x4& own, float columns, const NormArgs& A, Exchange& ex, int& turn) {
+  float mean = own[0], square = own[1], t = own[2], tx = own[3];
+  if constexpr (!kOne) {   // each 16 lanes take one wave's values a lane
+    if ((threadIdx.x & 63) == 0) ex.values[turn][threadIdx.x >> 6] = own;
+    __syncthreads();
+    const f32x4 v = ex.values[turn][threadIdx.x & 15];
+    mean = flk::row16_sum(v[0] * columns) * A.inv_width;
+    const float d = v[0] - mean;
+    square = flk::row16_sum(v[1] + columns * d * d);
+    if constexpr (kGrads) {
+      t = flk::row16_sum(v[2]);
+      tx = flk::row16_sum(v[3] + d * v[2]);
     }
     turn ^= 1;
   }
+  return Stats{mean, __builtin_amdgcn_rsqf(square * A.inv_width + A.eps), t, tx};
 }
 
-// Centres the row in xs (elements past the row's end become 0) and returns 1 / sqrt(v + eps).
-template <int kW, int kV>
-__device__ __forceinline__ float centre(float (&xs)[kV][8], const int (&left)[kV], const NormArgs& A,
-                                        float (*scratch)[2][kW / 64], int& turn) {
-  float sum = 0.0f, none = 0.0f;
-#pragma unroll
-  for (int c = 0; c < kV; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum += xs[c][i];
-  row_sums<kW>(sum, none, scratch, turn);
-  const float mean = sum * A.inv_width;
-  float square = 0.0f;
-#pragma unroll
-  for (int c = 0; c < kV; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      xs[c][i] = i < left[c] ? xs[c][i] - mean : 0.0f;
-      square += xs[c][i] * xs[c][i];
-    }
-  row_sums<kW>(square, none, scratch, turn);
-  return 1.0f / sqrtf(square * A.inv_width + A.eps);
-}
-
-template <typename T, typename P, int kW, int kV>
-__global__ __launch_bounds__(kW > kThreads ? kW : kThreads) void norm_kernel(const NormArgs A) {
-  constexpr int kRows = kW > kThreads ? 1 : kThreads / kW;   // rows per block
-  __shared__ float scratch[2][2][kW / 64];
-  int turn = 0;
-  const int lane = threadIdx.x % kW;
-  // Rows past kMaxBlocks blocks' are walked in turns, whole waves (one row a block: whole blocks).
-  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kW; row < A.rows; row += (int64_t)gridDim.x * kRows) {
-    const int64_t b = row / A.length, t = row - b * A.length;
-    const T* x = row_at<T>(A.x, b, t);
-    T* y = const_cast<T*>(row_at<T>(A.y, b, t));
-    int left[kV];
-    float xs[kV][8];
-  #pragma unroll
-    for (int c = 0; c < kV; ++c) {
-      const int at = (lane + kW * c) * 8;
-      left[c] = A.width - at;
-      const flk::Raw8<T> r = flk::load8(x + at, left[c]);
-  #pragma unroll
-      for (int i = 0; i < 8; ++i) xs[c][i] = (float)r.v[i];
-    }
-    const float q = centre<kW, kV>(xs, left, A, scratch, turn);
-    const P* factor = static_cast<const P*>(A.factor);
-    const P* offset = static_cast<const P*>(A.offset);
-    if (factor) factor += b * A.param_stride;
-    if (offset) offset += b * A.param_stride;
-  #pragma unroll
-    for (int c = 0; c < kV; ++c) {
-      const int at = (lane + kW * c) * 8;
-      if (left[c] <= 0) continue;
-      float out[8];
-  #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = xs[c][i] * q;
-      if (factor) {
-        const flk::Raw8<P> f = flk::load8(factor + at, left[c]);
-  #pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] *= (float)f.v[i] + A.add;
-      }
-      if (offset) {
-        const flk::Raw8<P> f = flk::load8(offset + at, left[c]);
-  #pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] += (float)f.v[i];
-      }
-      flk::store8(y + at, left[c], out);
-    }
+// A block's rows: slot's of every kSlots, first .. end - 1 of a group.
+struct Walk {
+  int64_t group, first, end;
+  __device__ __forceinline__ Walk(const NormArgs& A, int slot) {
+    group = blockIdx.x / A.blocks_per_group;
+    const int64_t begin = (int64_t)(blockIdx.x - group * A.blocks_per_group) * A.per_block;
+    first = begin + slot;
+    end = min(begin + A.per_block, A.group_rows);
   }
-}
+  template <typename T>
+  __device__ __forceinline__ T* row(const NormArgs& A, const Rows& r, int64_t at) const {
+    int64_t b = group, t = at;
+    if (A.group_rows != A.length) {   // one group of all entries' rows
+      b = (uint32_t)at / (uint32_t)A.length;
+      t = at - b * A.length;
+    }
+    return static_cast<T*>(const_cast<void*>(r.p)) + b * r.batch_stride + t * r.row_stride;
+  }
+};
 
-template <typename T, typename P, int kW, int kV>
-__global__ __launch_bounds__(kW > kThreads ? kW : kThreads) void norm_backward_kernel(const NormArgs A) {
-  constexpr int kRows = kW > kThreads ? 1 : kThreads / kW;
-  __shared__ float scratch[2][2][kW / 64];
-  __shared__ float sums[kRows > 1 ? 2 * kV * 8 * kW : 1];
+// kOne: a wave takes a row alone, kSlots rows a block; otherwise all of the block's waves take one.
+template <typename T, typename P, int kV, bool kOne, bool kNarrow, bool kBackward>
+__global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const NormArgs A) {
+  constexpr int kSlots = kOne ? 4 : 1;
+  __shared__ Exchange ex;
+  __shared__ float sums[kOne && kBackward ? 2 * kV * 8 * 64 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = kOne ? 1 : blockDim.x >> 6, slot = kOne ? wave : 0;
+  const int lanes = 64 * waves, width = A.width;
+  const Chunks<kV, kNarrow> chunks(width, kOne ? lane : (int)threadIdx.x, lanes);
+  auto columns_of = [&](int w) {
+    float n = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kV; ++c) n += (float)max(0, min(width - (lanes * c + w * 64) * 8, 512));
+    return n;
+  };
+  const float count = columns_of(kOne ? 0 : wave), inv_count = 1.0f / count;
+  const float columns = (lane & 15) < waves ? columns_of(lane & 15) : 0.0f;
+  if (!kOne && wave == 0 && lane >= 32 && (lane & 15) >= waves) ex.values[lane >> 4 & 1][lane & 15] = f32x4{};
   int turn = 0;
-  const int lane = threadIdx.x % kW, slot = threadIdx.x / kW;
-  const int64_t group = blockIdx.x / A.blocks_per_group;
-  const int64_t first = (int64_t)(blockIdx.x - group * A.blocks_per_group) * A.per_block;   // of the group's rows
-  const int64_t end = min(first + A.per_block, A.group_rows);
+  const Walk walk(A, slot);
+
   const P* factor = static_cast<const P*>(A.factor);
-  if (factor) factor += group * A.param_stride;
-  int left[kV];
-  flk::Raw8<P> f[kV];
-  float da[kV][8], dc[kV][8];
+  const P* offset = static_cast<const P*>(A.offset);
+  float a[kV][8], o[kBackward ? 1 : kV][8];
 #pragma unroll
   for (int c = 0; c < kV; ++c) {
-    const int at = (lane + kW * c) * 8;
-    left[c] = A.width - at;
-    if (factor) f[c] = flk::load8(factor + at, left[c]);
+    flk::Raw8<P> raw{};
+    if (factor) raw = chunks.load(factor + walk.group * A.param_stride, c, width);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (!factor) f[c].v[i] = (P)0.0f;
-      da[c][i] = dc[c][i] = 0.0f;
+    for (int i = 0; i < 8; ++i) a[c][i] = factor ? (float)raw.v[i] + A.add : 1.0f;
+    if constexpr (!kBackward) {
+      if (offset) raw = chunks.load(offset + walk.group * A.param_stride, c, width);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[c][i] = offset ? (float)raw.v[i] : 0.0f;
     }
   }
-  const float add = factor ? A.add : 1.0f;
-  // With several rows a block each slot walks its own rows without barriers; with one, all waves
-  // of the block walk the same rows.
-  for (int64_t r = first + slot; r < end; r += kRows) {
-    const int64_t row = group * A.group_rows + r;
-    const int64_t b = row / A.length, t = row - b * A.length;
-    const T* x = row_at<T>(A.x, b, t);
-    const T* dy = row_at<T>(A.dy, b, t);
-    T* dx = const_cast<T*>(row_at<T>(A.y, b, t));
-    float xs[kV][8];
-    flk::Raw8<T> g[kV];
+  float da[kBackward ? kV : 1][8] = {}, dc[kBackward ? kV : 1][8] = {};
+  // Whether all of this wave's columns count in the row's sums; where not, the others enter as zeros.
+  const bool whole = count == (float)(kV * 512);
+
+  // The next kDepth rows are on their way while a row is worked on.
+  constexpr int kDepth = sizeof(T) == 2 && kV == 1 ? 2 : 1;
+  flk::Raw8<T> x[kDepth][kV], g[kBackward ? kDepth : 1][kV];
+  auto fetch = [&](int d, int64_t r) {
+    const T* px = walk.template row<T>(A, A.x, r);
+    const T* pg = kBackward ? walk.template row<T>(A, A.dy, r) : nullptr;
 #pragma unroll
     for (int c = 0; c < kV; ++c) {
-      const int at = (lane + kW * c) * 8;
-      const flk::Raw8<T> raw = flk::load8(x + at, left[c]);
-      g[c] = flk::load8(dy + at, left[c]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) xs[c][i] = (float)raw.v[i];
+      x[d][c] = chunks.load(px, c, width);
+      if constexpr (kBackward) g[d][c] = chunks.load(pg, c, width);
     }
-    const float q = centre<kW, kV>(xs, left, A, scratch, turn);
-    float st = 0.0f, stn = 0.0f;
+  };
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d)
+    if (walk.first + d * kSlots < walk.end) fetch(d, walk.first + d * kSlots);
+  auto work = [&](int d, int64_t r) {
+    float xs[kV][8], gs[kBackward ? kV : 1][8];
 #pragma unroll
     for (int c = 0; c < kV; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float d = (float)g[c].v[i], n = xs[c][i] * q;
-        const float tt = d * ((float)f[c].v[i] + add);
-        xs[c][i] = n;
-        da[c][i] += d * n;
-        dc[c][i] += d;
-        st += tt;
-        stn += tt * n;
+        xs[c][i] = (float)x[d][c].v[i];
+        if constexpr (kBackward) gs[c][i] = (float)g[d][c].v[i];
       }
-    row_sums<kW>(st, stn, scratch, turn);
-    const float mt = st * A.inv_width, mtn = stn * A.inv_width;
+    if (r + kDepth * kSlots < walk.end) fetch(d, r + kDepth * kSlots);
+    auto leave_out = [&](float (&v)[8], int c) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = chunks.counts(c, i, width) ? v[i] : 0.0f;
+    };
+    f32x4 own{};
 #pragma unroll
     for (int c = 0; c < kV; ++c) {
-      if (left[c] <= 0) continue;
+      if (!whole) {
+        leave_out(xs[c], c);
+        if constexpr (kBackward) leave_out(gs[c], c);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) own[0] += xs[c][i];
+    }
+    own[0] = wave_sum(own[0]) * inv_count;
+#pragma unroll
+    for (int c = 0; c < kV; ++c) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) xs[c][i] -= own[0];
+      if (!whole) leave_out(xs[c], c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        own[1] += xs[c][i] * xs[c][i];
+        if constexpr (kBackward) {
+          dc[c][i] += gs[c][i];
+          const float t = gs[c][i] * a[c][i];
+          own[2] += t;
+          own[3] += t * xs[c][i];
+        }
+      }
+    }
+    own[1] = wave_sum(own[1]);
+    if constexpr (kBackward) {
+      own[2] = wave_sum(own[2]);
+      own[3] = wave_sum(own[3]);
+    }
+    const Stats st = join<kOne, kBackward>(own, columns, A, ex, turn);
+    const float shift = (own[0] - st.mean) * st.rstd;
+    const float mt = st.t * A.inv_width * st.rstd, mtn = st.rstd * st.tx * A.inv_width * st.rstd;
+    T* y = walk.template row<T>(A, A.y, r);
+#pragma unroll
+    for (int c = 0; c < kV; ++c) {
       float out[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float tt = (float)g[c].v[i] * ((float)f[c].v[i] + add);
-        out[i] = q * (tt - mt - xs[c][i] * mtn);
+        const float n = xs[c][i] * st.rstd + shift;
+        if constexpr (kBackward) {
+          out[i] = gs[c][i] * a[c][i] * st.rstd - mt - n * mtn;
+          da[c][i] += gs[c][i] * n;
+        } else {
+          out[i] = n * a[c][i] + o[c][i];
+        }
       }
-      flk::store8(dx + (lane + kW * c) * 8, left[c], out);
+      chunks.store(y, c, width, out);
     }
+  };
+  for (int64_t r = walk.first; r < walk.end; r += kDepth * kSlots) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d)
+      if (r + d * kSlots < walk.end) work(d, r + d * kSlots);
   }
-  if (!A.partial) return;
-  if constexpr (kRows > 1) {   // slot 0 adds the other slots' sums, one slot at a time
-    for (int s = 1; s < kRows; ++s) {
-      __syncthreads();
-      if (slot == s) {
+  if constexpr (kBackward) {
+    if (!A.partial) return;
+    if constexpr (kOne) {   // slot 0 adds the other slots' sums, one slot at a time
+      for (int s = 1; s < kSlots; ++s) {
+        __syncthreads();
 #pragma unroll
         for (int c = 0; c < kV; ++c)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            sums[(c * 8 + i) * kW + lane] = da[c][i];
-            sums[(kV * 8 + c * 8 + i) * kW + lane] = dc[c][i];
-          }
-      }
-      __syncthreads();
-      if (slot == 0) {
+          for (int i = 0; i < 8; ++i)
+            if (slot == s) {
+              sums[(c * 8 + i) * 64 + lane] = da[c][i];
+              sums[(kV * 8 + c * 8 + i) * 64 + lane] = dc[c][i];
+            }
+        __syncthreads();
 #pragma unroll
         for (int c = 0; c < kV; ++c)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            da[c][i] += sums[(c * 8 + i) * kW + lane];
-            dc[c][i] += sums[(kV * 8 + c * 8 + i) * kW + lane];
-          }
+          for (int i = 0; i < 8; ++i)
+            if (slot == 0) {
+              da[c][i] += sums[(c * 8 + i) * 64 + lane];
+              dc[c][i] += sums[(kV * 8 + c * 8 + i) * 64 + lane];
+            }
       }
+      if (slot) return;
     }
-    if (slot) return;
-  }
-  float* out = A.partial + (int64_t)blockIdx.x * 2 * A.width;
+    float* out = A.partial + (int64_t)blockIdx.x * 2 * width;
 #pragma unroll
-  for (int c = 0; c < kV; ++c) {
-    const int at = (lane + kW * c) * 8;
-    if (left[c] <= 0) continue;
-    flk::store8(out + at, left[c], da[c]);
-    flk::store8(out + A.width + at, left[c], dc[c]);
+    for (int c = 0; c < kV; ++c) {
+      chunks.store(out, c, width, da[c]);
+      chunks.store(out + width, c, width, dc[c]);
+    }
   }
 }
 
-// Adds a group's partial rows in order: 64 columns a block, four waves take every fourth row each.
+// Adds a group's partial rows in a fixed order: 64 columns a block, its waves every kJoinWaves-th row each, then the
+// waves' sums in order.
+constexpr int kJoinWaves = 16;
 template <typename P>
-__global__ __launch_bounds__(kThreads) void norm_params_kernel(const float* __restrict__ partial, int blocks, int width,
-                                                               int cuts, P* dfactor, P* doffset) {
-  __shared__ float part[4][64];
+__global__ __launch_bounds__(64 * kJoinWaves) void norm_params_kernel(const float* __restrict__ partial, int blocks,
+                                                                      int width, int cuts, P* dfactor, P* doffset) {
+  __shared__ float part[kJoinWaves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t group = blockIdx.x / cuts;
   const int col = (int)(blockIdx.x - group * cuts) * 64 + lane;
@@ -274,55 +329,70 @@ __global__ __launch_bounds__(kThreads) void norm_params_kernel(const float* __re
   if (!out) return;
   const float* src = partial + group * blocks * 2 * width + (int64_t)which * width + col;
   float sum = 0.0f;
-  if (col < width)
-    for (int i = wave; i < blocks; i += 4) sum += src[(int64_t)i * 2 * width];
+  if (col < width) {
+#pragma unroll 4
+    for (int i = wave; i < blocks; i += kJoinWaves) sum += src[(int64_t)i * 2 * width];
+  }
   part[wave][lane] = sum;
   __syncthreads();
-  if (wave == 0 && col < width) out[group * width + col] = (P)((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+  if (wave || col >= width) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWaves; ++w) sum += part[w][lane];
+  out[group * width + col] = (P)sum;
 }
 
-constexpr int kMaxWidth = 512 * 8 * 8;
+constexpr int kMaxWidth = 2 * kMaxWaves * 512;
 constexpr int kMaxRows = INT32_MAX;
 constexpr int64_t kMaxBlocks = 1 << 22;   // a launch's work-items are counted in 32 bits
 
-// Rows each backward block walks: about 512 blocks, so that two share a CU, but no more than 64
-// rows a block are needed to make the partial rows cheap.
-int backward_rows(int64_t group_rows, int64_t groups) {
-  const int64_t blocks = 512 / groups > 0 ? 512 / groups : 1;
-  const int64_t per = (group_rows + blocks - 1) / blocks;
-  return (int)(per < 4 ? 4 : per);
+// Rows a block walks.  Of the numbers of blocks a CU that keep up to `waves` waves on it, the one whose CUs
+// all get nearly the same number of rows, and then the largest; `least` rows a block at any rate.
+int rows_per_block(int64_t group_rows, int64_t groups, int width, int waves, int least) {
+  const int slots = width <= 512 ? 4 : 1, of_block = width <= 512 ? 4 : std::min((width + 511) / 512, kMaxWaves);
+  int64_t best = 0, load = INT64_MAX;
+  for (int per_cu = std::max(1, waves / of_block); per_cu >= std::max(1, waves / 2 / of_block); --per_cu) {
+    const int64_t blocks = std::max<int64_t>(1, 256 * per_cu / groups);
+    const int64_t per = (std::max<int64_t>(least, (group_rows + blocks - 1) / blocks) + slots - 1) / slots * slots;
+    const int64_t all = groups * ((group_rows + per - 1) / per), cu = (all + 255) / 256 * per;
+    if (cu < load) {
+      load = cu;
+      best = per;
+    }
+  }
+  return (int)best;
+}
+int forward_rows(int64_t group_rows, int64_t groups, int width) {
+  return rows_per_block(group_rows, groups, width, 24, 1);
+}
+int backward_rows(int64_t group_rows, int64_t groups, int width) {
+  return rows_per_block(group_rows, groups, width, 12, (int)std::min<int64_t>(4, 1 + group_rows * groups / 128));
 }
 
-template <typename T, typename P, int kW, int kV>
-int launch(const NormArgs& a, int64_t groups, bool backward, hipStream_t s) {
-  constexpr int threads = kW > kThreads ? kW : kThreads, rows = threads / kW;
-  if (backward)
-    norm_backward_kernel<T, P, kW, kV><<<dim3((unsigned)(groups * a.blocks_per_group)), threads, 0, s>>>(a);
+template <typename T, typename P, bool kBackward>
+int dispatch(const NormArgs& a, int64_t groups, hipStream_t s) {
+  const dim3 grid((unsigned)(groups * a.blocks_per_group));
+  const int chunks = (a.width + 7) / 8;
+  if (a.width < 8)
+    norm_kernel<T, P, 1, true, true, kBackward><<<grid, 256, 0, s>>>(a);
+  else if (a.width <= 512)
+    norm_kernel<T, P, 1, true, false, kBackward><<<grid, 256, 0, s>>>(a);
+  else if (a.width <= 512 * kMaxWaves)
+    norm_kernel<T, P, 1, false, false, kBackward><<<grid, (chunks + 63) / 64 * 64, 0, s>>>(a);
   else
-    norm_kernel<T, P, kW, kV><<<dim3((unsigned)std::min((a.rows + rows - 1) / rows, kMaxBlocks)), threads, 0, s>>>(a);
+    norm_kernel<T, P, 2, false, false, kBackward><<<grid, 64 * kMaxWaves, 0, s>>>(a);
   return flk_launch_status();
 }
 
-template <typename T, typename P>
-int dispatch(const NormArgs& a, int64_t groups, bool backward, hipStream_t s) {
-  if (a.width <= 512) return launch<T, P, 64, 1>(a, groups, backward, s);
-  if (a.width <= 1024) return launch<T, P, 64, 2>(a, groups, backward, s);
-  if (a.width <= 2048) return launch<T, P, 64, 4>(a, groups, backward, s);
-  if (a.width <= 3 * 1024) return launch<T, P, 64, 6>(a, groups, backward, s);
-  if (a.width <= 4096) return launch<T, P, 256, 2>(a, groups, backward, s);
-  if (a.width <= 8192) return launch<T, P, 256, 4>(a, groups, backward, s);
-  return launch<T, P, 512, 8>(a, groups, backward, s);
-}
-
-int dispatch_types(int dtype, int params, const NormArgs& a, int64_t groups, bool backward, hipStream_t s) {
-  if (dtype == FLK_F32) return params == FLK_F32 ? dispatch<float, float>(a, groups, backward, s) : FLK_E_UNSUPPORTED;
+template <bool kBackward>
+int dispatch_types(int dtype, int params, const NormArgs& a, int64_t groups, hipStream_t s) {
+  if (dtype == FLK_F32) return params == FLK_F32 ? dispatch<float, float, kBackward>(a, groups, s) : FLK_E_UNSUPPORTED;
   if (dtype == FLK_BF16) {
-    if (params == FLK_BF16) return dispatch<__bf16, __bf16>(a, groups, backward, s);
-    if (params == FLK_F32) return dispatch<__bf16, float>(a, groups, backward, s);
+    if (params == FLK_BF16) return dispatch<__bf16, __bf16, kBackward>(a, groups, s);
+    if (params == FLK_F32) return dispatch<__bf16, float, kBackward>(a, groups, s);
   }
   if (dtype == FLK_F16) {
-    if (params == FLK_F16) return dispatch<_Float16, _Float16>(a, groups, backward, s);
-    if (params == FLK_F32) return dispatch<_Float16, float>(a, groups, backward, s);
+    if (params == FLK_F16) return dispatch<_Float16, _Float16, kBackward>(a, groups, s);
+    if (params == FLK_F32) return dispatch<_Float16, float, kBackward>(a, groups, s);
   }
   return FLK_E_UNSUPPORTED;
 }
@@ -356,7 +426,7 @@ NormArgs common_args(const void* x, int64_t xb, int64_t xr, const void* factor, 
   a.inv_width = 1.0f / (float)width;
   a.length = length;
   a.width = width;
-  a.rows = (int64_t)batch * length;
+  a.group_rows = param_stride ? length : (int64_t)batch * length;
   return a;
 }
 
@@ -372,7 +442,11 @@ extern "C" int flk_layer_norm(const void* x, int64_t x_batch_stride, int64_t x_r
   NormArgs a = common_args(x, x_batch_stride, x_row_stride, factor, offset, param_batch_stride, add_one, eps, batch,
                            length, width);
   a.y = Rows{y, y_batch_stride, y_row_stride};
-  return dispatch_types(dtype, params_dtype, a, 0, false, static_cast<hipStream_t>(stream));
+  const int64_t groups = param_batch_stride ? batch : 1;
+  a.per_block = forward_rows(a.group_rows, groups, width);
+  a.blocks_per_group = (int)((a.group_rows + a.per_block - 1) / a.per_block);
+  if (groups * a.blocks_per_group > kMaxBlocks) return FLK_E_INVALID;
+  return dispatch_types<false>(dtype, params_dtype, a, groups, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int flk_layer_norm_backward_plan(int batch, int length, int width, int shared_params,
@@ -382,7 +456,7 @@ extern "C" int flk_layer_norm_backward_plan(int batch, int length, int width, in
   *workspace_bytes = 0;
   if (batch == 0 || length == 0) return FLK_OK;
   const int64_t groups = shared_params ? 1 : batch, group_rows = shared_params ? (int64_t)batch * length : length;
-  const int per = backward_rows(group_rows, groups);
+  const int per = backward_rows(group_rows, groups, width);
   *workspace_bytes = groups * ((group_rows + per - 1) / per) * 2 * width * 4;
   return FLK_OK;
 }
@@ -403,10 +477,8 @@ extern "C" int flk_layer_norm_backward(const void* dy, int64_t dy_batch_stride, 
                            length, width);
   a.dy = Rows{dy, dy_batch_stride, dy_row_stride};
   a.y = Rows{dx, dx_batch_stride, dx_row_stride};
-  const bool shared = param_batch_stride == 0;
-  const int64_t groups = shared ? 1 : batch;
-  a.group_rows = shared ? a.rows : length;
-  a.per_block = backward_rows(a.group_rows, groups);
+  const int64_t groups = param_batch_stride ? batch : 1;
+  a.per_block = backward_rows(a.group_rows, groups, width);
   a.blocks_per_group = (int)((a.group_rows + a.per_block - 1) / a.per_block);
   const int cuts = (width + 63) / 64;
   if (groups * a.blocks_per_group > kMaxBlocks || groups * cuts > kMaxBlocks) return FLK_E_INVALID;
@@ -417,17 +489,17 @@ extern "C" int flk_layer_norm_backward(const void* dy, int64_t dy_batch_stride, 
     a.partial = static_cast<float*>(workspace);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (const int st = dispatch_types(dtype, params_dtype, a, groups, true, s)) return st;
+  if (const int st = dispatch_types<true>(dtype, params_dtype, a, groups, s)) return st;
   if (!a.partial) return FLK_OK;
   const dim3 grid((unsigned)(groups * cuts), 2);
   if (params_dtype == FLK_F32)
-    norm_params_kernel<float><<<grid, kThreads, 0, s>>>(a.partial, a.blocks_per_group, width, cuts,
+    norm_params_kernel<float><<<grid, 64 * kJoinWaves, 0, s>>>(a.partial, a.blocks_per_group, width, cuts,
                                                         static_cast<float*>(dfactor), static_cast<float*>(doffset));
   else if (params_dtype == FLK_BF16)
-    norm_params_kernel<__bf16><<<grid, kThreads, 0, s>>>(a.partial, a.blocks_per_group, width, cuts,
+    norm_params_kernel<__bf16><<<grid, 64 * kJoinWaves, 0, s>>>(a.partial, a.blocks_per_group, width, cuts,
                                                          static_cast<__bf16*>(dfactor), static_cast<__bf16*>(doffset));
   else
-    norm_params_kernel<_Float16><<<grid, kThreads, 0, s>>>(a.partial, a.blocks_per_group, width, cuts,
+    norm_params_kernel<_Float16><<<grid, 64 * kJoinWaves, 0, s>>>(a.partial, a.blocks_per_group, width, cuts,
                                                            static_cast<_Float16*>(dfactor),
                                                            static_cast<_Float16*>(doffset));
   return flk_launch_status();

@@ -276,9 +276,197 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// FLK_BF16, FLK_F16, FLK_F32, or -1.
+int code_of(at::ScalarType t) {
+  return t == at::kBFloat16 ? FLK_BF16 : t == at::kHalf ? FLK_F16 : t == at::kFloat ? FLK_F32 : -1;
+}
+
+// A (..., N) tensor as (batch, length, N) rows read in place.
+struct Blocks {
+  const at::Tensor* t;
+  int batch, length, width;
+  int64_t batch_stride, row_stride;
+};
+
+bool blocks_from(PyObject* o, int device, Blocks& b) {
+  b.t = gpu_tensor(o, device);
+  if (!b.t || b.t->dim() < 1 || b.t->numel() == 0 || code_of(b.t->scalar_type()) < 0 || b.t->stride(-1) != 1)
+    return false;
+  const int64_t width = b.t->size(-1);
+  int64_t batch = 1, length = b.t->numel() / width;
+  b.batch_stride = 0;
+  b.row_stride = width;
+  if (b.t->dim() == 3) {
+    batch = b.t->size(0);
+    length = b.t->size(1);
+    b.batch_stride = b.t->stride(0);
+    b.row_stride = b.t->stride(1);
+  } else if (!b.t->is_contiguous()) {
+    return false;
+  }
+  if (width > INT32_MAX || batch > INT32_MAX || length > INT32_MAX) return false;
+  b.batch = (int)batch;
+  b.length = (int)length;
+  b.width = (int)width;
+  return true;
+}
+
+// The two parameters of a norm: dense, of one type, x's or float32.  Either may be None where `per_entry` is
+// false (then of shape (width,)); else both are given, a row for each batch entry.
+struct Params {
+  const at::Tensor *factor = nullptr, *offset = nullptr;
+  at::ScalarType dtype;
+};
+
+bool params_from(PyObject* factor, PyObject* offset, bool per_entry, const Blocks& x, int device, Params& p) {
+  p.dtype = x.t->scalar_type();
+  const at::Tensor* first = nullptr;
+  for (PyObject* o : {factor, offset}) {
+    if (o == Py_None && !per_entry) continue;
+    const at::Tensor* t = gpu_tensor(o, device);
+    if (!t || !t->is_contiguous()) return false;
+    const at::ScalarType dt = t->scalar_type();
+    if ((dt != at::kFloat && dt != x.t->scalar_type()) || (first && dt != first->scalar_type())) return false;
+    const bool fits = per_entry ? (t->dim() == 2 && t->size(0) == x.batch && t->size(1) == x.width) ||
+                                      (t->dim() == 3 && t->size(0) == x.batch && t->size(1) == 1 && t->size(2) == x.width)
+                                : t->dim() == 1 && t->size(0) == x.width;
+    if (!fits) return false;
+    first = t;
+    p.dtype = dt;
+    (o == factor ? p.factor : p.offset) = t;
+    if (factor == offset) p.factor = p.offset = t;
+  }
+  return true;
+}
+
+void* data_of(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+
+// (x, factor, offset, eps) -> y or None
+PyObject* norm_forward(PyObject* x_, PyObject* factor, PyObject* offset, PyObject* eps_, bool per_entry) {
+  const int device = device_of(x_);
+  Blocks x;
+  Params p;
+  float eps;
+  if (device < 0 || !gain_of(eps_, eps) || !blocks_from(x_, device, x) || (per_entry && x.t->dim() != 3) ||
+      !params_from(factor, offset, per_entry, x, device, p))
+    return none();
+  at::Tensor y;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    y = empty(x.t->sizes(), x.t->scalar_type(), device);
+    st = flk_layer_norm(x.t->data_ptr(), x.batch_stride, x.row_stride, code_of(x.t->scalar_type()), data_of(p.factor),
+                        data_of(p.offset), code_of(p.dtype), per_entry ? x.width : 0, per_entry, eps, x.batch, x.length,
+                        x.width, y.data_ptr(), (int64_t)x.length * x.width, x.width, stream_of(device));
+  }
+  return st == FLK_OK ? THPVariable_Wrap(y) : failed(st, "flk_layer_norm");
+}
+
+// (dy, x, factor, offset, eps) -> (dx, dfactor, doffset), or with `swap` (dx, doffset, dfactor); or None
+PyObject* norm_backward(PyObject* dy_, PyObject* x_, PyObject* factor, PyObject* offset, PyObject* eps_, bool per_entry,
+                        bool swap) {
+  const int device = device_of(x_);
+  Blocks x, dy;
+  Params p;
+  float eps;
+  if (device < 0 || !gain_of(eps_, eps) || !blocks_from(x_, device, x) || !blocks_from(dy_, device, dy) ||
+      dy.t->sizes() != x.t->sizes() || dy.t->scalar_type() != x.t->scalar_type() || (per_entry && x.t->dim() != 3) ||
+      !params_from(factor, offset, per_entry, x, device, p) || (!p.factor && !p.offset))
+    return none();
+  at::Tensor dx, df, dc;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    int64_t bytes = 0;
+    st = flk_layer_norm_backward_plan(x.batch, x.length, x.width, !per_entry, &bytes);
+    if (st == FLK_OK) {
+      const at::Tensor ws = empty({bytes}, at::kByte, device);
+      dx = empty(x.t->sizes(), x.t->scalar_type(), device);
+      if (p.factor) df = empty(p.factor->sizes(), p.dtype, device);
+      if (p.offset) dc = empty(p.offset->sizes(), p.dtype, device);
+      st = flk_layer_norm_backward(
+          dy.t->data_ptr(), dy.batch_stride, dy.row_stride, x.t->data_ptr(), x.batch_stride, x.row_stride,
+          code_of(x.t->scalar_type()), data_of(p.factor), code_of(p.dtype), per_entry ? x.width : 0, per_entry, eps,
+          x.batch, x.length, x.width, dx.data_ptr(), (int64_t)x.length * x.width, x.width,
+          p.factor ? df.data_ptr() : nullptr, p.offset ? dc.data_ptr() : nullptr, ws.data_ptr(), bytes,
+          stream_of(device));
+    }
+  }
+  if (st != FLK_OK) return failed(st, "flk_layer_norm_backward");
+  return swap ? tuple_of({dx, dc, df}) : tuple_of({dx, df, dc});   // an undefined tensor becomes None
+}
+
+// layer_norm(x, weight, bias, eps), modulate(x, shift, scale, eps)
+PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return n == 4 ? norm_forward(a[0], a[1], a[2], a[3], false) : none();
+  END_HANDLE_TH_ERRORS
+}
+PyObject* modulate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return n == 4 ? norm_forward(a[0], a[2], a[1], a[3], true) : none();
+  END_HANDLE_TH_ERRORS
+}
+// layer_norm_backward(dy, x, weight, bias, eps), modulate_backward(dy, x, shift, scale, eps)
+PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return n == 5 ? norm_backward(a[0], a[1], a[2], a[3], a[4], false, false) : none();
+  END_HANDLE_TH_ERRORS
+}
+PyObject* modulate_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return n == 5 ? norm_backward(a[0], a[1], a[3], a[2], a[4], true, true) : none();
+  END_HANDLE_TH_ERRORS
+}
+
+// swiglu(gu) -> h, swiglu_backward(dh, gu) -> dgu, or None
+PyObject* swiglu(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const int device = n == 1 ? device_of(a[0]) : -1;
+  Blocks gu;
+  if (device < 0 || !blocks_from(a[0], device, gu) || gu.width % 2) return none();
+  const int hidden = gu.width / 2;
+  at::Tensor h;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    at::DimVector shape(gu.t->sizes());
+    shape.back() = hidden;
+    h = empty(shape, gu.t->scalar_type(), device);
+    st = flk_swiglu(gu.t->data_ptr(), gu.batch_stride, gu.row_stride, code_of(gu.t->scalar_type()), gu.batch, gu.length,
+                    hidden, h.data_ptr(), (int64_t)gu.length * hidden, hidden, stream_of(device));
+  }
+  return st == FLK_OK ? THPVariable_Wrap(h) : failed(st, "flk_swiglu");
+  END_HANDLE_TH_ERRORS
+}
+PyObject* swiglu_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const int device = n == 2 ? device_of(a[1]) : -1;
+  Blocks dh, gu;
+  if (device < 0 || !blocks_from(a[1], device, gu) || gu.width % 2 || !blocks_from(a[0], device, dh) ||
+      dh.t->scalar_type() != gu.t->scalar_type())
+    return none();
+  at::DimVector shape(gu.t->sizes());
+  shape.back() = gu.width / 2;
+  if (dh.t->sizes() != at::IntArrayRef(shape)) return none();
+  at::Tensor dgu;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    dgu = empty(gu.t->sizes(), gu.t->scalar_type(), device);
+    st = flk_swiglu_backward(dh.t->data_ptr(), dh.batch_stride, dh.row_stride, gu.t->data_ptr(), gu.batch_stride,
+                             gu.row_stride, code_of(gu.t->scalar_type()), gu.batch, gu.length, dh.width, dgu.data_ptr(),
+                             (int64_t)gu.length * gu.width, gu.width, stream_of(device));
+  }
+  return st == FLK_OK ? THPVariable_Wrap(dgu) : failed(st, "flk_swiglu_backward");
+  END_HANDLE_TH_ERRORS
+}
+
 #define FLK_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FLK_METHOD(qk_prep), FLK_METHOD(attend_merged), FLK_METHOD(double_attention),
-                         FLK_METHOD(linear), {nullptr, nullptr, 0, nullptr}};
+                         FLK_METHOD(linear), FLK_METHOD(layer_norm), FLK_METHOD(layer_norm_backward),
+                         FLK_METHOD(modulate), FLK_METHOD(modulate_backward), FLK_METHOD(swiglu),
+                         FLK_METHOD(swiglu_backward), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

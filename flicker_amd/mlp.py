@@ -23,7 +23,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .kernels import _on_gpu
+from .kernels import _native, _on_gpu
 from .norm import _blocks, _dtype, _out_blocks, _output, _strides
 
 _GATE, _GATE_BACKWARD, _MATMUL, _MATMUL_BT, _MATMUL_AT = range(5)   # FLK_MLP_*
@@ -40,6 +40,10 @@ class Kept(NamedTuple):
 def swiglu(gu: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """silu(g) * u of gu (..., 2 * hidden) = [g | u] -> (..., hidden); bfloat16, float16 or float32.  gu and
     ``out`` may be columns of wider buffers."""
+    if out is None:
+        done = _native.swiglu(gu)
+        if done is not None:
+            return done
     code = _dtype("gu", gu)
     if gu.dim() == 0 or gu.shape[-1] == 0 or gu.shape[-1] % 2:
         raise ValueError(f"gu must be (..., 2 * hidden), got {tuple(gu.shape)}")
@@ -55,6 +59,10 @@ def swiglu(gu: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor
 
 def swiglu_backward(dh: torch.Tensor, gu: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """dgu = [dg | du] of ``swiglu(gu)`` for the incoming gradient dh; ``out`` may be gu itself."""
+    if out is None:
+        done = _native.swiglu_backward(dh, gu)
+        if done is not None:
+            return done
     code = _dtype("gu", gu)
     _on_gpu("dh", dh)
     if gu.dim() == 0 or gu.shape[-1] == 0 or gu.shape[-1] % 2:

@@ -9,7 +9,7 @@ float32 and every output is rounded once, where the reference rounds each step o
 bf16 (``w8a8.quantize_act_modulated`` reproduces those roundings); the two differ by bf16 ulps.
 
 x is bfloat16, float16 or float32, (..., width) with rows of any stride (a (B, L, width) view, such
-as one stream of a joint sequence, is read in place) and any width up to 32768; parameters are
+as one stream of a joint sequence, is read in place) and any width up to 16384; parameters are
 of x's type or float32.  Parameter gradients are sums over tokens in a fixed order.  For gradients through
 torch's autograd see ``flicker_amd.autograd``.
 """
@@ -21,7 +21,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .kernels import EPS, _on_gpu, _vector
+from .kernels import EPS, _native, _on_gpu, _vector
 
 _CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # FLK_BF16, FLK_F16, FLK_F32
 
@@ -147,6 +147,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                eps: float = EPS, out: torch.Tensor | None = None) -> torch.Tensor:
     """Layer norm over the last axis of x (..., width); ``weight`` and ``bias`` (width,) or None.  ``out`` may be
     a view with strided rows, or x itself."""
+    if out is None:
+        done = _native.layer_norm(x, weight, bias, eps)
+        if done is not None:
+            return done
     _check_x(x)
     weight, bias = _params((("weight", weight), ("bias", bias)), x, ((x.shape[-1],),))
     return _forward(x, weight, bias, False, False, eps, out)
@@ -156,6 +160,9 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
                         bias: torch.Tensor | None = None, *, eps: float = EPS):
     """(dx, dweight, dbias) of ``layer_norm(x, weight, bias)`` for the incoming gradient dy; None for a
     parameter that is None."""
+    done = _native.layer_norm_backward(dy, x, weight, bias, eps)
+    if done is not None:
+        return done
     _check_x(x)
     w, b = _params((("weight", weight), ("bias", bias)), x, ((x.shape[-1],),))
     dtype = next((p.dtype for p in (w, b) if p is not None), x.dtype)
@@ -176,6 +183,10 @@ def modulate(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *, eps: 
              out: torch.Tensor | None = None) -> torch.Tensor:
     """modules.py:38-40 -- (1 + scale) * layer_norm(x) + shift of x (B, L, width) with one row of shift and
     scale per batch entry, (B, width) or (B, 1, width).  ``out`` as for layer_norm."""
+    if out is None:
+        done = _native.modulate(x, shift, scale, eps)
+        if done is not None:
+            return done
     shift, scale = _modulation(x, shift, scale)
     return _forward(x, scale, shift, True, True, eps, out)
 
@@ -184,6 +195,9 @@ def modulate_backward(dy: torch.Tensor, x: torch.Tensor, shift: torch.Tensor, sc
                       eps: float = EPS):
     """(dx, dshift, dscale) of ``modulate(x, shift, scale)`` for the incoming gradient dy, the last two shaped as
     shift and scale."""
+    done = _native.modulate_backward(dy, x, shift, scale, eps)
+    if done is not None:
+        return done
     shift_row, scale_row = _modulation(x, shift, scale)
     dx, dscale, dshift = _backward(dy, x, scale_row, (True, True), scale_row.dtype, True, True, eps)
     return dx, dshift.view(shift.shape), dscale.view(scale.shape)

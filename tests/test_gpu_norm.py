@@ -68,7 +68,7 @@ def _norm_case(x, factor, offset, dy, over, eps=norm.EPS):
     return (y, y_tol), (dx, dx_tol), (dyn.sum(over), da_tol), (dyo.sum(over), (rows + 64) * U * np.abs(dyo).sum(over))
 
 
-WIDTHS = [1, 2, 7, 8, 64, 511, 513, 1000, 1536, 2049, 24 * 128, 4096, 5001, 8200]
+WIDTHS = [1, 2, 7, 8, 64, 511, 513, 1000, 1536, 2049, 24 * 128, 4096, 5001, 8200, 16384]
 
 
 @pytest.mark.parametrize("width", WIDTHS)
@@ -228,7 +228,7 @@ def test_norm_refusals(device):
     with pytest.raises(HipKernelError):
         norm.layer_norm(x, eps=-1.0)
     with pytest.raises(HipKernelError, match="unsupported"):
-        norm.layer_norm(torch.zeros(1, 40000, device=device))
+        norm.layer_norm(torch.zeros(1, 16392, device=device))
 
 
 def _gate_case(gu, dh):
@@ -323,3 +323,47 @@ def test_gradients_are_the_forward_pass_differences(device):
         near, far = slope(2.0 ** -5), slope(2.0 ** -4)
         noise = 300 * U * float((out.double().abs() * weight.abs()).sum()) * 2 ** 5
         assert abs(float((grad.double() * d.double()).sum()) - near) <= abs(far - near) + noise
+
+
+class Declines:
+    """A native call path that takes no call."""
+
+    def __getattr__(self, name):
+        return lambda *_: None
+
+
+@pytest.mark.parametrize("dtype,params", [("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp32")])
+@pytest.mark.parametrize("width", [1, 96, 1003])
+def test_native_path_equals_the_python_path(device, monkeypatch, dtype, params, width):
+    """Plain calls take the native path, and have the Python path's values, shapes and types."""
+    x, g = _stream(width, 2, 9, width, TYPES[dtype], device)
+    wide = torch.randn(2, 9, 5 + 2 * width, generator=g).to(TYPES[dtype]).to(device)
+    dy = torch.randn(2, 9, width, generator=g).to(TYPES[dtype]).to(device)
+    rows = [torch.randn(2, 1, width, generator=g).to(TYPES[params]).to(device) for _ in range(2)]
+    w, b = rows[0][0, 0], rows[1][1, 0]
+    calls = {
+        "modulate": lambda: norm.modulate(x, *rows),
+        "modulate_backward": lambda: norm.modulate_backward(dy, x, *rows),
+        "layer_norm": lambda: norm.layer_norm(x[0], w, None),
+        "layer_norm_backward": lambda: norm.layer_norm_backward(dy, x, None, b),
+        "swiglu": lambda: mlp.swiglu(wide[..., 5:]),
+        "swiglu_backward": lambda: mlp.swiglu_backward(dy, wide[..., 5:]),
+    }
+    taken = {
+        "modulate": norm._native.modulate(x, *rows, 1e-6), "layer_norm": norm._native.layer_norm(x[0], w, None, 1e-6),
+        "modulate_backward": norm._native.modulate_backward(dy, x, *rows, 1e-6),
+        "layer_norm_backward": norm._native.layer_norm_backward(dy, x, None, b, 1e-6),
+        "swiglu": norm._native.swiglu(wide[..., 5:]), "swiglu_backward": norm._native.swiglu_backward(dy, wide[..., 5:]),
+    }
+    assert all(v is not None for v in taken.values()), [k for k, v in taken.items() if v is None]
+    got = {k: f() for k, f in calls.items()}
+    monkeypatch.setattr(norm, "_native", Declines())
+    monkeypatch.setattr(mlp, "_native", Declines())
+    for k, f in calls.items():
+        for a, c, e in zip(*(v if isinstance(v, tuple) else (v,) for v in (got[k], f(), taken[k])), strict=True):
+            if c is None:
+                assert a is None and e is None
+                continue
+            for t in (a, e):
+                assert t.shape == c.shape and t.dtype == c.dtype and torch.equal(t, c), k
+    assert norm._native.modulate(x, *rows) is None

@@ -72,7 +72,7 @@ def test_layer_norm_checks(lib):
     assert _norm(lib, eps=-1.0) == INVALID and _norm(lib, eps=float("nan")) == INVALID
     assert _norm(lib, pstride=32) == INVALID
     assert _norm(lib, batch=65536, length=65536) == INVALID
-    assert _norm(lib, width=32769, pstride=0) == UNSUPPORTED
+    assert _norm(lib, width=16385, pstride=0) == UNSUPPORTED
     assert _norm(lib, batch=1, x=None) == INVALID and _norm(lib, batch=1, y=None) == INVALID
     assert _norm(lib, batch=1, x=P16 + 1) == ALIGN and _norm(lib, batch=1, dtype=F32, params=F32, y=P16 + 2) == ALIGN
     assert _norm(lib, batch=1, params=F32, factor=P16 + 2) == ALIGN
