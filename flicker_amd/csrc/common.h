@@ -56,6 +56,12 @@ __device__ __forceinline__ void dma16_at(const void* base, uint32_t voff, const 
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "{m0}"(lds), "v"(voff), "s"(base) : "memory");
 }
 
+// Four bytes per lane the same way, landing at lds_dst + 4 i.
+__device__ __forceinline__ void dma4_at(const void* base, uint32_t voff, const uint8_t* lds_dst) {
+  const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds_dst);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" :: "{m0}"(lds), "v"(voff), "s"(base) : "memory");
+}
+
 __device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace flk

@@ -10,29 +10,32 @@
 // g of a column holds u of the same column, and h leaves the registers as the only output.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "elems.h"
 
 namespace {
 
 using flk::f32x4;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // A block's tile: WN x WM waves across the columns and rows of D, each NF x MF fragments of 16 x 16.
-template <int WN, int WM, int NF, int MF, int BUFFERS, int PER_CU, int RING, int LEAD, int BAR>
+template <int WN, int WM, int NF, int MF, int BUFFERS, int PER_CU, int RING, int LEAD, int BAR, int AHEAD>
 struct Geometry {
   static constexpr int kWN = WN, kWM = WM, kNF = NF, kMF = MF;
+  static constexpr int kAhead = AHEAD;
   static constexpr int kRing = RING, kLead = LEAD, kBar = BAR;
   static constexpr int kBuffers = BUFFERS;   // stages in LDS
   static constexpr int kPerCU = PER_CU;      // blocks a CU holds
   static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
   static constexpr int kTB = 16 * NF * WN, kTA = 16 * MF * WM;
 };
-typedef Geometry<2, 4, 8, 4, 2, 1, 4, 3, 3> Large;    // 256 columns x 256 rows
-typedef Geometry<2, 4, 6, 4, 2, 1, 3, 2, 2> Medium;   // 192 x 256
-typedef Geometry<2, 2, 4, 4, 2, 2, 4, 3, 3> Small;    // 128 x 128, two blocks a CU
-typedef Geometry<2, 2, 4, 4, 4, 1, 4, 3, 3> Deep;     // 128 x 128, one block a CU with more stages in flight
-typedef Geometry<4, 1, 2, 2, 4, 2, 4, 2, 1> Few;      // 128 x 32: few rows, the columns' operand streams through
+typedef Geometry<2, 4, 8, 4, 2, 1, 4, 3, 3, 2> Large;    // 256 columns x 256 rows
+typedef Geometry<2, 4, 6, 4, 2, 1, 3, 2, 2, 2> Medium;   // 192 x 256
+typedef Geometry<2, 2, 4, 4, 2, 2, 4, 3, 3, 0> Small;    // 128 x 128, two blocks a CU
+typedef Geometry<2, 2, 4, 4, 4, 1, 4, 3, 3, 0> Deep;     // 128 x 128, one block a CU with more stages in flight
+typedef Geometry<4, 1, 2, 2, 4, 2, 4, 2, 1, 0> Few;      // 128 x 32: few rows, the columns' operand streams through
 
 constexpr int kK = 64;                // inner terms a stage
 constexpr int kKBytes = kK * 2;       // of one operand row: a 128-byte line
@@ -55,6 +58,7 @@ struct Product {
   float* gu;          // kGate: out, may be NULL; kGateBackward: in
   int hidden;         // kGate, kGateBackward
   int tiles_a, tiles_b;
+  bool stream;        // whether what the launch writes (kGateBackward: gu, which it reads) passes the caches by
   float* partial;     // kPartial: (splits, rows, cols) sums over `stages` stages each
   int splits, stages;
 };
@@ -106,6 +110,7 @@ __device__ __forceinline__ int slot_chunk(int h4) { return ((h4 & 1) << 1) | (h4
 template <typename T, bool kAcross, int kT, int kWaves>
 struct Half {
   typedef typename Mfma<T>::vec vec;
+  static constexpr int kRows = kT;
   static constexpr int kBytes = kT * kKBytes;
   static constexpr int kCopies = kBytes / 1024 / kWaves;   // copy instructions per wave
   static constexpr int kLine = kAcross ? kT * 2 : kKBytes;
@@ -121,6 +126,7 @@ struct Half {
   const uint8_t* base;          // the tile's first row / column
   int64_t step;                 // bytes from one stage to the next
   uint32_t from[kCopies];       // what this lane fetches, from base
+  uint32_t touched;
 
   // rows / terms beyond the operand repeat its last one; results of repeated rows are never stored, and
   // repeated terms are never fetched (tail).  kPair: see pair_column.
@@ -138,6 +144,16 @@ struct Half {
         from[i] = (uint32_t)column(line) * (uint32_t)pitch + chunk * 16;
     }
   }
+  // Touches one 128-byte line a lane of a stage far ahead, so that the L2 has it when the copies come: line i of
+  // the half.  What it brings lands in LDS that nothing reads.
+  template <typename Column>
+  __device__ __forceinline__ void init_touch(const Operand& o, int i, Column column) {
+    if constexpr (kAcross)
+      touched = (uint32_t)(i / (kT / 64)) * (uint32_t)(o.stride * 2) + 2u * (uint32_t)column(i % (kT / 64) * 64);
+    else
+      touched = (uint32_t)column(i) * (uint32_t)(o.stride * 2);
+  }
+  __device__ __forceinline__ void touch(int stage, uint8_t* lds) const { flk::dma4_at(base + stage * step, touched, lds); }
   __device__ __forceinline__ void copy(int i, int stage, uint8_t* lds, int wave) const {
     flk::dma16_at(base + stage * step, from[i], lds + (wave * kCopies + i) * 1024);
   }
@@ -206,15 +222,30 @@ __device__ __forceinline__ int out_swizzle(int row) {
   return row & mask;
 }
 
-template <typename T, int kChunks, int kRows>
+// Accesses that leave the caches to others where kStream is set.
+template <bool kStream, typename V>
+__device__ __forceinline__ void store(V* p, const V& v) {
+  if constexpr (kStream)
+    __builtin_nontemporal_store(v, p);
+  else
+    *p = v;
+}
+template <bool kStream, typename V>
+__device__ __forceinline__ V load(const V* p) {
+  if constexpr (kStream) return __builtin_nontemporal_load(p);
+  return *p;
+}
+
+template <bool kStream, typename T, int kChunks, int kRows>
 __device__ __forceinline__ void store_rows(const uint8_t* lds, T* d, int64_t stride, int64_t row0, int64_t rows,
                                            int col0, int cols, int lane) {
 #pragma unroll
   for (int it = 0; it < (kRows * kChunks + 63) / 64; ++it) {
     const int at = it * 64 + lane, r = at / kChunks, c = at % kChunks;
     if (kRows * kChunks % 64 && r >= kRows) break;
-    const uint4 v = *reinterpret_cast<const uint4*>(lds + (r * kChunks + (c ^ out_swizzle<kChunks>(r))) * 16);
-    if (row0 + r < rows && col0 + c * 8 < cols) *reinterpret_cast<uint4*>(d + (row0 + r) * stride + col0 + c * 8) = v;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(lds + (r * kChunks + (c ^ out_swizzle<kChunks>(r))) * 16);
+    if (row0 + r < rows && col0 + c * 8 < cols)
+      store<kStream>(reinterpret_cast<u32x4*>(d + (row0 + r) * stride + col0 + c * 8), v);
   }
 }
 
@@ -243,7 +274,9 @@ __global__ __launch_bounds__(G::kThreads, G::kThreads * G::kPerCU / 256) void ml
   // are read kLead groups ahead into a ring; kBar groups of a stage follow its barrier.
   constexpr int kGroups = 2 * kNF, kRing = G::kRing, kLead = G::kLead, kBar = G::kBar;
   static_assert(kGroups % kRing == 0 && kLead < kRing && kBar <= kLead && kMF <= kNF, "the fragment ring divides a stage");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kBuffers * kStage];
+  constexpr int kAhead = G::kAhead;
+  static_assert(kAhead == 0 || (kBuffers == 2 && G::kWaves == 8), "two waits: with a touch in flight, or without");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kBuffers * kStage + (kAhead ? 2048 : 0)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wb = wave / kWM, wa = wave % kWM, l16 = lane & 15, h4 = lane >> 4;
@@ -261,16 +294,26 @@ __global__ __launch_bounds__(G::kThreads, G::kThreads * G::kPerCU / 256) void ml
   HB hb;
   HA ha;
   const int64_t row0 = (int64_t)ta * kTA, col0 = (int64_t)tb * kTB;
+  // Blocks of a sweep share their row and column operands: each touches its share of both (kAhead).
+  const int share_b = min(kGroup, P.tiles_a), share_a = min(8, P.tiles_b);
+  const int part_b = (kTB + share_b - 1) / share_b, part_a = (kTA + share_a - 1) / share_a;
+  const int turn = (wave & 3) * 64, part = wave < 4 ? part_b : part_a;
+  const bool touches = kAhead > 0 && turn < part && P.tiles_a >= kGroup;
+  const int line = min((wave < 4 ? ta % share_b : tb % share_a) * part + min(turn + lane, part - 1), (wave < 4 ? kTB : kTA) - 1);
+  auto init = [&](auto& half, const Operand& o, int64_t first, auto column) __attribute__((always_inline)) {
+    half.init(o, first, wave, lane, column);
+    if constexpr (kAhead > 0) half.init_touch(o, min(line, half.kRows - 1), column);
+  };
   if constexpr (kE == kGate)
-    hb.init(P.b, 0, wave, lane, [&](int c) { return pair_column<16 * kNF, G::kWN>(tb, c, P.hidden); });
+    init(hb, P.b, 0, [&](int c) { return pair_column<16 * kNF, G::kWN>(tb, c, P.hidden); });
   else if constexpr (kBAcross)
-    hb.init(P.b, 0, wave, lane, [&](int c) { return min((int)col0 + c, P.b.rows - 8); });
+    init(hb, P.b, 0, [&](int c) { return min((int)col0 + c, P.b.rows - 8); });
   else
-    hb.init(P.b, col0, wave, lane, [&](int r) { return min(r, P.b.rows - 1 - (int)col0); });
+    init(hb, P.b, col0, [&](int r) { return min(r, P.b.rows - 1 - (int)col0); });
   if constexpr (kAAcross)
-    ha.init(P.a, 0, wave, lane, [&](int c) { return min((int)row0 + c, P.a.rows - 8); });
+    init(ha, P.a, 0, [&](int c) { return min((int)row0 + c, P.a.rows - 8); });
   else
-    ha.init(P.a, row0, wave, lane, [&](int r) { return min(r, P.a.rows - 1 - (int)row0); });
+    init(ha, P.a, row0, [&](int r) { return min(r, P.a.rows - 1 - (int)row0); });
 
   // Stages first .. first + stages - 1 of the inner axis; the axis' last may have fewer terms (left).
   const int all = (P.inner + kK - 1) / kK, left = P.inner - (all - 1) * kK;
@@ -313,7 +356,9 @@ __global__ __launch_bounds__(G::kThreads, G::kThreads * G::kPerCU / 256) void ml
   // next stage's first fragments.  After the last stage those reads take what is there; nothing uses it.
   // Copies return in order: while `later` whole stages follow the awaited one, theirs may be in flight.
   constexpr int kLater = kBuffers - 2;
+  constexpr int kTouch = kGroups - kBar - 4;   // the touch follows the stage's copies
   constexpr int kSpread = (kCopies + kBar + kNF - 1) / (kBar + kNF);   // copy instructions a group
+  static_assert(kAhead == 0 || (kBar + kTouch) * kSpread >= kCopies, "the touch comes after the last copy");
 #pragma unroll
   for (int s = 0; s < kBuffers; ++s) {
     if (s < whole)
@@ -342,12 +387,21 @@ __global__ __launch_bounds__(G::kThreads, G::kThreads * G::kPerCU / 256) void ml
       if (after == 0) {
         if (kLater > 0 && s + kBuffers <= whole)
           asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(kLater * kCopies) : "memory");
+        else if (touches && s + kAhead < whole)
+          asm volatile("s_waitcnt vmcnt(1) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         else
           asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (s + kBuffers >= whole && s + kBuffers < stages) tail_stage(s + kBuffers);
       }
       if (after >= 0) {
         if (s + kBuffers < whole) copy_some(s + kBuffers, after * kSpread, (after + 1) * kSpread);
+      } else if (kAhead > 0 && g == kTouch) {
+        if (touches && s + kAhead < whole) {
+          if (wave < 4)
+            hb.touch(first + s + kAhead, smem + kBuffers * kStage + wave * 256);
+          else
+            ha.touch(first + s + kAhead, smem + kBuffers * kStage + wave * 256);
+        }
       } else if ((kBar + g) * kSpread < kCopies) {
         if (s > 0 && s + kBuffers - 1 < whole) copy_some(s + kBuffers - 1, (kBar + g) * kSpread, (kBar + g + 1) * kSpread);
       }
@@ -374,103 +428,111 @@ __global__ __launch_bounds__(G::kThreads, G::kThreads * G::kPerCU / 256) void ml
   constexpr int kRows = 16 * kMF;
   T* d = static_cast<T*>(P.d);
   const int64_t wrow = row0 + wa * kRows;
-  if constexpr (kE == kPartial) {
-    float* out = P.partial + (int64_t)range * P.a.rows * P.b.rows;
-#pragma unroll
-    for (int m = 0; m < kMF; ++m) {
-      const int64_t row = wrow + m * 16 + l16;
-      if (row >= P.a.rows) continue;
-#pragma unroll
-      for (int n = 0; n < kNF; ++n) {
-        const int col = (int)col0 + wb * 16 * kNF + n * 16 + h4 * 4;
-        if (col < P.b.rows) *reinterpret_cast<f32x4*>(out + row * P.b.rows + col) = acc[n][m];
-      }
-    }
-  } else if constexpr (kE == kPlain) {
-    constexpr int kChunks = 2 * kNF;
-    uint8_t* out = smem + wave * (kRows * kChunks * 16);
-#pragma unroll
-    for (int n = 0; n < kNF; ++n)
-#pragma unroll
+  auto finish = [&](auto stream) __attribute__((always_inline)) {
+    constexpr bool kStream = decltype(stream)::value;
+    (void)kStream;
+    if constexpr (kE == kPartial) {
+      float* out = P.partial + (int64_t)range * P.a.rows * P.b.rows;
+  #pragma unroll
       for (int m = 0; m < kMF; ++m) {
-        const float x[4] = {acc[n][m][0], acc[n][m][1], acc[n][m][2], acc[n][m][3]};
-        put4<T, kChunks>(out, m * 16 + l16, n * 16 + h4 * 4, x);
-      }
-    store_rows<T, kChunks, kRows>(out, d, P.d_stride, wrow, P.a.rows, (int)col0 + wb * 16 * kNF, P.b.rows, lane);
-  } else if constexpr (kE == kGateBackward) {
-    // dh leaves as float32 rows of half the wave's columns at a time; a lane takes 8 columns of a row
-    // back, so that g and u are read, and dg and du written, in whole lines.
-    constexpr int kPass = kNF / 2, kChunks = kPass * 4, kParts = kPass * 2;   // chunks of 4, parts of 8 columns
-    constexpr int kTurns = (kRows * kParts + 63) / 64, kBatch = kTurns % 4 == 0 ? 4 : 3;
-    uint8_t* out = smem + wave * (kRows * kChunks * 16);
-#pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-#pragma unroll
-      for (int n = 0; n < kPass; ++n)
-#pragma unroll
-        for (int m = 0; m < kMF; ++m) {
-          const int r = m * 16 + l16;
-          *reinterpret_cast<f32x4*>(out + (r * kChunks + ((n * 4 + h4) ^ out_swizzle<kChunks>(r))) * 16) =
-              acc[pass * kPass + n][m];
-        }
-      const int wcol = (int)col0 + wb * 16 * kNF + pass * kPass * 16;
-#pragma unroll
-      for (int first = 0; first < kTurns; first += kBatch) {
-        f32x4 g[kBatch][2], u[kBatch][2];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int at = (first + i) * 64 + lane, r = at / kParts, col = wcol + at % kParts * 8;
-          if (r >= kRows || wrow + r >= P.a.rows || col >= P.hidden) continue;
-          const f32x4* src = reinterpret_cast<const f32x4*>(P.gu + (wrow + r) * 2 * P.hidden + col);
-          const f32x4* usrc = reinterpret_cast<const f32x4*>(P.gu + (wrow + r) * 2 * P.hidden + P.hidden + col);
-          g[i][0] = src[0];
-          g[i][1] = src[1];
-          u[i][0] = usrc[0];
-          u[i][1] = usrc[1];
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int at = (first + i) * 64 + lane, r = at / kParts, part = at % kParts, col = wcol + part * 8;
-          if (r >= kRows || wrow + r >= P.a.rows || col >= P.hidden) continue;
-          float dg[8], du[8];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const f32x4 dh = *reinterpret_cast<const f32x4*>(
-                out + (r * kChunks + ((part * 2 + c) ^ out_swizzle<kChunks>(r))) * 16);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) flk::gate_backward(dh[j], g[i][c][j], u[i][c][j], dg[c * 4 + j], du[c * 4 + j]);
-          }
-          T* dst = d + (wrow + r) * P.d_stride + col;
-          *reinterpret_cast<uint4*>(dst) = uint4{pack2<T>(dg[0], dg[1]), pack2<T>(dg[2], dg[3]), pack2<T>(dg[4], dg[5]),
-                                                 pack2<T>(dg[6], dg[7])};
-          *reinterpret_cast<uint4*>(dst + P.hidden) = uint4{pack2<T>(du[0], du[1]), pack2<T>(du[2], du[3]),
-                                                            pack2<T>(du[4], du[5]), pack2<T>(du[6], du[7])};
-        }
-      }
-    }
-  } else {
-    constexpr int kHalf = kNF / 2, kChunks = kNF;
-    uint8_t* out = smem + wave * (kRows * kChunks * 16);
-    const int wcol = tb * (kTB / 2) + wb * 16 * kHalf;
-#pragma unroll
-    for (int n = 0; n < kHalf; ++n)
-#pragma unroll
-      for (int m = 0; m < kMF; ++m) {
-        const f32x4 g = acc[n][m], u = acc[n + kHalf][m];
         const int64_t row = wrow + m * 16 + l16;
-        const int col = wcol + n * 16 + h4 * 4;
-        if (P.gu && row < P.a.rows && col < P.hidden) {
-          float* dst = P.gu + row * 2 * P.hidden + col;
-          *reinterpret_cast<f32x4*>(dst) = g;
-          *reinterpret_cast<f32x4*>(dst + P.hidden) = u;
+        if (row >= P.a.rows) continue;
+  #pragma unroll
+        for (int n = 0; n < kNF; ++n) {
+          const int col = (int)col0 + wb * 16 * kNF + n * 16 + h4 * 4;
+          if (col < P.b.rows) *reinterpret_cast<f32x4*>(out + row * P.b.rows + col) = acc[n][m];
         }
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = flk::gate(g[i], u[i]);
-        put4<T, kChunks>(out, m * 16 + l16, n * 16 + h4 * 4, x);
       }
-    store_rows<T, kChunks, kRows>(out, d, P.d_stride, wrow, P.a.rows, wcol, P.hidden, lane);
-  }
+    } else if constexpr (kE == kPlain) {
+      constexpr int kChunks = 2 * kNF;
+      uint8_t* out = smem + wave * (kRows * kChunks * 16);
+  #pragma unroll
+      for (int n = 0; n < kNF; ++n)
+  #pragma unroll
+        for (int m = 0; m < kMF; ++m) {
+          const float x[4] = {acc[n][m][0], acc[n][m][1], acc[n][m][2], acc[n][m][3]};
+          put4<T, kChunks>(out, m * 16 + l16, n * 16 + h4 * 4, x);
+        }
+      store_rows<kStream, T, kChunks, kRows>(out, d, P.d_stride, wrow, P.a.rows, (int)col0 + wb * 16 * kNF, P.b.rows, lane);
+    } else if constexpr (kE == kGateBackward) {
+      // dh leaves as float32 rows of half the wave's columns at a time; a lane takes 8 columns of a row
+      // back, so that g and u are read, and dg and du written, in whole lines.
+      constexpr int kPass = kNF / 2, kChunks = kPass * 4, kParts = kPass * 2;   // chunks of 4, parts of 8 columns
+      constexpr int kTurns = (kRows * kParts + 63) / 64, kBatch = kTurns % 4 == 0 ? 4 : 3;
+      uint8_t* out = smem + wave * (kRows * kChunks * 16);
+  #pragma unroll
+      for (int pass = 0; pass < 2; ++pass) {
+  #pragma unroll
+        for (int n = 0; n < kPass; ++n)
+  #pragma unroll
+          for (int m = 0; m < kMF; ++m) {
+            const int r = m * 16 + l16;
+            *reinterpret_cast<f32x4*>(out + (r * kChunks + ((n * 4 + h4) ^ out_swizzle<kChunks>(r))) * 16) =
+                acc[pass * kPass + n][m];
+          }
+        const int wcol = (int)col0 + wb * 16 * kNF + pass * kPass * 16;
+  #pragma unroll
+        for (int first = 0; first < kTurns; first += kBatch) {
+          f32x4 g[kBatch][2], u[kBatch][2];
+  #pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int at = (first + i) * 64 + lane, r = at / kParts, col = wcol + at % kParts * 8;
+            if (r >= kRows || wrow + r >= P.a.rows || col >= P.hidden) continue;
+            const f32x4* src = reinterpret_cast<const f32x4*>(P.gu + (wrow + r) * 2 * P.hidden + col);
+            const f32x4* usrc = reinterpret_cast<const f32x4*>(P.gu + (wrow + r) * 2 * P.hidden + P.hidden + col);
+            g[i][0] = load<kStream>(src);
+            g[i][1] = load<kStream>(src + 1);
+            u[i][0] = load<kStream>(usrc);
+            u[i][1] = load<kStream>(usrc + 1);
+          }
+  #pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int at = (first + i) * 64 + lane, r = at / kParts, part = at % kParts, col = wcol + part * 8;
+            if (r >= kRows || wrow + r >= P.a.rows || col >= P.hidden) continue;
+            float dg[8], du[8];
+  #pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const f32x4 dh = *reinterpret_cast<const f32x4*>(
+                  out + (r * kChunks + ((part * 2 + c) ^ out_swizzle<kChunks>(r))) * 16);
+  #pragma unroll
+              for (int j = 0; j < 4; ++j) flk::gate_backward(dh[j], g[i][c][j], u[i][c][j], dg[c * 4 + j], du[c * 4 + j]);
+            }
+            T* dst = d + (wrow + r) * P.d_stride + col;
+            *reinterpret_cast<uint4*>(dst) = uint4{pack2<T>(dg[0], dg[1]), pack2<T>(dg[2], dg[3]), pack2<T>(dg[4], dg[5]),
+                                                   pack2<T>(dg[6], dg[7])};
+            *reinterpret_cast<uint4*>(dst + P.hidden) = uint4{pack2<T>(du[0], du[1]), pack2<T>(du[2], du[3]),
+                                                              pack2<T>(du[4], du[5]), pack2<T>(du[6], du[7])};
+          }
+        }
+      }
+    } else {
+      constexpr int kHalf = kNF / 2, kChunks = kNF;
+      uint8_t* out = smem + wave * (kRows * kChunks * 16);
+      const int wcol = tb * (kTB / 2) + wb * 16 * kHalf;
+  #pragma unroll
+      for (int n = 0; n < kHalf; ++n)
+  #pragma unroll
+        for (int m = 0; m < kMF; ++m) {
+          const f32x4 g = acc[n][m], u = acc[n + kHalf][m];
+          const int64_t row = wrow + m * 16 + l16;
+          const int col = wcol + n * 16 + h4 * 4;
+          if (P.gu && row < P.a.rows && col < P.hidden) {
+            float* dst = P.gu + row * 2 * P.hidden + col;
+            store<kStream>(reinterpret_cast<f32x4*>(dst), g);
+            store<kStream>(reinterpret_cast<f32x4*>(dst + P.hidden), u);
+          }
+          float x[4];
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = flk::gate(g[i], u[i]);
+          put4<T, kChunks>(out, m * 16 + l16, n * 16 + h4 * 4, x);
+        }
+      store_rows<kStream, T, kChunks, kRows>(out, d, P.d_stride, wrow, P.a.rows, wcol, P.hidden, lane);
+    }
+  };
+  if (P.stream)
+    finish(std::true_type{});
+  else
+    finish(std::false_type{});
 }
 
 // Adds the ranges' partial sums in order and finishes as kE says, four columns a lane: of one row of D,
@@ -517,6 +579,7 @@ constexpr int kMaxDim = INT32_MAX - 256;
 constexpr int64_t kMaxStride = 1 << 22;   // 256 rows of one operand are addressed in 32 bits
 constexpr int64_t kMaxBlocks = 1 << 22;   // work-items of a launch are counted in 32 bits
 constexpr int kCUs = 256;
+constexpr int64_t kStreamBytes = 80 << 20;
 
 enum Tile { kLarge, kMedium, kSmall, kDeep, kFew, kTiles };
 
@@ -612,6 +675,7 @@ template <bool kAAcross, bool kBAcross, Epilogue kE>
 int launch(Product& p, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (p.a.stride > kMaxStride || p.b.stride > kMaxStride) return FLK_E_INVALID;
   const Choice c = choose(p.a.rows, p.b.rows, p.inner, kAAcross);
+  p.stream = (kE == kPlain || !p.gu ? 2LL * p.a.rows * (kE == kGate ? p.hidden : p.b.rows) : 8LL * p.a.rows * p.hidden) > kStreamBytes;
   const int64_t need = partial_bytes(c, p.a.rows, p.b.rows);
   if (need) {
     if (!workspace || workspace_bytes < need) return FLK_E_SCRATCH;
