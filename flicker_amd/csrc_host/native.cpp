@@ -462,11 +462,146 @@ PyObject* swiglu_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A (rows, cols) operand of a matrix product, its rows 16-byte aligned: t's last axis against all others.
+struct Matrix {
+  const at::Tensor* t;
+  int64_t rows, cols, stride;
+};
+
+bool matrix_from(PyObject* o, int device, Matrix& m) {
+  m.t = gpu_tensor(o, device);
+  if (!m.t || m.t->dim() < 1 || m.t->numel() == 0 || m.t->stride(-1) != 1 || !aligned16(*m.t)) return false;
+  const at::ScalarType dt = m.t->scalar_type();
+  if (dt != at::kBFloat16 && dt != at::kHalf) return false;
+  m.cols = m.t->size(-1);
+  m.rows = m.t->numel() / m.cols;
+  m.stride = m.cols;
+  if (m.t->dim() == 2)
+    m.stride = m.t->stride(0);
+  else if (!m.t->is_contiguous())
+    return false;
+  return m.cols % 8 == 0 && m.stride % 8 == 0 && m.stride >= m.cols && m.rows <= INT32_MAX && m.cols <= INT32_MAX;
+}
+
+// The operands of a gated MLP: x (..., width), w_in (width, 2 hidden), w_out (hidden, width) of one type.
+struct Mlp {
+  Matrix x, in, out;
+  int dtype, m, width, hidden;
+};
+
+bool mlp_from(PyObject* x, PyObject* w_in, PyObject* w_out, int device, Mlp& p) {
+  if (!matrix_from(x, device, p.x) || !matrix_from(w_in, device, p.in) || !matrix_from(w_out, device, p.out) ||
+      p.in.t->dim() != 2 || p.out.t->dim() != 2 || p.in.t->scalar_type() != p.x.t->scalar_type() ||
+      p.out.t->scalar_type() != p.x.t->scalar_type() || p.in.rows != p.x.cols || p.out.cols != p.x.cols ||
+      p.in.cols != 2 * p.out.rows || p.out.rows % 8)
+    return false;
+  p.dtype = code_of(p.x.t->scalar_type());
+  p.m = (int)p.x.rows;
+  p.width = (int)p.x.cols;
+  p.hidden = (int)p.out.rows;
+  return true;
+}
+
+// Workspace of one product; undefined where it needs none.
+int workspace(int product, int rows, int cols, int inner, int device, at::Tensor& ws, int64_t& bytes) {
+  bytes = 0;
+  const int st = flk_mlp_plan(product, rows, cols, inner, &bytes);
+  ws = st == FLK_OK && bytes ? empty({bytes}, at::kByte, device) : at::Tensor();
+  return st;
+}
+
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+int matmul(int product, const Matrix& a, const Matrix& b, int dtype, int rows, int cols, int inner, const at::Tensor& d,
+           int device) {
+  at::Tensor ws;
+  int64_t bytes;
+  const int st = workspace(product, rows, cols, inner, device, ws, bytes);
+  return st != FLK_OK ? st
+                      : flk_mlp_matmul(a.t->data_ptr(), a.stride, product == FLK_MLP_MATMUL_AT, b.t->data_ptr(), b.stride,
+                                       product == FLK_MLP_MATMUL_BT, dtype, rows, cols, inner, d.data_ptr(), cols, ptr(ws),
+                                       bytes, stream_of(device));
+}
+
+// gated_mlp(x, w_in, w_out, keep) -> (y, h, gu), h and gu None without keep; or None
+PyObject* gated_mlp(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const int device = n == 4 && PyBool_Check(a[3]) ? device_of(a[0]) : -1;
+  Mlp p;
+  if (device < 0 || !mlp_from(a[0], a[1], a[2], device, p)) return none();
+  const bool keep = a[3] == Py_True;
+  at::Tensor y, h, gu;
+  int st;
+  const char* what = "flk_mlp_gate";
+  {
+    pybind11::gil_scoped_release release;
+    const at::ScalarType dt = p.x.t->scalar_type();
+    y = empty(p.x.t->sizes(), dt, device);
+    h = empty({p.m, p.hidden}, dt, device);
+    if (keep) gu = empty({p.m, 2 * (int64_t)p.hidden}, at::kFloat, device);
+    at::Tensor ws;
+    int64_t bytes;
+    st = workspace(FLK_MLP_GATE, p.m, p.hidden, p.width, device, ws, bytes);
+    if (st == FLK_OK)
+      st = flk_mlp_gate(p.x.t->data_ptr(), p.x.stride, p.in.t->data_ptr(), p.in.stride, p.dtype, p.m, p.width, p.hidden,
+                        h.data_ptr(), p.hidden, static_cast<float*>(ptr(gu)), ptr(ws), bytes, stream_of(device));
+    if (st == FLK_OK) {
+      what = "flk_mlp_matmul";
+      st = matmul(FLK_MLP_MATMUL, Matrix{&h, p.m, p.hidden, p.hidden}, p.out, p.dtype, p.m, p.width, p.hidden, y, device);
+    }
+    if (!keep) h = at::Tensor();
+  }
+  return st == FLK_OK ? tuple_of({y, h, gu}) : failed(st, what);
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_mlp_backward(dy, x, w_in, w_out, h, gu) -> (dx, dw_in, dw_out) or None
+PyObject* gated_mlp_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const int device = n == 6 ? device_of(a[1]) : -1;
+  Mlp p;
+  Matrix dy;
+  if (device < 0 || !mlp_from(a[1], a[2], a[3], device, p) || !matrix_from(a[0], device, dy) ||
+      dy.t->sizes() != p.x.t->sizes() || dy.t->scalar_type() != p.x.t->scalar_type())
+    return none();
+  const at::Tensor* h = dense(a[4], device, p.x.t->scalar_type(), {p.m, p.hidden});
+  const at::Tensor* gu = dense(a[5], device, at::kFloat, {p.m, 2 * (int64_t)p.hidden});
+  if (!h || !gu) return none();
+  at::Tensor dx, dw_in, dw_out;
+  int st;
+  const char* what = "flk_mlp_gate_backward";
+  {
+    pybind11::gil_scoped_release release;
+    const at::ScalarType dt = p.x.t->scalar_type();
+    const int wide = 2 * p.hidden;
+    dx = empty(p.x.t->sizes(), dt, device);
+    dw_in = empty({p.width, wide}, dt, device);
+    dw_out = empty({p.hidden, p.width}, dt, device);
+    const at::Tensor dgu = empty({p.m, wide}, dt, device);
+    at::Tensor ws;
+    int64_t bytes;
+    st = workspace(FLK_MLP_GATE_BACKWARD, p.m, p.hidden, p.width, device, ws, bytes);
+    if (st == FLK_OK)
+      st = flk_mlp_gate_backward(dy.t->data_ptr(), dy.stride, p.out.t->data_ptr(), p.out.stride, gu->data_ptr<float>(),
+                                 p.dtype, p.m, p.width, p.hidden, dgu.data_ptr(), wide, ptr(ws), bytes, stream_of(device));
+    const Matrix d{&dgu, p.m, wide, wide};
+    if (st == FLK_OK) {
+      what = "flk_mlp_matmul";
+      st = matmul(FLK_MLP_MATMUL_AT, Matrix{h, p.m, p.hidden, p.hidden}, dy, p.dtype, p.hidden, p.width, p.m, dw_out, device);
+    }
+    if (st == FLK_OK) st = matmul(FLK_MLP_MATMUL_AT, p.x, d, p.dtype, p.width, wide, p.m, dw_in, device);
+    if (st == FLK_OK) st = matmul(FLK_MLP_MATMUL_BT, d, p.in, p.dtype, p.m, p.width, wide, dx, device);
+  }
+  return st == FLK_OK ? tuple_of({dx, dw_in, dw_out}) : failed(st, what);
+  END_HANDLE_TH_ERRORS
+}
+
 #define FLK_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FLK_METHOD(qk_prep), FLK_METHOD(attend_merged), FLK_METHOD(double_attention),
                          FLK_METHOD(linear), FLK_METHOD(layer_norm), FLK_METHOD(layer_norm_backward),
                          FLK_METHOD(modulate), FLK_METHOD(modulate_backward), FLK_METHOD(swiglu),
-                         FLK_METHOD(swiglu_backward), {nullptr, nullptr, 0, nullptr}};
+                         FLK_METHOD(swiglu_backward), FLK_METHOD(gated_mlp), FLK_METHOD(gated_mlp_backward),
+                         {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -138,6 +138,10 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, keep:
     """(silu(x @ w_g) * (x @ w_u)) @ w_out with w_in = [w_g | w_u]: x (..., width), w_in (width, 2 * hidden), w_out
     (hidden, width), all bfloat16 or all float16, widths multiples of 8 -> (..., width).  With ``keep`` also
     returns the ``Kept`` that gated_mlp_backward takes.  ``out`` must be contiguous."""
+    if out is None:
+        done = _native.gated_mlp(x, w_in, w_out, keep)
+        if done is not None:
+            return (done[0], Kept(done[1], done[2])) if keep else done[0]
     xr, w_in, w_out, width, hidden = _operands(x, w_in, w_out)
     m = xr.shape[0]
     out = _output(out, x.shape, x)
@@ -157,6 +161,9 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, keep:
 def gated_mlp_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, kept: Kept):
     """(dx, dw_in, dw_out) of ``gated_mlp(x, w_in, w_out, keep=True)`` for the incoming gradient dy and the
     ``kept`` that call returned."""
+    done = _native.gated_mlp_backward(dy, x, w_in, w_out, *kept)
+    if done is not None:
+        return done
     xr, wi, wo, width, hidden = _operands(x, w_in, w_out)
     m = xr.shape[0]
     if dy.shape != x.shape:

@@ -16,7 +16,7 @@ import torch
 
 from flicker_amd import _lib, autograd, mlp, modules, norm
 from oracle import mlp as M
-from tests.test_gpu_norm import TINY, _close, _f64, _gate_case
+from tests.test_gpu_norm import TINY, Declines, _close, _f64, _gate_case
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -335,3 +335,24 @@ def test_autograd_refuses_capture_with_gradients(device):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, norm.layer_norm(x, w.detach()))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("m,width,hidden", [(1, 256, 264), (77, 72, 136), (600, 64, 64)])
+def test_native_path_equals_the_python_path(device, monkeypatch, dtype, m, width, hidden):
+    """Plain calls take the native path, and have the Python path's values, shapes and types."""
+    x, dy, w_in, w_out = _operands(m, m, width, hidden, dtype, device)
+    wide = torch.zeros(hidden, width + 8, dtype=dtype, device=device)
+    wide[:, :width] = w_out
+    w_out = wide[:, :width]
+    x3, dy3 = x.view(1, m, width), dy.view(1, m, width)
+    taken = mlp._native.gated_mlp(x3, w_in, w_out, True)
+    assert taken is not None and mlp._native.gated_mlp(x3, w_in, w_out, False)[1:] == (None, None)
+    assert mlp._native.gated_mlp_backward(dy3, x3, w_in, w_out, *taken[1:]) is not None
+    y, kept = mlp.gated_mlp(x3, w_in, w_out, keep=True)
+    got = (y, *kept, mlp.gated_mlp(x3, w_in, w_out), *mlp.gated_mlp_backward(dy3, x3, w_in, w_out, kept))
+    monkeypatch.setattr(mlp, "_native", Declines())
+    y, kept = mlp.gated_mlp(x3, w_in, w_out, keep=True)
+    want = (y, *kept, mlp.gated_mlp(x3, w_in, w_out), *mlp.gated_mlp_backward(dy3, x3, w_in, w_out, kept))
+    for a, b in zip(got, want, strict=True):
+        assert a.shape == b.shape and a.dtype == b.dtype and a.is_contiguous() and torch.equal(a, b)
