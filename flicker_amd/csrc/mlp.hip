@@ -7,7 +7,22 @@
 // Each is D (rows, cols) = A B with float32 sums, computed transposed (D^T = B^T A^T: the MFMA's A
 // operand holds 16 columns of D, its B operand 16 rows), so that a lane ends with four neighbouring
 // columns of one row.  The gate's product takes g's and u's columns into one tile: a lane that holds
-// g of a column holds u of the same column, and h leaves the registers as the only output.
+// g of a column holds u of the same column, and h leaves the registers as the only output.  h, y, dgu
+// and the gradients are rounded once, to the operands' type, which the matrix cores take; g and u are kept in
+// float32 for the backward pass: rounded to 16 bits they would add 1.5 roundings to dg and du.
+//
+// What bounds them (4096 tokens, width 3 * 1024, hidden 9 * 1024, random bf16; times of one box):
+//   * Large products, the MFMA under the chip's power limit: gate 354 us (1.31 PFLOP/s), y 167 us
+//     (1.39), dWin 366 us (1.27); the same launches on constant operands take 20% less, at higher
+//     clocks.  A library product of 8192^3 reaches 1.37 on the same box.  Whole rounds of tiles count
+//     as much: 18 * 16 tiles of 256 x 256 on 256 CUs take two rounds for one and an eighth.
+//   * The gate's backward pass (294 us) and the forward pass that keeps g and u (404 us): also the
+//     float32 g and u, 302 MB each way, in the epilogue, which no MFMA of the same block covers.
+//   * 512 tokens: the weights' latency, one stage ahead (95 us with the weights in the caches, 134 without).
+//   * One token: HBM, the weights read once (42 us for 170 MB, two split products and two joins).
+// Timed and left: 192 x 192 tiles (no faster a column than 192 x 256), stages of 32 terms in three buffers
+// with two 256 x 128 blocks a CU (20% slower), fragment rings of 4 to 8 read 3 to 6 groups ahead
+// (all within 3%), barriers 2 to 4 groups before a stage's end (within 2%).
 
 #include <algorithm>
 #include <type_traits>
@@ -24,10 +39,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 template <int WN, int WM, int NF, int MF, int BUFFERS, int PER_CU, int RING, int LEAD, int BAR, int AHEAD>
 struct Geometry {
   static constexpr int kWN = WN, kWM = WM, kNF = NF, kMF = MF;
-  static constexpr int kAhead = AHEAD;
-  static constexpr int kRing = RING, kLead = LEAD, kBar = BAR;
   static constexpr int kBuffers = BUFFERS;   // stages in LDS
   static constexpr int kPerCU = PER_CU;      // blocks a CU holds
+  static constexpr int kRing = RING, kLead = LEAD, kBar = BAR;   // column fragments in flight, see mlp_kernel
+  static constexpr int kAhead = AHEAD;       // stages that a touch is ahead of the stage worked on (0: none)
   static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
   static constexpr int kTB = 16 * NF * WN, kTA = 16 * MF * WM;
 };
@@ -294,7 +309,9 @@ __global__ __launch_bounds__(G::kThreads, G::kThreads * G::kPerCU / 256) void ml
   HB hb;
   HA ha;
   const int64_t row0 = (int64_t)ta * kTA, col0 = (int64_t)tb * kTB;
-  // Blocks of a sweep share their row and column operands: each touches its share of both (kAhead).
+  // Blocks of a sweep share their row and column operands.  Each touches its share of both a little before
+  // all of them copy the lines, so that one miss serves all (forward and backward 2-4% faster at 4096
+  // and 16384 tokens; further ahead, or every block all of its lines, slower).  Sweeps of fewer rows gain nothing.
   const int share_b = min(kGroup, P.tiles_a), share_a = min(8, P.tiles_b);
   const int part_b = (kTB + share_b - 1) / share_b, part_a = (kTA + share_a - 1) / share_a;
   const int turn = (wave & 3) * 64, part = wave < 4 ? part_b : part_a;
@@ -350,11 +367,12 @@ __global__ __launch_bounds__(G::kThreads, G::kThreads * G::kPerCU / 256) void ml
 #pragma unroll
     for (int m = 0; m < kMF; ++m) acc[n][m] = f32x4{};
 
-  // kBuffers stages of two inner steps each.  Step 0 reads step 1's fragments as it goes; step 1 reads its
-  // own last column fragments, then -- every wave done reading the stage, the next one landed
-  // everywhere (the barrier) -- refills the stage's buffer with the stage kBuffers on and reads the
-  // next stage's first fragments.  After the last stage those reads take what is there; nothing uses it.
-  // Copies return in order: while `later` whole stages follow the awaited one, theirs may be in flight.
+  // kBuffers stages of two inner steps each.  Fragments are read from the stage as the groups before go; kBar
+  // groups before its end -- every wave done reading the stage, the next one landed everywhere (the
+  // barrier) -- the stage's buffer begins to take the stage kBuffers on, a copy instruction or two a
+  // group (all at once they fill the address units and stall the MFMAs: 4%), and the next stage's
+  // first fragments are read.  After the last stage those reads take what is there; nothing uses it.
+  // Copies return in order: while kLater whole stages follow the awaited one, theirs may be in flight.
   constexpr int kLater = kBuffers - 2;
   constexpr int kTouch = kGroups - kBar - 4;   // the touch follows the stage's copies
   constexpr int kSpread = (kCopies + kBar + kNF - 1) / (kBar + kNF);   // copy instructions a group
@@ -579,6 +597,8 @@ constexpr int kMaxDim = INT32_MAX - 256;
 constexpr int64_t kMaxStride = 1 << 22;   // 256 rows of one operand are addressed in 32 bits
 constexpr int64_t kMaxBlocks = 1 << 22;   // work-items of a launch are counted in 32 bits
 constexpr int kCUs = 256;
+// Outputs larger than this leave the caches alone (nontemporal): what follows reads them from HBM anyway, and
+// the operands stay.  4096 tokens, float32 g and u: 464 -> 404 us; at 65 MB the same costs 13%.
 constexpr int64_t kStreamBytes = 80 << 20;
 
 enum Tile { kLarge, kMedium, kSmall, kDeep, kFew, kTiles };

@@ -22,6 +22,14 @@
 // rows; blocks write them as partial rows, which a second kernel adds in a fixed order: the
 // gradients do not depend on timing.
 //
+// Measured (bf16, width 3 * 1024): forward 4 x 4096 rows in 46 us, 4.4 TB/s (a large copy's rate is 5.2), backward
+// 4608 rows in 27 us (85 MB of operands and 13 MB of partial rows, twice); 512 rows in 4.5 and 12 us, launches and
+// the latency of a few rows each.  What it took: a wave a row held 48 columns a lane and waited for its
+// 12 reductions with 2 waves a SIMD (65 and 176 us at 4 x 4096 rows); several waves a row that
+// each add up the others' values from LDS, one after the other, spend 1800 cycles a row on that
+// (53 and 94), where sixteen lanes take one wave's values each and add them by DPP (46 and 69).  Fetching
+// more than two rows ahead gains nothing; nor does a join of 16 columns a block.
+//
 // A row's last chunk starts 8 columns before its end, so that every load is a whole one; the columns that
 // it shares with the lane before are left out of its sums and stores.
 

@@ -5,7 +5,8 @@
 //
 // float32 arithmetic, each output rounded once.  HBM bounds it: three values move per output
 // forwards, five per pair of outputs backwards; a lane takes 8 columns of both halves, so
-// every access is 16 bytes (32 for float32) and neighbouring lanes' are adjacent.
+// every access is 16 bytes (32 for float32) and neighbouring lanes' are adjacent.  4608 x 9216 bf16 from a row of 27648:
+// forward 41-49 us (5.2-6.2 TB/s, as much of it as the caches hold), backward 84 us (5.0), a large copy's rate.
 
 #include "elems.h"
 
