@@ -199,6 +199,23 @@ def test_gated_mlp_shapes_and_views(device):
     assert torch.equal(mlp.gated_mlp(x[0], w_in, w_out), mlp.gated_mlp(x[:1], w_in, w_out)[0])
 
 
+def test_offsets_past_32_bits(device):
+    """The last tokens of a call whose g and u hold more than 2^31 values, on whole numbers (g and u exact)."""
+    m, width, hidden, last = 2 ** 17 + 300, 64, 8192 + 8, 300
+    x, w_in = _whole(1, (last, width), torch.bfloat16, device, 3), _whole(2, (width, 2 * hidden), torch.bfloat16, device, 1) * 2.0 ** -4
+    w_out, dy = _whole(3, (hidden, width), torch.bfloat16, device, 1) * 2.0 ** -6, _whole(4, (last, width), torch.bfloat16, device, 3)
+    big_x, big_dy = (torch.zeros(m, width, dtype=torch.bfloat16, device=device) for _ in range(2))
+    big_x[-last:], big_dy[-last:] = x, dy
+    y, kept = mlp.gated_mlp(big_x, w_in, w_out, keep=True)
+    want_y, want = mlp.gated_mlp(x, w_in, w_out, keep=True)
+    assert torch.equal(kept.gu[-last:], want.gu) and torch.equal(kept.h[-last:], want.h) and not kept.gu[:-last].any()
+    got = mlp.gated_mlp_backward(big_dy, big_x, w_in, w_out, kept)
+    exact = _mlp_case(*map(_f64, (x, dy, w_in, w_out)), torch.bfloat16)
+    assert not y[:-last].any() and not got[0][:-last].any()
+    for name, value in (("y", y[-last:]), ("dx", got[0][-last:]), ("dw_in", got[1]), ("dw_out", got[2])):
+        _close(name, value, *exact[name])
+
+
 def test_gated_mlp_not_finite(device):
     """A token's not-finite value stays in its row of y and dx, whatever rows share its tile."""
     x, dy, w_in, w_out = _operands(5, 40, 64, 64, torch.bfloat16, device)

@@ -325,6 +325,28 @@ def test_gradients_are_the_forward_pass_differences(device):
         assert abs(float((grad.double() * d.double()).sum()) - near) <= abs(far - near) + noise
 
 
+def test_offsets_past_32_bits(device):
+    """The last rows of tensors of more than 2^31 elements are those of a call on them alone."""
+    width, rows = 8192, 2 ** 18 + 700
+    part, g = _stream(8, 1, 700, width, torch.bfloat16, device)
+    x = torch.zeros(1, rows, width, dtype=torch.bfloat16, device=device)
+    x[:, -700:] = part
+    shift, scale = (torch.randn(1, width, generator=g).to(torch.bfloat16).to(device) for _ in range(2))
+    assert torch.equal(norm.modulate(x, shift, scale)[:, -700:], norm.modulate(part, shift, scale))
+    dx, dshift, dscale = norm.modulate_backward(x, x, shift, scale)
+    want = norm.modulate_backward(part, part, shift, scale)
+    assert torch.equal(dx[:, -700:], want[0]) and not dx[:, :-700].any()
+    # the other rows add zeros to the sums, in another order of float32 additions: 1e-4 of the terms' absolute sum
+    n = M._stats(_f64(part), norm.EPS)[0]
+    for got, exact, terms in ((dshift, want[1], np.abs(_f64(part))), (dscale, want[2], np.abs(_f64(part) * n))):
+        off = np.abs(_f64(got) - _f64(exact))[0]
+        assert (off <= 2.0 ** -7 * np.abs(_f64(exact))[0] + 1e-4 * terms[0].sum(0)).all()
+    h = mlp.swiglu(x)
+    assert torch.equal(h[:, -700:], mlp.swiglu(part)) and not h[:, :-700].any()
+    dgu = mlp.swiglu_backward(h, x)
+    assert torch.equal(dgu[:, -700:], mlp.swiglu_backward(mlp.swiglu(part), part)) and not dgu[:, :-700].any()
+
+
 class Declines:
     """A native call path that takes no call."""
 

@@ -141,6 +141,8 @@ def test_mlp_checks(lib):
     assert mm(rows=1, inner=0) == INVALID and mm(rows=1, x=None) == INVALID
     assert mm(rows=1, inner=60) == UNSUPPORTED and mm(rows=1, cols=124) == UNSUPPORTED
     assert mm(at=1, rows=60, xr=64) == UNSUPPORTED
+    assert mm(rows=1, xr=(1 << 22) + 8) == INVALID and mm(rows=1, wr=(1 << 22) + 8) == INVALID
+    assert gate(m=1, wr=(1 << 22) + 8) == INVALID and back(m=1, xr=(1 << 22) + 8) == INVALID
     assert mm(rows=1, xr=68) == ALIGN and mm(rows=1, w=P16 + 8) == ALIGN
     size = ctypes.c_int64(-1)
     for product in range(5):
