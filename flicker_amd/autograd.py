@@ -17,11 +17,15 @@ from . import norm as _norm
 from .kernels import EPS
 
 
-def _recorded(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) \
-            and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+def _not_captured() -> None:
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("flicker_amd.autograd is not captured into a graph with gradients: capture the explicit "
                            "forward and backward calls of flicker_amd.norm and flicker_amd.mlp")
+
+
+def _recorded(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _not_captured()
 
 
 def _first_only(backward):
@@ -31,6 +35,7 @@ def _first_only(backward):
     def run(ctx, *grads):
         if torch.is_grad_enabled():
             raise RuntimeError("flicker_amd.autograd has first derivatives only: create_graph=True is not supported")
+        _not_captured()
         return backward(ctx, *grads)
     return run
 
@@ -85,7 +90,7 @@ class _GatedMLP(torch.autograd.Function):
     @_first_only
     def backward(ctx, dy):
         x, w_in, w_out, h, gu = ctx.saved_tensors
-        return _mlp.gated_mlp_backward(dy, x, w_in, w_out, _mlp.Kept(h, gu))
+        return _mlp.gated_mlp_backward(dy, x, w_in, w_out, _mlp.Kept(h, gu), wanted=ctx.needs_input_grad)
 
 
 def layer_norm(x, weight=None, bias=None, *, eps: float = EPS) -> torch.Tensor:

@@ -158,12 +158,15 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, keep:
     return (out, Kept(h, gu)) if keep else out
 
 
-def gated_mlp_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, kept: Kept):
+def gated_mlp_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, kept: Kept, *,
+                       wanted: tuple[bool, bool, bool] = (True, True, True)):
     """(dx, dw_in, dw_out) of ``gated_mlp(x, w_in, w_out, keep=True)`` for the incoming gradient dy and the
-    ``kept`` that call returned."""
-    done = _native.gated_mlp_backward(dy, x, w_in, w_out, *kept)
-    if done is not None:
-        return done
+    ``kept`` that call returned.  Where ``wanted`` is false (frozen weights) a gradient is None, and its product
+    is not computed."""
+    if all(wanted):
+        done = _native.gated_mlp_backward(dy, x, w_in, w_out, *kept)
+        if done is not None:
+            return done
     xr, wi, wo, width, hidden = _operands(x, w_in, w_out)
     m = xr.shape[0]
     if dy.shape != x.shape:
@@ -174,18 +177,23 @@ def gated_mlp_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor, w_
         _on_gpu(f"kept.{name}", t)
         if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
             raise ValueError(f"kept.{name} must be contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx, dw_in, dw_out = (torch.empty(t.shape, dtype=x.dtype, device=x.device) if want else None
+                         for t, want in zip((x, w_in, w_out), wanted, strict=True))
     if m == 0:
-        return dx, torch.zeros(w_in.shape, dtype=x.dtype, device=x.device), \
-            torch.zeros(w_out.shape, dtype=x.dtype, device=x.device)
-    dw_in = torch.empty(w_in.shape, dtype=x.dtype, device=x.device)
-    dw_out = torch.empty(w_out.shape, dtype=x.dtype, device=x.device)
-    dgu = torch.empty((m, 2 * hidden), dtype=x.dtype, device=x.device)
-    ws, nbytes = _workspace(_GATE_BACKWARD, m, hidden, width, x.device)
-    _lib.run("flk_mlp_gate_backward", (gr, wo, gu, dgu, ws), gr.data_ptr(), gr.stride(0), wo.data_ptr(), wo.stride(0),
-             gu.data_ptr(), _dtype("x", x), m, width, hidden, dgu.data_ptr(), 2 * hidden, _lib.ptr(ws), nbytes,
-             _lib.stream_of(x))
-    _matmul(h, gr, dw_out, a_t=True)
-    _matmul(xr, dgu, dw_in, a_t=True)
-    _matmul(dgu, wi, dx.view(m, width), b_t=True)
+        for dw in (dw_in, dw_out):
+            if dw is not None:
+                dw.zero_()
+        return dx, dw_in, dw_out
+    if dx is not None or dw_in is not None:
+        dgu = torch.empty((m, 2 * hidden), dtype=x.dtype, device=x.device)
+        ws, nbytes = _workspace(_GATE_BACKWARD, m, hidden, width, x.device)
+        _lib.run("flk_mlp_gate_backward", (gr, wo, gu, dgu, ws), gr.data_ptr(), gr.stride(0), wo.data_ptr(),
+                 wo.stride(0), gu.data_ptr(), _dtype("x", x), m, width, hidden, dgu.data_ptr(), 2 * hidden, _lib.ptr(ws),
+                 nbytes, _lib.stream_of(x))
+    if dw_out is not None:
+        _matmul(h, gr, dw_out, a_t=True)
+    if dw_in is not None:
+        _matmul(xr, dgu, dw_in, a_t=True)
+    if dx is not None:
+        _matmul(dgu, wi, dx.view(m, width), b_t=True)
     return dx, dw_in, dw_out

@@ -231,6 +231,23 @@ def test_gated_mlp_not_finite(device):
     assert got[1].isnan().any()
 
 
+@pytest.mark.parametrize("wanted", [(True, False, False), (False, True, False), (False, False, True), (True, True, False),
+                                    (False, False, False)])
+def test_gated_mlp_wanted_gradients(device, wanted):
+    x, dy, w_in, w_out = _operands(6, 50, 64, 72, torch.bfloat16, device)
+    _, kept = mlp.gated_mlp(x, w_in, w_out, keep=True)
+    every = mlp.gated_mlp_backward(dy, x, w_in, w_out, kept)
+    for got, want, asked in zip(mlp.gated_mlp_backward(dy, x, w_in, w_out, kept, wanted=wanted), every, wanted, strict=True):
+        assert torch.equal(got, want) if asked else got is None
+    none = mlp.gated_mlp_backward(dy[:0], x[:0], w_in, w_out, mlp.Kept(kept.h[:0], kept.gu[:0]), wanted=wanted)
+    assert [t is not None for t in none] == list(wanted) and not any(t.any() for t in none if t is not None)
+    leaves = [t.clone().requires_grad_(a) for t, a in zip((x, w_in, w_out), wanted)]
+    if any(wanted):
+        autograd.gated_mlp(*leaves).backward(dy)
+        for leaf, want, asked in zip(leaves, every, wanted):
+            assert torch.equal(leaf.grad, want) if asked else leaf.grad is None
+
+
 def test_gated_mlp_refusals(device):
     x, dy, w_in, w_out = _operands(1, 4, 64, 72, torch.bfloat16, device)
     with pytest.raises(TypeError, match="bfloat16 or float16"):

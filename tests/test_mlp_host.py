@@ -161,3 +161,14 @@ def test_python_refuses_host_tensors_and_bad_calls():
             call()
     with pytest.raises(TypeError, match="torch.Tensor"):
         norm.layer_norm([1.0, 2.0])
+
+
+def test_autograd_refuses_a_captured_backward_pass(monkeypatch):
+    """A backward pass of an eager forward pass, under capture: refused before it computes anything."""
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="explicit"):
+        autograd._Swiglu.backward(None, None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    with torch.enable_grad(), pytest.raises(RuntimeError, match="first derivatives only"):
+        autograd._Swiglu.backward(None, None)
