@@ -11,14 +11,25 @@ struct Raw8 {
   T v[8];
 };
 
-// Eight elements at p, of which the first `count` exist (the rest read as zero).  The copy of a whole
-// chunk assumes no more than the element's own alignment; the target's unaligned access mode
-// makes it one 16-byte load (two for float32) all the same.
+// A whole chunk is read and written as 16-byte words (two for float32) that assume no more than a 16-bit
+// element's alignment: the target's unaligned access mode takes them as they are.
+typedef uint32_t word __attribute__((ext_vector_type(4), aligned(2), may_alias));
 template <typename T>
+constexpr int kWords = sizeof(Raw8<T>) / 16;
+
+// Eight elements at p, of which the first `count` exist (the rest read as zero).  kStream: the access leaves
+// the caches to others (nontemporal).
+template <bool kStream = false, typename T>
 __device__ __forceinline__ Raw8<T> load8(const T* p, int count) {
   Raw8<T> r;
   if (count >= 8) {
-    __builtin_memcpy(&r, p, sizeof(r));
+    word w[kWords<T>];
+#pragma unroll
+    for (int i = 0; i < kWords<T>; ++i) {
+      const word* at = reinterpret_cast<const word*>(p) + i;
+      w[i] = kStream ? __builtin_nontemporal_load(at) : *at;
+    }
+    __builtin_memcpy(&r, &w, sizeof(r));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.v[i] = i < count ? p[i] : (T)0.0f;
@@ -26,13 +37,22 @@ __device__ __forceinline__ Raw8<T> load8(const T* p, int count) {
   return r;
 }
 
-template <typename T>
+template <bool kStream = false, typename T>
 __device__ __forceinline__ void store8(T* p, int count, const float (&x)[8]) {
   Raw8<T> r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) r.v[i] = (T)x[i];
   if (count >= 8) {
-    __builtin_memcpy(p, &r, sizeof(r));
+    word w[kWords<T>];
+    __builtin_memcpy(&w, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < kWords<T>; ++i) {
+      word* at = reinterpret_cast<word*>(p) + i;
+      if constexpr (kStream)
+        __builtin_nontemporal_store(w[i], at);
+      else
+        *at = w[i];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)

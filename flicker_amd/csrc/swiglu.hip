@@ -42,20 +42,20 @@ __global__ __launch_bounds__(kThreads) void swiglu_kernel(const GateArgs A) {
     const int at = (in_row - ahead * A.chunks) * 8, left = A.hidden - at;
     const int64_t b = row / A.length, t = row - b * A.length;
     const T* gu = row_at<T>(A.gu, b, t) + at;
-    const flk::Raw8<T> g8 = flk::load8(gu, left), u8 = flk::load8(gu + A.hidden, left);
+    const flk::Raw8<T> g8 = flk::load8<true>(gu, left), u8 = flk::load8<true>(gu + A.hidden, left);
     T* out = row_at<T>(A.out, b, t) + at;
     float o0[8], o1[8];
     if constexpr (kBackward) {
-      const flk::Raw8<T> d8 = flk::load8(row_at<T>(A.dh, b, t) + at, left);
+      const flk::Raw8<T> d8 = flk::load8<true>(row_at<T>(A.dh, b, t) + at, left);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         flk::gate_backward((float)d8.v[i], (float)g8.v[i], (float)u8.v[i], o0[i], o1[i]);
-      flk::store8(out + A.hidden, left, o1);
+      flk::store8<true>(out + A.hidden, left, o1);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) o0[i] = flk::gate((float)g8.v[i], (float)u8.v[i]);
     }
-    flk::store8(out, left, o0);
+    flk::store8<true>(out, left, o0);
   }
 }
 
