@@ -25,13 +25,13 @@
 // y and dx are stored past the caches: 4608 rows forward 13.3 -> 11.0 us, and no slower a product that reads y
 // next; the rows read are not (13.3 -> 16.7: the last cache often has them), nor the partial rows, read again at once.
 //
-// Measured (bf16, width 3 * 1024): forward 4 x 4096 rows in 46 us, 4.4 TB/s (a large copy's rate is 5.2), backward
-// 4608 rows in 27 us (85 MB of operands and 13 MB of partial rows, twice); 512 rows in 4.5 and 12 us, launches and
-// the latency of a few rows each.  What it took: a wave a row held 48 columns a lane and waited for its
-// 12 reductions with 2 waves a SIMD (65 and 176 us at 4 x 4096 rows); several waves a row that
-// each add up the others' values from LDS, one after the other, spend 1800 cycles a row on that
-// (53 and 94), where sixteen lanes take one wave's values each and add them by DPP (46 and 69).  Fetching
-// more than two rows ahead gains nothing; nor does a join of 16 columns a block.
+// Measured (bf16, width 3 * 1024, among other passes): forward 4 x 4096 rows in 41.7 us, 4.8 TB/s (a large copy's
+// rate is 5.2), backward 4608 rows in 24.9 us (85 MB of operands, and 13 MB of partial rows written and read); 512
+// rows in 4.1 and 11 us, launches and the latency of a few rows each.  What it took, at 4 x 4096 rows: a wave a
+// row held 48 columns a lane and waited for its reductions with 2 waves a SIMD (65 us forward, 176
+// backward); several waves a row that each add up the others' values from LDS, one after the other, spend 1800
+// cycles a row on that (53, 94), where sixteen lanes take one wave's values each and add them by DPP (46, 69).
+// Fetching more than two rows ahead gains nothing; nor does a join of 16 columns a block.
 //
 // A row's last chunk starts 8 columns before its end, so that every load is a whole one; the columns that
 // it shares with the lane before are left out of its sums and stores.

@@ -5,8 +5,10 @@
 //
 // float32 arithmetic, each output rounded once.  HBM bounds it: three values move per output
 // forwards, five per pair of outputs backwards; a lane takes 8 columns of both halves, so
-// every access is 16 bytes (32 for float32) and neighbouring lanes' are adjacent.  4608 x 9216 bf16 from a row of 27648:
-// forward 41-49 us (5.2-6.2 TB/s, as much of it as the caches hold), backward 84 us (5.0), a large copy's rate.
+// every access is 16 bytes (32 for float32) and neighbouring lanes' are adjacent.  All of it passes the caches by
+// (nontemporal): operands and outputs are larger than they are, and smaller ones lose nothing.  4608 x 9216
+// bf16 from a row of 27648: forward 42 us (6.0 TB/s; 49 through the caches), backward 66 (6.4; 83); a large copy
+// reaches 5.2.
 
 #include "elems.h"
 
