@@ -6,7 +6,7 @@
 // float32 arithmetic, each output rounded once.  HBM bounds it: three values move per output
 // forwards, five per pair of outputs backwards; a lane takes 8 columns of both halves, so
 // every access is 16 bytes (32 for float32) and neighbouring lanes' are adjacent.  All of it passes the caches by
-// (nontemporal): operands and outputs are larger than they are, and smaller ones lose nothing.  4608 x 9216
+// (nontemporal): at the blocks' sizes operands and outputs are as large as they are.  4608 x 9216
 // bf16 from a row of 27648: forward 42 us (6.0 TB/s; 49 through the caches), backward 66 (6.4; 83); a large copy
 // reaches 5.2.
 
