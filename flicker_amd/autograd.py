@@ -1,6 +1,7 @@
 """``norm`` and ``mlp`` under torch's autograd: the same functions, differentiable.
 
-Each call records the matching ``*_backward`` call; first derivatives only.  They are not captured into a HIP
+Each call records the matching ``*_backward`` call; first derivatives only, and no forward mode (an operand
+with a tangent raises NotImplementedError).  They are not captured into a HIP
 graph with gradients: autograd accumulates into a leaf on the stream of whichever graph of that leaf is
 alive, which need not be the captured one, so such a call is refused -- capture the explicit forward
 and backward calls of ``norm`` and ``mlp`` instead, which touch no leaves.
@@ -23,9 +24,12 @@ def _not_captured() -> None:
                            "forward and backward calls of flicker_amd.norm and flicker_amd.mlp")
 
 
-def _recorded(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _recorded(*tensors) -> bool:
+    """Whether autograd records a call on these operands."""
+    recorded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if recorded:
         _not_captured()
+    return recorded
 
 
 def _first_only(backward):
@@ -81,7 +85,9 @@ class _Swiglu(torch.autograd.Function):
 
 class _GatedMLP(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_in, w_out):
+    def forward(ctx, x, w_in, w_out, keep):
+        if not keep:
+            return _mlp.gated_mlp(x, w_in, w_out)
         y, kept = _mlp.gated_mlp(x, w_in, w_out, keep=True)
         ctx.save_for_backward(x, w_in, w_out, *kept)
         return y
@@ -90,7 +96,7 @@ class _GatedMLP(torch.autograd.Function):
     @_first_only
     def backward(ctx, dy):
         x, w_in, w_out, h, gu = ctx.saved_tensors
-        return _mlp.gated_mlp_backward(dy, x, w_in, w_out, _mlp.Kept(h, gu), wanted=ctx.needs_input_grad)
+        return *_mlp.gated_mlp_backward(dy, x, w_in, w_out, _mlp.Kept(h, gu), wanted=ctx.needs_input_grad[:3]), None
 
 
 def layer_norm(x, weight=None, bias=None, *, eps: float = EPS) -> torch.Tensor:
@@ -114,7 +120,4 @@ def swiglu(gu) -> torch.Tensor:
 def gated_mlp(x, w_in, w_out) -> torch.Tensor:
     """mlp.gated_mlp, differentiable in x, w_in and w_out; keeps what the backward pass needs only where one
     of them requires a gradient."""
-    _recorded(x, w_in, w_out)
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_in, w_out))):
-        return _mlp.gated_mlp(x, w_in, w_out)
-    return _GatedMLP.apply(x, w_in, w_out)
+    return _GatedMLP.apply(x, w_in, w_out, _recorded(x, w_in, w_out))

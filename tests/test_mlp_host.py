@@ -172,3 +172,24 @@ def test_autograd_refuses_a_captured_backward_pass(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     with torch.enable_grad(), pytest.raises(RuntimeError, match="first derivatives only"):
         autograd._Swiglu.backward(None, None)
+
+
+def test_autograd_refuses_forward_mode(monkeypatch):
+    """An operand with a tangent, with and without recorded gradients beside it: no result without its tangent."""
+    import torch.autograd.forward_ad as fwd
+    monkeypatch.setattr(autograd._norm, "layer_norm", lambda x, w, b, eps: x * 2)
+    monkeypatch.setattr(autograd._norm, "modulate", lambda x, shift, scale, eps: x * 2)
+    monkeypatch.setattr(autograd._mlp, "swiglu", lambda gu: gu[..., :4] * 2)
+    monkeypatch.setattr(autograd._mlp, "gated_mlp", lambda x, w_in, w_out, keep=False:
+                        (x * 2, mlp.Kept(x[:, :1], x[:, :1])) if keep else x * 2)
+    x, w_in, w_out = torch.randn(3, 8), torch.randn(8, 16), torch.randn(8, 8)
+    assert torch.equal(autograd.gated_mlp(x, w_in, w_out), x * 2)
+    assert not autograd.gated_mlp(x, w_in, w_out).requires_grad
+    assert autograd.gated_mlp(x, w_in.requires_grad_(), w_out).requires_grad
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: autograd.layer_norm(dual), lambda: autograd.modulate(dual, x, x), lambda: autograd.swiglu(dual),
+                     lambda: autograd.gated_mlp(dual, w_in, w_out), lambda: autograd.gated_mlp(dual, w_in.detach(), w_out),
+                     lambda: autograd.gated_mlp(x, w_in.detach(), fwd.make_dual(w_out, torch.ones_like(w_out)))):
+            with pytest.raises(NotImplementedError):
+                call()
