@@ -354,7 +354,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void norm_params_kernel(const floa
 
 constexpr int kMaxWidth = 2 * kMaxWaves * 512;
 constexpr int kMaxRows = INT32_MAX;
-constexpr int64_t kMaxBlocks = 1 << 22;   // a launch's work-items are counted in 32 bits
+constexpr int kMaxGroups = 1 << 22;       // batch entries with parameters of their own
+constexpr int64_t kMaxItems = 1LL << 31;  // of one launch, whose work-items are counted in 32 bits
 
 // Rows a block walks.  Of the numbers of blocks a CU that keep up to `waves` waves on it, the one whose CUs
 // all get nearly the same number of rows, and then the largest; `least` rows a block at any rate.
@@ -379,19 +380,56 @@ int backward_rows(int64_t group_rows, int64_t groups, int width) {
   return rows_per_block(group_rows, groups, width, 12, (int)std::min<int64_t>(4, 1 + group_rows * groups / 128));
 }
 
+// Threads of a block.
+int threads_of(int width) { return width <= 512 ? 256 : std::min(((width + 7) / 8 + 63) / 64, kMaxWaves) * 64; }
+
+// Group g's rows and parameters.
+template <typename T, typename P>
+NormArgs from_group(NormArgs a, int64_t g) {
+  if (g == 0) return a;   // the only one where the groups are not batch entries
+  for (Rows* r : {&a.x, &a.dy, &a.y})
+    if (r->p) r->p = static_cast<const T*>(r->p) + g * r->batch_stride;
+  for (const void** p : {&a.factor, &a.offset})
+    if (*p) *p = static_cast<const P*>(*p) + g * a.param_stride;
+  if (a.partial) a.partial += g * a.blocks_per_group * 2 * a.width;
+  return a;
+}
+
 template <typename T, typename P, bool kBackward>
-int dispatch(const NormArgs& a, int64_t groups, hipStream_t s) {
-  const dim3 grid((unsigned)(groups * a.blocks_per_group));
-  const int chunks = (a.width + 7) / 8;
-  if (a.width < 8)
-    norm_kernel<T, P, 1, true, true, kBackward><<<grid, 256, 0, s>>>(a);
-  else if (a.width <= 512)
-    norm_kernel<T, P, 1, true, false, kBackward><<<grid, 256, 0, s>>>(a);
-  else if (a.width <= 512 * kMaxWaves)
-    norm_kernel<T, P, 1, false, false, kBackward><<<grid, (chunks + 63) / 64 * 64, 0, s>>>(a);
-  else
-    norm_kernel<T, P, 2, false, false, kBackward><<<grid, 64 * kMaxWaves, 0, s>>>(a);
-  return flk_launch_status();
+int dispatch(const NormArgs& all, int64_t groups, hipStream_t s) {
+  const int threads = threads_of(all.width);
+  const int64_t most = kMaxItems / threads / all.blocks_per_group;   // groups of one launch
+  for (int64_t first = 0; first < groups; first += most) {
+    const NormArgs a = from_group<T, P>(all, first);
+    const dim3 grid((unsigned)(std::min(most, groups - first) * a.blocks_per_group));
+    if (a.width < 8)
+      norm_kernel<T, P, 1, true, true, kBackward><<<grid, threads, 0, s>>>(a);
+    else if (a.width <= 512)
+      norm_kernel<T, P, 1, true, false, kBackward><<<grid, threads, 0, s>>>(a);
+    else if (a.width <= 512 * kMaxWaves)
+      norm_kernel<T, P, 1, false, false, kBackward><<<grid, threads, 0, s>>>(a);
+    else
+      norm_kernel<T, P, 2, false, false, kBackward><<<grid, threads, 0, s>>>(a);
+    if (const int st = flk_launch_status()) return st;
+  }
+  return FLK_OK;
+}
+
+template <typename P>
+int join_params(const NormArgs& a, int64_t groups, void* dfactor, void* doffset, hipStream_t s) {
+  const int cuts = (a.width + 63) / 64;
+  const int64_t most = kMaxItems / (64 * kJoinWaves) / cuts;
+  for (int64_t first = 0; first < groups; first += most) {
+    const dim3 grid((unsigned)(std::min(most, groups - first) * cuts), 2);
+    P* df = static_cast<P*>(dfactor);
+    P* dc = static_cast<P*>(doffset);
+    norm_params_kernel<P><<<grid, 64 * kJoinWaves, 0, s>>>(a.partial + first * a.blocks_per_group * 2 * a.width,
+                                                           a.blocks_per_group, a.width, cuts,
+                                                           df ? df + first * a.width : nullptr,
+                                                           dc ? dc + first * a.width : nullptr);
+    if (const int st = flk_launch_status()) return st;
+  }
+  return FLK_OK;
 }
 
 template <bool kBackward>
@@ -415,7 +453,7 @@ int check(int dtype, int params, const void* x, const void* y, const void* facto
   if (dtype < FLK_BF16 || dtype > FLK_F32 || params < FLK_BF16 || params > FLK_F32) return FLK_E_INVALID;
   if (batch < 0 || length < 0 || width <= 0 || !(eps >= 0.0f) || param_stride < 0) return FLK_E_INVALID;
   if (param_stride && param_stride < width) return FLK_E_INVALID;
-  if ((int64_t)batch * length > kMaxRows) return FLK_E_INVALID;
+  if ((int64_t)batch * length > kMaxRows || (param_stride && batch > kMaxGroups)) return FLK_E_INVALID;
   if (width > kMaxWidth) return FLK_E_UNSUPPORTED;
   if (batch == 0 || length == 0) return FLK_OK;
   if (!x || !y) return FLK_E_INVALID;
@@ -456,14 +494,13 @@ extern "C" int flk_layer_norm(const void* x, int64_t x_batch_stride, int64_t x_r
   const int64_t groups = param_batch_stride ? batch : 1;
   a.per_block = forward_rows(a.group_rows, groups, width);
   a.blocks_per_group = (int)((a.group_rows + a.per_block - 1) / a.per_block);
-  if (groups * a.blocks_per_group > kMaxBlocks) return FLK_E_INVALID;
   return dispatch_types<false>(dtype, params_dtype, a, groups, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int flk_layer_norm_backward_plan(int batch, int length, int width, int shared_params,
                                             int64_t* workspace_bytes) {
   if (batch < 0 || length < 0 || width <= 0 || !workspace_bytes) return FLK_E_INVALID;
-  if ((int64_t)batch * length > kMaxRows) return FLK_E_INVALID;
+  if ((int64_t)batch * length > kMaxRows || (!shared_params && batch > kMaxGroups)) return FLK_E_INVALID;
   *workspace_bytes = 0;
   if (batch == 0 || length == 0) return FLK_OK;
   const int64_t groups = shared_params ? 1 : batch, group_rows = shared_params ? (int64_t)batch * length : length;
@@ -491,8 +528,6 @@ extern "C" int flk_layer_norm_backward(const void* dy, int64_t dy_batch_stride, 
   const int64_t groups = param_batch_stride ? batch : 1;
   a.per_block = backward_rows(a.group_rows, groups, width);
   a.blocks_per_group = (int)((a.group_rows + a.per_block - 1) / a.per_block);
-  const int cuts = (width + 63) / 64;
-  if (groups * a.blocks_per_group > kMaxBlocks || groups * cuts > kMaxBlocks) return FLK_E_INVALID;
   if (dfactor || doffset) {
     const int64_t need = groups * a.blocks_per_group * 2 * width * 4;
     if (!workspace || workspace_bytes < need) return FLK_E_SCRATCH;
@@ -502,16 +537,7 @@ extern "C" int flk_layer_norm_backward(const void* dy, int64_t dy_batch_stride, 
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (const int st = dispatch_types<true>(dtype, params_dtype, a, groups, s)) return st;
   if (!a.partial) return FLK_OK;
-  const dim3 grid((unsigned)(groups * cuts), 2);
-  if (params_dtype == FLK_F32)
-    norm_params_kernel<float><<<grid, 64 * kJoinWaves, 0, s>>>(a.partial, a.blocks_per_group, width, cuts,
-                                                        static_cast<float*>(dfactor), static_cast<float*>(doffset));
-  else if (params_dtype == FLK_BF16)
-    norm_params_kernel<__bf16><<<grid, 64 * kJoinWaves, 0, s>>>(a.partial, a.blocks_per_group, width, cuts,
-                                                         static_cast<__bf16*>(dfactor), static_cast<__bf16*>(doffset));
-  else
-    norm_params_kernel<_Float16><<<grid, 64 * kJoinWaves, 0, s>>>(a.partial, a.blocks_per_group, width, cuts,
-                                                           static_cast<_Float16*>(dfactor),
-                                                           static_cast<_Float16*>(doffset));
-  return flk_launch_status();
+  if (params_dtype == FLK_F32) return join_params<float>(a, groups, dfactor, doffset, s);
+  if (params_dtype == FLK_BF16) return join_params<__bf16>(a, groups, dfactor, doffset, s);
+  return join_params<_Float16>(a, groups, dfactor, doffset, s);
 }

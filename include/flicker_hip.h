@@ -412,7 +412,8 @@ int flk_w8a8_qk_prep_pair(const int8_t* xq0, const int8_t* wq_t0, const float* a
  *            b*batch_stride + t*row_stride + j, strides in elements, any of them
  *   factor, offset  (width,) rows of type params_dtype (dtype itself or FLK_F32), one per batch
  *            entry at b*param_batch_stride, or one for all (stride 0); NULL: a = 1, c = 0
- * y may be x.  Any alignment of whole elements; width at most 16384. */
+ * y may be x.  Any alignment of whole elements; width at most 16384 (else FLK_E_UNSUPPORTED), batch * length at
+ * most 2^31 - 1 and, with a row of parameters per batch entry, batch at most 2^22 (else FLK_E_INVALID). */
 int flk_layer_norm(const void* x, int64_t x_batch_stride, int64_t x_row_stride, int dtype, const void* factor,
                    const void* offset, int params_dtype, int64_t param_batch_stride, int add_one, float eps, int batch,
                    int length, int width, void* y, int64_t y_batch_stride, int64_t y_row_stride, void* stream);

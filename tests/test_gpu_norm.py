@@ -122,6 +122,36 @@ def test_many_rows(device):
         _close(label, got, *want)
 
 
+def test_more_parameter_rows_than_one_launch_takes(device):
+    """Per-token modulation of many tokens: every entry's outputs are those of a call on fewer entries."""
+    batch, width, part = 65536 + 3, 4096, 16384
+    g = torch.Generator(device).manual_seed(12)
+    x, dy, shift, scale = (torch.randn(batch, 1, width, generator=g, device=device, dtype=torch.bfloat16) for _ in range(4))
+    print(f"modulate batch={batch} width={width}", flush=True)
+    y = norm.modulate(x, shift, scale)
+    print(f"modulate_backward batch={batch} width={width}", flush=True)
+    grads = norm.modulate_backward(dy, x, shift, scale)
+    assert torch.equal(grads[1], dy)   # a sum of one row
+    for at in range(0, batch, part):
+        s = slice(at, at + part)
+        assert torch.equal(y[s], norm.modulate(x[s], shift[s], scale[s]))
+        for got, want in zip(grads, norm.modulate_backward(dy[s], x[s], shift[s], scale[s])):
+            assert torch.equal(got[s], want)
+
+
+def test_most_batch_entries(device):
+    """2^22 entries with blocks of 576 threads, more work-items than one launch takes, of one row and no parameters."""
+    from flicker_amd import _lib
+    batch, width = 1 << 22, 4104
+    x = torch.randn(1, width, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(device)
+    want = norm.layer_norm(x)
+    y = torch.zeros(batch, width, dtype=torch.bfloat16, device=device)
+    print(f"flk_layer_norm batch={batch} width={width}", flush=True)
+    _lib.run("flk_layer_norm", (x, y), x.data_ptr(), 0, width, 0, None, None, 0, width, 0, 1e-6, batch, 1, width, y.data_ptr(),
+             width, width, _lib.stream_of(x))
+    assert all(bool((part == want).all()) for part in y.split(1 << 18))
+
+
 def test_optional_parameters(device):
     x, g = _stream(7, 2, 5, 72, torch.float32, device)
     w, b = torch.randn(72, generator=g).to(device), torch.randn(72, generator=g).to(device)

@@ -102,6 +102,24 @@ def test_layer_norm_backward_checks(lib):
     assert lib.flk_layer_norm_backward_plan(1, 4, 8, 0, None) == INVALID
 
 
+def test_norm_batch_limits(lib):
+    """Each side of the limit on parameter rows, before anything is launched: the plan and the launch agree, and
+    no product of batch and width is in the way."""
+    most = 1 << 22
+    size = ctypes.c_int64(-1)
+    for batch, width, status in ((65535, 4096, OK), (65536, 4096, OK), (65537, 4096, OK), (most, 64, OK), (most, 16384, OK),
+                                 (most + 1, 64, INVALID)):
+        assert lib.flk_layer_norm_backward_plan(batch, 1, width, 0, ctypes.byref(size)) == status
+        assert status != OK or size.value >= batch * 2 * width * 4
+        # a workspace of no bytes is the last thing that is refused
+        assert _norm_backward(lib, batch=batch, length=1, width=width, pstride=width, nbytes=0) == (SCRATCH if status == OK else status)
+    assert _norm(lib, batch=most + 1, length=1) == INVALID
+    assert _norm(lib, batch=most, length=0) == OK
+    # one row of parameters for all entries: no limit but the rows'
+    assert lib.flk_layer_norm_backward_plan(most + 1, 1, 64, 1, ctypes.byref(size)) == OK
+    assert _norm_backward(lib, batch=most + 1, length=1, pstride=0, nbytes=0) == SCRATCH
+
+
 def test_swiglu_checks(lib):
     def call(dtype=BF16, batch=0, length=3, hidden=5, gu=P16, h=P16):
         return lib.flk_swiglu(gu, 0, 10, dtype, batch, length, hidden, h, 0, 5, None)
