@@ -27,6 +27,7 @@ from .kernels import _native, _on_gpu
 from .norm import _blocks, _dtype, _out_blocks, _output, _strides
 
 _GATE, _GATE_BACKWARD, _MATMUL, _MATMUL_BT, _MATMUL_AT = range(5)   # FLK_MLP_*
+_MAX_STRIDE = 1 << 22   # elements between two rows of an operand of the products
 
 
 class Kept(NamedTuple):
@@ -80,7 +81,8 @@ def swiglu_backward(dh: torch.Tensor, gu: torch.Tensor, *, out: torch.Tensor | N
 
 
 def _matrix(name: str, t: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
-    """A 2-D view with a contiguous last axis and 16-byte aligned rows (a copy where t has none)."""
+    """A 2-D view with a contiguous last axis and 16-byte aligned rows at most _MAX_STRIDE apart (a copy where t
+    has none)."""
     _on_gpu(name, t)
     if t.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
@@ -89,7 +91,7 @@ def _matrix(name: str, t: torch.Tensor, dtype: torch.dtype | None = None) -> tor
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     row = t.stride(0)
-    if t.stride(1) != 1 or row % 8 or row < t.shape[1] or t.data_ptr() % 16:
+    if t.stride(1) != 1 or row % 8 or not t.shape[1] <= row <= _MAX_STRIDE or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 

@@ -199,6 +199,21 @@ def test_gated_mlp_shapes_and_views(device):
     assert torch.equal(mlp.gated_mlp(x[0], w_in, w_out), mlp.gated_mlp(x[:1], w_in, w_out)[0])
 
 
+def test_rows_far_apart(device):
+    """Each image's first token in place, whose rows are more than 2^22 elements apart."""
+    x, dy, w_in, w_out = _operands(11, 3, 64, 72, torch.bfloat16, device)
+    long = torch.zeros(2, 3, 2 ** 16 + 1, 64, dtype=torch.bfloat16, device=device)
+    far_x, far_dy = long[0, :, 0], long[1, :, 0]
+    far_x.copy_(x)
+    far_dy.copy_(dy)
+    want, kept = mlp.gated_mlp(x, w_in, w_out, keep=True)
+    y, far_kept = mlp.gated_mlp(far_x, w_in, w_out, keep=True)
+    assert torch.equal(y, want)
+    for got, exact in zip(mlp.gated_mlp_backward(far_dy, far_x, w_in, w_out, far_kept),
+                          mlp.gated_mlp_backward(dy, x, w_in, w_out, kept)):
+        assert torch.equal(got, exact)
+
+
 def test_offsets_past_32_bits(device):
     """The last tokens of a call whose g and u hold more than 2^31 values, on whole numbers (g and u exact)."""
     m, width, hidden, last = 2 ** 17 + 300, 64, 8192 + 8, 300

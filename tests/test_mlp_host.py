@@ -169,6 +169,21 @@ def test_mlp_checks(lib):
     assert lib.flk_mlp_plan(0, -1, 8, 8, ctypes.byref(size)) == INVALID and lib.flk_mlp_plan(0, 1, 8, 8, None) == INVALID
 
 
+def test_operand_layouts_of_the_products(lib, monkeypatch):
+    """Rows further apart than the products address, or off 16 bytes, are copied; others are read in place."""
+    monkeypatch.setattr(mlp, "_on_gpu", lambda name, t: None)
+    most = 1 << 22
+    memory = torch.zeros(2 * most + 64, dtype=torch.bfloat16)
+    for row, offset, taken in ((most, 0, True), (most + 8, 0, False), (64, 0, True), (68, 0, False), (64, 4, False)):
+        t = memory[offset:].as_strided((2, 64), (row, 1))
+        t[1, 63] = 3.0
+        m = mlp._matrix("x", t)
+        assert torch.equal(m, t) and m.stride(1) == 1 and (m.data_ptr() == t.data_ptr()) == taken
+        assert lib.flk_mlp_matmul(P16, m.stride(0), 0, P16, 8, 0, BF16, 0, 8, 64, P16, 8, None, 0, None) == OK
+    first = torch.zeros(3, most // 64 + 1, 64, dtype=torch.bfloat16)[:, 0]   # each image's first token
+    assert mlp._matrix("x", first).stride(0) == 64
+
+
 def test_python_refuses_host_tensors_and_bad_calls():
     x = torch.zeros(2, 3, 16, dtype=torch.bfloat16)
     for call in (lambda: norm.layer_norm(x), lambda: norm.modulate(x, x[:, 0], x[:, 0]), lambda: mlp.swiglu(x),
