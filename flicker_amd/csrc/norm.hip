@@ -141,7 +141,8 @@ __device__ __forceinline__ Stats join(const f32x4& own, float columns, const Nor
     }
     turn ^= 1;
   }
-  return Stats{mean, __builtin_amdgcn_rsqf(square * A.inv_width + A.eps), t, tx};
+  // rsqrtf, not the bare instruction, which takes the subnormal variances that eps = 0 lets through for zero
+  return Stats{mean, rsqrtf(square * A.inv_width + A.eps), t, tx};
 }
 
 // A block's rows: slot's of every kSlots, first .. end - 1 of a group.

@@ -180,6 +180,26 @@ def test_eps_and_constant_rows(device):
             _close(label, got, *want)
 
 
+@pytest.mark.parametrize("width", [64, 1024, 16384])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_small_variance_without_eps(device, width, dtype):
+    """Rows of +-2^-66, whose squares and variance are float32 subnormals (2^-132, exact): n is exactly +-1, and
+    with dy = n / 2 + 1 (+ 1 on the first half) every mean that dx takes is a sum of few powers of two."""
+    sign = torch.ones(width, device=device)
+    sign[1::2] = -1.0
+    x = (sign * 2.0 ** -66).to(TYPES[dtype]).repeat(3, 1)
+    assert torch.equal(norm.layer_norm(x, eps=0.0), sign.to(x.dtype).repeat(3, 1))
+    dy = (sign / 2 + 1).repeat(3, 1)
+    dy[:, :width // 2] += 1.0
+    dy = dy.to(x.dtype)
+    one = torch.ones(width, dtype=x.dtype, device=device)
+    dx, dw, db = norm.layer_norm_backward(dy, x, one, one, eps=0.0)
+    half = torch.full((3, width), -0.5, device=device)   # dy - mean dy - n mean(dy n)
+    half[:, :width // 2] = 0.5
+    assert torch.equal(dx, (half * 2.0 ** 66).to(x.dtype))
+    assert torch.equal(dw, (3 * dy[0].float() * sign).to(x.dtype)) and torch.equal(db, (3 * dy[0].float()).to(x.dtype))
+
+
 def test_not_finite_values_stay_in_their_rows(device):
     x = torch.randn(1, 6, 80, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(device)
     clean = norm.layer_norm(x)
