@@ -22,8 +22,9 @@
 // rows; blocks write them as partial rows, which a second kernel adds in a fixed order: the
 // gradients do not depend on timing.
 //
-// y and dx are stored past the caches: 4608 rows forward 13.3 -> 11.0 us, and no slower a product that reads y
-// next; the rows read are not (13.3 -> 16.7: the last cache often has them), nor the partial rows, read again at once.
+// 16-bit y and dx are stored past the caches: 4608 rows forward 13.3 -> 11.0 us, and no slower a product that reads y
+// next (float32: see kStreamBytes); the rows read are not (13.3 -> 16.7: the last cache often has them), nor the
+// partial rows, read again at once.
 //
 // Measured (bf16, width 3 * 1024, among other passes): forward 4 x 4096 rows in 41.7 us, 4.8 TB/s (a large copy's
 // rate is 5.2), backward 4608 rows in 24.9 us (85 MB of operands, and 13 MB of partial rows written and read); 512
@@ -165,8 +166,9 @@ struct Walk {
   }
 };
 
-// kOne: a wave takes a row alone, kSlots rows a block; otherwise all of the block's waves take one.
-template <typename T, typename P, int kV, bool kOne, bool kNarrow, bool kBackward>
+// kOne: a wave takes a row alone, kSlots rows a block; otherwise all of the block's waves take one.  kStream: y and
+// dx leave the caches to others (nontemporal).
+template <typename T, typename P, int kV, bool kOne, bool kNarrow, bool kBackward, bool kStream>
 __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const NormArgs A) {
   constexpr int kSlots = kOne ? 4 : 1;
   __shared__ Exchange ex;
@@ -284,7 +286,7 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
           out[i] = n * a[c][i] + o[c][i];
         }
       }
-      chunks.template store<true>(y, c, width, out);
+      chunks.template store<kStream>(y, c, width, out);
     }
   };
   for (int64_t r = walk.first; r < walk.end; r += kDepth * kSlots) {
@@ -356,6 +358,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void norm_params_kernel(const floa
 constexpr int kMaxWidth = 2 * kMaxWaves * 512;
 constexpr int kMaxRows = INT32_MAX;
 constexpr int kMaxGroups = 1 << 22;       // batch entries with parameters of their own
+// Float32 outputs up to this size pass the caches by, as 16-bit ones of any size do: 1200 x 24 * 128 forward 7.0 us
+// (through the caches 8.2), backward 15.8 (16.4).  Larger ones do not: 2048 rows 10.5 and 21.4 us (past the caches
+// 11.0 and 22.4), with what reads the output next 19.7 and 29.3 (21.0 and 32.3); 16384 x 1000 47 and 70 (56 and 78).
+constexpr int64_t kStreamBytes = 18 << 20;
 constexpr int64_t kMaxItems = 1LL << 31;  // of one launch, whose work-items are counted in 32 bits
 
 // Rows a block walks.  Of the numbers of blocks a CU that keep up to `waves` waves on it, the one whose CUs
@@ -396,24 +402,31 @@ NormArgs from_group(NormArgs a, int64_t g) {
   return a;
 }
 
-template <typename T, typename P, bool kBackward>
-int dispatch(const NormArgs& all, int64_t groups, hipStream_t s) {
+template <typename T, typename P, bool kBackward, bool kStream>
+int launch(const NormArgs& all, int64_t groups, hipStream_t s) {
   const int threads = threads_of(all.width);
   const int64_t most = kMaxItems / threads / all.blocks_per_group;   // groups of one launch
   for (int64_t first = 0; first < groups; first += most) {
     const NormArgs a = from_group<T, P>(all, first);
     const dim3 grid((unsigned)(std::min(most, groups - first) * a.blocks_per_group));
     if (a.width < 8)
-      norm_kernel<T, P, 1, true, true, kBackward><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 1, true, true, kBackward, kStream><<<grid, threads, 0, s>>>(a);
     else if (a.width <= 512)
-      norm_kernel<T, P, 1, true, false, kBackward><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 1, true, false, kBackward, kStream><<<grid, threads, 0, s>>>(a);
     else if (a.width <= 512 * kMaxWaves)
-      norm_kernel<T, P, 1, false, false, kBackward><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 1, false, false, kBackward, kStream><<<grid, threads, 0, s>>>(a);
     else
-      norm_kernel<T, P, 2, false, false, kBackward><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 2, false, false, kBackward, kStream><<<grid, threads, 0, s>>>(a);
     if (const int st = flk_launch_status()) return st;
   }
   return FLK_OK;
+}
+
+template <typename T, typename P, bool kBackward>
+int dispatch(const NormArgs& a, int64_t groups, hipStream_t s) {
+  if constexpr (sizeof(T) == 4)
+    if (a.group_rows * groups * a.width * 4 > kStreamBytes) return launch<T, P, kBackward, false>(a, groups, s);
+  return launch<T, P, kBackward, true>(a, groups, s);
 }
 
 template <typename P>

@@ -5,10 +5,12 @@
 //
 // float32 arithmetic, each output rounded once.  HBM bounds it: three values move per output
 // forwards, five per pair of outputs backwards; a lane takes 8 columns of both halves, so
-// every access is 16 bytes (32 for float32) and neighbouring lanes' are adjacent.  All of it passes the caches by
-// (nontemporal): at the blocks' sizes operands and outputs are as large as they are.  4608 x 9216
+// every access is 16 bytes (32 for float32) and neighbouring lanes' are adjacent.  16-bit operands and outputs
+// pass the caches by (nontemporal): at the blocks' sizes they are as large as the caches.  4608 x 9216
 // bf16 from a row of 27648: forward 42 us (6.0 TB/s; 49 through the caches), backward 66 (6.4; 83); a large copy
-// reaches 5.2.
+// reaches 5.2.  Float32 ones do not: 512 x 9216 forward 10.6 us (past the caches 12.5), backward 17.8 (19.7), 1536 rows
+// between two neighbours that write gu and read h 78 (84) and 103 (112); 4608 rows 90.6 (92.1; 5.6 TB/s) and 150
+// (157; 5.7), the same between neighbours.
 
 #include "elems.h"
 
@@ -34,6 +36,7 @@ __device__ __forceinline__ T* row_at(const Rows& r, int64_t b, int64_t t) {
 
 template <typename T, bool kBackward>
 __global__ __launch_bounds__(kThreads) void swiglu_kernel(const GateArgs A) {
+  constexpr bool kStream = sizeof(T) == 2;
   for (int64_t first = (int64_t)blockIdx.x * kThreads; first < A.total; first += (int64_t)gridDim.x * kThreads) {
     // The block's first row is scalar; a lane's own is at most kThreads rows on.
     const int64_t row0 = first / A.chunks;
@@ -44,20 +47,20 @@ __global__ __launch_bounds__(kThreads) void swiglu_kernel(const GateArgs A) {
     const int at = (in_row - ahead * A.chunks) * 8, left = A.hidden - at;
     const int64_t b = row / A.length, t = row - b * A.length;
     const T* gu = row_at<T>(A.gu, b, t) + at;
-    const flk::Raw8<T> g8 = flk::load8<true>(gu, left), u8 = flk::load8<true>(gu + A.hidden, left);
+    const flk::Raw8<T> g8 = flk::load8<kStream>(gu, left), u8 = flk::load8<kStream>(gu + A.hidden, left);
     T* out = row_at<T>(A.out, b, t) + at;
     float o0[8], o1[8];
     if constexpr (kBackward) {
-      const flk::Raw8<T> d8 = flk::load8<true>(row_at<T>(A.dh, b, t) + at, left);
+      const flk::Raw8<T> d8 = flk::load8<kStream>(row_at<T>(A.dh, b, t) + at, left);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         flk::gate_backward((float)d8.v[i], (float)g8.v[i], (float)u8.v[i], o0[i], o1[i]);
-      flk::store8<true>(out + A.hidden, left, o1);
+      flk::store8<kStream>(out + A.hidden, left, o1);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) o0[i] = flk::gate((float)g8.v[i], (float)u8.v[i]);
     }
-    flk::store8<true>(out, left, o0);
+    flk::store8<kStream>(out, left, o0);
   }
 }
 

@@ -106,6 +106,20 @@ def test_layer_norm_rows(device, batch, length, width, dtype):
     assert all(torch.equal(a, b) for a, b in zip(grads, again)), "the sums' order does not depend on timing"
 
 
+@pytest.mark.parametrize("length,width", [(700000, 7), (50001, 100), (333, 16001)])
+def test_large_float32_outputs(device, length, width):
+    """Float32 outputs past 18 MB are stored through the caches, by kernels of their own for narrow, ordinary and wide rows."""
+    assert 4 * length * width > 18 << 20
+    print(f"layer_norm length={length} width={width} float32", flush=True)
+    x, g = _stream(width, 1, length, width, torch.float32, device)
+    weight, bias = ((1 + 0.2 * torch.randn(width, generator=g)).to(device) for _ in range(2))
+    dy = torch.randn(x.shape, generator=g).to(device)
+    y, dx, da, dc = _norm_case(_f64(x), _f64(weight), _f64(bias), _f64(dy), (0, 1))
+    _close("y", norm.layer_norm(x, weight, bias), *y)
+    for label, got, want in zip(("dx", "dweight", "dbias"), norm.layer_norm_backward(dy, x, weight, bias), (dx, da, dc)):
+        _close(label, got, *want)
+
+
 def test_many_rows(device):
     """Enough rows that every block of the backward pass walks many, with as many batch entries as rows too."""
     x, g = _stream(5, 4, 9000, 40, torch.bfloat16, device)
