@@ -615,7 +615,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // estimated time over tiles and numbers of ranges.  A tile's blocks run in rounds of what the GPU
 // holds; a stage takes the measured time below with one or two blocks on a CU, a round some more to
 // fill its first stages and to write its tiles, and split products pay a second launch and write
-// and read their partial sums (6 TB/s, mostly from the caches).
+// and read their partial sums (6 TB/s, mostly from the caches).  splits 0: no tile's launch holds the product.
 Choice choose(int64_t rows, int64_t cols, int64_t inner, bool a_across) {
   struct Cost {
     int rows, cols, per_cu;
@@ -631,7 +631,7 @@ Choice choose(int64_t rows, int64_t cols, int64_t inner, bool a_across) {
   };
   static constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48};
   const int64_t all = ceil_div(inner, kK);
-  Choice best{kLarge, 1, (int)all};
+  Choice best{kLarge, 0, (int)all};
   double least = 1e300;
   for (int tile = 0; tile < kTiles; ++tile) {
     const Cost& c = kCost[tile];
@@ -641,6 +641,7 @@ Choice choose(int64_t rows, int64_t cols, int64_t inner, bool a_across) {
       if (want == 1 ? !c.whole : !c.split || want > all) continue;
       const int64_t stages = ceil_div(all, want), splits = ceil_div(all, stages);
       const int64_t blocks = tiles * splits, rounds = blocks / slots, rest = blocks - rounds * slots;
+      if (blocks > kMaxBlocks) continue;
       double us = rounds * (c.stage[c.per_cu - 1] * stages + c.round);
       if (rest) us += c.stage[rest > kCUs] * stages + c.round;
       if (splits > 1) us += 3.0 + 8.0 * splits * rows * cols / 6e6;
@@ -660,7 +661,6 @@ int launch_tiles(Product& p, hipStream_t s) {
   p.tiles_a = (int)ceil_div(p.a.rows, G::kTA);
   p.tiles_b = (int)(kE == kGate ? ceil_div(p.hidden, G::kTB / 2) : ceil_div(p.b.rows, G::kTB));
   const int64_t blocks = (int64_t)p.tiles_a * p.tiles_b * p.splits;
-  if (blocks > kMaxBlocks) return FLK_E_INVALID;
   mlp_kernel<T, kAAcross, kBAcross, kE, G><<<dim3((unsigned)blocks), G::kThreads, 0, s>>>(p);
   return flk_launch_status();
 }
@@ -695,6 +695,7 @@ template <bool kAAcross, bool kBAcross, Epilogue kE>
 int launch(Product& p, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (p.a.stride > kMaxStride || p.b.stride > kMaxStride) return FLK_E_INVALID;
   const Choice c = choose(p.a.rows, p.b.rows, p.inner, kAAcross);
+  if (!c.splits) return FLK_E_INVALID;
   p.stream = (kE == kPlain || !p.gu ? 2LL * p.a.rows * (kE == kGate ? p.hidden : p.b.rows) : 8LL * p.a.rows * p.hidden) > kStreamBytes;
   const int64_t need = partial_bytes(c, p.a.rows, p.b.rows);
   if (need) {
@@ -717,8 +718,10 @@ extern "C" int flk_mlp_plan(int product, int rows, int cols, int inner, int64_t*
   const int64_t columns = product == FLK_MLP_GATE ? 2LL * cols : cols;
   if (rows > kMaxDim || columns > kMaxDim || inner > kMaxDim) return FLK_E_INVALID;
   *workspace_bytes = 0;
-  if (rows && cols && inner) *workspace_bytes = partial_bytes(choose(rows, columns, inner, product == FLK_MLP_MATMUL_AT), rows, columns);
-  return FLK_OK;
+  if (!rows || !cols || !inner) return FLK_OK;
+  const Choice c = choose(rows, columns, inner, product == FLK_MLP_MATMUL_AT);
+  *workspace_bytes = partial_bytes(c, rows, columns);
+  return c.splits ? FLK_OK : FLK_E_INVALID;
 }
 
 extern "C" int flk_mlp_gate(const void* x, int64_t x_row_stride, const void* w_in, int64_t w_in_row_stride, int dtype,

@@ -449,7 +449,7 @@ int flk_swiglu_backward(const void* dh, int64_t dh_batch_stride, int64_t dh_row_
 /* The matrix products of the gated MLP y = (silu(x Wg) * (x Wu)) Wout and of its gradients, on bf16 or
  * fp16 operands (dtype) with float32 sums.  Strides are in elements between rows; every pointer
  * is 16-byte aligned, and widths (all sizes but the token count) and strides are multiples of 8; an
- * operand's stride is at most 2^22 (FLK_E_INVALID).
+ * operand's stride is at most 2^22, and an output at most 2^22 tiles of 256 x 256 (FLK_E_INVALID).
  * Every output row is dense in its last axis; outputs overlap no input.  Products that would leave
  * most of the GPU idle are cut along their inner axis: their partial sums go through `workspace`
  * (16-byte aligned; flk_mlp_plan's bytes for the same product and sizes) and are added in a fixed

@@ -231,6 +231,20 @@ def test_offsets_past_32_bits(device):
         _close(name, value, *exact[name])
 
 
+def test_more_tokens_than_small_tiles(device):
+    """Tokens for more than 2^22 tiles of 128 rows, on whole numbers: the first and the last are those of a short call."""
+    m, part = (1 << 29) + 136, 300
+    x, w_in = _whole(1, (part, 8), torch.bfloat16, device, 3), _whole(2, (8, 16), torch.bfloat16, device, 1) * 2.0 ** -2
+    w_out = _whole(3, (8, 8), torch.bfloat16, device, 1)
+    long = torch.zeros(m, 8, dtype=torch.bfloat16, device=device)
+    long[:part], long[-part:] = x, x
+    want = mlp.gated_mlp(x, w_in, w_out)
+    print(f"gated_mlp m={m}", flush=True)
+    y = mlp.gated_mlp(long, w_in, w_out)
+    assert torch.equal(y[:part], want) and torch.equal(y[-part:], want)
+    assert not any(bool(rest.any()) for rest in y[part:-part].split(1 << 26))
+
+
 def test_gated_mlp_not_finite(device):
     """A token's not-finite value stays in its row of y and dx, whatever rows share its tile."""
     x, dy, w_in, w_out = _operands(5, 40, 64, 64, torch.bfloat16, device)

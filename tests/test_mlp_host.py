@@ -169,6 +169,20 @@ def test_mlp_checks(lib):
     assert lib.flk_mlp_plan(0, -1, 8, 8, ctypes.byref(size)) == INVALID and lib.flk_mlp_plan(0, 1, 8, 8, None) == INVALID
 
 
+def test_mlp_tile_limits(lib):
+    """Products past 2^22 tiles of 256 x 256 are refused by the plan and by the launch, and no smaller ones: where
+    smaller tiles would be too many for one launch, larger ones are taken."""
+    size = ctypes.c_int64(-1)
+    most = 256 << 22
+    for product in range(4):
+        assert lib.flk_mlp_plan(product, most, 8, 8, ctypes.byref(size)) == OK and size.value == 0
+        assert lib.flk_mlp_plan(product, most + 1, 8, 8, ctypes.byref(size)) == INVALID
+    gate = lambda m: lib.flk_mlp_gate(P16, 8, P16, 16, BF16, m, 8, 8, P16, 8, None, None, 0, None)  # noqa: E731
+    back = lambda m: lib.flk_mlp_gate_backward(P16, 8, P16, 8, P16, BF16, m, 8, 8, P16, 16, None, 0, None)  # noqa: E731
+    for f in (gate, back):
+        assert f(most + 1) == INVALID
+
+
 def test_operand_layouts_of_the_products(lib, monkeypatch):
     """Rows further apart than the products address, or off 16 bytes, are copied; others are read in place."""
     monkeypatch.setattr(mlp, "_on_gpu", lambda name, t: None)
