@@ -64,6 +64,7 @@ SIGNATURES = {
     "flk_swiglu": (_i, [_p, _i64, _i64, _i, _i, _i, _i, _p, _i64, _i64, _p]),
     "flk_swiglu_backward": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i, _i, _i, _i, _p, _i64, _i64, _p]),
     "flk_mlp_plan": (_i, [_i, _i, _i, _i, ctypes.POINTER(ctypes.c_int64)]),
+    "flk_mlp_kernel": (ctypes.c_char_p, [_i, _i, _i, _i]),
     "flk_mlp_gate": (_i, [_p, _i64, _p, _i64, _i, _i, _i, _i, _p, _i64, _p, _p, _i64, _p]),
     "flk_mlp_gate_backward": (_i, [_p, _i64, _p, _i64, _p, _i, _i, _i, _i, _p, _i64, _p, _i64, _p]),
     "flk_mlp_matmul": (_i, [_p, _i64, _i, _p, _i64, _i, _i, _i, _i, _i, _p, _i64, _p, _i64, _p]),

@@ -724,6 +724,15 @@ extern "C" int flk_mlp_plan(int product, int rows, int cols, int inner, int64_t*
   return c.splits ? FLK_OK : FLK_E_INVALID;
 }
 
+extern "C" const char* flk_mlp_kernel(int product, int rows, int cols, int inner) {
+  static constexpr const char* kNames[kTiles][2] = {{"256x256", ""}, {"192x256", ""}, {"128x128 x2", "128x128 x2 split"},
+                                                    {"128x128 deep", "128x128 deep split"}, {"", "128x32 split"}};
+  int64_t bytes = 0;
+  if (flk_mlp_plan(product, rows, cols, inner, &bytes) != FLK_OK || !rows || !cols || !inner) return "";
+  const Choice c = choose(rows, product == FLK_MLP_GATE ? 2LL * cols : cols, inner, product == FLK_MLP_MATMUL_AT);
+  return kNames[c.tile][c.splits > 1];
+}
+
 extern "C" int flk_mlp_gate(const void* x, int64_t x_row_stride, const void* w_in, int64_t w_in_row_stride, int dtype,
                             int m, int width, int hidden, void* h, int64_t h_row_stride, float* gu, void* workspace,
                             int64_t workspace_bytes, void* stream) {

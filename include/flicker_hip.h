@@ -472,6 +472,9 @@ int flk_swiglu_backward(const void* dh, int64_t dh_batch_stride, int64_t dh_row_
 #define FLK_MLP_MATMUL_BT 3      /* ... with b_transposed                               */
 #define FLK_MLP_MATMUL_AT 4      /* ... with a_transposed                               */
 int flk_mlp_plan(int product, int rows, int cols, int inner, int64_t* workspace_bytes);
+/* The tile, columns x rows, that a product runs on ("x2": two blocks a CU; "deep": one with more stages in
+ * flight; "split": cut along the inner axis); "" for sizes that are empty or refused. */
+const char* flk_mlp_kernel(int product, int rows, int cols, int inner);
 int flk_mlp_gate(const void* x, int64_t x_row_stride, const void* w_in, int64_t w_in_row_stride, int dtype, int m,
                  int width, int hidden, void* h, int64_t h_row_stride, float* gu, void* workspace,
                  int64_t workspace_bytes, void* stream);

@@ -148,6 +148,101 @@ def hidden_sum(a, b):
     return a.shape[1] * U * (a @ b)
 
 
+# Each product on each of its tiles (tests/test_mlp_host.py asserts which one a size takes): four row tiles, whose blocks
+# touch their operands' lines ahead, five to seven, which sweep in two groups, and outputs that pass the caches by (past
+# 80 MB; the gate's g and u); one stage of 64 terms, a ragged one after none, one and more whole stages.  The tokens'
+# axis, inside in the fifth product, has any length.
+SHORT, ODD = (64, 72, 136, 200, 328), (64, 71, 133, 200, 331)
+TILES = [(product, tile, rows // 8 * 8 if product == mlp._MATMUL_AT else rows, cols, ODD if product == mlp._MATMUL_AT else inner)
+         for product in (mlp._MATMUL, mlp._MATMUL_BT, mlp._MATMUL_AT, mlp._GATE_BACKWARD) for tile, rows, cols, inner in (
+             ("256x256", 779, 12368, SHORT), ("256x256", 1547, 7600, SHORT), ("192x256", 779, 9352, SHORT),
+             ("192x256", 8203, 928, SHORT), ("128x128 x2", 779, 4672, SHORT), ("128x128 deep", 1035, 304, SHORT))]
+TILES += [(mlp._GATE, tile, rows, cols, SHORT) for tile, rows, cols in (
+    ("256x256", 779, 6232), ("256x256", 1291, 4048), ("256x256", 267, 12368), ("192x256", 779, 4776), ("192x256", 1291, 3008),
+    ("192x256", 267, 10912), ("128x128 x2", 779, 2384), ("128x128 deep", 779, 200))]
+TILES += [(product, tile, rows, cols, (200,)) for product, tile, rows, cols in (
+    (mlp._MATMUL, "256x256", 3347, 12576), (mlp._MATMUL_BT, "192x256", 3347, 13928), (mlp._MATMUL_AT, "256x256", 3344, 12576),
+    (mlp._MATMUL_AT, "192x256", 3344, 13928), (mlp._GATE, "192x256", 2315, 4568), (mlp._GATE, "256x256", 779, 13512),
+    (mlp._GATE, "256x256", 3347, 12576), (mlp._GATE_BACKWARD, "192x256", 2315, 4568), (mlp._GATE_BACKWARD, "256x256", 779, 13512),
+    (mlp._GATE_BACKWARD, "128x128 x2", 1291, 10808))]
+TILES += [(product, "128x128 deep split", 2072, 72, (1000,)) for product in range(5)]
+TILES += [(product, "128x128 x2 split", 520, 2192, (4040,)) for product in range(1, 5)] + [(mlp._GATE, "128x128 x2 split", 267, 1832, (4040,))]
+TILES += [(product, "128x32 split", 45, 200, (520,)) for product in range(4)]
+
+
+def _inside(t):
+    """t in the middle of a larger buffer of NaNs, rows 16-byte aligned."""
+    wide = torch.full((t.shape[0] + 2, -(-t.shape[1] // 8) * 8 + 16), float("nan"), dtype=t.dtype, device=t.device)
+    wide[1:-1, 8:8 + t.shape[1]] = t
+    return wide[1:-1, 8:8 + t.shape[1]]
+
+
+@pytest.mark.parametrize("product,tile,rows,cols,inners", TILES)
+@pytest.mark.parametrize("dtype", BOTH)
+def test_every_tile(device, product, tile, rows, cols, inners, dtype):
+    """Whole numbers, whose sums are exact, inside NaNs that no result may hold.  The gate's g is at least 64, where
+    1 + exp(-g) is 1: h = g u, dg = dh u and du = dh g in one float32 product each."""
+    for inner in inners:
+        print(f"product {product} {tile} rows={rows} cols={cols} inner={inner} {dtype}", flush=True)
+        assert _lib.lib().flk_mlp_kernel(product, rows, cols, inner).decode() == tile
+        ws, nbytes = mlp._workspace(product, rows, cols, inner, device)
+        a = _inside(_whole(1, (rows, inner), dtype, device, 3))
+        code, stream = mlp._dtype("a", a), _lib.stream_of(a)
+        if product == mlp._GATE:
+            a.abs_().add_(1.0)
+            w = _inside(_whole(2, (inner, 2 * cols), dtype, device, 2))
+            w[:, :cols].abs_().clamp_(1.0)
+            w[:, cols:] *= 2.0 ** -10
+            gu, h = torch.full((rows, 2 * cols), 77.0, device=device), _inside(torch.full((rows, cols), 77.0, dtype=dtype, device=device))
+            want = (a.double() @ w.double()).float()
+            for kept in (gu, None):
+                h.fill_(77.0)
+                _lib.run("flk_mlp_gate", (a, w, h, kept, ws), a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(0), code, rows, inner,
+                         cols, h.data_ptr(), h.stride(0), _lib.ptr(kept), _lib.ptr(ws), nbytes, stream)
+                assert torch.equal(h, (want[:, :cols] * want[:, cols:]).to(dtype))
+            assert torch.equal(gu, want)
+            continue
+        b = _inside(_whole(2, (cols, inner), dtype, device, 3))
+        exact = (a.double() @ b.double().t()).float()
+        if product == mlp._GATE_BACKWARD:
+            g = torch.Generator(device).manual_seed(3)
+            gu = torch.randn(rows, 2 * cols, generator=g, device=device)
+            gu[:, :cols].abs_().add_(64.0)
+            d = _inside(torch.full((rows, 2 * cols), 77.0, dtype=dtype, device=device))
+            _lib.run("flk_mlp_gate_backward", (a, b, gu, d, ws), a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), gu.data_ptr(),
+                     code, rows, inner, cols, d.data_ptr(), d.stride(0), _lib.ptr(ws), nbytes, stream)
+            assert torch.equal(d[:, :cols], (exact * gu[:, cols:]).to(dtype)) and torch.equal(d[:, cols:], (exact * gu[:, :cols]).to(dtype))
+        else:
+            d = _inside(torch.full((rows, cols), 77.0, dtype=dtype, device=device))
+            a_t, b_t = product == mlp._MATMUL_AT, product == mlp._MATMUL_BT
+            mlp._matmul(_inside(a.t()) if a_t else a, b if b_t else _inside(b.t()), d, a_t=a_t, b_t=b_t)
+            assert torch.equal(d, exact.to(dtype))
+        wide = d._base
+        wide[1:-1, 8:8 + d.shape[1]] = float("nan")
+        assert bool(wide.isnan().all())   # nothing beside the output is written
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_gate_on_large_tiles(device, dtype):
+    """The gate and its gradients of ordinary values on 256 x 256 tiles, at the first and last rows."""
+    rows, inner = 1291, 136
+    for cols, scale in ((4048, 2.0 ** -6), (8104, 2.0 ** -6)):
+        print(f"gate m={rows} width={inner} hidden={cols} {dtype}", flush=True)
+        pick = torch.cat((torch.arange(20), torch.arange(rows - 20, rows))).to(device)
+        x, w = _whole(1, (rows, inner), dtype, device, 3), _whole(2, (inner, 2 * cols), dtype, device, 1) * scale
+        gu, h = torch.empty(rows, 2 * cols, device=device), torch.empty(rows, cols, dtype=dtype, device=device)
+        _lib.run("flk_mlp_gate", (x, w, h, gu), x.data_ptr(), inner, w.data_ptr(), 2 * cols, mlp._dtype("x", x), rows, inner, cols,
+                 h.data_ptr(), cols, gu.data_ptr(), None, 0, _lib.stream_of(x))
+        want = _f64(x[pick]) @ _f64(w)
+        assert np.array_equal(_f64(gu[pick]), want)
+        _close("h", h[pick], *_gate_case(want, np.zeros((len(pick), cols)))[0])
+        dy, w_out = _whole(3, (rows, inner), dtype, device, 3), _whole(4, (cols, inner), dtype, device, 2) * 2.0 ** -6
+        dgu = torch.empty(rows, 2 * cols, dtype=dtype, device=device)
+        _lib.run("flk_mlp_gate_backward", (dy, w_out, gu, dgu), dy.data_ptr(), inner, w_out.data_ptr(), inner, gu.data_ptr(),
+                 mlp._dtype("x", x), rows, inner, cols, dgu.data_ptr(), 2 * cols, None, 0, _lib.stream_of(x))
+        _close("dgu", dgu[pick], *_gate_case(want, _f64(dy[pick]) @ _f64(w_out).T)[1])
+
+
 @pytest.mark.parametrize("m,width,hidden", [(1, 64, 64), (1, 512, 1536), (5, 256, 264), (24, 136, 320), (77, 512, 512),
                                             (200, 72, 136), (512, 256, 768), (1000, 200, 424)])
 @pytest.mark.parametrize("dtype", BOTH)

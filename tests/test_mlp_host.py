@@ -183,6 +183,21 @@ def test_mlp_tile_limits(lib):
         assert f(most + 1) == INVALID
 
 
+def test_tiles_of_the_tested_sizes(lib):
+    """The GPU tests' sizes reach every tile of every product, so that a change of the costs that choose between them
+    does not leave one untested."""
+    from tests.test_gpu_mlp import TILES
+    reached = set()
+    for product, tile, rows, cols, inners in TILES:
+        for inner in inners:
+            assert lib.flk_mlp_kernel(product, rows, cols, inner).decode() == tile, (product, rows, cols, inner)
+        reached.add((product, tile))
+    names = {"256x256", "192x256", "128x128 x2", "128x128 x2 split", "128x128 deep", "128x128 deep split", "128x32 split"}
+    assert reached == {(p, n) for p in range(5) for n in names} - {(mlp._MATMUL_AT, "128x32 split")}
+    for bad in ((5, 1, 8, 8), (-1, 1, 8, 8), (0, 0, 8, 8), (0, 1, 0, 8), (0, 1, 8, 0), (0, -1, 8, 8), (0, 2 ** 30 + 1, 8, 8)):
+        assert lib.flk_mlp_kernel(*bad) == b""
+
+
 def test_operand_layouts_of_the_products(lib, monkeypatch):
     """Rows further apart than the products address, or off 16 bytes, are copied; others are read in place."""
     monkeypatch.setattr(mlp, "_on_gpu", lambda name, t: None)
