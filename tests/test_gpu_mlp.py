@@ -264,6 +264,25 @@ def test_gated_mlp(device, m, width, hidden, dtype):
     assert all(torch.equal(a, b) for a, b in zip(again, (got["dx"], got["dw_in"], got["dw_out"])))
 
 
+@pytest.mark.parametrize("m,width,hidden", [(1, 256, 768), (77, 512, 136), (1291, 136, 4048)])
+@pytest.mark.parametrize("dtype", BOTH)
+def test_nothing_but_h_and_dgu_is_rounded_between_the_products(device, m, width, hidden, dtype):
+    """y from the h that the call keeps, and the gradients from that h and dgu, are off by their float32 sums and
+    their own rounding only."""
+    print(f"gated_mlp m={m} width={width} hidden={hidden} {dtype}", flush=True)
+    x, dy, w_in, w_out = _operands(m, m, width, hidden, dtype, device)
+    y, kept = mlp.gated_mlp(x, w_in, w_out, keep=True)
+    dgu = torch.empty(m, 2 * hidden, dtype=dtype, device=device)
+    ws, nbytes = mlp._workspace(mlp._GATE_BACKWARD, m, hidden, width, device)
+    _lib.run("flk_mlp_gate_backward", (dy, w_out, kept.gu, dgu, ws), dy.data_ptr(), width, w_out.data_ptr(), width,
+             kept.gu.data_ptr(), mlp._dtype("x", x), m, width, hidden, dgu.data_ptr(), 2 * hidden, _lib.ptr(ws), nbytes,
+             _lib.stream_of(x))
+    h, d, wi, wo, xs, g = map(_f64, (kept.h, dgu, w_in, w_out, x, dy))
+    dx, dw_in, dw_out = mlp.gated_mlp_backward(dy, x, w_in, w_out, kept)
+    for name, got, a, b in (("y", y, h, wo), ("dx", dx, d, wi.T), ("dw_in", dw_in, xs.T, d), ("dw_out", dw_out, h.T, g)):
+        _close(name, got, a @ b, hidden_sum(np.abs(a), np.abs(b)))
+
+
 def test_gated_mlp_shapes_and_views(device):
     """Batches, one token, rows of a wider buffer, weights inside wider ones, and the operands' gradients' shapes."""
     x, dy, w_in, w_out = _operands(3, 42, 64, 72, torch.bfloat16, device)
