@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from .kernels import _native, _on_gpu
-from .norm import _blocks, _dtype, _out_blocks, _output, _strides
+from .norm import _blocks, _dtype, _out_blocks, _output, _refuse_overlap, _strides
 
 _GATE, _GATE_BACKWARD, _MATMUL, _MATMUL_BT, _MATMUL_AT = range(5)   # FLK_MLP_*
 _MAX_STRIDE = 1 << 22   # elements between two rows of an operand of the products
@@ -40,7 +40,7 @@ class Kept(NamedTuple):
 
 def swiglu(gu: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """silu(g) * u of gu (..., 2 * hidden) = [g | u] -> (..., hidden); bfloat16, float16 or float32.  gu and
-    ``out`` may be columns of wider buffers."""
+    ``out`` may be columns of wider buffers, and ``out`` one of gu's halves; any other overlap is refused."""
     if out is None:
         done = _native.swiglu(gu)
         if done is not None:
@@ -49,17 +49,20 @@ def swiglu(gu: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor
     if gu.dim() == 0 or gu.shape[-1] == 0 or gu.shape[-1] % 2:
         raise ValueError(f"gu must be (..., 2 * hidden), got {tuple(gu.shape)}")
     hidden = gu.shape[-1] // 2
-    out = _output(out, (*gu.shape[:-1], hidden), gu)
+    given, out = out is not None, _output(out, (*gu.shape[:-1], hidden), gu)
     if gu.numel() == 0:
         return out
     gb, ob = _blocks(gu), _out_blocks(out)
+    if given:
+        _refuse_overlap("gu", ob, gb, (0, hidden))
     _lib.run("flk_swiglu", (gu, out), gb.data_ptr(), *_strides(gb), code, gb.shape[0], gb.shape[1], hidden,
              ob.data_ptr(), *_strides(ob), _lib.stream_of(gu))
     return out
 
 
 def swiglu_backward(dh: torch.Tensor, gu: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
-    """dgu = [dg | du] of ``swiglu(gu)`` for the incoming gradient dh; ``out`` may be gu itself."""
+    """dgu = [dg | du] of ``swiglu(gu)`` for the incoming gradient dh; ``out`` may be gu itself, and dh one of its
+    halves; any other overlap is refused."""
     if out is None:
         done = _native.swiglu_backward(dh, gu)
         if done is not None:
@@ -71,10 +74,13 @@ def swiglu_backward(dh: torch.Tensor, gu: torch.Tensor, *, out: torch.Tensor | N
     hidden = gu.shape[-1] // 2
     if dh.shape != (*gu.shape[:-1], hidden) or dh.dtype != gu.dtype:
         raise ValueError(f"dh must be {gu.dtype} {(*gu.shape[:-1], hidden)}, got {dh.dtype} {tuple(dh.shape)}")
-    out = _output(out, gu.shape, gu)
+    given, out = out is not None, _output(out, gu.shape, gu)
     if gu.numel() == 0:
         return out
     gb, db, ob = _blocks(gu), _blocks(dh), _out_blocks(out)
+    if given:
+        _refuse_overlap("gu", ob, gb, (0,))
+        _refuse_overlap("dh", ob, db, (0, -hidden))
     _lib.run("flk_swiglu_backward", (dh, gu, out), db.data_ptr(), *_strides(db), gb.data_ptr(), *_strides(gb), code,
              gb.shape[0], gb.shape[1], hidden, ob.data_ptr(), *_strides(ob), _lib.stream_of(gu))
     return out
@@ -139,16 +145,19 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, *, keep:
               out: torch.Tensor | None = None):
     """(silu(x @ w_g) * (x @ w_u)) @ w_out with w_in = [w_g | w_u]: x (..., width), w_in (width, 2 * hidden), w_out
     (hidden, width), all bfloat16 or all float16, widths multiples of 8 -> (..., width).  With ``keep`` also
-    returns the ``Kept`` that gated_mlp_backward takes.  ``out`` must be contiguous."""
+    returns the ``Kept`` that gated_mlp_backward takes.  ``out`` must be contiguous; it may
+    overlap x, but not w_out."""
     if out is None:
         done = _native.gated_mlp(x, w_in, w_out, keep)
         if done is not None:
             return (done[0], Kept(done[1], done[2])) if keep else done[0]
     xr, w_in, w_out, width, hidden = _operands(x, w_in, w_out)
     m = xr.shape[0]
-    out = _output(out, x.shape, x)
+    given, out = out is not None, _output(out, x.shape, x)
     if not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be contiguous and 16-byte aligned")
+    if given and m:
+        _refuse_overlap("w_out", out.view(m, width), w_out)
     h = torch.empty((m, hidden), dtype=x.dtype, device=x.device)
     gu = torch.empty((m, 2 * hidden), dtype=torch.float32, device=x.device) if keep else None
     if m:

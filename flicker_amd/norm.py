@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -61,13 +62,42 @@ def _out_blocks(out: torch.Tensor) -> torch.Tensor:
             out = out.view(1, -1, out.shape[-1])
         except RuntimeError:
             raise ValueError(f"out {tuple(out.shape)} with strides {out.stride()} has no common row stride") from None
-    batch, length, width = out.shape
-    row = out.stride(1) if length > 1 else width
-    entry = out.stride(0) if batch > 1 else width
-    apart = entry >= (length - 1) * row + width or row >= (batch - 1) * entry + width
-    if (width > 1 and out.stride(2) != 1) or min(row, entry) < width or not (apart or min(batch, length) == 1):
+    if not _rows_apart(out):
         raise ValueError(f"out needs contiguous rows that do not overlap, got strides {out.stride()}")
     return out
+
+
+def _rows_apart(t: torch.Tensor) -> bool:
+    """Whether (B, L, N) has contiguous rows that do not overlap."""
+    batch, length, width = t.shape
+    row = t.stride(1) if length > 1 else width
+    entry = t.stride(0) if batch > 1 else width
+    apart = entry >= (length - 1) * row + width or row >= (batch - 1) * entry + width
+    return (width <= 1 or t.stride(2) == 1) and min(row, entry) >= width and (apart or min(batch, length) == 1)
+
+
+def _elements(t: torch.Tensor) -> np.ndarray:
+    """``t``'s addresses as an array that is never read."""
+    class Memory:
+        __array_interface__ = {"version": 3, "typestr": f"|V{t.element_size()}", "data": (t.data_ptr(), True),
+                               "shape": tuple(t.shape), "strides": tuple(s * t.element_size() for s in t.stride())}
+    return np.asarray(Memory())
+
+
+def _end(t: torch.Tensor) -> int:
+    return t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _refuse_overlap(name: str, out: torch.Tensor, t: torch.Tensor, columns=()) -> None:
+    """Refuses an output over an input ``t`` that is still being read.  In place, row by row, is not refused: both are
+    (B, L, N) blocks of the same strides, and out's rows begin one of ``columns`` after t's."""
+    if out.data_ptr() >= _end(t) or t.data_ptr() >= _end(out):
+        return
+    if (out.data_ptr() - t.data_ptr()) in [c * t.element_size() for c in columns] and _rows_apart(t) and all(
+            a == b or n == 1 for n, a, b in zip(t.shape[:2], out.stride(), t.stride())):
+        return
+    if np.shares_memory(_elements(out), _elements(t)):
+        raise ValueError(f"out shares memory with {name}, and not in place")
 
 
 def _param(name: str, t: torch.Tensor | None, shape, x: torch.Tensor) -> torch.Tensor | None:
@@ -92,12 +122,17 @@ def _params(named, x, shapes):
 
 def _forward(x, factor, offset, per_entry: bool, add_one: bool, eps: float, out):
     code = _dtype("x", x)
-    out = _output(out, x.shape, x)
+    given, out = out is not None, _output(out, x.shape, x)
     yb = _out_blocks(out)
     if x.numel() == 0:
         return out
     xb = _blocks(x)
     batch, length, width = xb.shape
+    if given:
+        _refuse_overlap("x", yb, xb, (0,))
+        for p in (factor, offset):
+            if p is not None:
+                _refuse_overlap("a parameter", yb, p)
     param = factor if factor is not None else offset
     _lib.run("flk_layer_norm", (x, factor, offset, out), xb.data_ptr(), *_strides(xb), code, _lib.ptr(factor),
              _lib.ptr(offset), code if param is None else _CODES[param.dtype], width if per_entry else 0,
@@ -146,7 +181,7 @@ def _check_x(x: torch.Tensor) -> None:
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
                eps: float = EPS, out: torch.Tensor | None = None) -> torch.Tensor:
     """Layer norm over the last axis of x (..., width); ``weight`` and ``bias`` (width,) or None.  ``out`` may be
-    a view with strided rows, or x itself."""
+    a view with strided rows, or x itself; any other overlap with an operand is refused."""
     if out is None:
         done = _native.layer_norm(x, weight, bias, eps)
         if done is not None:

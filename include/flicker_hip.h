@@ -412,8 +412,9 @@ int flk_w8a8_qk_prep_pair(const int8_t* xq0, const int8_t* wq_t0, const float* a
  *            b*batch_stride + t*row_stride + j, strides in elements, any of them
  *   factor, offset  (width,) rows of type params_dtype (dtype itself or FLK_F32), one per batch
  *            entry at b*param_batch_stride, or one for all (stride 0); NULL: a = 1, c = 0
- * y may be x.  Any alignment of whole elements; width at most 16384 (else FLK_E_UNSUPPORTED), batch * length at
- * most 2^31 - 1 and, with a row of parameters per batch entry, batch at most 2^22 (else FLK_E_INVALID). */
+ * y may be x, and overlaps no operand otherwise.  Any alignment of whole elements; width at most
+ * 16384 (else FLK_E_UNSUPPORTED), batch * length at most 2^31 - 1 and, with a row of parameters per batch
+ * entry, batch at most 2^22 (else FLK_E_INVALID). */
 int flk_layer_norm(const void* x, int64_t x_batch_stride, int64_t x_row_stride, int dtype, const void* factor,
                    const void* offset, int params_dtype, int64_t param_batch_stride, int add_one, float eps, int batch,
                    int length, int width, void* y, int64_t y_batch_stride, int64_t y_row_stride, void* stream);
@@ -436,12 +437,13 @@ int flk_layer_norm_backward(const void* dy, int64_t dy_batch_stride, int64_t dy_
 /* h = silu(g) * u of gu = [g | u], silu(z) = z / (1 + exp(-z)), in float32, rounded once: the gate of
  * the blocks' MLP (modules.py:157-167, 185-200).
  *   gu  (batch, length, 2*hidden), h (batch, length, hidden) of type dtype, laid out as in
- *       flk_layer_norm: gu may be columns of a wider projection, h columns of a wider buffer. */
+ *       flk_layer_norm: gu may be columns of a wider projection, h columns of a wider buffer.  h may be
+ *       one half of gu, row in row, and overlaps it in no other way. */
 int flk_swiglu(const void* gu, int64_t gu_batch_stride, int64_t gu_row_stride, int dtype, int batch, int length,
                int hidden, void* h, int64_t h_batch_stride, int64_t h_row_stride, void* stream);
 
 /* dgu = [dg | du] for the incoming gradient dh, with s = 1 / (1 + exp(-g)):
- *   dg = dh u s (1 + g (1 - s)),  du = dh g s.   dgu may be gu. */
+ *   dg = dh u s (1 + g (1 - s)),  du = dh g s.   dgu may be gu, and dh one half of dgu. */
 int flk_swiglu_backward(const void* dh, int64_t dh_batch_stride, int64_t dh_row_stride, const void* gu,
                         int64_t gu_batch_stride, int64_t gu_row_stride, int dtype, int batch, int length, int hidden,
                         void* dgu, int64_t dgu_batch_stride, int64_t dgu_row_stride, void* stream);

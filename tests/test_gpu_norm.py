@@ -352,6 +352,40 @@ def test_swiglu_in_place_of_a_single_block(device):
         mlp.swiglu_backward(gu, gu)
 
 
+def test_outputs_over_their_operands(device):
+    """In place where each lane writes what it has read, beside the operands in one buffer, and refused otherwise."""
+    wide = torch.randn(2, 5, 200, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(device)
+    for at in (20, 60):   # silu(g) u over g, over u
+        w = wide.clone()
+        want = mlp.swiglu(w[..., 20:100].contiguous())
+        assert torch.equal(mlp.swiglu(w[..., 20:100], out=w[..., at:at + 40]), want)
+        w = wide.clone()
+        out, dh = w[..., 20:100], w[..., at:at + 40]   # the gradient where dh was
+        gu = wide[..., 100:180]
+        want = mlp.swiglu_backward(dh.contiguous(), gu)
+        assert torch.equal(mlp.swiglu_backward(dh, gu, out=out), want)
+    w = wide.clone()
+    want = norm.layer_norm(w[..., 20:100].contiguous())
+    assert torch.equal(norm.layer_norm(w[..., 20:100], out=w[..., 100:180]), want)
+    assert torch.equal(w[..., 20:100], wide[..., 20:100])
+    for call in (lambda: mlp.swiglu(w[..., 20:100], out=w[..., 21:61]), lambda: mlp.swiglu(w[..., 20:100], out=w[..., 10:50]),
+                 lambda: mlp.swiglu(w[:, :4, 20:100], out=w[:, 1:, 20:60]),
+                 lambda: mlp.swiglu_backward(wide[..., 100:140], w[..., 20:100], out=w[..., 21:101]),
+                 lambda: mlp.swiglu_backward(w[..., 70:110], wide[..., 20:100], out=w[..., 20:100]),
+                 lambda: norm.layer_norm(w[..., 20:100], out=w[..., 21:101]), lambda: norm.layer_norm(w[:, :4], out=w[:, 1:]),
+                 lambda: norm.layer_norm(wide, w[0, 0], out=w)):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+    # rows of parameters that are not dense are copied before anything is written
+    want = norm.modulate(wide, wide[:, 0].clone(), wide[:, 1].clone())
+    w = wide.clone()
+    assert torch.equal(norm.modulate(w, w[:, 0], w[:, 1], out=w), want)
+    x, w_in = wide[0, :, :64].contiguous(), wide[..., :160].reshape(10, 160)[:8].repeat(8, 1)
+    w_out = torch.zeros(80 * 64, dtype=torch.bfloat16, device=device)
+    with pytest.raises(ValueError, match="shares memory"):
+        mlp.gated_mlp(x, w_in, w_out.view(80, 64), out=w_out[:5 * 64].view(5, 64))
+
+
 def test_autograd_matches_the_explicit_calls(device):
     x, g = _stream(4, 2, 9, 56, torch.bfloat16, device)
     x.requires_grad_()

@@ -213,6 +213,50 @@ def test_operand_layouts_of_the_products(lib, monkeypatch):
     assert mlp._matrix("x", first).stride(0) == 64
 
 
+def _owners(t, hidden, chunk):
+    """Address -> the lanes of t's elements there; a lane takes `chunk` columns of a row, of both halves of a wide one."""
+    found = {}
+    for b, r, c in np.ndindex(*t.shape):
+        at = t.data_ptr() + t.element_size() * (b * t.stride(0) + r * t.stride(1) + c * t.stride(2))
+        found.setdefault(at, set()).add((b, r, c % hidden // chunk))
+    return found
+
+
+def test_overlapping_outputs_are_refused():
+    """Random views of one small buffer, element by element: an output is accepted where no lane writes what another
+    reads, and refused only where it shares memory."""
+    r = np.random.RandomState(0)
+    memory = torch.zeros(2000)
+    accepted, refused, in_place = 0, 0, set()
+    for _ in range(3000):
+        kind, hidden = r.choice(["norm", "swiglu", "dh"]), int(r.choice([3, 8, 16, 20]))
+        columns = {"norm": (0,), "swiglu": (0, hidden), "dh": (0, -hidden)}[kind]
+        shape = (int(r.randint(1, 4)), int(r.randint(1, 4)))
+        row = int(r.choice([hidden, 2 * hidden, 2 * hidden + 5, 50]))
+        strides = (int(r.choice([0, row * shape[1], row * shape[1] + 7, 200])), int(r.choice([row, row, 2 * hidden])), 1)
+        t = memory[40 + int(r.randint(0, 60)):].as_strided((*shape, hidden * (1 + (kind == "swiglu"))), strides)
+        if r.rand() < 0.5:
+            strides = (row * shape[1], row, 1)
+        start = t.storage_offset() + int(r.choice([*columns, r.randint(-40, 60), r.randint(-40, 300)]))
+        out = memory[start:].as_strided((*shape, hidden * (1 + (kind == "dh"))), strides)
+        if not norm._rows_apart(out):
+            continue
+        chunk = hidden if kind == "norm" else 8   # a norm's rows are read whole before they are written
+        written, read = _owners(out, hidden, chunk), _owners(t, hidden, chunk)
+        shared = written.keys() & read.keys()
+        try:
+            norm._refuse_overlap("t", out, t, columns)
+        except ValueError as error:
+            assert shared and "shares memory with t" in str(error)
+            refused += 1
+            continue
+        assert all(read[at] == written[at] and len(read[at]) == 1 for at in shared), (kind, out.stride(), start, t.stride(), t.storage_offset())
+        accepted += not shared
+        if shared:
+            in_place.add((kind, out.data_ptr() == t.data_ptr()))
+    assert accepted > 300 and refused > 300 and len(in_place) == 5, (accepted, refused, in_place)
+
+
 def test_python_refuses_host_tensors_and_bad_calls():
     x = torch.zeros(2, 3, 16, dtype=torch.bfloat16)
     for call in (lambda: norm.layer_norm(x), lambda: norm.modulate(x, x[:, 0], x[:, 0]), lambda: mlp.swiglu(x),
