@@ -10,8 +10,9 @@ buffer that linear2 reads (modules.py:185-200).
 
 ``*_backward`` take the incoming gradient and the forward call's operands.  Sums are float32 and outputs are
 rounded once; between the two projections h, and backwards [dg | du], are rounded to the operands' type,
-which the matrix cores take, while g and u stay float32.  For gradients through torch's autograd see
-``flicker_amd.autograd``.
+which the matrix cores take, while g and u stay float32.  In float16 that rounding has the type's range: an h
+past 65504 is infinite, and a dg or du below 2^-25 is zero (bfloat16 has float32's range).  For gradients
+through torch's autograd see ``flicker_amd.autograd``.
 """
 
 from __future__ import annotations

@@ -455,7 +455,7 @@ int flk_swiglu_backward(const void* dh, int64_t dh_batch_stride, int64_t dh_row_
  * Every output row is dense in its last axis; outputs overlap no input.  Products that would leave
  * most of the GPU idle are cut along their inner axis: their partial sums go through `workspace`
  * (16-byte aligned; flk_mlp_plan's bytes for the same product and sizes) and are added in a fixed
- * order.
+ * order.  h and dgu are rounded to dtype: in fp16 an h past 65504 is infinite, and a dg or du below 2^-25 zero.
  *
  * flk_mlp_gate: h (m, hidden) = silu(g) * u of [g | u] = x (m, width) w_in (width, 2*hidden); gu, if
  * not NULL, receives [g | u] as float32 (m, 2*hidden), dense, which the backward pass needs.

@@ -359,6 +359,22 @@ def test_more_tokens_than_small_tiles(device):
     assert not any(bool(rest.any()) for rest in y[part:-part].split(1 << 26))
 
 
+def test_range_between_the_products(device):
+    """h and dgu have the operands' type's range: in float16 h = 300 * 300 is infinite, and du = 2^-27 silu(1) zero."""
+    def one(value, dtype):
+        t = torch.zeros(1, 8, dtype=dtype, device=device)
+        t[0, 0] = value
+        return t
+    for dtype, y, zero in ((torch.bfloat16, 90112.0, False), (torch.float16, float("inf"), True)):
+        w_in, w_out = torch.zeros(8, 16, dtype=dtype, device=device), torch.eye(8, dtype=dtype, device=device)
+        w_in[0, 0] = w_in[0, 8] = 1.0
+        assert mlp.gated_mlp(one(300.0, dtype), w_in, w_out)[0, 0] == y   # 90000 to 8 bits: 176 * 512
+        x, dy = one(1.0, dtype), one(2.0 ** -13, dtype)
+        _, kept = mlp.gated_mlp(x, w_in, w_out * 2.0 ** -14, keep=True)
+        dx, dw_in, _ = mlp.gated_mlp_backward(dy, x, w_in, w_out * 2.0 ** -14, kept)
+        assert bool((dw_in == 0).all()) == bool((dx == 0).all()) == zero
+
+
 def test_gated_mlp_not_finite(device):
     """A token's not-finite value stays in its row of y and dx, whatever rows share its tile."""
     x, dy, w_in, w_out = _operands(5, 40, 64, 64, torch.bfloat16, device)
