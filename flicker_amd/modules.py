@@ -143,7 +143,8 @@ def single_attention(linear1_out, q_scale, k_scale, freqs: Freqs | PositionIds, 
 def mlp_section(x, shift, scale, w_in, w_out):
     """modules.py:157-167 (per stream) -- a double block's MLP: the gated MLP of modulate(x, shift, scale), before
     the block's gate and residual.  x (B, L, hidden) bf16 or fp16, shift and scale (B, hidden) or (B, 1, hidden),
-    w_in (hidden, 2 * mlp), w_out (mlp, hidden).  Its gradients are those of ``norm.modulate`` and
-    ``mlp.gated_mlp``, or ``autograd``'s."""
+    w_in (hidden, 2 * mlp), w_out (mlp, hidden).  Not recorded by torch's autograd, whatever requires gradients: a
+    program that trains calls ``autograd.gated_mlp(autograd.modulate(x, shift, scale), w_in, w_out)``, or the
+    ``*_backward`` functions of ``norm`` and ``mlp``."""
     from . import mlp, norm
     return mlp.gated_mlp(norm.modulate(x, shift, scale), w_in, w_out)
