@@ -1,10 +1,10 @@
 """``norm`` and ``mlp`` under torch's autograd: the same functions, differentiable.
 
 Each call records the matching ``*_backward`` call; first derivatives only, and no forward mode (an operand
-with a tangent raises NotImplementedError).  They are not captured into a HIP
-graph with gradients: autograd accumulates into a leaf on the stream of whichever graph of that leaf is
-alive, which need not be the captured one, so such a call is refused -- capture the explicit forward
-and backward calls of ``norm`` and ``mlp`` instead, which touch no leaves.
+with a tangent raises NotImplementedError).  They are not captured into a HIP graph with gradients: autograd
+accumulates into a leaf on the stream of whichever graph of that leaf is alive, which need not be the captured
+one, so such a call is refused -- capture the explicit forward and backward calls of ``norm`` and ``mlp``
+instead, which touch no leaves.
 """
 
 from __future__ import annotations

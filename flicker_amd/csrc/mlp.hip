@@ -144,7 +144,7 @@ struct Half {
   uint32_t touched;
 
   // rows / terms beyond the operand repeat its last one; results of repeated rows are never stored, and
-  // repeated terms are never fetched (tail).  kPair: see pair_column.
+  // repeated terms are never fetched (tail).
   template <typename Column>
   __device__ __forceinline__ void init(const Operand& o, int64_t first, int wave, int lane, Column column) {
     const int64_t pitch = o.stride * 2;
@@ -160,7 +160,8 @@ struct Half {
     }
   }
   // Touches one 128-byte line a lane of a stage far ahead, so that the L2 has it when the copies come: line i of
-  // the half.  What it brings lands in LDS that nothing reads.
+  // the half.  What it brings lands in LDS that nothing reads.  Across, where a half's columns are 48 of g and 48 of
+  // u in turn (the gate on Medium), columns 64 i are not where its lines begin: some of them are left out.
   template <typename Column>
   __device__ __forceinline__ void init_touch(const Operand& o, int i, Column column) {
     if constexpr (kAcross)
@@ -615,7 +616,9 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // estimated time over tiles and numbers of ranges.  A tile's blocks run in rounds of what the GPU
 // holds; a stage takes the measured time below with one or two blocks on a CU, a round some more to
 // fill its first stages and to write its tiles, and split products pay a second launch and write
-// and read their partial sums (6 TB/s, mostly from the caches).  splits 0: no tile's launch holds the product.
+// and read their partial sums (6 TB/s, mostly from the caches).  What an epilogue reads and writes is not counted: of
+// 2961 tokens, 1000 wide, the gate that keeps g and u over 2728 columns takes 72 us where this says 47, its
+// backward pass 52 for 24; the tiles compared pay about the same for it.  splits 0: no tile's launch holds the product.
 Choice choose(int64_t rows, int64_t cols, int64_t inner, bool a_across) {
   struct Cost {
     int rows, cols, per_cu;

@@ -16,8 +16,8 @@
 // one barrier a row, forwards and backwards.
 //
 // HBM bounds both directions: a row is read once and held in registers, one 8-element chunk a lane
-// (two past 8192 columns), so a lane owns few columns and a CU has many rows in flight.  The
-// backward pass recomputes m and q from the row it has to read anyway, so the forward pass
+// (two past 8192 columns, where the backward pass spills 14 registers, 28 with float32 rows), so a lane owns
+// few columns and a CU has many rows in flight.  The backward pass recomputes m and q from the row it has to read anyway, so the forward pass
 // keeps nothing.  Its column sums stay in the lanes that own the columns while a block walks its
 // rows; blocks write them as partial rows, which a second kernel adds in a fixed order: the
 // gradients do not depend on timing.
@@ -28,11 +28,14 @@
 //
 // Measured (bf16, width 3 * 1024, among other passes): forward 4 x 4096 rows in 41.7 us, 4.8 TB/s (a large copy's
 // rate is 5.2), backward 4608 rows in 24.9 us (85 MB of operands, and 13 MB of partial rows written and read); 512
-// rows in 4.1 and 11 us, launches and the latency of a few rows each.  What it took, at 4 x 4096 rows: a wave a
+// rows in 4.1 and 11 us: a launch and three latencies one after the other, the factor's, the offset's and the first
+// row's.  Widths past 8192, 1000 x 16384: 12.6 us forward, 39 backward (2.5 TB/s), float32 27 and 77.  What it took, at 4 x 4096 rows: a wave a
 // row held 48 columns a lane and waited for its reductions with 2 waves a SIMD (65 us forward, 176
 // backward); several waves a row that each add up the others' values from LDS, one after the other, spend 1800
 // cycles a row on that (53, 94), where sixteen lanes take one wave's values each and add them by DPP (46, 69).
-// Fetching more than two rows ahead gains nothing; nor does a join of 16 columns a block.
+// Fetching more than two rows ahead gains nothing as the loop is: its fetches are conditional, and once a turn it waits
+// for all that is outstanding, stores included.  A join of 16 columns a block gains nothing at this width (96 blocks
+// of 64 columns; at 1000 columns they are 32 on 256 CUs, and the join takes 5 us all the same).
 //
 // A row's last chunk starts 8 columns before its end, so that every load is a whole one; the columns that
 // it shares with the lane before are left out of its sums and stores.
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
   // Whether all of this wave's columns count in the row's sums; where not, the others enter as zeros.
   const bool whole = count == (float)(kV * 512);
 
-  // The next kDepth rows are on their way while a row is worked on.
+  // The next kDepth rows are asked for, one as each row is begun; those of the loop's next turn are waited for before it.
   constexpr int kDepth = sizeof(T) == 2 && kV == 1 ? 2 : 1;
   flk::Raw8<T> x[kDepth][kV], g[kBackward ? kDepth : 1][kV];
   auto fetch = [&](int d, int64_t r) {

@@ -10,7 +10,7 @@
 // bf16 from a row of 27648: forward 42 us (6.0 TB/s; 49 through the caches), backward 66 (6.4; 83); a large copy
 // reaches 5.2.  Float32 ones do not: 512 x 9216 forward 10.6 us (past the caches 12.5), backward 17.8 (19.7), 1536 rows
 // between two neighbours that write gu and read h 78 (84) and 103 (112); 4608 rows 90.6 (92.1; 5.6 TB/s) and 150
-// (157; 5.7), the same between neighbours.
+// (157; 5.7), within 2% between neighbours.
 
 #include "elems.h"
 

@@ -407,6 +407,7 @@ def test_autograd_matches_the_explicit_calls(device):
         torch.autograd.grad(autograd.swiglu(gu).sum(), gu, create_graph=True)
 
 
+# The steps are h = 2^-5 and 2 h = 2^-4; the docstring's 1/8 is no step of this test.
 def test_gradients_are_the_forward_pass_differences(device):
     """A float32 norm and gate moved along a direction.  The central difference with h = 1/8 is off by
     h^2 / 6 times the third derivative along it, which the differences with h and 2 h show: their
