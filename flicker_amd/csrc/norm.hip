@@ -23,8 +23,9 @@
 // gradients do not depend on timing.
 //
 // 16-bit y and dx are stored past the caches: 4608 rows forward 13.3 -> 11.0 us, and no slower a product that reads y
-// next (float32: see kStreamBytes); the rows read are not (13.3 -> 16.7: the last cache often has them), nor the
-// partial rows, read again at once.
+// next (float32: see kStreamBytes).  Past 50 MB an elementwise reader finds less of it: 9216 rows 22.0 us alone (through
+// the caches 25.0), 47.5 with such a reader (42.4); 4608 rows 22.1 (22.4).  The rows read are not (13.3 -> 16.7: the last
+// cache often has them), nor the partial rows, read again at once.
 //
 // Measured (bf16, width 3 * 1024, among other passes): forward 4 x 4096 rows in 41.7 us, 4.8 TB/s (a large copy's
 // rate is 5.2), backward 4608 rows in 24.9 us (85 MB of operands, and 13 MB of partial rows written and read); 512
