@@ -34,7 +34,8 @@ def _rounded(exact, dtype):
     return torch.from_numpy(exact).to(torch.float32).to(dtype)
 
 
-# rows, cols, inner: one of everything, tile edges and either side of them, ragged, long inner axes
+# rows, cols, inner: one of everything, edges of the 128-wide tiles and either side of them, ragged, long inner axes (larger
+# tiles: TILES)
 SIZES = [(1, 8, 8), (1, 512, 1000), (3, 64, 96), (16, 128, 64), (17, 136, 72), (33, 8, 2048), (64, 72, 40), (100, 256, 256),
          (129, 248, 136), (255, 264, 200), (257, 512, 64), (300, 1024, 328), (512, 520, 72), (1000, 776, 1160)]
 
