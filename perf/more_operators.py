@@ -96,8 +96,9 @@ def draw(rng):
         else:
             queries = _log_int(rng, 1, min(LONGEST, math.isqrt(MOST_PAIRS // (batch * heads))))
             keys = queries if rng.random() < 0.7 else _log_int(rng, 1, min(LONGEST, MOST_PAIRS // (batch * heads * queries)))
-        mask = rng.choice(("all", "all", "padding", "random", "empty"))
-        text = rng.randint(0, min(keys, TEXT)) if mask in ("padding", "empty") else 0
+        keys = max(keys, 4)     # with one key kept the gradients of q and k are zero, and what is left of them is noise
+        mask = rng.choice(("all", "all", "padding", "random" if keys >= 64 else "all", "empty"))
+        text = rng.randint(0, min(keys - 4, TEXT)) if mask in ("padding", "empty") else 0
         return _attention(None, step, dtype, batch, heads, kv_heads, queries, keys, mask, text,
                           rng.choice(("heads", "tokens")))
     tokens = _log_int(rng, 1, LONGEST // batch)
@@ -197,9 +198,9 @@ def prepare(case, seed):
     dtype, batch = TYPES[case["dtype"]], case["batch"]
     state = {"kind": case["kind"], "step": case["step"]}
     if case["kind"] == "attention":
-        # logits with a deviation of about two, q scaled by 1 / sqrt(DIM)
-        state["q"] = _heads(gen, case, case["heads"], case["queries"], 1.5 / math.sqrt(DIM))
-        state["k"] = _heads(gen, case, case["kv_heads"], case["keys"], 1.5)
+        # norm scales of 1.2: logits with a deviation of 1.4; q comes scaled by 1 / sqrt(DIM)
+        state["q"] = _heads(gen, case, case["heads"], case["queries"], 1.2 / math.sqrt(DIM))
+        state["k"] = _heads(gen, case, case["kv_heads"], case["keys"], 1.2)
         state["v"] = _heads(gen, case, case["kv_heads"], case["keys"], None)
         state["mask"] = _key_mask(gen, case)
         if case["step"] == "train":
@@ -310,8 +311,8 @@ def _framework(s):
         from flicker_amd import attention
         if s["step"] == "forward":
             return attention.attention(s["q"], s["k"], s["v"], key_mask=s["mask"])
-        o, lse = attention.attention(s["q"], s["k"], s["v"], key_mask=s["mask"], keep=True)
-        return o, *attention.attention_backward(s["do"], s["q"], s["k"], s["v"], o, lse, key_mask=s["mask"])
+        o, kept = attention.attention(s["q"], s["k"], s["v"], key_mask=s["mask"], keep=True)
+        return o, *attention.attention_backward(s["do"], s["q"], s["k"], s["v"], kept, key_mask=s["mask"])
     if s["kind"] == "qk_prep":
         from flicker_amd import kernels
         freqs = kernels.Freqs(s["cos"], s["sin"], s["gain"])
