@@ -17,6 +17,7 @@ LIB_PATH = pathlib.Path(__file__).resolve().with_name("libflicker_hip.so")
 
 _p, _i, _i64, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 _ip = ctypes.POINTER(ctypes.c_int)
+_sp = ctypes.POINTER(ctypes.c_int64)
 
 # name -> (restype, argtypes); one entry per function of include/flicker_hip.h
 SIGNATURES = {
@@ -67,6 +68,10 @@ SIGNATURES = {
     "flk_mlp_kernel": (ctypes.c_char_p, [_i, _i, _i, _i]),
     "flk_mlp_gate": (_i, [_p, _i64, _p, _i64, _i, _i, _i, _i, _p, _i64, _p, _p, _i64, _p]),
     "flk_mlp_gate_backward": (_i, [_p, _i64, _p, _i64, _p, _i, _i, _i, _i, _p, _i64, _p, _i64, _p]),
+    "flk_attention_plan": (_i, [_i, _i, _i, _i, _i, _i, _i, _sp]),
+    "flk_attention": (_i, [_p, _sp, _p, _sp, _p, _sp, _i, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _sp, _p, _p, _p, _i64, _p]),
+    "flk_attention_backward": (_i, [*[_p, _sp] * 5, _p, _p, _i, _p, _i64, _i, _i, _i, _i, _i, _i, *[_p, _sp] * 3,
+                                    _p, _i64, _p]),
     "flk_mlp_matmul": (_i, [_p, _i64, _i, _p, _i64, _i, _i, _i, _i, _i, _p, _i64, _p, _i64, _p]),
 }
 

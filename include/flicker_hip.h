@@ -487,6 +487,39 @@ int flk_mlp_matmul(const void* a, int64_t a_row_stride, int a_transposed, const 
                    int b_transposed, int dtype, int rows, int cols, int inner, void* d, int64_t d_row_stride,
                    void* workspace, int64_t workspace_bytes, void* stream);
 
+/* softmax(q k^T) v of any lengths, over the keys that a mask keeps, and its gradients.  q comes scaled.
+ *   q        (batch, heads, queries, head_dim) of type dtype (FLK_BF16, FLK_F16); every tensor's strides are
+ *            three values, from one batch entry, head and row to the next, in elements, multiples of 8; its
+ *            last axis is dense and its pointer 16-byte aligned
+ *   k, v     (batch, kv_heads, keys, head_dim); kv_heads divides heads, and head h reads key head
+ *            h / (heads / kv_heads)
+ *   key_mask (batch, keys) bytes, not zero where the key is kept, or NULL: all are.  What k and v hold
+ *            elsewhere is not read into any result, whatever it is
+ *   o        (batch, heads, queries, head_dim); 0 for a query that keeps no key
+ *   low      o's rounding error in its own type, (batch, queries, heads, head_dim), dense, or NULL
+ *   lse      (batch, heads, queries) float32, log sum exp of each row (-inf for one without keys), or NULL
+ * head_dim is 128 (else FLK_E_UNSUPPORTED); queries and keys at most 2^28, and batch * heads * queries and
+ * batch * kv_heads * keys (lengths rounded up to 32) at most 2^27 (else FLK_E_INVALID).  `workspace` (256-byte
+ * aligned; the plan's bytes for the same sizes, `masked` whether there is a mask) is free again when the
+ * call's kernels have run, and needs no initial value. */
+int flk_attention_plan(int batch, int heads, int kv_heads, int queries, int keys, int masked, int backward,
+                       int64_t* workspace_bytes);
+int flk_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                  const int64_t* v_strides, int dtype, const void* key_mask, int64_t mask_batch_stride, int batch,
+                  int heads, int kv_heads, int queries, int keys, int head_dim, void* o, const int64_t* o_strides,
+                  void* low, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients of flk_attention for d_o, the gradient of o (of o's shape, any strides as above), from the
+ * forward call's operands and its o, low and lse: dq, dk and dv, shaped as q, k and v.  P and dS
+ * are rounded to dtype between the products.  The gradients of masked keys are zero.  Nothing is written when
+ * batch, queries or keys is 0.  Sums are in a fixed order. */
+int flk_attention_backward(const void* d_o, const int64_t* d_o_strides, const void* q, const int64_t* q_strides,
+                           const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                           const void* o, const int64_t* o_strides, const void* low, const float* lse, int dtype,
+                           const void* key_mask, int64_t mask_batch_stride, int batch, int heads, int kv_heads, int queries,
+                           int keys, int head_dim, void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides,
+                           void* dv, const int64_t* dv_strides, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
