@@ -68,6 +68,14 @@ SIGNATURES = {
     "flk_mlp_kernel": (ctypes.c_char_p, [_i, _i, _i, _i]),
     "flk_mlp_gate": (_i, [_p, _i64, _p, _i64, _i, _i, _i, _i, _p, _i64, _p, _p, _i64, _p]),
     "flk_mlp_gate_backward": (_i, [_p, _i64, _p, _i64, _p, _i, _i, _i, _i, _p, _i64, _p, _i64, _p]),
+    "flk_qk_prep_backward_plan": (_i, [_i, _i, _i, _sp]),
+    "flk_qk_prep_backward": (_i, [*[_p, _sp] * 3, _p, _i64, _i64, _p, _p, _i64, _p, _p, _i, _f, _i, _i, _i, _i, _p, _i64, _i64,
+                                  _p, _p, _p, _i64, _p]),
+    "flk_residual_norm": (_i, [*[_p, _i64, _i64] * 2, _i, _p, _p, _p, _i, _i64, _i, _f, _i, _i, _i, *[_p, _i64, _i64] * 2,
+                               _p]),
+    "flk_residual_norm_backward_plan": (_i, [_i, _i, _i, _i, _sp]),
+    "flk_residual_norm_backward": (_i, [*[_p, _i64, _i64] * 4, _i, _p, _p, _i, _i64, _i, _f, _i, _i, _i,
+                                        *[_p, _i64, _i64] * 2, _p, _p, _p, _p, _i64, _p]),
     "flk_attention_plan": (_i, [_i, _i, _i, _i, _i, _i, _i, _sp]),
     "flk_attention": (_i, [_p, _sp, _p, _sp, _p, _sp, _i, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _sp, _p, _p, _p, _i64, _p]),
     "flk_attention_backward": (_i, [*[_p, _sp] * 5, _p, _p, _i, _p, _i64, _i, _i, _i, _i, _i, _i, *[_p, _sp] * 3,

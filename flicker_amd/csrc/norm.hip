@@ -8,6 +8,11 @@
 //   dx_j = q (t_j - mean(t) - n_j mean(t n))
 //   dfactor_j = sum over the rows that share it of dy_j n_j,  doffset_j = sum of dy_j
 //
+// The residual form (modules.py:157-167, between a block's two halves) takes x + gate * branch for x, with a gate row like
+// the factor's; it stores that sum as r beside y.  Backward, with the gradient dr of r that comes in beside dy,
+// everything of the sum's gradient d = dr + dx is known row by row: dx = d, dbranch = gate d, dgate = sum of d branch.  The sum
+// is recomputed in float32 from x and branch, which have to be read anyway for dgate, rather than from the rounded r.
+//
 // All arithmetic is float32 and every output is rounded once.  Sums of squares of an uncentred residual
 // stream, whose tokens sit off zero, would cancel, so each wave centres its part of the row on its own
 // mean, and the waves' (mean, centred squares) are joined by the parallel form of the variance:
@@ -58,8 +63,10 @@ struct Rows {            // row t of batch entry b at p + b * batch_stride + t *
 
 struct NormArgs {
   Rows x, dy, y;         // y: the output (dx backwards)
+  Rows branch, dr, r;    // the residual form's; r: the sum (dbranch backwards)
   const void* factor;    // NULL: 1
   const void* offset;    // NULL: 0
+  const void* gate;      // the residual form's
   int64_t param_stride;  // elements from one batch entry's row to the next (0: one row for all)
   float add;             // a = factor + add
   float eps, inv_width;
@@ -67,7 +74,7 @@ struct NormArgs {
   // Blocks walk `per_block` rows of one group: of one batch entry's, or, where all share the parameters, of all.
   int64_t group_rows;
   int per_block, blocks_per_group;
-  float* partial;        // backward: column sums (block, 2, width), or NULL
+  float* partial;        // backward: column sums (block, 2, width; the residual form 3), or NULL
 };
 
 // Sum over 64 lanes without leaving the registers; every lane ends with the same value.
@@ -172,11 +179,11 @@ struct Walk {
 
 // kOne: a wave takes a row alone, kSlots rows a block; otherwise all of the block's waves take one.  kStream: y and
 // dx leave the caches to others (nontemporal).
-template <typename T, typename P, int kV, bool kOne, bool kNarrow, bool kBackward, bool kStream>
+template <typename T, typename P, int kV, bool kOne, bool kNarrow, bool kBackward, bool kStream, bool kResidual>
 __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const NormArgs A) {
-  constexpr int kSlots = kOne ? 4 : 1;
+  constexpr int kSlots = kOne ? 4 : 1, kSums = kResidual ? 3 : 2;
   __shared__ Exchange ex;
-  __shared__ float sums[kOne && kBackward ? 2 * kV * 8 * 64 : 1];
+  __shared__ float sums[kOne && kBackward ? kSums * kV * 8 * 64 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int waves = kOne ? 1 : blockDim.x >> 6, slot = kOne ? wave : 0;
   const int lanes = 64 * waves, width = A.width;
@@ -195,7 +202,8 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
 
   const P* factor = static_cast<const P*>(A.factor);
   const P* offset = static_cast<const P*>(A.offset);
-  float a[kV][8], o[kBackward ? 1 : kV][8];
+  const P* gate = static_cast<const P*>(A.gate);
+  float a[kV][8], o[kBackward ? 1 : kV][8], gt[kResidual ? kV : 1][8];
 #pragma unroll
   for (int c = 0; c < kV; ++c) {
     flk::Raw8<P> raw{};
@@ -207,21 +215,31 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[c][i] = offset ? (float)raw.v[i] : 0.0f;
     }
+    if constexpr (kResidual) {
+      raw = chunks.load(gate + walk.group * A.param_stride, c, width);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) gt[c][i] = (float)raw.v[i];
+    }
   }
-  float da[kBackward ? kV : 1][8] = {}, dc[kBackward ? kV : 1][8] = {};
+  float da[kBackward ? kV : 1][8] = {}, dc[kBackward ? kV : 1][8] = {}, dg[kBackward && kResidual ? kV : 1][8] = {};
   // Whether all of this wave's columns count in the row's sums; where not, the others enter as zeros.
   const bool whole = count == (float)(kV * 512);
 
   // The next kDepth rows are asked for, one as each row is begun; those of the loop's next turn are waited for before it.
   constexpr int kDepth = sizeof(T) == 2 && kV == 1 ? 2 : 1;
-  flk::Raw8<T> x[kDepth][kV], g[kBackward ? kDepth : 1][kV];
+  flk::Raw8<T> x[kDepth][kV], g[kBackward ? kDepth : 1][kV], br[kResidual ? kDepth : 1][kV];
+  flk::Raw8<T> gr[kBackward && kResidual ? kDepth : 1][kV];
   auto fetch = [&](int d, int64_t r) {
     const T* px = walk.template row<T>(A, A.x, r);
     const T* pg = kBackward ? walk.template row<T>(A, A.dy, r) : nullptr;
+    const T* pb = kResidual ? walk.template row<T>(A, A.branch, r) : nullptr;
+    const T* pr = kResidual && kBackward ? walk.template row<T>(A, A.dr, r) : nullptr;
 #pragma unroll
     for (int c = 0; c < kV; ++c) {
       x[d][c] = chunks.load(px, c, width);
+      if constexpr (kResidual) br[d][c] = chunks.load(pb, c, width);
       if constexpr (kBackward) g[d][c] = chunks.load(pg, c, width);
+      if constexpr (kBackward && kResidual) gr[d][c] = chunks.load(pr, c, width);
     }
   };
 #pragma unroll
@@ -229,13 +247,23 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
     if (walk.first + d * kSlots < walk.end) fetch(d, walk.first + d * kSlots);
   auto work = [&](int d, int64_t r) {
     float xs[kV][8], gs[kBackward ? kV : 1][8];
+    flk::Raw8<T> bs[kResidual ? kV : 1], rs[kBackward && kResidual ? kV : 1];
 #pragma unroll
     for (int c = 0; c < kV; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         xs[c][i] = (float)x[d][c].v[i];
+        if constexpr (kResidual) xs[c][i] += gt[c][i] * (float)br[d][c].v[i];
         if constexpr (kBackward) gs[c][i] = (float)g[d][c].v[i];
       }
+    if constexpr (kResidual) {
+#pragma unroll
+      for (int c = 0; c < kV; ++c) {
+        bs[c] = br[d][c];
+        if constexpr (kBackward) rs[c] = gr[d][c];
+        else chunks.template store<kStream>(walk.template row<T>(A, A.r, r), c, width, xs[c]);
+      }
+    }
     if (r + kDepth * kSlots < walk.end) fetch(d, r + kDepth * kSlots);
     auto leave_out = [&](float (&v)[8], int c) {
 #pragma unroll
@@ -286,11 +314,20 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
         if constexpr (kBackward) {
           out[i] = gs[c][i] * a[c][i] * st.rstd - mt - n * mtn;
           da[c][i] += gs[c][i] * n;
+          if constexpr (kResidual) {
+            out[i] += (float)rs[c].v[i];
+            dg[c][i] += out[i] * (float)bs[c].v[i];
+          }
         } else {
           out[i] = n * a[c][i] + o[c][i];
         }
       }
       chunks.template store<kStream>(y, c, width, out);
+      if constexpr (kBackward && kResidual) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] *= gt[c][i];
+        chunks.template store<kStream>(walk.template row<T>(A, A.r, r), c, width, out);
+      }
     }
   };
   for (int64_t r = walk.first; r < walk.end; r += kDepth * kSlots) {
@@ -310,6 +347,7 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
             if (slot == s) {
               sums[(c * 8 + i) * 64 + lane] = da[c][i];
               sums[(kV * 8 + c * 8 + i) * 64 + lane] = dc[c][i];
+              if constexpr (kResidual) sums[(kV * 16 + c * 8 + i) * 64 + lane] = dg[c][i];
             }
         __syncthreads();
 #pragma unroll
@@ -319,15 +357,17 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
             if (slot == 0) {
               da[c][i] += sums[(c * 8 + i) * 64 + lane];
               dc[c][i] += sums[(kV * 8 + c * 8 + i) * 64 + lane];
+              if constexpr (kResidual) dg[c][i] += sums[(kV * 16 + c * 8 + i) * 64 + lane];
             }
       }
       if (slot) return;
     }
-    float* out = A.partial + (int64_t)blockIdx.x * 2 * width;
+    float* out = A.partial + (int64_t)blockIdx.x * kSums * width;
 #pragma unroll
     for (int c = 0; c < kV; ++c) {
       chunks.template store<false>(out, c, width, da[c]);
       chunks.template store<false>(out + width, c, width, dc[c]);
+      if constexpr (kResidual) chunks.template store<false>(out + 2 * width, c, width, dg[c]);
     }
   }
 }
@@ -336,20 +376,20 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
 // waves' sums in order.
 constexpr int kJoinWaves = 16;
 template <typename P>
-__global__ __launch_bounds__(64 * kJoinWaves) void norm_params_kernel(const float* __restrict__ partial, int blocks,
-                                                                      int width, int cuts, P* dfactor, P* doffset) {
+__global__ __launch_bounds__(64 * kJoinWaves) void norm_params_kernel(const float* __restrict__ partial, int blocks, int width,
+                                                                      int cuts, P* dfactor, P* doffset, P* dgate) {
   __shared__ float part[kJoinWaves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t group = blockIdx.x / cuts;
   const int col = (int)(blockIdx.x - group * cuts) * 64 + lane;
-  const int which = blockIdx.y;              // 0: factor, 1: offset
-  P* out = which ? doffset : dfactor;
+  const int which = blockIdx.y, sums = gridDim.y;   // 0: factor, 1: offset, 2: gate
+  P* out = which == 2 ? dgate : which ? doffset : dfactor;
   if (!out) return;
-  const float* src = partial + group * blocks * 2 * width + (int64_t)which * width + col;
+  const float* src = partial + group * blocks * sums * width + (int64_t)which * width + col;
   float sum = 0.0f;
   if (col < width) {
 #pragma unroll 4
-    for (int i = wave; i < blocks; i += kJoinWaves) sum += src[(int64_t)i * 2 * width];
+    for (int i = wave; i < blocks; i += kJoinWaves) sum += src[(int64_t)i * sums * width];
   }
   part[wave][lane] = sum;
   __syncthreads();
@@ -394,19 +434,21 @@ int backward_rows(int64_t group_rows, int64_t groups, int width) {
 // Threads of a block.
 int threads_of(int width) { return width <= 512 ? 256 : std::min(((width + 7) / 8 + 63) / 64, kMaxWaves) * 64; }
 
+int sums_of(const NormArgs& a) { return a.gate ? 3 : 2; }   // column sums of the backward pass
+
 // Group g's rows and parameters.
 template <typename T, typename P>
 NormArgs from_group(NormArgs a, int64_t g) {
   if (g == 0) return a;   // the only one where the groups are not batch entries
-  for (Rows* r : {&a.x, &a.dy, &a.y})
+  for (Rows* r : {&a.x, &a.dy, &a.y, &a.branch, &a.dr, &a.r})
     if (r->p) r->p = static_cast<const T*>(r->p) + g * r->batch_stride;
-  for (const void** p : {&a.factor, &a.offset})
+  for (const void** p : {&a.factor, &a.offset, &a.gate})
     if (*p) *p = static_cast<const P*>(*p) + g * a.param_stride;
-  if (a.partial) a.partial += g * a.blocks_per_group * 2 * a.width;
+  if (a.partial) a.partial += g * a.blocks_per_group * sums_of(a) * a.width;
   return a;
 }
 
-template <typename T, typename P, bool kBackward, bool kStream>
+template <typename T, typename P, bool kBackward, bool kStream, bool kResidual>
 int launch(const NormArgs& all, int64_t groups, hipStream_t s) {
   const int threads = threads_of(all.width);
   const int64_t most = kMaxItems / threads / all.blocks_per_group;   // groups of one launch
@@ -414,52 +456,58 @@ int launch(const NormArgs& all, int64_t groups, hipStream_t s) {
     const NormArgs a = from_group<T, P>(all, first);
     const dim3 grid((unsigned)(std::min(most, groups - first) * a.blocks_per_group));
     if (a.width < 8)
-      norm_kernel<T, P, 1, true, true, kBackward, kStream><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 1, true, true, kBackward, kStream, kResidual><<<grid, threads, 0, s>>>(a);
     else if (a.width <= 512)
-      norm_kernel<T, P, 1, true, false, kBackward, kStream><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 1, true, false, kBackward, kStream, kResidual><<<grid, threads, 0, s>>>(a);
     else if (a.width <= 512 * kMaxWaves)
-      norm_kernel<T, P, 1, false, false, kBackward, kStream><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 1, false, false, kBackward, kStream, kResidual><<<grid, threads, 0, s>>>(a);
     else
-      norm_kernel<T, P, 2, false, false, kBackward, kStream><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 2, false, false, kBackward, kStream, kResidual><<<grid, threads, 0, s>>>(a);
     if (const int st = flk_launch_status()) return st;
   }
   return FLK_OK;
 }
 
-template <typename T, typename P, bool kBackward>
+template <typename T, typename P, bool kBackward, bool kResidual>
 int dispatch(const NormArgs& a, int64_t groups, hipStream_t s) {
   if constexpr (sizeof(T) == 4)
-    if (a.group_rows * groups * a.width * 4 > kStreamBytes) return launch<T, P, kBackward, false>(a, groups, s);
-  return launch<T, P, kBackward, true>(a, groups, s);
+    if (a.group_rows * groups * a.width * 4 > kStreamBytes) return launch<T, P, kBackward, false, kResidual>(a, groups, s);
+  return launch<T, P, kBackward, true, kResidual>(a, groups, s);
 }
 
 template <typename P>
-int join_params(const NormArgs& a, int64_t groups, void* dfactor, void* doffset, hipStream_t s) {
+int join_params(const NormArgs& a, int64_t groups, void* dfactor, void* doffset, void* dgate, hipStream_t s) {
   const int cuts = (a.width + 63) / 64;
-  const int64_t most = kMaxItems / (64 * kJoinWaves) / cuts;
+  const int64_t most = kMaxItems / (64 * kJoinWaves) / sums_of(a) / cuts;
   for (int64_t first = 0; first < groups; first += most) {
-    const dim3 grid((unsigned)(std::min(most, groups - first) * cuts), 2);
-    P* df = static_cast<P*>(dfactor);
-    P* dc = static_cast<P*>(doffset);
-    norm_params_kernel<P><<<grid, 64 * kJoinWaves, 0, s>>>(a.partial + first * a.blocks_per_group * 2 * a.width,
-                                                           a.blocks_per_group, a.width, cuts,
-                                                           df ? df + first * a.width : nullptr,
-                                                           dc ? dc + first * a.width : nullptr);
+    const dim3 grid((unsigned)(std::min(most, groups - first) * cuts), sums_of(a));
+    auto rows = [&](void* p) { return p ? static_cast<P*>(p) + first * a.width : nullptr; };
+    norm_params_kernel<P><<<grid, 64 * kJoinWaves, 0, s>>>(a.partial + first * a.blocks_per_group * sums_of(a) * a.width,
+                                                           a.blocks_per_group, a.width, cuts, rows(dfactor),
+                                                           rows(doffset), rows(dgate));
     if (const int st = flk_launch_status()) return st;
   }
   return FLK_OK;
 }
 
-template <bool kBackward>
+// Adds the column sums up, where there are any.
+int join_types(int params, const NormArgs& a, int64_t groups, void* dfactor, void* doffset, void* dgate, hipStream_t s) {
+  if (!a.partial) return FLK_OK;
+  if (params == FLK_F32) return join_params<float>(a, groups, dfactor, doffset, dgate, s);
+  if (params == FLK_BF16) return join_params<__bf16>(a, groups, dfactor, doffset, dgate, s);
+  return join_params<_Float16>(a, groups, dfactor, doffset, dgate, s);
+}
+
+template <bool kBackward, bool kResidual>
 int dispatch_types(int dtype, int params, const NormArgs& a, int64_t groups, hipStream_t s) {
-  if (dtype == FLK_F32) return params == FLK_F32 ? dispatch<float, float, kBackward>(a, groups, s) : FLK_E_UNSUPPORTED;
+  if (dtype == FLK_F32) return params == FLK_F32 ? dispatch<float, float, kBackward, kResidual>(a, groups, s) : FLK_E_UNSUPPORTED;
   if (dtype == FLK_BF16) {
-    if (params == FLK_BF16) return dispatch<__bf16, __bf16, kBackward>(a, groups, s);
-    if (params == FLK_F32) return dispatch<__bf16, float, kBackward>(a, groups, s);
+    if (params == FLK_BF16) return dispatch<__bf16, __bf16, kBackward, kResidual>(a, groups, s);
+    if (params == FLK_F32) return dispatch<__bf16, float, kBackward, kResidual>(a, groups, s);
   }
   if (dtype == FLK_F16) {
-    if (params == FLK_F16) return dispatch<_Float16, _Float16, kBackward>(a, groups, s);
-    if (params == FLK_F32) return dispatch<_Float16, float, kBackward>(a, groups, s);
+    if (params == FLK_F16) return dispatch<_Float16, _Float16, kBackward, kResidual>(a, groups, s);
+    if (params == FLK_F32) return dispatch<_Float16, float, kBackward, kResidual>(a, groups, s);
   }
   return FLK_E_UNSUPPORTED;
 }
@@ -512,7 +560,7 @@ extern "C" int flk_layer_norm(const void* x, int64_t x_batch_stride, int64_t x_r
   const int64_t groups = param_batch_stride ? batch : 1;
   a.per_block = forward_rows(a.group_rows, groups, width);
   a.blocks_per_group = (int)((a.group_rows + a.per_block - 1) / a.per_block);
-  return dispatch_types<false>(dtype, params_dtype, a, groups, static_cast<hipStream_t>(stream));
+  return dispatch_types<false, false>(dtype, params_dtype, a, groups, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int flk_layer_norm_backward_plan(int batch, int length, int width, int shared_params,
@@ -553,9 +601,77 @@ extern "C" int flk_layer_norm_backward(const void* dy, int64_t dy_batch_stride, 
     a.partial = static_cast<float*>(workspace);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (const int st = dispatch_types<true>(dtype, params_dtype, a, groups, s)) return st;
-  if (!a.partial) return FLK_OK;
-  if (params_dtype == FLK_F32) return join_params<float>(a, groups, dfactor, doffset, s);
-  if (params_dtype == FLK_BF16) return join_params<__bf16>(a, groups, dfactor, doffset, s);
-  return join_params<_Float16>(a, groups, dfactor, doffset, s);
+  if (const int st = dispatch_types<true, false>(dtype, params_dtype, a, groups, s)) return st;
+  return join_types(params_dtype, a, groups, dfactor, doffset, nullptr, s);
+}
+
+extern "C" int flk_residual_norm(const void* x, int64_t x_batch_stride, int64_t x_row_stride, const void* branch,
+                                 int64_t branch_batch_stride, int64_t branch_row_stride, int dtype, const void* gate,
+                                 const void* factor, const void* offset, int params_dtype, int64_t param_batch_stride,
+                                 int add_one, float eps, int batch, int length, int width, void* r, int64_t r_batch_stride,
+                                 int64_t r_row_stride, void* y, int64_t y_batch_stride, int64_t y_row_stride,
+                                 void* stream) {
+  if (const int st = check(dtype, params_dtype, x, y, factor, offset, param_batch_stride, eps, batch, length, width))
+    return st;
+  if (const int st = check(dtype, params_dtype, branch, r, gate, nullptr, param_batch_stride, eps, batch, length, width))
+    return st;
+  if (batch == 0 || length == 0) return FLK_OK;
+  if (!gate) return FLK_E_INVALID;
+  NormArgs a = common_args(x, x_batch_stride, x_row_stride, factor, offset, param_batch_stride, add_one, eps, batch,
+                           length, width);
+  a.y = Rows{y, y_batch_stride, y_row_stride};
+  a.branch = Rows{branch, branch_batch_stride, branch_row_stride};
+  a.r = Rows{r, r_batch_stride, r_row_stride};
+  a.gate = gate;
+  const int64_t groups = param_batch_stride ? batch : 1;
+  a.per_block = forward_rows(a.group_rows, groups, width);
+  a.blocks_per_group = (int)((a.group_rows + a.per_block - 1) / a.per_block);
+  return dispatch_types<false, true>(dtype, params_dtype, a, groups, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int flk_residual_norm_backward_plan(int batch, int length, int width, int shared_params,
+                                               int64_t* workspace_bytes) {
+  if (const int st = flk_layer_norm_backward_plan(batch, length, width, shared_params, workspace_bytes)) return st;
+  *workspace_bytes = *workspace_bytes / 2 * 3;
+  return FLK_OK;
+}
+
+extern "C" int flk_residual_norm_backward(const void* dr, int64_t dr_batch_stride, int64_t dr_row_stride, const void* dy,
+                                          int64_t dy_batch_stride, int64_t dy_row_stride, const void* x,
+                                          int64_t x_batch_stride, int64_t x_row_stride, const void* branch,
+                                          int64_t branch_batch_stride, int64_t branch_row_stride, int dtype,
+                                          const void* gate, const void* factor, int params_dtype,
+                                          int64_t param_batch_stride, int add_one, float eps, int batch, int length,
+                                          int width, void* dx, int64_t dx_batch_stride, int64_t dx_row_stride,
+                                          void* dbranch, int64_t dbranch_batch_stride, int64_t dbranch_row_stride,
+                                          void* dgate, void* dfactor, void* doffset, void* workspace,
+                                          int64_t workspace_bytes, void* stream) {
+  const struct {
+    const void *in, *out, *row, *sum;
+  } all[] = {{x, dx, factor, dfactor}, {branch, dbranch, gate, dgate}, {dy, dx, nullptr, doffset}, {dr, dx, nullptr, nullptr}};
+  for (const auto& t : all)
+    if (const int st = check(dtype, params_dtype, t.in, t.out, t.row, t.sum, param_batch_stride, eps, batch, length, width))
+      return st;
+  if (batch == 0 || length == 0) return FLK_OK;   // the sums over no rows are the caller's to clear
+  if (!gate) return FLK_E_INVALID;
+  NormArgs a = common_args(x, x_batch_stride, x_row_stride, factor, nullptr, param_batch_stride, add_one, eps, batch,
+                           length, width);
+  a.dy = Rows{dy, dy_batch_stride, dy_row_stride};
+  a.dr = Rows{dr, dr_batch_stride, dr_row_stride};
+  a.branch = Rows{branch, branch_batch_stride, branch_row_stride};
+  a.y = Rows{dx, dx_batch_stride, dx_row_stride};
+  a.r = Rows{dbranch, dbranch_batch_stride, dbranch_row_stride};
+  a.gate = gate;
+  const int64_t groups = param_batch_stride ? batch : 1;
+  a.per_block = backward_rows(a.group_rows, groups, width);
+  a.blocks_per_group = (int)((a.group_rows + a.per_block - 1) / a.per_block);
+  if (dgate || dfactor || doffset) {
+    const int64_t need = groups * a.blocks_per_group * 3 * width * 4;
+    if (!workspace || workspace_bytes < need) return FLK_E_SCRATCH;
+    if (!flk_host_aligned(workspace, 16)) return FLK_E_ALIGN;
+    a.partial = static_cast<float*>(workspace);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (const int st = dispatch_types<true, true>(dtype, params_dtype, a, groups, s)) return st;
+  return join_types(params_dtype, a, groups, dfactor, doffset, dgate, s);
 }

@@ -5,6 +5,7 @@ tensors on an MI355X; every computation runs in the HIP kernels of libflicker_hi
 
   Freqs, EPS, ROW_TILES, row_tile, lane_pair     kernels.py:12-31
   qk_prep                                         kernels.py:57-91  -> flk_qk_prep
+  qk_prep_backward  its gradients                 -> flk_qk_prep_backward
   SCORE_TILES, EXP_LIMIT, logit_bound             kernels.py:94-101
   attend                                          kernels.py:105-145 -> flk_attend
   attend_merged = merge_heads(attend(...))        + modules.py:63-65 -> flk_attend_to
@@ -19,6 +20,7 @@ accepts ``PositionIds``: the kernel then computes the RoPE lanes from the positi
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import NamedTuple
 
@@ -272,6 +274,61 @@ def qk_prep(qkv: torch.Tensor, q_scale: torch.Tensor, k_scale: torch.Tensor,
         raise ValueError(f"qk_prep needs a row tile dividing L={length} (rows={tile_rows})")
     _on_gpu("qkv", qkv)
     return _launch_qk_prep(qkv, q_scale, k_scale, freqs, num_heads, out, out_offset)
+
+
+def qk_prep_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, qkv: torch.Tensor, q_scale: torch.Tensor,
+                     k_scale: torch.Tensor, freqs: Freqs | PositionIds, num_heads: int, *, offset: int = 0,
+                     out: torch.Tensor | None = None):
+    """(dqkv, dq_scale, dk_scale) of ``qk_prep(qkv, q_scale, k_scale, freqs, num_heads)`` for the incoming gradients dq,
+    dk and dv (B, H, L_out, D) bf16 of its outputs, of which it takes the rows from ``offset`` (a stream's place in the joint
+    sequence, as ``out_offset``).  Any L; the roundings inside qk_prep pass gradients through.  ``out`` may be a
+    (B, L, 3*H*D) bf16 view with 16-byte aligned rows (columns of linear1's gradient) that overlaps no operand."""
+    _on_gpu("qkv", qkv)
+    if qkv.dim() != 3:
+        raise ValueError(f"qkv must be (B, L, 3*H*D), got {tuple(qkv.shape)}")
+    if num_heads <= 0:
+        raise ValueError(f"num_heads must be positive, got {num_heads}")
+    scale_shapes = q_scale.shape, k_scale.shape
+    qkv, q_scale, k_scale, freqs, rope, dim = _qk_operands(qkv, q_scale, k_scale, freqs, num_heads)
+    if isinstance(freqs, PositionIds):
+        from .rope import rope_lanes
+        freqs = rope_lanes(rope, freqs.q_gain, freqs.axes_dim, freqs.theta)
+        rope = freqs.cos, freqs.sin
+    cos, sin = rope
+    batch, length, width = qkv.shape
+    grads = []
+    for name, t in (("dq", dq), ("dk", dk), ("dv", dv)):
+        _on_gpu(name, t)
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+        if t.dim() != 4 or t.shape != dq.shape or t.shape[:2] != (batch, num_heads) or t.shape[3] != dim:
+            raise ValueError(f"dq, dk and dv must be ({batch}, {num_heads}, L_out, {dim}) of one shape, got "
+                             f"{tuple(t.shape)} for {name}")
+        if offset < 0 or offset + length > t.shape[2]:
+            raise ValueError(f"offset {offset} + L {length} exceeds the gradients' length {t.shape[2]}")
+        grads.append(_dense_rows(t[:, :, offset:offset + length]))
+    if out is None:
+        out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+    else:
+        _on_gpu("out", out)
+        if (out.shape != qkv.shape or out.dtype != qkv.dtype or out.stride(2) != 1 or out.stride(0) % 8
+                or out.stride(1) % 8 or out.data_ptr() % 16):
+            raise ValueError(f"out must be a bf16 {tuple(qkv.shape)} view with contiguous, 16-byte aligned rows")
+    make = torch.empty if out.numel() else torch.zeros   # sums over no rows
+    dscales = tuple(make(shape, dtype=q_scale.dtype, device=qkv.device) for shape in scale_shapes)
+    if out.numel() == 0:
+        return out, *dscales
+    size = ctypes.c_int64(0)
+    _lib.check(_lib.lib().flk_qk_prep_backward_plan(batch, length, num_heads, ctypes.byref(size)),
+               "flk_qk_prep_backward_plan")
+    ws = torch.empty(size.value, dtype=torch.uint8, device=qkv.device)
+    _lib.run("flk_qk_prep_backward", (*grads, qkv, cos, sin, q_scale, k_scale, out, *dscales, ws),
+             *(x for t in grads for x in (t.data_ptr(), (ctypes.c_int64 * 3)(*t.stride()[:3]))), qkv.data_ptr(),
+             qkv.stride(0), qkv.stride(1), cos.data_ptr(), sin.data_ptr(), cos.stride(0), q_scale.data_ptr(),
+             k_scale.data_ptr(), int(q_scale.dtype == torch.float32), float(freqs.q_gain), batch, length, num_heads, dim,
+             out.data_ptr(), out.stride(0), out.stride(1), dscales[0].data_ptr(), dscales[1].data_ptr(), ws.data_ptr(),
+             size.value, _lib.stream_of(qkv))
+    return out, *dscales
 
 
 SCORE_TILES = (2304, 1536, 1152, 512, 256, 128)

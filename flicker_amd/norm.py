@@ -2,6 +2,8 @@
 
   layer_norm   (x - mean) / sqrt(var + eps) * weight + bias        (src/flicker/nn.py:17-21 is weight = bias = None)
   modulate     (1 + scale) * layer_norm(x) + shift, a row of each per image   (src/flicker/modules.py:38-40)
+  residual_modulate   r = x + gate * branch and modulate of that sum: what ends one part of a block and begins
+               the next                                              (src/flicker/modules.py:157-167, 185-200)
 
 ``*_backward`` take the incoming gradient and the forward call's arguments and return the gradients
 in the order of those arguments; nothing is kept from the forward call.  All arithmetic is
@@ -236,3 +238,68 @@ def modulate_backward(dy: torch.Tensor, x: torch.Tensor, shift: torch.Tensor, sc
     shift_row, scale_row = _modulation(x, shift, scale)
     dx, dscale, dshift = _backward(dy, x, scale_row, (True, True), scale_row.dtype, True, True, eps)
     return dx, dshift.view(shift.shape), dscale.view(scale.shape)
+
+
+def _residual(x, branch, gate, shift, scale):
+    """Checked (gate, shift, scale) rows."""
+    if gate is None:
+        raise TypeError("residual_modulate needs a gate")
+    shift_row, scale_row = _modulation(x, shift, scale)
+    _same("branch", branch, x)
+    batch, _, width = x.shape
+    gate = _param("gate", gate, ((batch, width), (batch, 1, width)), x)
+    if gate.dtype != scale_row.dtype:
+        raise TypeError(f"gate, shift and scale must share one dtype, got {gate.dtype} and {scale_row.dtype}")
+    return _vector(gate), shift_row, scale_row
+
+
+def _same(name: str, t: torch.Tensor, x: torch.Tensor) -> None:
+    _on_gpu(name, t)
+    if t.shape != x.shape or t.dtype != x.dtype:
+        raise ValueError(f"{name} must be {x.dtype} {tuple(x.shape)} like x, got {t.dtype} {tuple(t.shape)}")
+
+
+def _rows(t: torch.Tensor) -> tuple[int, int, int]:
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def residual_modulate(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor, shift: torch.Tensor,
+                      scale: torch.Tensor, *, eps: float = EPS) -> tuple[torch.Tensor, torch.Tensor]:
+    """(r, y) with r = x + gate * branch and y = (1 + scale) * layer_norm(r) + shift: x and branch (B, L, width), one row
+    of gate, shift and scale per batch entry, (B, width) or (B, 1, width).  y is of the unrounded sum."""
+    gate, shift, scale = _residual(x, branch, gate, shift, scale)
+    r, y = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    if x.numel() == 0:
+        return r, y
+    xb, bb = _blocks(x), _blocks(branch)
+    batch, length, width = x.shape
+    _lib.run("flk_residual_norm", (x, branch, gate, scale, shift, r, y), *_rows(xb), *_rows(bb), _CODES[x.dtype],
+             gate.data_ptr(), scale.data_ptr(), shift.data_ptr(), _CODES[scale.dtype], width, 1, float(eps), batch, length,
+             width, *_rows(r), *_rows(y), _lib.stream_of(x))
+    return r, y
+
+
+def residual_modulate_backward(dr: torch.Tensor, dy: torch.Tensor, x: torch.Tensor, branch: torch.Tensor,
+                               gate: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *, eps: float = EPS):
+    """(dx, dbranch, dgate, dshift, dscale) of ``residual_modulate`` for the incoming gradients dr of r and dy of y, the
+    last three shaped as gate, shift and scale."""
+    shapes = gate, shift, scale
+    gate, shift, scale = _residual(x, branch, gate, shift, scale)
+    _same("dr", dr, x)
+    _same("dy", dy, x)
+    batch, length, width = x.shape
+    dx, dbranch = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    make = torch.empty if x.numel() else torch.zeros   # sums over no rows
+    dgate, dshift, dscale = (make(t.shape, dtype=t.dtype, device=x.device) for t in shapes)
+    if x.numel() == 0:
+        return dx, dbranch, dgate, dshift, dscale
+    size = ctypes.c_int64(0)
+    _lib.check(_lib.lib().flk_residual_norm_backward_plan(batch, length, width, 0, ctypes.byref(size)),
+               "flk_residual_norm_backward_plan")
+    ws = torch.empty(size.value, dtype=torch.uint8, device=x.device)
+    rb, yb, xb, bb = (_blocks(t) for t in (dr, dy, x, branch))
+    _lib.run("flk_residual_norm_backward", (dr, dy, x, branch, gate, scale, dx, dbranch, dgate, dscale, dshift, ws),
+             *_rows(rb), *_rows(yb), *_rows(xb), *_rows(bb), _CODES[x.dtype], gate.data_ptr(), scale.data_ptr(),
+             _CODES[scale.dtype], width, 1, float(eps), batch, length, width, *_rows(dx), *_rows(dbranch),
+             dgate.data_ptr(), dscale.data_ptr(), dshift.data_ptr(), ws.data_ptr(), size.value, _lib.stream_of(x))
+    return dx, dbranch, dgate, dshift, dscale

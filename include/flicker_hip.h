@@ -404,6 +404,24 @@ int flk_w8a8_qk_prep_pair(const int8_t* xq0, const int8_t* wq_t0, const float* a
                           int num_heads, int head_dim, void* q_out, void* k_out, void* v_out,
                           int64_t out_length, void* stream);
 
+/* Gradients of flk_qk_prep: of the projection and of both norm scales, for the gradients dq, dk and dv of its
+ * outputs.  The roundings inside qk_prep pass gradients through; sums are float32, in a fixed order.
+ *   dq, dk, dv  (batch, num_heads, length, head_dim) bf16; strides are three values, from one batch entry, head and
+ *            row to the next, in elements, multiples of 8, the last axis dense: rows of a joint sequence's
+ *            gradients are taken in place
+ *   qkv, cos, sin, table_row_stride, q_scale, k_scale, scale_is_f32, q_gain  flk_qk_prep's
+ *   dqkv     (batch, length, 3*num_heads*head_dim) bf16, strides in elements, multiples of 8; v's section is
+ *            dv bit for bit.  It overlaps no operand
+ *   dq_scale, dk_scale  (head_dim,) of the scales' type; not written when batch or length is 0
+ * `workspace` (16-byte aligned, the plan's bytes) needs no initial value. */
+int flk_qk_prep_backward_plan(int batch, int length, int num_heads, int64_t* workspace_bytes);
+int flk_qk_prep_backward(const void* dq, const int64_t* dq_strides, const void* dk, const int64_t* dk_strides,
+                         const void* dv, const int64_t* dv_strides, const void* qkv, int64_t qkv_batch_stride,
+                         int64_t qkv_row_stride, const float* cos, const float* sin, int64_t table_row_stride,
+                         const void* q_scale, const void* k_scale, int scale_is_f32, float q_gain, int batch, int length,
+                         int num_heads, int head_dim, void* dqkv, int64_t dqkv_batch_stride, int64_t dqkv_row_stride,
+                         void* dq_scale, void* dk_scale, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Layer norm over the last axis with a per-channel factor and offset:
  *   y = (x - mean) / sqrt(var + eps) * a + c,  a = factor (+ 1 with add_one), c = offset
  * in float32, rounded once.  Replaces layer_norm (src/flicker/nn.py:17-21) and, with add_one and
@@ -433,6 +451,28 @@ int flk_layer_norm_backward(const void* dy, int64_t dy_batch_stride, int64_t dy_
                             int params_dtype, int64_t param_batch_stride, int add_one, float eps, int batch, int length,
                             int width, void* dx, int64_t dx_batch_stride, int64_t dx_row_stride, void* dfactor,
                             void* doffset, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The layer norm of a gated residual sum, and the sum (modules.py:157-167):
+ *   r = x + gate * branch,  y = the layer norm of r as flk_layer_norm's, of the unrounded sum
+ * x, branch, r and y are laid out as flk_layer_norm's x; gate is a row like factor and not NULL.  r and y overlap
+ * each other and the operands nowhere. */
+int flk_residual_norm(const void* x, int64_t x_batch_stride, int64_t x_row_stride, const void* branch,
+                      int64_t branch_batch_stride, int64_t branch_row_stride, int dtype, const void* gate,
+                      const void* factor, const void* offset, int params_dtype, int64_t param_batch_stride, int add_one,
+                      float eps, int batch, int length, int width, void* r, int64_t r_batch_stride, int64_t r_row_stride,
+                      void* y, int64_t y_batch_stride, int64_t y_row_stride, void* stream);
+
+/* Its gradients for the gradients dr of r and dy of y: dx, dbranch, and the parameters' rows as
+ * flk_layer_norm_backward's (any of them NULL; the workspace is not needed when all are). */
+int flk_residual_norm_backward_plan(int batch, int length, int width, int shared_params, int64_t* workspace_bytes);
+int flk_residual_norm_backward(const void* dr, int64_t dr_batch_stride, int64_t dr_row_stride, const void* dy,
+                               int64_t dy_batch_stride, int64_t dy_row_stride, const void* x, int64_t x_batch_stride,
+                               int64_t x_row_stride, const void* branch, int64_t branch_batch_stride,
+                               int64_t branch_row_stride, int dtype, const void* gate, const void* factor,
+                               int params_dtype, int64_t param_batch_stride, int add_one, float eps, int batch, int length,
+                               int width, void* dx, int64_t dx_batch_stride, int64_t dx_row_stride, void* dbranch,
+                               int64_t dbranch_batch_stride, int64_t dbranch_row_stride, void* dgate, void* dfactor,
+                               void* doffset, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* h = silu(g) * u of gu = [g | u], silu(z) = z / (1 + exp(-z)), in float32, rounded once: the gate of
  * the blocks' MLP (modules.py:157-167, 185-200).
