@@ -26,6 +26,8 @@ from . import _lib
 from .kernels import HEAD_DIM, _on_gpu
 from .norm import _CODES
 
+_MAX_ROW = 1 << 25   # elements between two rows
+
 
 class Kept(NamedTuple):
     """What attention keeps for its backward pass: the o that it returned, ``low``, what o's rounding left of it, in o's
@@ -37,8 +39,9 @@ class Kept(NamedTuple):
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` (B, H, L, D), or a copy where its last axis is not dense or its rows are not 16-byte aligned."""
-    if t.numel() and (t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride(), t.shape[:3]) if n > 1)):
+    """``t`` (B, H, L, D), or a copy where its last axis is not dense or its rows are not 16-byte aligned or too far apart."""
+    if t.numel() and (t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride(), t.shape[:3]) if n > 1)
+                      or (t.shape[2] > 1 and t.stride(2) > _MAX_ROW)):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 

@@ -9,6 +9,7 @@
 // no gradient.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -16,15 +17,16 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kRowBytes = kD * 2;
-constexpr int kTile = 64;              // rows of a staged tile, keys of a mask word
-constexpr int kUnit = 32;              // rows of a unit: the contraction length of one MFMA
+constexpr int kUnit = 32;              // rows of a unit: the contraction length of one MFMA, keys of a mask word
 constexpr int kUnitBytes = kUnit * kRowBytes;
-constexpr int kTileBytes = kTile * kRowBytes;
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;              // two a SIMD
 constexpr int kThreads = 64 * kWaves;
-constexpr int kBlock = 32 * kWaves;    // queries (or keys) of a block, 32 a wave
+constexpr int kQueries = 32 * kWaves;  // queries of a block, 32 a wave
+constexpr int kKeys = 16 * kWaves;     // keys of a block of attention_dkv_kernel, 32 a pair of waves
+constexpr int kLead = 4;               // slots between an operand's LDS read and its MFMAs
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int64_t kMaxItems = 1LL << 31;
+constexpr int64_t kMaxRow = 1LL << 25;   // elements between two rows: a unit's byte offsets stay below 2^31
 
 using flk::f32x4;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -70,11 +72,11 @@ struct Tensor {   // element d of row t of head h of batch entry b at p + b * ba
   }
 };
 
-// What the mask's bytes come to: of batch entry b the words words[b * tiles + t], bit i of word t set where key 64 t + i
-// is kept, the tiles live[b * tiles + n], n < counts[b], whose words are not zero, in order.  NULL words: all are kept.
+// What the mask's bytes come to: of batch entry b the words bits[b * units + u], bit i of word u set where key 32 u + i is
+// kept, and the units live[b * units + n].x, n < counts[b], whose words (.y) are not zero, in order.  NULL: all are kept.
 struct Mask {
-  const uint64_t* words;
-  const int* live;
+  const uint32_t* bits;
+  const uint2* live;
   const int* counts;
 };
 
@@ -82,38 +84,45 @@ struct Args {
   Tensor q, k, v, o, dO, dq, dk, dv;
   void* low;        // (batch, queries, heads, 128): what o's rounding left, in the same type
   float* lse;       // (batch, heads, queries)
-  float* stats;     // (batch, heads, units, 2, 32): a unit's log2(e) lse and -delta; rows past the end inf and 0
+  float* stats;     // (batch * heads * q_units + 1, 2, 32): a unit's log2(e) lse and -delta; inf and 0 in rows past the
+                    // end and in the last unit
   Mask mask;
-  int batch, heads, kv_heads, group, queries, keys, tiles, units;
+  int batch, heads, kv_heads, group, queries, keys, q_units, k_units;
 };
 
-// Which bits of tile t are kept.
-__device__ __forceinline__ uint64_t kept(const Args& A, int b, int t) {
-  if (A.mask.words) return A.mask.words[(int64_t)b * A.tiles + t];
-  const int left = A.keys - t * kTile;
-  return left >= 64 ? ~0ull : (1ull << left) - 1;
-}
-__device__ __forceinline__ int live_tiles(const Args& A, int b) { return A.mask.words ? A.mask.counts[b] : A.tiles; }
-__device__ __forceinline__ int live_tile(const Args& A, int b, int n) {
-  return A.mask.words ? A.mask.live[(int64_t)b * A.tiles + n] : n;
+// Which keys of unit u are kept.
+__device__ __forceinline__ uint32_t kept(const Args& A, int b, int u) {
+  if (A.mask.bits) return A.mask.bits[(int64_t)b * A.k_units + u];
+  const int left = A.keys - u * kUnit;
+  return left >= kUnit ? ~0u : (1u << left) - 1;
 }
 
 __device__ __forceinline__ int swz(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
 
-// Operands of a staged tile, whose 16-byte chunk c of row r sits in place c ^ swz(r).
-struct Places {
-  int row[4];   // 16 rows x 32 d as they are: row lane % 16, d step st
-  int col[8];   // 16 d x 32 rows transposed: d tile dt
+// LDS holds units of 32 rows of 256 bytes, whose 16-byte chunk c of row r sits in place c ^ swz(r).
+struct Places {   // a lane's byte offsets of its operands within a unit
+  int row[4];     // 16 rows x 32 d as they are: row lane % 16, d step st
+  int col[8];     // 16 d x 32 rows transposed: d tile dt
 };
 __device__ __forceinline__ Places places() {
   Places at;
   const int lane = threadIdx.x & 63, h = lane >> 4, col = lane & 15;
+  // k-slots 8h .. 8h + 7 of a row operand are d chunk 4 st + hperm, 0, 2, 1, 3 for h = 0 .. 3: lanes l and l + 32 then read
+  // neighbouring chunks, on distinct banks however the read is split.
   const int hperm = ((h & 1) << 1) | (h >> 1);
 #pragma unroll
-  for (int st = 0; st < 4; ++st) at.row[st] = col * kRowBytes + ((((st << 2) | hperm) ^ swz(col)) << 4);
+  for (int st = 0; st < 4; ++st) {
+    at.row[st] = col * kRowBytes + ((((st << 2) | hperm) ^ swz(col)) << 4);
+    asm volatile("" : "+v"(at.row[st]));
+  }
+  // The transposing read hands lane 4a + b of a lane group element b of its source lanes a, a + 4, a + 8, a + 12: source lane
+  // s of group h points at row 4h + s / 4, d 16 dt + 4 (s % 4), so the k-slots are rows 4h .. + 3 and those + 16.
   const int r = h * 4 + (col >> 2);
 #pragma unroll
-  for (int dt = 0; dt < 8; ++dt) at.col[dt] = r * kRowBytes + (((2 * dt + ((col & 3) >> 1)) ^ swz(r)) << 4) + (col & 1) * 8;
+  for (int dt = 0; dt < 8; ++dt) {
+    at.col[dt] = r * kRowBytes + (((2 * dt + ((col & 3) >> 1)) ^ swz(r)) << 4) + (col & 1) * 8;
+    asm volatile("" : "+v"(at.col[dt]));
+  }
   return at;
 }
 template <typename T>
@@ -126,16 +135,79 @@ __device__ __forceinline__ vec8<T> col_operand(const uint8_t* unit, const Places
   const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(unit + at.col[dt] + 16 * kRowBytes));
   return __builtin_bit_cast(vec8<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-
-// Stages 64 rows from `first`, those that `bits` leaves out as zeros.
-__device__ __forceinline__ void stage(uint8_t* dst, const uint16_t* src, int64_t stride, int first, uint64_t bits) {
-  for (int i = threadIdx.x; i < kTile * 16; i += kThreads) {
-    const int r = i >> 4, c = i & 15;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (bits >> r & 1) x = *reinterpret_cast<const uint4*>(src + (int64_t)(first + r) * stride + c * 8);
-    *reinterpret_cast<uint4*>(dst + r * kRowBytes + ((c ^ swz(r)) << 4)) = x;
-  }
+// P^T or dS^T of group g as the right operand of a product over a unit's rows: the packed words of its two accumulators.
+template <typename T>
+__device__ __forceinline__ vec8<T> packed(const uint32_t (&p)[8], int g) {
+  return __builtin_bit_cast(vec8<T>, make_uint4(p[4 * g], p[4 * g + 1], p[4 * g + 2], p[4 * g + 3]));
 }
+
+// Copies of a tensor's units into LDS: each wave 4 rows of 32, 16 bytes a lane, straight from memory.
+struct Copies {
+  const uint16_t* head;
+  int64_t row;
+  uint32_t at, at_last;   // a lane's source offset in a unit, and in the last, whose rows past the end repeat the last row
+  int last;               // that unit
+  __device__ __forceinline__ Copies(const uint16_t* head, int64_t row, int rows) : head(head), row(row) {
+    const int lane = threadIdx.x & 63, r = (threadIdx.x >> 6) * 4 + (lane >> 4);
+    const uint32_t chunk = ((lane & 15) ^ swz(r)) << 4;
+    last = (rows - 1) / kUnit;
+    at = (uint32_t)(r * row * 2) + chunk;
+    at_last = (uint32_t)(min(r, rows - 1 - last * kUnit) * row * 2) + chunk;
+  }
+  __device__ __forceinline__ void start(uint8_t* slot, int unit) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    flk::dma16_at(head + (int64_t)unit * kUnit * row, unit == last ? at_last : at, slot + wave * 4 * kRowBytes);
+  }
+};
+
+// Clears this wave's rows of a unit that `bits` leaves out: 0 * what they hold would be NaN for infinities.  Their copy has
+// landed; the others see zeros after the next barrier.
+__device__ __forceinline__ void clear_rows(uint8_t* slot, uint32_t bits) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t mine = bits >> (4 * wave) & 15;
+  if (mine == 15) return;
+  if (!(mine >> (lane >> 4) & 1))
+    *reinterpret_cast<uint4*>(slot + wave * 4 * kRowBytes + lane * 16) = make_uint4(0, 0, 0, 0);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+// What the accumulators of a unit's S start from: 0, -inf for the rows (keys) that `bits` leaves out.
+__device__ __forceinline__ f32x4 bias_of(uint32_t bits, int kt) {
+  const uint32_t mine = bits >> (16 * kt + (threadIdx.x >> 4 & 3) * 4);
+  f32x4 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = mine >> i & 1 ? 0.0f : -INFINITY;
+  return x;
+}
+
+// The key units of a batch entry that have kept keys, asked for one after the other from 0; past the last: the last one with
+// no key kept.  A masked entry's list is fetched 64 units at a time, one a lane.
+template <bool kMasked>
+struct Units {
+  const uint2* live;
+  int n;
+  uint32_t tail;
+  uint2 some;
+  __device__ __forceinline__ Units(const Args& A, int b) {
+    if constexpr (kMasked) {
+      n = __builtin_amdgcn_readfirstlane(A.mask.counts[b]);
+      live = A.mask.live + (int64_t)b * A.k_units;
+    } else {
+      n = A.k_units;
+      tail = kept(A, b, n - 1);
+    }
+  }
+  __device__ __forceinline__ void get(int i, int& unit, uint32_t& bits) {
+    if constexpr (kMasked) {
+      if ((i & 63) == 0) some = live[min(i + (int)(threadIdx.x & 63), n - 1)];
+      unit = __builtin_amdgcn_readlane(some.x, i & 63);
+      bits = i < n ? __builtin_amdgcn_readlane(some.y, i & 63) : 0u;
+    } else {
+      unit = min(i, n - 1);
+      bits = i < n - 1 ? ~0u : i == n - 1 ? tail : 0u;
+    }
+  }
+};
 
 // The wave's two groups of 16 rows from row0 as the right operand: row lane % 16 of group g, d step st; zeros past `end`.
 template <typename T>
@@ -181,285 +253,654 @@ __device__ __forceinline__ float across(float x) {   // the four lane groups' su
   return x + __shfl_xor(x, 32);
 }
 
+// The end of an iteration: the copies started one iteration ago have landed (`kCopies` of them a wave and iteration), and
+// every wave's; no wait for LDS reads, which touch nothing that the next copies write.
+template <int kCopies>
+__device__ __forceinline__ void landed() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopies) : "memory");
+}
+__device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
+
 template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_kernel(const Args A) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kTileBytes];
-  const int lane = threadIdx.x & 63, h4 = lane >> 4;
-  const int blocks = (A.queries + kBlock - 1) / kBlock;
-  const int bh = blockIdx.x / blocks, b = bh / A.heads, h = bh - b * A.heads;
-  const int q0 = (blockIdx.x - bh * blocks) * kBlock + (threadIdx.x >> 6) * 32;
-  vec8<T> q[4][2];
-  load_rows<T>(q, A.q.at<T>(b, h), A.q.row, q0, A.queries);
-  const Places at = places();
-  f32x4 acc[8][2] = {};
-  float m[2] = {-1e30f, -1e30f}, l[2] = {}, l_exact[2] = {};   // sums of the rounded and of the unrounded P
-  const int n = live_tiles(A, b);
-  for (int i = 0; i < n; ++i) {
-    const int t = live_tile(A, b, i);
-    const uint64_t bits = kept(A, b, t);
-    __syncthreads();
-    stage(smem, A.k.at<uint16_t>(b, h / A.group), A.k.row, t * kTile, bits);
-    stage(smem + kTileBytes, A.v.at<uint16_t>(b, h / A.group), A.v.row, t * kTile, bits);
-    __syncthreads();
-    for (int u = 0; u < 2; ++u) {
-      f32x4 s[2][2] = {};
+struct Forward {
+  vec8<T> x[4][2];         // Q^T
+  f32x4 acc[8][2];         // O^T
+  vec8<T> ops[2 * kLead];  // operand of slot n in ops[n % (2 kLead)]
+  f32x4 l[2];              // sums of the rounded P (register 0 of lanes 0-15)
+  vec8<T> ones;            // row 0 ones, rows 1-15 zeros
+  float sum[2];            // with kKeep: of the unrounded P, this lane's
+  float top[2], limit[2];  // the maximum that P is taken against, and where it has to rise
+  Places at;
+};
+
+constexpr float kSlack = 6.0f;   // how far S may pass the maximum it is taken against: P stays below 2^9
+
+// Phase u: S(u+1) = K(u+1) Q^T and O^T += V(u-1)^T P(u-1)^T on the matrix pipe while the vector units turn S(u) into P(u).
+template <bool kBias, bool kKeep, typename T, typename Hook>
+__device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur)[4], f32x4 (&s_next)[4],
+                                              const uint32_t (&p_prev)[8], uint32_t (&p_cur)[8], const uint8_t* k_unit,
+                                              const uint8_t* v_unit, const uint8_t* k_after, uint32_t bits_next,
+                                              Hook&& hook) {
+  f32x4 sv[4];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+  for (int i = 0; i < 4; ++i) {
+    sv[i] = s_cur[i];
+    asm volatile("" : "+v"(sv[i]));
+  }
+  // A row's P are exp(S - top) with the top of an earlier unit until S passes it by kSlack: then it rises to the row's
+  // maximum, and what has been summed, P(u-1) among it, is scaled when this phase has added P(u-1).
+  float high[2];
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          const vec8<T> a = row_operand<T>(smem + u * kUnitBytes, at, st, kt);
+  for (int g = 0; g < 2; ++g) {
+    high[g] = fmaxf(fmaxf(sv[2 * g][0], sv[2 * g][1]), sv[2 * g][2]);
+    high[g] = fmaxf(fmaxf(high[g], sv[2 * g][3]), sv[2 * g + 1][0]);
+    high[g] = fmaxf(fmaxf(high[g], sv[2 * g + 1][1]), sv[2 * g + 1][2]);
+    high[g] = fmaxf(high[g], sv[2 * g + 1][3]);
+  }
+  const bool rise = __any(high[0] > w.limit[0] || high[1] > w.limit[1]);
+  float factor[2] = {1.0f, 1.0f};
+  if (rise) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g) s[g][kt] = mfma(a, q[st][g], s[g][kt]);
-        }
-      uint32_t p[2][4];
+    for (int g = 0; g < 2; ++g) {
+      float t = fmaxf(high[g], __shfl_xor(high[g], 16));
+      t = fmaxf(fmaxf(t, __shfl_xor(t, 32)), w.top[g]);
+      factor[g] = __builtin_amdgcn_exp2f((w.top[g] - t) * kLog2e);
+      w.top[g] = t;
+      w.limit[g] = t + kSlack;
+      if constexpr (kKeep) w.sum[g] *= factor[g];
+    }
+  }
+  const float base[2] = {w.top[0] * -kLog2e, w.top[1] * -kLog2e};
+  f32x4 start[2] = {};
+  if constexpr (kBias) {
+    if (bits_next != ~0u) {
+      start[0] = bias_of(bits_next, 0);
+      start[1] = bias_of(bits_next, 1);
+    }
+  }
+  float t[16], e[16];
+  auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, base[n >> 3]); };
+  auto exp = [&](int n) { e[n] = __builtin_amdgcn_exp2f(t[n]); };
+  auto put = [&](int n) {
+    p_cur[n >> 1] = pack<T>(e[n], e[n + 1]);
+    asm volatile("" : "+v"(p_cur[n >> 1]));   // keeps the pack in its slot
+    if constexpr (kKeep) w.sum[n >> 3] += e[n] + e[n + 1];
+  };
+  const vec8<T> pb[2] = {packed<T>(p_prev, 0), packed<T>(p_prev, 1)};
+  scaled(0);
+  scaled(1);
+  exp(0);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        float top = m[g];
+  for (int n = 0; n < 16; ++n) {
+    const vec8<T>& a = w.ops[n % (2 * kLead)];
+    if (n < 8) {
+      const int st = n >> 1, kt = n & 1;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool on = bits >> (u * 32 + (e >> 2) * 16 + h4 * 4 + (e & 3)) & 1;
-          s[g][e >> 2][e & 3] = on ? s[g][e >> 2][e & 3] * kLog2e : -INFINITY;
-          top = fmaxf(top, s[g][e >> 2][e & 3]);
-        }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float f = __builtin_amdgcn_exp2f(m[g] - top);
-        m[g] = top;
-        l[g] *= f;
-        l_exact[g] *= f;
+      for (int g = 0; g < 2; ++g)
+        s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : kBias ? start[kt] : f32x4{});
+    } else {
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) acc[dt][g] *= f;
+      for (int g = 0; g < 2; ++g) w.acc[n - 8][g] = mfma(a, pb[g], w.acc[n - 8][g]);
+      if (n == 15) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x0 = __builtin_amdgcn_exp2f(s[g][e >> 1][(e & 1) * 2] - top);
-          const float x1 = __builtin_amdgcn_exp2f(s[g][e >> 1][(e & 1) * 2 + 1] - top);
-          l[g] += (float)(T)x0 + (float)(T)x1;
-          l_exact[g] += x0 + x1;
-          p[g][e] = pack<T>(x0, x1);
-        }
-      }
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) {
-        const vec8<T> a = col_operand<T>(smem + kTileBytes + u * kUnitBytes, at, dt);
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-          acc[dt][g] = mfma(a, __builtin_bit_cast(vec8<T>, make_uint4(p[g][0], p[g][1], p[g][2], p[g][3])), acc[dt][g]);
+        for (int g = 0; g < 2; ++g) w.l[g] = mfma(w.ones, pb[g], w.l[g]);
       }
     }
+    const int m = n + kLead;
+    vec8<T>& to = w.ops[m % (2 * kLead)];
+    if (m < 8) to = row_operand<T>(k_unit, w.at, m >> 1, m & 1);
+    else if (m < 16) to = col_operand<T>(v_unit, w.at, m - 8);
+    else to = row_operand<T>(k_after, w.at, (m - 16) >> 1, m & 1);
+    if (n + 2 < 16) scaled(n + 2);
+    if (n + 1 < 16) exp(n + 1);
+    if (n & 1) put(n - 1);
+    hook(n);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (rise) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] *= factor[g];
+      // l's row 0 sits in the lanes 0-15, whose columns are these queries
+      w.l[g] *= factor[g];
+    }
+  }
+}
+
+constexpr int kKRing = 4, kVRing = 4;   // forward: units of K and of V in LDS
+
+template <typename T, bool kMasked, bool kKeep>
+__global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[(kKRing + kVRing) * kUnitBytes];
+  const int lane = threadIdx.x & 63, h4 = lane >> 4;
+  const int blocks = (A.queries + kQueries - 1) / kQueries;
+  const int bh = blockIdx.x / blocks, b = bh / A.heads, h = bh - b * A.heads;
+  const int q0 = (blockIdx.x - bh * blocks) * kQueries + (threadIdx.x >> 6) * 32;
+  Units<kMasked> units(A, b);
+  const int n = units.n;
+  Forward<T> w;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
+    w.l[g] = f32x4{};
+    w.sum[g] = 0.0f;
+    w.top[g] = w.limit[g] = -1e30f;
+  }
+  if (n) {
+    auto k_slot = [&](int i) { return smem + (i & (kKRing - 1)) * kUnitBytes; };
+    auto v_slot = [&](int i) { return smem + (kKRing + (i & (kVRing - 1))) * kUnitBytes; };
+    const Copies kc(A.k.at<uint16_t>(b, h / A.group), A.k.row, A.keys), vc(A.v.at<uint16_t>(b, h / A.group), A.v.row, A.keys);
+    int unit[5];          // of the iterations u .. u + 4
+    uint32_t bits[5];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      units.get(i, unit[i], bits[i]);
+      kc.start(k_slot(i), unit[i]);
+    }
+    vc.start(v_slot(0), unit[0]);
+    load_rows<T>(w.x, A.q.at<T>(b, h), A.q.row, q0, A.queries);
+    w.at = places();
+    const T one = (T)((lane & 15) == 0 ? 1.0f : 0.0f);
+    w.ones = vec8<T>{one, one, one, one, one, one, one, one};
+    reinterpret_cast<uint4*>(v_slot(-1))[threadIdx.x] = make_uint4(0, 0, 0, 0);   // V(-1), times P(-1) = 0
+    landed<0>();
+    for (int i = 0; i < 4; ++i) clear_rows(k_slot(i), bits[i]);
+    clear_rows(v_slot(0), bits[0]);
+    __syncthreads();
+    f32x4 s0[4], s1[4];
+    uint32_t p0[8], p1[8] = {};
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const f32x4 start = bias_of(bits[0], kt);
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const vec8<T> a = row_operand<T>(k_slot(0), w.at, st, kt);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : start);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
+    __syncthreads();   // K(0) has been read: iteration 0 copies K(4) over it
+    auto iteration = [&](auto bias, int u, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8],
+                         uint32_t(&p_cur)[8]) {
+      constexpr bool kBias = decltype(bias)::value;
+      units.get(u + 4, unit[4], bits[4]);
+      forward_phase<kBias, kKeep>(w, s_cur, s_next, p_prev, p_cur, k_slot(u + 1), v_slot(u - 1), k_slot(u + 2), bits[1],
+                                  [&](int slot) {
+                                    if (slot == 1) kc.start(k_slot(u + 4), unit[4]);
+                                    if (slot == 3) vc.start(v_slot(u + 1), unit[1]);
+                                  });
+      landed<2>();
+      if constexpr (kBias) {
+        clear_rows(k_slot(u + 3), bits[3]);
+        clear_rows(v_slot(u), bits[0]);
+      }
+      barrier();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        unit[i] = unit[i + 1];
+        bits[i] = bits[i + 1];
+      }
+    };
+    int u = 0;
+    if constexpr (!kMasked)   // while no unit in reach is cut off: u + 4 < n - 1
+      for (; u + 6 < n; u += 2) {
+        iteration(std::false_type{}, u, s0, s1, p1, p0);
+        iteration(std::false_type{}, u + 1, s1, s0, p0, p1);
+      }
+    for (; u <= n; u += 2) {
+      iteration(std::true_type{}, u, s0, s1, p1, p0);
+      iteration(std::true_type{}, u + 1, s1, s0, p0, p1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy writes LDS that the block has left
   }
   float scale[2];
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    const float sum = across(l[g]), exact = across(l_exact[g]);
-    scale[g] = sum > 0.0f ? 1.0f / sum : 0.0f;
-    const int r = q0 + g * 16 + (lane & 15);
-    if (A.lse && h4 == 0 && r < A.queries)
-      A.lse[(int64_t)bh * A.queries + r] = sum > 0.0f ? (m[g] + __builtin_amdgcn_logf(exact)) * kLn2 : -INFINITY;
+    const float l = __shfl(w.l[g][0], lane & 15);
+    scale[g] = l > 0.0f ? 1.0f / l : 0.0f;
+    if constexpr (kKeep) {
+      const float sum = across(w.sum[g]);
+      const int r = q0 + g * 16 + (lane & 15);
+      if (h4 == 0 && r < A.queries)
+        A.lse[(int64_t)bh * A.queries + r] = l > 0.0f ? w.top[g] + __builtin_amdgcn_logf(sum) * kLn2 : -INFINITY;
+    }
   }
-  T* low = static_cast<T*>(A.low);
+  T* low = kKeep ? static_cast<T*>(A.low) : nullptr;
   if (low) low += ((int64_t)b * A.queries * A.heads + h) * kD;
-  store_rows<T>(acc, scale, A.o.at<T>(b, h), A.o.row, q0, A.queries, low, (int64_t)A.heads * kD);
+  store_rows<T>(w.acc, scale, A.o.at<T>(b, h), A.o.row, q0, A.queries, low, (int64_t)A.heads * kD);
 }
 
 // dq, and the stats that attention_dkv_kernel reads.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_dq_kernel(const Args A) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kTileBytes];
-  const int lane = threadIdx.x & 63, h4 = lane >> 4;
-  const int blocks = (A.queries + kBlock - 1) / kBlock;
-  const int bh = blockIdx.x / blocks, b = bh / A.heads, h = bh - b * A.heads;
-  const int q0 = (blockIdx.x - bh * blocks) * kBlock + (threadIdx.x >> 6) * 32;
-  vec8<T> q[4][2], g0[4][2], o[4][2], low[4][2];
-  load_rows<T>(q, A.q.at<T>(b, h), A.q.row, q0, A.queries);
-  load_rows<T>(g0, A.dO.at<T>(b, h), A.dO.row, q0, A.queries);
-  load_rows<T>(o, A.o.at<T>(b, h), A.o.row, q0, A.queries);
-  load_rows<T>(low, static_cast<const T*>(A.low) + ((int64_t)b * A.queries * A.heads + h) * kD, (int64_t)A.heads * kD, q0,
-               A.queries);
-  float lse[2], delta[2];
+struct Dq {
+  vec8<T> x[4][2], g[4][2];   // Q^T, dO^T
+  f32x4 acc[8][2];            // dQ^T
+  vec8<T> ops[2 * kLead];
+  float lse[2], delta[2];     // -log2(e) lse, -delta
+  Places at;
+};
+
+// Phase u: S(u+1) = K(u+1) Q^T, dP(u+1) = V(u+1) dO^T and dQ^T += K(u-1)^T dS(u-1)^T, while dS(u) is formed.
+template <bool kBias, typename T, typename Hook>
+__device__ __forceinline__ void dq_phase(Dq<T>& w, const f32x4 (&s_cur)[4], const f32x4 (&d_cur)[4], f32x4 (&s_next)[4],
+                                         f32x4 (&d_next)[4], const uint32_t (&p_prev)[8], uint32_t (&p_cur)[8],
+                                         const uint8_t* k_unit, const uint8_t* v_unit, const uint8_t* k_before,
+                                         const uint8_t* k_after, uint32_t bits_next, Hook&& hook) {
+  f32x4 sv[4], dv[4];
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int r = q0 + g * 16 + (lane & 15);
-    const float x = r < A.queries ? A.lse[(int64_t)bh * A.queries + r] : -INFINITY;
-    lse[g] = x == -INFINITY ? INFINITY : x * kLog2e;
-    float sum = 0.0f;
-#pragma unroll
-    for (int st = 0; st < 4; ++st)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += (float)g0[st][g][e] * ((float)o[st][g][e] + (float)low[st][g][e]);
-    delta[g] = x == -INFINITY ? 0.0f : across(sum);
-    if (h4 == 0 && r < A.units * kUnit) {
-      float* st = A.stats + ((int64_t)bh * A.units + r / kUnit) * 2 * kUnit + r % kUnit;
-      st[0] = lse[g];
-      st[kUnit] = -delta[g];
+  for (int i = 0; i < 4; ++i) {
+    sv[i] = s_cur[i];
+    dv[i] = d_cur[i];
+    asm volatile("" : "+v"(sv[i]), "+v"(dv[i]));
+  }
+  f32x4 start[2] = {};
+  if constexpr (kBias) {
+    if (bits_next != ~0u) {
+      start[0] = bias_of(bits_next, 0);
+      start[1] = bias_of(bits_next, 1);
     }
   }
-  const Places at = places();
-  f32x4 acc[8][2] = {};
-  const int n = live_tiles(A, b);
-  for (int i = 0; i < n; ++i) {
-    const int t = live_tile(A, b, i);
-    const uint64_t bits = kept(A, b, t);
-    __syncthreads();
-    stage(smem, A.k.at<uint16_t>(b, h / A.group), A.k.row, t * kTile, bits);
-    stage(smem + kTileBytes, A.v.at<uint16_t>(b, h / A.group), A.v.row, t * kTile, bits);
-    __syncthreads();
-    for (int u = 0; u < 2; ++u) {
-      f32x4 s[2][2] = {}, dp[2][2];
+  float t[16], e[16];
+  auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, w.lse[n >> 3]); };
+  auto exp = [&](int n) { e[n] = __builtin_amdgcn_exp2f(t[n]); };
+  auto put = [&](int n) {
+    const float x = e[n] * (dv[n >> 2][n & 3] + w.delta[n >> 3]), y = e[n + 1] * (dv[n >> 2][(n & 3) + 1] + w.delta[n >> 3]);
+    p_cur[n >> 1] = pack<T>(x, y);
+    asm volatile("" : "+v"(p_cur[n >> 1]));
+  };
+  const vec8<T> pb[2] = {packed<T>(p_prev, 0), packed<T>(p_prev, 1)};
+  scaled(0);
+  scaled(1);
+  exp(0);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+  for (int n = 0; n < 24; ++n) {
+    const vec8<T>& a = w.ops[n % (2 * kLead)];
+    const int st = (n & 7) >> 1, kt = n & 1;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) dp[g][kt] = f32x4{-delta[g], -delta[g], -delta[g], -delta[g]};
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          const vec8<T> a = row_operand<T>(smem + u * kUnitBytes, at, st, kt);
-          const vec8<T> c = row_operand<T>(smem + kTileBytes + u * kUnitBytes, at, st, kt);
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            s[g][kt] = mfma(a, q[st][g], s[g][kt]);
-            dp[g][kt] = mfma(c, g0[st][g], dp[g][kt]);
-          }
-        }
-      }
-      uint32_t ds[2][4];
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          float x[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const bool on = bits >> (u * 32 + (e >> 2) * 16 + h4 * 4 + (e & 3) + j) & 1;
-            x[j] = on ? __builtin_amdgcn_exp2f(s[g][e >> 2][(e & 3) + j] * kLog2e - lse[g]) * dp[g][e >> 2][(e & 3) + j]
-                      : 0.0f;
-          }
-          ds[g][e >> 1] = pack<T>(x[0], x[1]);
-        }
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) {
-        const vec8<T> a = col_operand<T>(smem + u * kUnitBytes, at, dt);
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-          acc[dt][g] = mfma(a, __builtin_bit_cast(vec8<T>, make_uint4(ds[g][0], ds[g][1], ds[g][2], ds[g][3])), acc[dt][g]);
-      }
+    for (int g = 0; g < 2; ++g) {
+      if (n < 8) s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : kBias ? start[kt] : f32x4{});
+      else if (n < 16) d_next[2 * g + kt] = mfma(a, w.g[st][g], st ? d_next[2 * g + kt] : f32x4{});
+      else w.acc[n - 16][g] = mfma(a, pb[g], w.acc[n - 16][g]);
     }
+    const int m = n + kLead;
+    vec8<T>& to = w.ops[m % (2 * kLead)];
+    if (m < 8) to = row_operand<T>(k_unit, w.at, m >> 1, m & 1);
+    else if (m < 16) to = row_operand<T>(v_unit, w.at, (m - 8) >> 1, m & 1);
+    else if (m < 24) to = col_operand<T>(k_before, w.at, m - 16);
+    else to = row_operand<T>(k_after, w.at, (m - 24) >> 1, m & 1);
+    if (n + 2 < 16) scaled(n + 2);
+    if (n + 1 < 16) exp(n + 1);
+    if (n < 16 && n & 1) put(n - 1);
+    hook(n);
+    __builtin_amdgcn_sched_barrier(0);
   }
-  const float one[2] = {1.0f, 1.0f};
-  store_rows<T>(acc, one, A.dq.at<T>(b, h), A.dq.row, q0, A.queries);
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void attention_dkv_kernel(const Args A) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kTileBytes];
+constexpr int kDqKRing = 8, kDqVRing = 4;
+
+template <typename T, bool kMasked>
+__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[(kDqKRing + kDqVRing) * kUnitBytes];
   const int lane = threadIdx.x & 63, h4 = lane >> 4;
-  const int blocks = (A.keys + kBlock - 1) / kBlock;
-  const int bh = blockIdx.x / blocks, b = bh / A.kv_heads, h = bh - b * A.kv_heads;
-  const int first = (blockIdx.x - bh * blocks) * kBlock, k0 = first + (threadIdx.x >> 6) * 32;
-  vec8<T> k[4][2], v[4][2];
-  load_rows<T>(k, A.k.at<T>(b, h), A.k.row, k0, A.keys);
-  load_rows<T>(v, A.v.at<T>(b, h), A.v.row, k0, A.keys);
-  bool on[2];
-  float one[2];
+  const int blocks = (A.queries + kQueries - 1) / kQueries;
+  const int bh = blockIdx.x / blocks, b = bh / A.heads, h = bh - b * A.heads;
+  const int q0 = (blockIdx.x - bh * blocks) * kQueries + (threadIdx.x >> 6) * 32;
+  Units<kMasked> units(A, b);
+  const int n = units.n;
+  Dq<T> w;
+  load_rows<T>(w.g, A.dO.at<T>(b, h), A.dO.row, q0, A.queries);
+  {
+    vec8<T> o[4][2], low[4][2];
+    load_rows<T>(o, A.o.at<T>(b, h), A.o.row, q0, A.queries);
+    load_rows<T>(low, static_cast<const T*>(A.low) + ((int64_t)b * A.queries * A.heads + h) * kD, (int64_t)A.heads * kD, q0,
+                 A.queries);
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int r = k0 + g * 16 + (lane & 15);
-    on[g] = r < A.keys && (kept(A, b, r / kTile) >> (r % kTile) & 1);
-    one[g] = 1.0f;
+    for (int g = 0; g < 2; ++g) {
+      const int r = q0 + g * 16 + (lane & 15);
+      const float x = r < A.queries ? A.lse[(int64_t)bh * A.queries + r] : -INFINITY;
+      float sum = 0.0f;
 #pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      k[st][g] = on[g] ? k[st][g] : vec8<T>{};
-      v[st][g] = on[g] ? v[st][g] : vec8<T>{};
-    }
-  }
-  const Places at = places();
-  f32x4 dk[8][2] = {}, dv[8][2] = {};
-  bool any = false;
-  for (int t = first / kTile; t < min(A.tiles, (first + kBlock) / kTile); ++t) any |= kept(A, b, t) != 0;
-  const int tiles = (A.queries + kTile - 1) / kTile, n = any ? tiles * A.group : 0;
-  for (int i = 0; i < n; ++i) {
-    const int hq = h * A.group + i / tiles, t = i % tiles;
-    const int left = A.queries - t * kTile;
-    const uint64_t bits = left >= 64 ? ~0ull : (1ull << left) - 1;
-    __syncthreads();
-    stage(smem, A.q.at<uint16_t>(b, hq), A.q.row, t * kTile, bits);
-    stage(smem + kTileBytes, A.dO.at<uint16_t>(b, hq), A.dO.row, t * kTile, bits);
-    __syncthreads();
-    for (int u = 0; u < 2 && t * 2 + u < A.units; ++u) {
-      const float* stats = A.stats + (((int64_t)b * A.heads + hq) * A.units + t * 2 + u) * 2 * kUnit;
-      f32x4 s[2][2] = {}, dp[2][2], lse[2];
+      for (int st = 0; st < 4; ++st)
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        lse[kt] = *reinterpret_cast<const f32x4*>(stats + kt * 16 + h4 * 4);
-#pragma unroll
-        for (int g = 0; g < 2; ++g) dp[g][kt] = *reinterpret_cast<const f32x4*>(stats + kUnit + kt * 16 + h4 * 4);
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          const vec8<T> a = row_operand<T>(smem + u * kUnitBytes, at, st, kt);
-          const vec8<T> c = row_operand<T>(smem + kTileBytes + u * kUnitBytes, at, st, kt);
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            s[g][kt] = mfma(a, k[st][g], s[g][kt]);
-            dp[g][kt] = mfma(c, v[st][g], dp[g][kt]);
-          }
-        }
-      }
-      uint32_t p[2][4], ds[2][4];
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          float x[2], y[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            x[j] = __builtin_amdgcn_exp2f(s[g][e >> 2][(e & 3) + j] * kLog2e - lse[e >> 2][(e & 3) + j]);
-            y[j] = x[j] * dp[g][e >> 2][(e & 3) + j];
-          }
-          p[g][e >> 1] = pack<T>(x[0], x[1]);
-          ds[g][e >> 1] = pack<T>(y[0], y[1]);
-        }
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) {
-        const vec8<T> a = col_operand<T>(smem + kTileBytes + u * kUnitBytes, at, dt);
-        const vec8<T> c = col_operand<T>(smem + u * kUnitBytes, at, dt);
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          dv[dt][g] = mfma(a, __builtin_bit_cast(vec8<T>, make_uint4(p[g][0], p[g][1], p[g][2], p[g][3])), dv[dt][g]);
-          dk[dt][g] = mfma(c, __builtin_bit_cast(vec8<T>, make_uint4(ds[g][0], ds[g][1], ds[g][2], ds[g][3])), dk[dt][g]);
-        }
+        for (int e = 0; e < 8; ++e) sum += (float)w.g[st][g][e] * ((float)o[st][g][e] + (float)low[st][g][e]);
+      sum = across(sum);
+      w.lse[g] = x == -INFINITY ? -INFINITY : x * -kLog2e;
+      w.delta[g] = x == -INFINITY ? 0.0f : -sum;
+      if (h4 == 0 && r < A.q_units * kUnit) {
+        float* st = A.stats + ((int64_t)bh * A.q_units + r / kUnit) * 2 * kUnit + r % kUnit;
+        st[0] = -w.lse[g];
+        st[kUnit] = w.delta[g];
       }
     }
+    if (blockIdx.x == 0 && threadIdx.x < 2 * kUnit)
+      A.stats[(int64_t)A.batch * A.heads * A.q_units * 2 * kUnit + threadIdx.x] = threadIdx.x < kUnit ? INFINITY : 0.0f;
   }
 #pragma unroll
   for (int g = 0; g < 2; ++g)
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
-      dk[dt][g] = on[g] ? dk[dt][g] : f32x4{};
-      dv[dt][g] = on[g] ? dv[dt][g] : f32x4{};
+    for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
+  if (n) {
+    auto k_slot = [&](int i) { return smem + (i & (kDqKRing - 1)) * kUnitBytes; };
+    auto v_slot = [&](int i) { return smem + (kDqKRing + (i & (kDqVRing - 1))) * kUnitBytes; };
+    const Copies kc(A.k.at<uint16_t>(b, h / A.group), A.k.row, A.keys), vc(A.v.at<uint16_t>(b, h / A.group), A.v.row, A.keys);
+    int unit[5];
+    uint32_t bits[5];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      units.get(i, unit[i], bits[i]);
+      kc.start(k_slot(i), unit[i]);
+      if (i < 3) vc.start(v_slot(i), unit[i]);
     }
-  store_rows<T>(dk, one, A.dk.at<T>(b, h), A.dk.row, k0, A.keys);
-  store_rows<T>(dv, one, A.dv.at<T>(b, h), A.dv.row, k0, A.keys);
+    load_rows<T>(w.x, A.q.at<T>(b, h), A.q.row, q0, A.queries);
+    w.at = places();
+    reinterpret_cast<uint4*>(k_slot(-1))[threadIdx.x] = make_uint4(0, 0, 0, 0);   // K(-1), times dS(-1) = 0
+    landed<0>();
+    for (int i = 0; i < 4; ++i) {
+      clear_rows(k_slot(i), bits[i]);
+      if (i < 3) clear_rows(v_slot(i), bits[i]);
+    }
+    __syncthreads();
+    f32x4 s0[4], s1[4], d0[4], d1[4];
+    uint32_t p0[8], p1[8] = {};
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const f32x4 start = bias_of(bits[0], kt);
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const vec8<T> a = row_operand<T>(k_slot(0), w.at, st, kt), c = row_operand<T>(v_slot(0), w.at, st, kt);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : start);
+          d0[2 * g + kt] = mfma(c, w.g[st][g], st ? d0[2 * g + kt] : f32x4{});
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
+    auto iteration = [&](auto bias, int u, const f32x4(&s_cur)[4], const f32x4(&d_cur)[4], f32x4(&s_next)[4],
+                         f32x4(&d_next)[4], const uint32_t(&p_prev)[8], uint32_t(&p_cur)[8]) {
+      constexpr bool kBias = decltype(bias)::value;
+      units.get(u + 4, unit[4], bits[4]);
+      dq_phase<kBias>(w, s_cur, d_cur, s_next, d_next, p_prev, p_cur, k_slot(u + 1), v_slot(u + 1), k_slot(u - 1),
+                      k_slot(u + 2), bits[1], [&](int slot) {
+                        if (slot == 1) kc.start(k_slot(u + 4), unit[4]);
+                        if (slot == 3) vc.start(v_slot(u + 3), unit[3]);
+                      });
+      landed<2>();
+      if constexpr (kBias) {
+        clear_rows(k_slot(u + 3), bits[3]);
+        clear_rows(v_slot(u + 2), bits[2]);
+      }
+      barrier();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        unit[i] = unit[i + 1];
+        bits[i] = bits[i + 1];
+      }
+    };
+    int u = 0;
+    if constexpr (!kMasked)
+      for (; u + 6 < n; u += 2) {
+        iteration(std::false_type{}, u, s0, d0, s1, d1, p1, p0);
+        iteration(std::false_type{}, u + 1, s1, d1, s0, d0, p0, p1);
+      }
+    for (; u <= n; u += 2) {
+      iteration(std::true_type{}, u, s0, d0, s1, d1, p1, p0);
+      iteration(std::true_type{}, u + 1, s1, d1, s0, d0, p0, p1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  const float one[2] = {1.0f, 1.0f};
+  store_rows<T>(w.acc, one, A.dq.at<T>(b, h), A.dq.row, q0, A.queries);
 }
 
-// The mask's words and live tiles of one batch entry a block; a thread a tile, 1024 tiles a turn.
+// dk and dv of 128 keys, 32 a pair of waves: the first holds K^T and dV^T, forms S and P and hands P on through LDS, the second holds
+// V^T and dK^T, forms dP and dS one unit later.
+template <typename T>
+struct Dkv {
+  vec8<T> x[4][2];         // K^T (V^T)
+  f32x4 acc[8][2];         // dV^T (dK^T)
+  vec8<T> ops[2 * kLead];
+  f32x4 stat[2];           // this phase's log2(e) lse (-delta) of the rows of each accumulator
+  Places at;
+};
+
+// The first wave's phase u: S(u+1) = Q(u+1) K^T and dV^T += dO(u-1)^T P(u-1) while P(u) is formed.  The second's:
+// dP(u) = dO(u) V^T and dK^T += Q(u-2)^T dS(u-2) while dS(u-1) = P(u-1) (dP(u-1) - delta) is formed; dP starts from
+// -delta.  `stats`: of the next phase; `hand`: where P goes (comes from).
+template <bool kSecond, typename T, typename Hook>
+__device__ __forceinline__ void dkv_phase(Dkv<T>& w, const f32x4 (&s_cur)[4], f32x4 (&s_next)[4], const uint32_t (&p_prev)[8],
+                                          uint32_t (&p_cur)[8], const uint8_t* rows, const uint8_t* cols,
+                                          const uint8_t* rows_after, const uint8_t* stats, uint8_t* hand, Hook&& hook) {
+  const int lane = threadIdx.x & 63;
+  f32x4* const mine = reinterpret_cast<f32x4*>(hand) + lane;   // accumulator i at mine[64 i]
+  f32x4 sv[4], e4[4], stat_next[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sv[i] = s_cur[i];
+    asm volatile("" : "+v"(sv[i]));
+    if constexpr (kSecond) e4[i] = mine[64 * i];
+  }
+  float t[16];
+  auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, -w.stat[n >> 2 & 1][n & 3]); };
+  auto exp = [&](int n) { e4[n >> 2][n & 3] = __builtin_amdgcn_exp2f(t[n]); };
+  auto put = [&](int n) {
+    float x = e4[n >> 2][n & 3], y = e4[n >> 2][(n & 3) + 1];
+    if constexpr (kSecond) {
+      x *= sv[n >> 2][n & 3];
+      y *= sv[n >> 2][(n & 3) + 1];
+    }
+    p_cur[n >> 1] = pack<T>(x, y);
+    asm volatile("" : "+v"(p_cur[n >> 1]));
+  };
+  const vec8<T> pb[2] = {packed<T>(p_prev, 0), packed<T>(p_prev, 1)};
+  if constexpr (!kSecond) {
+    scaled(0);
+    scaled(1);
+    exp(0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int n = 0; n < 16; ++n) {
+    const vec8<T>& a = w.ops[n % (2 * kLead)];
+    if (n < 8) {
+      const int st = n >> 1, kt = n & 1;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : kSecond ? w.stat[kt] : f32x4{});
+    } else {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) w.acc[n - 8][g] = mfma(a, pb[g], w.acc[n - 8][g]);
+    }
+    const int m = n + kLead;
+    vec8<T>& to = w.ops[m % (2 * kLead)];
+    if (m < 8) to = row_operand<T>(rows, w.at, m >> 1, m & 1);
+    else if (m < 16) to = col_operand<T>(cols, w.at, m - 8);
+    else to = row_operand<T>(rows_after, w.at, (m - 16) >> 1, m & 1);
+    if (n >= 9 && n < 11) stat_next[n - 9] = *reinterpret_cast<const f32x4*>(
+        stats + (kSecond ? kUnit * 4 : 0) + (n - 9) * 64 + (lane >> 4) * 16);
+    if constexpr (kSecond) {
+      if (n >= 8) put(2 * (n - 8));
+    } else {
+      if (n + 2 < 16) scaled(n + 2);
+      if (n + 1 < 16) exp(n + 1);
+      if (n & 1) put(n - 1);
+      if ((n & 3) == 3) mine[64 * (n >> 2)] = e4[n >> 2];
+    }
+    hook(n);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  w.stat[0] = stat_next[0];
+  w.stat[1] = stat_next[1];
+}
+
+constexpr int kQRing = 8, kORing = 5, kStatRing = 8;   // units of Q, of dO and of their stats in LDS
+constexpr int kStatBytes = 2 * kUnit * 4, kHandBytes = 4096;
+constexpr int kDkvStats = (kQRing + kORing) * kUnitBytes, kDkvHands = kDkvStats + kStatRing * kStatBytes;
+constexpr int kDkvBytes = kDkvHands + kWaves * kHandBytes;   // two hands a pair of waves
+
+// The query units of the heads that share a key head, one after the other.
+struct Queries {
+  const uint16_t* head;
+  int64_t row, next;     // elements from one row and one head to the next
+  int units, left, unit;
+  __device__ __forceinline__ Queries(const Tensor& t, int b, int h, int units, int heads)
+      : head(t.at<uint16_t>(b, h)), row(t.row), next(t.head), units(units), left(heads), unit(0) {}
+  __device__ __forceinline__ void step() {   // past the last unit: the last
+    if (unit + 1 < units) {
+      ++unit;
+    } else if (left > 1) {
+      --left;
+      unit = 0;
+      head += next;
+    }
+  }
+};
+
+template <bool kSecond, typename T>
+__device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, int b, int h, int k0, bool any) {
+  const int lane = threadIdx.x & 63, pair = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  Dkv<T> w;
+  const Tensor& own = kSecond ? A.v : A.k;
+  load_rows<T>(w.x, own.at<T>(b, h), own.row, k0, A.keys);
+  bool on[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int r = k0 + g * 16 + (lane & 15);
+    on[g] = r < A.keys && (kept(A, b, r / kUnit) >> (r % kUnit) & 1);
+#pragma unroll
+    for (int st = 0; st < 4; ++st) w.x[st][g] = on[g] ? w.x[st][g] : vec8<T>{};
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
+  }
+  if (any) {
+    const int n = A.q_units * A.group;
+    auto q_slot = [&](int i) { return smem + (i & (kQRing - 1)) * kUnitBytes; };
+    auto o_slot = [&](int i) { return smem + (kQRing + i) * kUnitBytes; };   // i in its ring
+    auto stat_slot = [&](int i) { return smem + kDkvStats + (i & (kStatRing - 1)) * kStatBytes; };
+    auto hand = [&](int i) { return smem + kDkvHands + (pair * 2 + (i & 1)) * kHandBytes; };
+    const Copies qc(nullptr, A.q.row, A.queries), oc(nullptr, A.dO.row, A.queries);
+    Queries qs(A.q, b, h * A.group, A.q_units, A.group), os(A.dO, b, h * A.group, A.q_units, A.group);
+    const float* stats = A.stats + ((int64_t)b * A.heads + h * A.group) * A.q_units * 2 * kUnit;
+    const float* none = A.stats + (int64_t)A.batch * A.heads * A.q_units * 2 * kUnit;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto copy = [&](const Copies& c, Queries& from, uint8_t* slot) {
+      flk::dma16_at(from.head + (int64_t)from.unit * kUnit * from.row, from.unit == c.last ? c.at_last : c.at,
+                    slot + wave * 4 * kRowBytes);
+      from.step();
+    };
+    // every wave copies all of a unit's stats: as many copies a wave as the waits count
+    auto copy_stats = [&](int i) {
+      flk::dma4_at(i < n ? stats + (int64_t)i * 2 * kUnit : none, lane * 4, stat_slot(i));
+    };
+    for (int i = 0; i < 4; ++i) copy(qc, qs, q_slot(i));
+    for (int i = 0; i < 3; ++i) {
+      copy(oc, os, o_slot(i));
+      copy_stats(i);
+    }
+    w.at = places();
+    // Q(-1), Q(-2), dO(-1) and P(-1), which the first iterations read, times zeros
+    reinterpret_cast<uint4*>(q_slot(-1))[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4*>(q_slot(-2))[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4*>(o_slot(kORing - 1))[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    if (!kSecond)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<f32x4*>(hand(1))[64 * i + lane] = f32x4{};
+    landed<0>();
+    __syncthreads();
+    f32x4 s0[4] = {}, s1[4];
+    uint32_t p0[8], p1[8] = {};
+    if constexpr (!kSecond) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          const vec8<T> a = row_operand<T>(q_slot(0), w.at, st, kt);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) s0[2 * g + kt] = mfma(a, w.x[st][g], s0[2 * g + kt]);
+        }
+    }
+    const uint8_t* first = kSecond ? o_slot(0) : q_slot(1);
+#pragma unroll
+    for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(first, w.at, m >> 1, m & 1);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+      w.stat[kt] = *reinterpret_cast<const f32x4*>(stat_slot(0) + (kSecond ? kUnit * 4 : 0) + kt * 64 + (lane >> 4) * 16);
+    int o = 0;   // u's place in dO's ring
+    auto o_at = [&](int d) { return o_slot(o + d >= kORing ? o + d - kORing : o + d); };
+    auto iteration = [&](int u, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8], uint32_t(&p_cur)[8]) {
+      const uint8_t* rows = kSecond ? o_at(0) : q_slot(u + 1);
+      const uint8_t* cols = kSecond ? q_slot(u - 2) : o_at(kORing - 1);
+      const uint8_t* after = kSecond ? o_at(1) : q_slot(u + 2);
+      dkv_phase<kSecond>(w, s_cur, s_next, p_prev, p_cur, rows, cols, after, stat_slot(u + 1), hand(kSecond ? u - 1 : u),
+                         [&](int slot) {
+                           if (slot == 1) copy(qc, qs, q_slot(u + 4));
+                           if (slot == 3) copy(oc, os, o_at(3));
+                           if (slot == 5) copy_stats(u + 3);
+                         });
+      if constexpr (!kSecond) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // P is in its hand
+      landed<3>();
+      barrier();
+      o = o + 1 == kORing ? 0 : o + 1;
+    };
+    // the second wave's last unit goes into dK at u = n + 1
+    for (int u = 0; u < n + 2; u += 2) {
+      iteration(u, s0, s1, p1, p0);
+      iteration(u + 1, s1, s0, p0, p1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = on[g] ? w.acc[dt][g] : f32x4{};
+  const float one[2] = {1.0f, 1.0f};
+  const Tensor& out = kSecond ? A.dk : A.dv;
+  store_rows<T>(w.acc, one, out.at<T>(b, h), out.row, k0, A.keys);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(const Args A) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kDkvBytes];
+  const int blocks = (A.keys + kKeys - 1) / kKeys;
+  const int bh = blockIdx.x / blocks, b = bh / A.kv_heads, h = bh - b * A.kv_heads;
+  const int first = (blockIdx.x - bh * blocks) * kKeys;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  bool any = false;
+  for (int u = first / kUnit; u < min(A.k_units, (first + kKeys) / kUnit); ++u) any |= kept(A, b, u) != 0;
+  const int k0 = first + (wave & 3) * 32;
+  if (wave < 4) dkv_wave<false, T>(A, smem, b, h, k0, any);
+  else dkv_wave<true, T>(A, smem, b, h, k0, any);
+}
+
+// The mask's words and live units, one batch entry a block, a thread a unit, 1024 units a turn.
 constexpr int kPlanWaves = 16;
 __global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const uint8_t* mask, int64_t batch_stride, int keys,
-                                                                         int tiles, uint64_t* words, int* live, int* counts) {
+                                                                         int units, uint32_t* words, uint2* live,
+                                                                         int* counts) {
   __shared__ int found[kPlanWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint8_t* row = mask + blockIdx.x * batch_stride;
-  words += (int64_t)blockIdx.x * tiles;
-  live += (int64_t)blockIdx.x * tiles;
+  words += (int64_t)blockIdx.x * units;
+  live += (int64_t)blockIdx.x * units;
   int count = 0;
-  for (int t0 = 0; t0 < tiles; t0 += 64 * kPlanWaves) {
-    uint64_t mine = 0;   // of tile t0 + threadIdx.x
+  for (int u0 = 0; u0 < units; u0 += 64 * kPlanWaves) {
+    uint32_t mine = 0;   // of unit u0 + threadIdx.x
 #pragma unroll 8
-    for (int i = 0; i < 64; ++i) {
-      const int key = (t0 + wave * 64 + i) * kTile + lane;   // at most keys + 65535
-      const uint64_t bits = __ballot(key < keys && row[key] != 0);
-      mine = lane == i ? bits : mine;
+    for (int i = 0; i < 32; ++i) {
+      const int key = (u0 + wave * 64 + 2 * i) * kUnit + lane;   // at most keys + 32767
+      const uint64_t both = __ballot(key < keys && row[key] != 0);
+      if (lane >> 1 == i) mine = (uint32_t)(lane & 1 ? both >> 32 : both);
     }
-    const int t = t0 + threadIdx.x;
+    const int u = u0 + threadIdx.x;
     const uint64_t any = __ballot(mine != 0);
-    if (t < tiles) words[t] = mine;
+    if (u < units) words[u] = mine;
     if (lane == 0) found[wave] = __popcll(any);
     __syncthreads();
     int at = count;
@@ -467,29 +908,27 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const u
       if (w < wave) at += found[w];
       count += found[w];
     }
-    if (mine) live[at + __popcll(any & ((1ull << lane) - 1))] = t;
+    if (mine) live[at + __popcll(any & ((1ull << lane) - 1))] = make_uint2(u, mine);
     __syncthreads();
   }
   if (threadIdx.x == 0) counts[blockIdx.x] = count;
 }
 
-int64_t mask_bytes(int batch, int keys) {
-  const int64_t tiles = (keys + kTile - 1) / kTile;
-  return (batch * (tiles * 12 + 4) + 255) / 256 * 256;
-}
+int units_of(int rows) { return (rows + kUnit - 1) / kUnit; }
+int64_t mask_bytes(int batch, int keys) { return ((int64_t)batch * (units_of(keys) * 12LL + 4) + 255) / 256 * 256; }
 int64_t stats_bytes(int batch, int heads, int queries) {
-  return (int64_t)batch * heads * ((queries + kUnit - 1) / kUnit) * 2 * kUnit * 4;
+  return ((int64_t)batch * heads * units_of(queries) + 1) * 2 * kUnit * 4;
 }
 
 // Lays the mask's words and lists out in `workspace` and starts the kernel that fills them.
 int plan_mask(const void* mask, int64_t batch_stride, Args& A, uint8_t* workspace, hipStream_t s) {
   if (!mask) return FLK_OK;
-  uint64_t* words = reinterpret_cast<uint64_t*>(workspace);
-  int* live = reinterpret_cast<int*>(words + (int64_t)A.batch * A.tiles);
-  int* counts = live + (int64_t)A.batch * A.tiles;
-  A.mask = Mask{words, live, counts};
-  attention_mask_kernel<<<A.batch, 64 * kPlanWaves, 0, s>>>(static_cast<const uint8_t*>(mask), batch_stride, A.keys, A.tiles,
-                                                            words, live, counts);
+  uint2* live = reinterpret_cast<uint2*>(workspace);
+  uint32_t* bits = reinterpret_cast<uint32_t*>(live + (int64_t)A.batch * A.k_units);
+  int* counts = reinterpret_cast<int*>(bits + (int64_t)A.batch * A.k_units);
+  A.mask = Mask{bits, live, counts};
+  attention_mask_kernel<<<A.batch, 64 * kPlanWaves, 0, s>>>(static_cast<const uint8_t*>(mask), batch_stride, A.keys,
+                                                            A.k_units, bits, live, counts);
   return flk_launch_status();
 }
 
@@ -503,6 +942,7 @@ bool sizes_ok(int batch, int heads, int kv_heads, int queries, int keys) {
 int check_tensor(const void* p, const int64_t* strides) {
   if (!p || !strides) return FLK_E_INVALID;
   if (!flk_host_aligned(p, 16) || strides[0] % 8 || strides[1] % 8 || strides[2] % 8) return FLK_E_ALIGN;
+  if (strides[2] < 0 || strides[2] > kMaxRow) return FLK_E_INVALID;
   return FLK_OK;
 }
 Tensor tensor(const void* p, const int64_t* s) { return Tensor{const_cast<void*>(p), s[0], s[1], s[2]}; }
@@ -515,9 +955,22 @@ Args sizes(int batch, int heads, int kv_heads, int queries, int keys) {
   A.group = heads / kv_heads;
   A.queries = queries;
   A.keys = keys;
-  A.tiles = (keys + kTile - 1) / kTile;
-  A.units = (queries + kUnit - 1) / kUnit;
+  A.q_units = units_of(queries);
+  A.k_units = units_of(keys);
   return A;
+}
+
+template <typename T, typename Launch>
+void forward(const Args& A, Launch&& launch) {
+  if (A.mask.bits) A.lse ? launch(attention_kernel<T, true, true>) : launch(attention_kernel<T, true, false>);
+  else A.lse ? launch(attention_kernel<T, false, true>) : launch(attention_kernel<T, false, false>);
+}
+
+template <typename T>
+void backward(const Args& A, dim3 of_q, dim3 of_k, hipStream_t s) {
+  if (A.mask.bits) attention_dq_kernel<T, true><<<of_q, kThreads, 0, s>>>(A);
+  else attention_dq_kernel<T, false><<<of_q, kThreads, 0, s>>>(A);
+  attention_dkv_kernel<T><<<of_k, kThreads, 0, s>>>(A);
 }
 
 }  // namespace
@@ -557,9 +1010,11 @@ extern "C" int flk_attention(const void* q, const int64_t* q_strides, const void
   A.lse = lse;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (const int st = plan_mask(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace), s)) return st;
-  const dim3 grid((unsigned)((int64_t)batch * heads * ((queries + kBlock - 1) / kBlock)));
-  if (dtype == FLK_BF16) attention_kernel<__bf16><<<grid, kThreads, 0, s>>>(A);
-  else attention_kernel<_Float16><<<grid, kThreads, 0, s>>>(A);
+  if (keys == 0) A.k_units = 0;
+  const dim3 grid((unsigned)((int64_t)batch * heads * ((queries + kQueries - 1) / kQueries)));
+  auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(A); };
+  if (dtype == FLK_BF16) forward<__bf16>(A, launch);
+  else forward<_Float16>(A, launch);
   return flk_launch_status();
 }
 
@@ -600,14 +1055,9 @@ extern "C" int flk_attention_backward(const void* d_o, const int64_t* d_o_stride
   A.stats = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + of_mask);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (const int st = plan_mask(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace), s)) return st;
-  const dim3 of_q((unsigned)((int64_t)batch * heads * ((queries + kBlock - 1) / kBlock)));
-  const dim3 of_k((unsigned)((int64_t)batch * kv_heads * ((keys + kBlock - 1) / kBlock)));
-  if (dtype == FLK_BF16) {
-    attention_dq_kernel<__bf16><<<of_q, kThreads, 0, s>>>(A);
-    attention_dkv_kernel<__bf16><<<of_k, kThreads, 0, s>>>(A);
-  } else {
-    attention_dq_kernel<_Float16><<<of_q, kThreads, 0, s>>>(A);
-    attention_dkv_kernel<_Float16><<<of_k, kThreads, 0, s>>>(A);
-  }
+  const dim3 of_q((unsigned)((int64_t)batch * heads * ((queries + kQueries - 1) / kQueries)));
+  const dim3 of_k((unsigned)((int64_t)batch * kv_heads * ((keys + kKeys - 1) / kKeys)));
+  if (dtype == FLK_BF16) backward<__bf16>(A, of_q, of_k, s);
+  else backward<_Float16>(A, of_q, of_k, s);
   return flk_launch_status();
 }
