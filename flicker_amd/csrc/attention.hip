@@ -97,6 +97,13 @@ __device__ __forceinline__ uint32_t kept(const Args& A, int b, int u) {
   return left >= kUnit ? ~0u : (1u << left) - 1;
 }
 
+// Hardware deals blocks round-robin over the 8 XCDs, each with an L2 of its own: this numbering gives each XCD
+// neighbouring blocks, which read the same head's rows.
+__device__ __forceinline__ int block_of() {
+  const int p = blockIdx.x, xcd = p & 7, per = gridDim.x >> 3, extra = gridDim.x & 7;
+  return xcd * per + min(xcd, extra) + (p >> 3);
+}
+
 __device__ __forceinline__ int swz(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
 
 // LDS holds units of 32 rows of 256 bytes, whose 16-byte chunk c of row r sits in place c ^ swz(r).
@@ -376,8 +383,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[(kKRing + kVRing) * kUnitBytes];
   const int lane = threadIdx.x & 63, h4 = lane >> 4;
   const int blocks = (A.queries + kQueries - 1) / kQueries;
-  const int bh = blockIdx.x / blocks, b = bh / A.heads, h = bh - b * A.heads;
-  const int q0 = (blockIdx.x - bh * blocks) * kQueries + (threadIdx.x >> 6) * 32;
+  const int block = block_of(), bh = block / blocks, b = bh / A.heads, h = bh - b * A.heads;
+  const int q0 = (block - bh * blocks) * kQueries + (threadIdx.x >> 6) * 32;
   Units<kMasked> units(A, b);
   const int n = units.n;
   Forward<T> w;
@@ -549,8 +556,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
   __shared__ __attribute__((aligned(1024))) uint8_t smem[(kDqKRing + kDqVRing) * kUnitBytes];
   const int lane = threadIdx.x & 63, h4 = lane >> 4;
   const int blocks = (A.queries + kQueries - 1) / kQueries;
-  const int bh = blockIdx.x / blocks, b = bh / A.heads, h = bh - b * A.heads;
-  const int q0 = (blockIdx.x - bh * blocks) * kQueries + (threadIdx.x >> 6) * 32;
+  const int block = block_of(), bh = block / blocks, b = bh / A.heads, h = bh - b * A.heads;
+  const int q0 = (block - bh * blocks) * kQueries + (threadIdx.x >> 6) * 32;
   Units<kMasked> units(A, b);
   const int n = units.n;
   Dq<T> w;
@@ -869,8 +876,8 @@ template <typename T>
 __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kDkvBytes];
   const int blocks = (A.keys + kKeys - 1) / kKeys;
-  const int bh = blockIdx.x / blocks, b = bh / A.kv_heads, h = bh - b * A.kv_heads;
-  const int first = (blockIdx.x - bh * blocks) * kKeys;
+  const int block = block_of(), bh = block / blocks, b = bh / A.kv_heads, h = bh - b * A.kv_heads;
+  const int first = (block - bh * blocks) * kKeys;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   bool any = false;
   for (int u = first / kUnit; u < min(A.k_units, (first + kKeys) / kUnit); ++u) any |= kept(A, b, u) != 0;
