@@ -276,11 +276,11 @@ struct Forward {
   f32x4 l[2];              // sums of the rounded P (register 0 of lanes 0-15)
   vec8<T> ones;            // row 0 ones, rows 1-15 zeros
   float sum[2];            // with kKeep: of the unrounded P, this lane's
-  float top[2], limit[2];  // the maximum that P is taken against, and where it has to rise
+  float top[2], base[2];   // the maximum that P is taken against, and -log2(e) times it
   Places at;
 };
 
-constexpr float kSlack = 6.0f;   // how far S may pass the maximum it is taken against: P stays below 2^9
+constexpr float kSlack = 9.0f;   // P stays below 2^9
 
 // Phase u: S(u+1) = K(u+1) Q^T and O^T += V(u-1)^T P(u-1)^T on the matrix pipe while the vector units turn S(u) into P(u).
 template <bool kBias, bool kKeep, typename T, typename Hook>
@@ -294,30 +294,6 @@ __device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur
     sv[i] = s_cur[i];
     asm volatile("" : "+v"(sv[i]));
   }
-  // A row's P are exp(S - top) with the top of an earlier unit until S passes it by kSlack: then it rises to the row's
-  // maximum, and what has been summed, P(u-1) among it, is scaled when this phase has added P(u-1).
-  float high[2];
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    high[g] = fmaxf(fmaxf(sv[2 * g][0], sv[2 * g][1]), sv[2 * g][2]);
-    high[g] = fmaxf(fmaxf(high[g], sv[2 * g][3]), sv[2 * g + 1][0]);
-    high[g] = fmaxf(fmaxf(high[g], sv[2 * g + 1][1]), sv[2 * g + 1][2]);
-    high[g] = fmaxf(high[g], sv[2 * g + 1][3]);
-  }
-  const bool rise = __any(high[0] > w.limit[0] || high[1] > w.limit[1]);
-  float factor[2] = {1.0f, 1.0f};
-  if (rise) {
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      float t = fmaxf(high[g], __shfl_xor(high[g], 16));
-      t = fmaxf(fmaxf(t, __shfl_xor(t, 32)), w.top[g]);
-      factor[g] = __builtin_amdgcn_exp2f((w.top[g] - t) * kLog2e);
-      w.top[g] = t;
-      w.limit[g] = t + kSlack;
-      if constexpr (kKeep) w.sum[g] *= factor[g];
-    }
-  }
-  const float base[2] = {w.top[0] * -kLog2e, w.top[1] * -kLog2e};
   f32x4 start[2] = {};
   if constexpr (kBias) {
     if (bits_next != ~0u) {
@@ -325,13 +301,14 @@ __device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur
       start[1] = bias_of(bits_next, 1);
     }
   }
-  float t[16], e[16];
-  auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, base[n >> 3]); };
+  float t[16], e[16], high = -INFINITY, sum[2] = {};
+  auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, w.base[n >> 3]); };
   auto exp = [&](int n) { e[n] = __builtin_amdgcn_exp2f(t[n]); };
   auto put = [&](int n) {
     p_cur[n >> 1] = pack<T>(e[n], e[n + 1]);
     asm volatile("" : "+v"(p_cur[n >> 1]));   // keeps the pack in its slot
-    if constexpr (kKeep) w.sum[n >> 3] += e[n] + e[n + 1];
+    high = fmaxf(fmaxf(high, t[n]), t[n + 1]);
+    if constexpr (kKeep) sum[n >> 3] += e[n] + e[n + 1];
   };
   const vec8<T> pb[2] = {packed<T>(p_prev, 0), packed<T>(p_prev, 1)};
   scaled(0);
@@ -365,14 +342,35 @@ __device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur
     hook(n);
     __builtin_amdgcn_sched_barrier(0);
   }
-  if (rise) {
+  // A row's P are exp(S - top) with the top of an earlier unit, until an exponent passes kSlack: then top rises to the row's
+  // maximum, what has been summed is scaled, and this unit's P are formed again.
+  if (__any(high > kSlack)) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
+      float x = sv[2 * g][0];
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] *= factor[g];
-      // l's row 0 sits in the lanes 0-15, whose columns are these queries
-      w.l[g] *= factor[g];
+      for (int n = 1; n < 8; ++n) x = fmaxf(x, sv[2 * g + (n >> 2)][n & 3]);
+      x = fmaxf(x, __shfl_xor(x, 16));
+      x = fmaxf(fmaxf(x, __shfl_xor(x, 32)), w.top[g]);
+      const float factor = __builtin_amdgcn_exp2f((w.top[g] - x) * kLog2e);
+      w.top[g] = x;
+      w.base[g] = x * -kLog2e;
+      sum[g] = 0.0f;
+      w.sum[g] *= factor;
+      w.l[g] *= factor;   // row 0 of l sits in the lanes 0-15, whose columns are these queries
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] *= factor;
+#pragma unroll
+      for (int n = 8 * g; n < 8 * g + 8; ++n) {
+        scaled(n);
+        exp(n);
+        if (n & 1) put(n - 1);
+      }
     }
+  }
+  if constexpr (kKeep) {
+    w.sum[0] += sum[0];
+    w.sum[1] += sum[1];
   }
 }
 
@@ -394,7 +392,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
     w.l[g] = f32x4{};
     w.sum[g] = 0.0f;
-    w.top[g] = w.limit[g] = -1e30f;
+    w.top[g] = -1e30f;
+    w.base[g] = 1e30f * kLog2e;
   }
   if (n) {
     auto k_slot = [&](int i) { return smem + (i & (kKRing - 1)) * kUnitBytes; };
@@ -759,14 +758,11 @@ struct Queries {
   int units, left, unit;
   __device__ __forceinline__ Queries(const Tensor& t, int b, int h, int units, int heads)
       : head(t.at<uint16_t>(b, h)), row(t.row), next(t.head), units(units), left(heads), unit(0) {}
-  __device__ __forceinline__ void step() {   // past the last unit: the last
-    if (unit + 1 < units) {
-      ++unit;
-    } else if (left > 1) {
-      --left;
-      unit = 0;
-      head += next;
-    }
+  __device__ __forceinline__ void step() {   // past the last unit: the last; selects, not branches, inside a phase
+    const bool more = unit + 1 < units, wrap = !more && left > 1;
+    unit = more ? unit + 1 : wrap ? 0 : unit;
+    left -= wrap;
+    head += wrap ? next : 0;
   }
 };
 
