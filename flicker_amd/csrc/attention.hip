@@ -431,19 +431,20 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
 #pragma unroll
     for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
     __syncthreads();   // K(0) has been read: iteration 0 copies K(4) over it
-    auto iteration = [&](auto bias, int u, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8],
-                         uint32_t(&p_cur)[8]) {
+    // r: u's place in the rings; a literal in the unrolled loop, where LDS addresses are then a lane's constants
+    auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8],
+                         uint32_t(&p_cur)[8]) __attribute__((always_inline)) {
       constexpr bool kBias = decltype(bias)::value;
       units.get(u + 4, unit[4], bits[4]);
-      forward_phase<kBias, kKeep>(w, s_cur, s_next, p_prev, p_cur, k_slot(u + 1), v_slot(u - 1), k_slot(u + 2), bits[1],
+      forward_phase<kBias, kKeep>(w, s_cur, s_next, p_prev, p_cur, k_slot(r + 1), v_slot(r - 1), k_slot(r + 2), bits[1],
                                   [&](int slot) {
-                                    if (slot == 1) kc.start(k_slot(u + 4), unit[4]);
-                                    if (slot == 3) vc.start(v_slot(u + 1), unit[1]);
+                                    if (slot == 1) kc.start(k_slot(r), unit[4]);
+                                    if (slot == 3) vc.start(v_slot(r + 1), unit[1]);
                                   });
       landed<2>();
       if constexpr (kBias) {
-        clear_rows(k_slot(u + 3), bits[3]);
-        clear_rows(v_slot(u), bits[0]);
+        clear_rows(k_slot(r + 3), bits[3]);
+        clear_rows(v_slot(r), bits[0]);
       }
       barrier();
 #pragma unroll
@@ -453,14 +454,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
       }
     };
     int u = 0;
-    if constexpr (!kMasked)   // while no unit in reach is cut off: u + 4 < n - 1
-      for (; u + 6 < n; u += 2) {
-        iteration(std::false_type{}, u, s0, s1, p1, p0);
-        iteration(std::false_type{}, u + 1, s1, s0, p0, p1);
+    if constexpr (!kMasked)   // while no unit that an iteration clears or starts from is the last
+      for (; u + 8 < n; u += 4) {
+        iteration(std::false_type{}, u, 0, s0, s1, p1, p0);
+        iteration(std::false_type{}, u + 1, 1, s1, s0, p0, p1);
+        iteration(std::false_type{}, u + 2, 2, s0, s1, p1, p0);
+        iteration(std::false_type{}, u + 3, 3, s1, s0, p0, p1);
       }
     for (; u <= n; u += 2) {
-      iteration(std::true_type{}, u, s0, s1, p1, p0);
-      iteration(std::true_type{}, u + 1, s1, s0, p0, p1);
+      iteration(std::true_type{}, u, u, s0, s1, p1, p0);
+      iteration(std::true_type{}, u + 1, u + 1, s1, s0, p0, p1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy writes LDS that the block has left
   }
