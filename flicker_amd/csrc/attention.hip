@@ -150,22 +150,29 @@ __device__ __forceinline__ vec8<T> packed(const uint32_t (&p)[8], int g) {
 
 // Copies of a tensor's units into LDS: each wave 4 rows of 32, 16 bytes a lane, straight from memory.
 struct Copies {
-  const uint16_t* head;
-  int64_t row;
+  const char* head;
+  uint32_t step;          // bytes from one unit to the next
   uint32_t at, at_last;   // a lane's source offset in a unit, and in the last, whose rows past the end repeat the last row
   int last;               // that unit
-  __device__ __forceinline__ Copies(const uint16_t* head, int64_t row, int rows) : head(head), row(row) {
+  __device__ __forceinline__ Copies(const uint16_t* head, int64_t row, int rows)
+      : head(reinterpret_cast<const char*>(head)), step((uint32_t)row * kUnit * 2) {
     const int lane = threadIdx.x & 63, r = (threadIdx.x >> 6) * 4 + (lane >> 4);
     const uint32_t chunk = ((lane & 15) ^ swz(r)) << 4;
     last = (rows - 1) / kUnit;
     at = (uint32_t)(r * row * 2) + chunk;
     at_last = (uint32_t)(min(r, rows - 1 - last * kUnit) * row * 2) + chunk;
   }
-  __device__ __forceinline__ void start(uint8_t* slot, int unit) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    flk::dma16_at(head + (int64_t)unit * kUnit * row, unit == last ? at_last : at, slot + wave * 4 * kRowBytes);
+  // Unit `unit` of the head into the slot whose byte 0 of this wave's rows is `lds`.  kInside: it is not the last.
+  template <bool kInside>
+  __device__ __forceinline__ void start(unsigned lds, int unit) const {
+    flk::dma16_lds(head + (uint64_t)(uint32_t)unit * step, kInside || unit != last ? at : at_last, lds);
   }
 };
+
+// Where this wave's 4 rows of the unit at the start of LDS go.
+__device__ __forceinline__ unsigned wave_rows(const uint8_t* smem) {
+  return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)smem + (threadIdx.x >> 6) * 4 * kRowBytes);
+}
 
 // Clears this wave's rows of a unit that `bits` leaves out: 0 * what they hold would be NaN for infinities.  Their copy has
 // landed; the others see zeros after the next barrier.
@@ -212,6 +219,18 @@ struct Units {
     } else {
       unit = min(i, n - 1);
       bits = i < n - 1 ? ~0u : i == n - 1 ? tail : 0u;
+    }
+  }
+  // The units of u .. u + 4, of which a masked entry has fetched the first four.
+  __device__ __forceinline__ void look(int u, int (&unit)[5], uint32_t (&bits)[5]) {
+#pragma unroll
+    for (int i = kMasked ? 4 : 0; i < 5; ++i) get(u + i, unit[i], bits[i]);
+  }
+  static __device__ __forceinline__ void shift(int (&unit)[5], uint32_t (&bits)[5]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unit[i] = unit[i + 1];
+      bits[i] = bits[i + 1];
     }
   }
 };
@@ -398,15 +417,18 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
   if (n) {
     auto k_slot = [&](int i) { return smem + (i & (kKRing - 1)) * kUnitBytes; };
     auto v_slot = [&](int i) { return smem + (kKRing + (i & (kVRing - 1))) * kUnitBytes; };
+    const unsigned lds = wave_rows(smem);
+    auto k_lds = [&](int i) { return lds + (i & (kKRing - 1)) * kUnitBytes; };
+    auto v_lds = [&](int i) { return lds + (kKRing + (i & (kVRing - 1))) * kUnitBytes; };
     const Copies kc(A.k.at<uint16_t>(b, h / A.group), A.k.row, A.keys), vc(A.v.at<uint16_t>(b, h / A.group), A.v.row, A.keys);
     int unit[5];          // of the iterations u .. u + 4
     uint32_t bits[5];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       units.get(i, unit[i], bits[i]);
-      kc.start(k_slot(i), unit[i]);
+      kc.start<false>(k_lds(i), unit[i]);
     }
-    vc.start(v_slot(0), unit[0]);
+    vc.start<false>(v_lds(0), unit[0]);
     load_rows<T>(w.x, A.q.at<T>(b, h), A.q.row, q0, A.queries);
     w.at = places();
     const T one = (T)((lane & 15) == 0 ? 1.0f : 0.0f);
@@ -434,12 +456,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
     // r: u's place in the rings; a literal in the unrolled loop, where LDS addresses are then a lane's constants
     auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8],
                          uint32_t(&p_cur)[8]) __attribute__((always_inline)) {
-      constexpr bool kBias = decltype(bias)::value;
-      units.get(u + 4, unit[4], bits[4]);
+      constexpr bool kBias = decltype(bias)::value, kAhead = !kMasked && !kBias;
+      if constexpr (!kAhead) units.look(u, unit, bits);
       forward_phase<kBias, kKeep>(w, s_cur, s_next, p_prev, p_cur, k_slot(r + 1), v_slot(r - 1), k_slot(r + 2), bits[1],
                                   [&](int slot) {
-                                    if (slot == 1) kc.start(k_slot(r), unit[4]);
-                                    if (slot == 3) vc.start(v_slot(r + 1), unit[1]);
+                                    if (slot == 1) kc.start<kAhead>(k_lds(r), kAhead ? u + 4 : unit[4]);
+                                    if (slot == 3) vc.start<kAhead>(v_lds(r + 1), kAhead ? u + 1 : unit[1]);
                                   });
       landed<2>();
       if constexpr (kBias) {
@@ -447,20 +469,17 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
         clear_rows(v_slot(r), bits[0]);
       }
       barrier();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        unit[i] = unit[i + 1];
-        bits[i] = bits[i + 1];
-      }
+      if constexpr (kMasked) units.shift(unit, bits);
+    };
+    auto turn = [&](auto bias, int u) __attribute__((always_inline)) {
+      iteration(bias, u, 0, s0, s1, p1, p0);
+      iteration(bias, u + 1, 1, s1, s0, p0, p1);
+      iteration(bias, u + 2, 2, s0, s1, p1, p0);
+      iteration(bias, u + 3, 3, s1, s0, p0, p1);
     };
     int u = 0;
-    if constexpr (!kMasked)   // while no unit that an iteration clears or starts from is the last
-      for (; u + 8 < n; u += 4) {
-        iteration(std::false_type{}, u, 0, s0, s1, p1, p0);
-        iteration(std::false_type{}, u + 1, 1, s1, s0, p0, p1);
-        iteration(std::false_type{}, u + 2, 2, s0, s1, p1, p0);
-        iteration(std::false_type{}, u + 3, 3, s1, s0, p0, p1);
-      }
+    // the last unit is out of reach of what a turn copies, clears and starts from
+    for (; u + 8 < n; u += 4) turn(std::bool_constant<kMasked>{}, u);
     for (; u <= n; u += 2) {
       iteration(std::true_type{}, u, u, s0, s1, p1, p0);
       iteration(std::true_type{}, u + 1, u + 1, s1, s0, p0, p1);
@@ -551,7 +570,7 @@ __device__ __forceinline__ void dq_phase(Dq<T>& w, const f32x4 (&s_cur)[4], cons
   }
 }
 
-constexpr int kDqKRing = 8, kDqVRing = 4;
+constexpr int kDqKRing = 6, kDqVRing = 3;
 
 template <typename T, bool kMasked>
 __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A) {
@@ -595,20 +614,24 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
   if (n) {
-    auto k_slot = [&](int i) { return smem + (i & (kDqKRing - 1)) * kUnitBytes; };
-    auto v_slot = [&](int i) { return smem + (kDqKRing + (i & (kDqVRing - 1))) * kUnitBytes; };
+    // i: 0 .. 11, a place in K's ring plus up to 5; V's divides it
+    auto k_slot = [&](int i) { return smem + (i >= kDqKRing ? i - kDqKRing : i) * kUnitBytes; };
+    auto v_slot = [&](int i) { return smem + (kDqKRing + i % kDqVRing) * kUnitBytes; };
+    const unsigned lds = wave_rows(smem);
+    auto k_lds = [&](int i) { return lds + (i >= kDqKRing ? i - kDqKRing : i) * kUnitBytes; };
+    auto v_lds = [&](int i) { return lds + (kDqKRing + i % kDqVRing) * kUnitBytes; };
     const Copies kc(A.k.at<uint16_t>(b, h / A.group), A.k.row, A.keys), vc(A.v.at<uint16_t>(b, h / A.group), A.v.row, A.keys);
     int unit[5];
     uint32_t bits[5];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       units.get(i, unit[i], bits[i]);
-      kc.start(k_slot(i), unit[i]);
-      if (i < 3) vc.start(v_slot(i), unit[i]);
+      kc.start<false>(k_lds(i), unit[i]);
+      if (i < 3) vc.start<false>(v_lds(i), unit[i]);
     }
     load_rows<T>(w.x, A.q.at<T>(b, h), A.q.row, q0, A.queries);
     w.at = places();
-    reinterpret_cast<uint4*>(k_slot(-1))[threadIdx.x] = make_uint4(0, 0, 0, 0);   // K(-1), times dS(-1) = 0
+    reinterpret_cast<uint4*>(k_slot(kDqKRing - 1))[threadIdx.x] = make_uint4(0, 0, 0, 0);   // K(-1), times dS(-1) = 0
     landed<0>();
     for (int i = 0; i < 4; ++i) {
       clear_rows(k_slot(i), bits[i]);
@@ -632,36 +655,38 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
     }
 #pragma unroll
     for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
-    auto iteration = [&](auto bias, int u, const f32x4(&s_cur)[4], const f32x4(&d_cur)[4], f32x4(&s_next)[4],
-                         f32x4(&d_next)[4], const uint32_t(&p_prev)[8], uint32_t(&p_cur)[8]) {
-      constexpr bool kBias = decltype(bias)::value;
-      units.get(u + 4, unit[4], bits[4]);
-      dq_phase<kBias>(w, s_cur, d_cur, s_next, d_next, p_prev, p_cur, k_slot(u + 1), v_slot(u + 1), k_slot(u - 1),
-                      k_slot(u + 2), bits[1], [&](int slot) {
-                        if (slot == 1) kc.start(k_slot(u + 4), unit[4]);
-                        if (slot == 3) vc.start(v_slot(u + 3), unit[3]);
+    __syncthreads();   // V(0) has been read: iteration 0 copies V(3) over it
+    // r: u's place in K's ring
+    auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[4], const f32x4(&d_cur)[4], f32x4(&s_next)[4],
+                         f32x4(&d_next)[4], const uint32_t(&p_prev)[8], uint32_t(&p_cur)[8]) __attribute__((always_inline)) {
+      constexpr bool kBias = decltype(bias)::value, kAhead = !kMasked && !kBias;
+      if constexpr (!kAhead) units.look(u, unit, bits);
+      dq_phase<kBias>(w, s_cur, d_cur, s_next, d_next, p_prev, p_cur, k_slot(r + 1), v_slot(r + 1), k_slot(r + 5),
+                      k_slot(r + 2), bits[1], [&](int slot) {
+                        if (slot == 1) kc.start<kAhead>(k_lds(r + 4), kAhead ? u + 4 : unit[4]);
+                        if (slot == 3) vc.start<kAhead>(v_lds(r), kAhead ? u + 3 : unit[3]);
                       });
       landed<2>();
       if constexpr (kBias) {
-        clear_rows(k_slot(u + 3), bits[3]);
-        clear_rows(v_slot(u + 2), bits[2]);
+        clear_rows(k_slot(r + 3), bits[3]);
+        clear_rows(v_slot(r + 2), bits[2]);
       }
       barrier();
+      if constexpr (kMasked) units.shift(unit, bits);
+    };
+    auto turn = [&](auto bias, int u) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        unit[i] = unit[i + 1];
-        bits[i] = bits[i + 1];
+      for (int r = 0; r < kDqKRing; r += 2) {
+        iteration(bias, u + r, r, s0, d0, s1, d1, p1, p0);
+        iteration(bias, u + r + 1, r + 1, s1, d1, s0, d0, p0, p1);
       }
     };
-    int u = 0;
-    if constexpr (!kMasked)
-      for (; u + 6 < n; u += 2) {
-        iteration(std::false_type{}, u, s0, d0, s1, d1, p1, p0);
-        iteration(std::false_type{}, u + 1, s1, d1, s0, d0, p0, p1);
-      }
+    int u = 0, r = 0;
+    for (; u + 10 < n; u += kDqKRing) turn(std::bool_constant<kMasked>{}, u);
     for (; u <= n; u += 2) {
-      iteration(std::true_type{}, u, s0, d0, s1, d1, p1, p0);
-      iteration(std::true_type{}, u + 1, s1, d1, s0, d0, p0, p1);
+      iteration(std::true_type{}, u, r, s0, d0, s1, d1, p1, p0);
+      iteration(std::true_type{}, u + 1, r + 1, s1, d1, s0, d0, p0, p1);
+      r = r + 2 == kDqKRing ? 0 : r + 2;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
@@ -680,13 +705,13 @@ struct Dkv {
   Places at;
 };
 
-// The first wave's phase u: S(u+1) = Q(u+1) K^T and dV^T += dO(u-1)^T P(u-1) while P(u) is formed.  The second's:
-// dP(u) = dO(u) V^T and dK^T += Q(u-2)^T dS(u-2) while dS(u-1) = P(u-1) (dP(u-1) - delta) is formed; dP starts from
-// -delta.  `stats`: of the next phase; `hand`: where P goes (comes from).
+// The first wave's phase u: S(u+1) = Q(u+1) K^T, then dV^T += dO(u-1)^T P(u-1), while P(u) is formed.  The second's:
+// dK^T += Q(u-2)^T dS(u-2), then dP(u) = dO(u) V^T, which starts from -delta, while dS(u-1) = P(u-1) (dP(u-1) - delta) is
+// formed from what the first wave left in `hand`.  `after`: the next phase's first operands, `stats` its stats.
 template <bool kSecond, typename T, typename Hook>
 __device__ __forceinline__ void dkv_phase(Dkv<T>& w, const f32x4 (&s_cur)[4], f32x4 (&s_next)[4], const uint32_t (&p_prev)[8],
-                                          uint32_t (&p_cur)[8], const uint8_t* rows, const uint8_t* cols,
-                                          const uint8_t* rows_after, const uint8_t* stats, uint8_t* hand, Hook&& hook) {
+                                          uint32_t (&p_cur)[8], const uint8_t* rows, const uint8_t* cols, const uint8_t* after,
+                                          const uint8_t* stats, uint8_t* hand, Hook&& hook) {
   const int lane = threadIdx.x & 63;
   f32x4* const mine = reinterpret_cast<f32x4*>(hand) + lane;   // accumulator i at mine[64 i]
   f32x4 sv[4], e4[4], stat_next[2];
@@ -718,20 +743,20 @@ __device__ __forceinline__ void dkv_phase(Dkv<T>& w, const f32x4 (&s_cur)[4], f3
 #pragma unroll
   for (int n = 0; n < 16; ++n) {
     const vec8<T>& a = w.ops[n % (2 * kLead)];
-    if (n < 8) {
-      const int st = n >> 1, kt = n & 1;
+    if ((n < 8) != kSecond) {
+      const int st = (n & 7) >> 1, kt = n & 1;
 #pragma unroll
       for (int g = 0; g < 2; ++g)
         s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : kSecond ? w.stat[kt] : f32x4{});
     } else {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) w.acc[n - 8][g] = mfma(a, pb[g], w.acc[n - 8][g]);
+      for (int g = 0; g < 2; ++g) w.acc[n & 7][g] = mfma(a, pb[g], w.acc[n & 7][g]);
     }
     const int m = n + kLead;
     vec8<T>& to = w.ops[m % (2 * kLead)];
-    if (m < 8) to = row_operand<T>(rows, w.at, m >> 1, m & 1);
-    else if (m < 16) to = col_operand<T>(cols, w.at, m - 8);
-    else to = row_operand<T>(rows_after, w.at, (m - 16) >> 1, m & 1);
+    const bool of_rows = (m & 8) == (kSecond ? 8 : 0);
+    if (of_rows) to = row_operand<T>(m < 16 ? rows : after, w.at, (m & 7) >> 1, m & 1);
+    else to = col_operand<T>(m < 16 ? cols : after, w.at, m & 7);
     if (n >= 9 && n < 11) stat_next[n - 9] = *reinterpret_cast<const f32x4*>(
         stats + (kSecond ? kUnit * 4 : 0) + (n - 9) * 64 + (lane >> 4) * 16);
     if constexpr (kSecond) {
@@ -749,23 +774,39 @@ __device__ __forceinline__ void dkv_phase(Dkv<T>& w, const f32x4 (&s_cur)[4], f3
   w.stat[1] = stat_next[1];
 }
 
-constexpr int kQRing = 8, kORing = 5, kStatRing = 8;   // units of Q, of dO and of their stats in LDS
+constexpr int kQRing = 8, kORing = 4, kStatRing = 8;   // units of Q, of dO and of their stats in LDS
 constexpr int kStatBytes = 2 * kUnit * 4, kHandBytes = 4096;
 constexpr int kDkvStats = (kQRing + kORing) * kUnitBytes, kDkvHands = kDkvStats + kStatRing * kStatBytes;
 constexpr int kDkvBytes = kDkvHands + kWaves * kHandBytes;   // two hands a pair of waves
 
-// The query units of the heads that share a key head, one after the other.
+// The units of the query heads that share a key head, one after the other.
 struct Queries {
-  const uint16_t* head;
-  int64_t row, next;     // elements from one row and one head to the next
-  int units, left, unit;
+  const char* at;        // the next unit
+  int64_t step, wrap;    // bytes to the one after it, and from a head's last unit to the next head's first
+  int units, unit, left; // its index in its head; heads from its on
   __device__ __forceinline__ Queries(const Tensor& t, int b, int h, int units, int heads)
-      : head(t.at<uint16_t>(b, h)), row(t.row), next(t.head), units(units), left(heads), unit(0) {}
-  __device__ __forceinline__ void step() {   // past the last unit: the last; selects, not branches, inside a phase
-    const bool more = unit + 1 < units, wrap = !more && left > 1;
-    unit = more ? unit + 1 : wrap ? 0 : unit;
-    left -= wrap;
-    head += wrap ? next : 0;
+      : at(reinterpret_cast<const char*>(t.at<uint16_t>(b, h))),
+        step(t.row * kUnit * 2),
+        wrap((t.head - (units - 1) * (t.row * kUnit)) * 2),
+        units(units),
+        unit(0),
+        left(heads) {}
+  // Whether a head's last unit is none of the next kCount.
+  template <int kCount>
+  __device__ __forceinline__ bool inside() const {
+    return unit + kCount < units;
+  }
+  template <bool kInside>
+  __device__ __forceinline__ void next() {   // past the last unit of all: the last; selects, not branches, inside a phase
+    if constexpr (kInside) {
+      at += step;
+      ++unit;
+    } else {
+      const bool more = unit + 1 < units, wraps = !more && left > 1;
+      at += more ? step : wraps ? wrap : 0;
+      unit = more ? unit + 1 : wraps ? 0 : unit;
+      left -= wraps;
+    }
   }
 };
 
@@ -788,33 +829,39 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, int b, in
   if (any) {
     const int n = A.q_units * A.group;
     auto q_slot = [&](int i) { return smem + (i & (kQRing - 1)) * kUnitBytes; };
-    auto o_slot = [&](int i) { return smem + (kQRing + i) * kUnitBytes; };   // i in its ring
+    auto o_slot = [&](int i) { return smem + (kQRing + (i & (kORing - 1))) * kUnitBytes; };
     auto stat_slot = [&](int i) { return smem + kDkvStats + (i & (kStatRing - 1)) * kStatBytes; };
     auto hand = [&](int i) { return smem + kDkvHands + (pair * 2 + (i & 1)) * kHandBytes; };
+    const unsigned lds = wave_rows(smem);
+    auto q_lds = [&](int i) { return lds + (i & (kQRing - 1)) * kUnitBytes; };
+    auto o_lds = [&](int i) { return lds + (kQRing + (i & (kORing - 1))) * kUnitBytes; };
+    const unsigned stat_lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)smem) + kDkvStats;
     const Copies qc(nullptr, A.q.row, A.queries), oc(nullptr, A.dO.row, A.queries);
     Queries qs(A.q, b, h * A.group, A.q_units, A.group), os(A.dO, b, h * A.group, A.q_units, A.group);
-    const float* stats = A.stats + ((int64_t)b * A.heads + h * A.group) * A.q_units * 2 * kUnit;
-    const float* none = A.stats + (int64_t)A.batch * A.heads * A.q_units * 2 * kUnit;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    auto copy = [&](const Copies& c, Queries& from, uint8_t* slot) {
-      flk::dma16_at(from.head + (int64_t)from.unit * kUnit * from.row, from.unit == c.last ? c.at_last : c.at,
-                    slot + wave * 4 * kRowBytes);
-      from.step();
+    const char* stats =
+        reinterpret_cast<const char*>(A.stats + ((int64_t)b * A.heads + h * A.group) * A.q_units * 2 * kUnit);
+    const char* none = reinterpret_cast<const char*>(A.stats + (int64_t)A.batch * A.heads * A.q_units * 2 * kUnit);
+    auto copy = [&](auto inside, const Copies& c, Queries& from, unsigned to) __attribute__((always_inline)) {
+      constexpr bool kInside = decltype(inside)::value;
+      flk::dma16_lds(from.at, kInside || from.unit != c.last ? c.at : c.at_last, to);
+      from.template next<kInside>();
     };
     // every wave copies all of a unit's stats: as many copies a wave as the waits count
-    auto copy_stats = [&](int i) {
-      flk::dma4_at(i < n ? stats + (int64_t)i * 2 * kUnit : none, lane * 4, stat_slot(i));
+    auto copy_stats = [&](auto inside, int i, int r) __attribute__((always_inline)) {
+      const char* from = stats + (int64_t)i * kStatBytes;
+      if constexpr (!decltype(inside)::value) from = i < n ? from : none;
+      flk::dma4_lds(from, lane * 4, stat_lds + (r & (kStatRing - 1)) * kStatBytes);
     };
-    for (int i = 0; i < 4; ++i) copy(qc, qs, q_slot(i));
+    for (int i = 0; i < 4; ++i) copy(std::false_type{}, qc, qs, q_lds(i));
     for (int i = 0; i < 3; ++i) {
-      copy(oc, os, o_slot(i));
-      copy_stats(i);
+      if (i < 2) copy(std::false_type{}, oc, os, o_lds(i));
+      copy_stats(std::false_type{}, i, i);
     }
     w.at = places();
     // Q(-1), Q(-2), dO(-1) and P(-1), which the first iterations read, times zeros
     reinterpret_cast<uint4*>(q_slot(-1))[threadIdx.x] = make_uint4(0, 0, 0, 0);
     reinterpret_cast<uint4*>(q_slot(-2))[threadIdx.x] = make_uint4(0, 0, 0, 0);
-    reinterpret_cast<uint4*>(o_slot(kORing - 1))[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4*>(o_slot(-1))[threadIdx.x] = make_uint4(0, 0, 0, 0);
     if (!kSecond)
 #pragma unroll
       for (int i = 0; i < 4; ++i) reinterpret_cast<f32x4*>(hand(1))[64 * i + lane] = f32x4{};
@@ -832,33 +879,38 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, int b, in
           for (int g = 0; g < 2; ++g) s0[2 * g + kt] = mfma(a, w.x[st][g], s0[2 * g + kt]);
         }
     }
-    const uint8_t* first = kSecond ? o_slot(0) : q_slot(1);
 #pragma unroll
-    for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(first, w.at, m >> 1, m & 1);
+    for (int m = 0; m < kLead; ++m)
+      w.ops[m] = kSecond ? col_operand<T>(q_slot(-2), w.at, m) : row_operand<T>(q_slot(1), w.at, m >> 1, m & 1);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
       w.stat[kt] = *reinterpret_cast<const f32x4*>(stat_slot(0) + (kSecond ? kUnit * 4 : 0) + kt * 64 + (lane >> 4) * 16);
-    int o = 0;   // u's place in dO's ring
-    auto o_at = [&](int d) { return o_slot(o + d >= kORing ? o + d - kORing : o + d); };
-    auto iteration = [&](int u, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8], uint32_t(&p_cur)[8]) {
-      const uint8_t* rows = kSecond ? o_at(0) : q_slot(u + 1);
-      const uint8_t* cols = kSecond ? q_slot(u - 2) : o_at(kORing - 1);
-      const uint8_t* after = kSecond ? o_at(1) : q_slot(u + 2);
-      dkv_phase<kSecond>(w, s_cur, s_next, p_prev, p_cur, rows, cols, after, stat_slot(u + 1), hand(kSecond ? u - 1 : u),
+    // r: u's place in the rings, 8 more or less; inside: no copy of it is of a head's last unit
+    auto iteration = [&](auto inside, int u, int r, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8],
+                         uint32_t(&p_cur)[8]) __attribute__((always_inline)) {
+      const uint8_t* rows = kSecond ? o_slot(r) : q_slot(r + 1);
+      const uint8_t* cols = kSecond ? q_slot(r - 2) : o_slot(r - 1);
+      const uint8_t* after = kSecond ? q_slot(r - 1) : q_slot(r + 2);
+      dkv_phase<kSecond>(w, s_cur, s_next, p_prev, p_cur, rows, cols, after, stat_slot(r + 1), hand(kSecond ? r - 1 : r),
                          [&](int slot) {
-                           if (slot == 1) copy(qc, qs, q_slot(u + 4));
-                           if (slot == 3) copy(oc, os, o_at(3));
-                           if (slot == 5) copy_stats(u + 3);
+                           if (slot == 1) copy(inside, qc, qs, q_lds(r + 4));
+                           if (slot == 3) copy(inside, oc, os, o_lds(r + 2));
+                           if (slot == 5) copy_stats(inside, u + 3, r + 3);
                          });
       if constexpr (!kSecond) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // P is in its hand
       landed<3>();
       barrier();
-      o = o + 1 == kORing ? 0 : o + 1;
     };
-    // the second wave's last unit goes into dK at u = n + 1
-    for (int u = 0; u < n + 2; u += 2) {
-      iteration(u, s0, s1, p1, p0);
-      iteration(u + 1, s1, s0, p0, p1);
+    int u = 0;
+    for (; qs.template inside<kQRing>() && u + kQRing <= n; u += kQRing)
+#pragma unroll
+      for (int r = 0; r < kQRing; r += 2) {
+        iteration(std::true_type{}, u + r, r, s0, s1, p1, p0);
+        iteration(std::true_type{}, u + r + 1, r + 1, s1, s0, p0, p1);
+      }
+    for (; u < n + 2; u += 2) {   // the second wave's last unit goes into dK at u = n + 1
+      iteration(std::false_type{}, u, u, s0, s1, p1, p0);
+      iteration(std::false_type{}, u + 1, u + 1, s1, s0, p0, p1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
