@@ -88,6 +88,11 @@ struct Args {
                     // end and in the last unit
   Mask mask;
   int batch, heads, kv_heads, group, queries, keys, q_units, k_units;
+  // The blocks from `whole` on are cut into `splits` along the units they walk: partial sums of 256 rows, in order, each
+  // with its rows' (top, l, sum) in the forward pass, which attention_join_kernel adds up.
+  int whole, splits;
+  float* part;      // (cut, 256, 128)
+  float* part_top;  // (cut, 256, 4)
 };
 
 // Which keys of unit u are kept.
@@ -99,10 +104,33 @@ __device__ __forceinline__ uint32_t kept(const Args& A, int b, int u) {
 
 // Hardware deals blocks round-robin over the 8 XCDs, each with an L2 of its own: this numbering gives each XCD
 // neighbouring blocks, which read the same head's rows.
-__device__ __forceinline__ int block_of() {
-  const int p = blockIdx.x, xcd = p & 7, per = gridDim.x >> 3, extra = gridDim.x & 7;
+__device__ __forceinline__ int by_xcd(int p, int total) {
+  const int xcd = p & 7, per = total >> 3, extra = total & 7;
   return xcd * per + min(xcd, extra) + (p >> 3);
 }
+
+// What a hardware block takes: a block, or one of its cuts.
+struct Piece {
+  int block, cut, split, splits;   // cut: its place among the partial sums, -1 for a whole block
+  __device__ __forceinline__ explicit Piece(const Args& A) {
+    const int p = blockIdx.x;
+    if (p < A.whole) {
+      block = by_xcd(p, A.whole);
+      cut = -1;
+      split = 0;
+      splits = 1;
+    } else {
+      const int i = by_xcd(p - A.whole, gridDim.x - A.whole);
+      splits = A.splits;
+      block = A.whole + i / splits;
+      split = i % splits;
+      cut = splits > 1 ? i : -1;
+    }
+  }
+  // Its part of n units.
+  __device__ __forceinline__ int first(int n) const { return split * (n / splits) + min(split, n % splits); }
+  __device__ __forceinline__ int count(int n) const { return n / splits + (split < n % splits); }
+};
 
 __device__ __forceinline__ int swz(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
 
@@ -199,17 +227,15 @@ __device__ __forceinline__ f32x4 bias_of(uint32_t bits, int kt) {
 template <bool kMasked>
 struct Units {
   const uint2* live;
-  int n;
+  int first, n;
   uint32_t tail;
   uint2 some;
-  __device__ __forceinline__ Units(const Args& A, int b) {
-    if constexpr (kMasked) {
-      n = __builtin_amdgcn_readfirstlane(A.mask.counts[b]);
-      live = A.mask.live + (int64_t)b * A.k_units;
-    } else {
-      n = A.k_units;
-      tail = kept(A, b, n - 1);
-    }
+  __device__ __forceinline__ Units(const Args& A, int b, const Piece& piece) {
+    const int all = kMasked ? __builtin_amdgcn_readfirstlane(A.mask.counts[b]) : A.k_units;
+    first = piece.first(all);
+    n = piece.count(all);
+    if constexpr (kMasked) live = A.mask.live + (int64_t)b * A.k_units + first;
+    else tail = first + n == all ? kept(A, b, all - 1) : ~0u;
   }
   __device__ __forceinline__ void get(int i, int& unit, uint32_t& bits) {
     if constexpr (kMasked) {
@@ -217,7 +243,7 @@ struct Units {
       unit = __builtin_amdgcn_readlane(some.x, i & 63);
       bits = i < n ? __builtin_amdgcn_readlane(some.y, i & 63) : 0u;
     } else {
-      unit = min(i, n - 1);
+      unit = first + min(i, n - 1);
       bits = i < n - 1 ? ~0u : i == n - 1 ? tail : 0u;
     }
   }
@@ -271,6 +297,18 @@ __device__ __forceinline__ void store_rows(const f32x4 (&acc)[8][2], const float
         *reinterpret_cast<uint2*>(low + (int64_t)r * low_stride + dt * 16 + h * 4) = w;
       }
     }
+  }
+}
+
+// The same unscaled as float32 rows of a cut's partial sums, for rows below `end`.
+__device__ __forceinline__ void store_part(const f32x4 (&acc)[8][2], float* dst, int row0, int end) {
+  const int lane = threadIdx.x & 63, h = lane >> 4;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int r = row0 + g * 16 + (lane & 15);
+    if (r >= end) continue;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(dst + r * kD + dt * 16 + h * 4) = acc[dt][g];
   }
 }
 
@@ -400,9 +438,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[(kKRing + kVRing) * kUnitBytes];
   const int lane = threadIdx.x & 63, h4 = lane >> 4;
   const int blocks = (A.queries + kQueries - 1) / kQueries;
-  const int block = block_of(), bh = block / blocks, b = bh / A.heads, h = bh - b * A.heads;
-  const int q0 = (block - bh * blocks) * kQueries + (threadIdx.x >> 6) * 32;
-  Units<kMasked> units(A, b);
+  const Piece piece(A);
+  const int block = piece.block, bh = block / blocks, b = bh / A.heads, h = bh - b * A.heads;
+  const int first = (block - bh * blocks) * kQueries, q0 = first + (threadIdx.x >> 6) * 32;
+  Units<kMasked> units(A, b, piece);
   const int n = units.n;
   Forward<T> w;
 #pragma unroll
@@ -438,53 +477,79 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
     for (int i = 0; i < 4; ++i) clear_rows(k_slot(i), bits[i]);
     clear_rows(v_slot(0), bits[0]);
     __syncthreads();
-    f32x4 s0[4], s1[4];
-    uint32_t p0[8], p1[8] = {};
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const f32x4 start = bias_of(bits[0], kt);
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        const vec8<T> a = row_operand<T>(k_slot(0), w.at, st, kt);
-#pragma unroll
-        for (int g = 0; g < 2; ++g) s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : start);
+    if (__builtin_amdgcn_readfirstlane(q0) >= A.queries) {   // no queries: this wave's share of the copies
+      __syncthreads();
+      const int turns = n > 8 ? (n - 5) / 4 * 4 : 0, all = turns + (n - turns + 2) / 2 * 2;   // as the loops below
+      for (int u = 0; u < all; ++u) {
+        units.look(u, unit, bits);
+        kc.start<false>(k_lds(u), unit[4]);
+        vc.start<false>(v_lds(u + 1), unit[1]);
+        landed<2>();
+        clear_rows(k_slot(u + 3), bits[3]);
+        clear_rows(v_slot(u), bits[0]);
+        barrier();
+        if constexpr (kMasked) units.shift(unit, bits);
       }
-    }
+    } else {
+      f32x4 s0[4], s1[4];
+      uint32_t p0[8], p1[8] = {};
 #pragma unroll
-    for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
-    __syncthreads();   // K(0) has been read: iteration 0 copies K(4) over it
-    // r: u's place in the rings; a literal in the unrolled loop, where LDS addresses are then a lane's constants
-    auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8],
-                         uint32_t(&p_cur)[8]) __attribute__((always_inline)) {
-      constexpr bool kBias = decltype(bias)::value, kAhead = !kMasked && !kBias;
-      if constexpr (!kAhead) units.look(u, unit, bits);
-      forward_phase<kBias, kKeep>(w, s_cur, s_next, p_prev, p_cur, k_slot(r + 1), v_slot(r - 1), k_slot(r + 2), bits[1],
-                                  [&](int slot) {
-                                    if (slot == 1) kc.start<kAhead>(k_lds(r), kAhead ? u + 4 : unit[4]);
-                                    if (slot == 3) vc.start<kAhead>(v_lds(r + 1), kAhead ? u + 1 : unit[1]);
-                                  });
-      landed<2>();
-      if constexpr (kBias) {
-        clear_rows(k_slot(r + 3), bits[3]);
-        clear_rows(v_slot(r), bits[0]);
+      for (int kt = 0; kt < 2; ++kt) {
+        const f32x4 start = bias_of(bits[0], kt);
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          const vec8<T> a = row_operand<T>(k_slot(0), w.at, st, kt);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : start);
+        }
       }
-      barrier();
-      if constexpr (kMasked) units.shift(unit, bits);
-    };
-    auto turn = [&](auto bias, int u) __attribute__((always_inline)) {
-      iteration(bias, u, 0, s0, s1, p1, p0);
-      iteration(bias, u + 1, 1, s1, s0, p0, p1);
-      iteration(bias, u + 2, 2, s0, s1, p1, p0);
-      iteration(bias, u + 3, 3, s1, s0, p0, p1);
-    };
-    int u = 0;
-    // the last unit is out of reach of what a turn copies, clears and starts from
-    for (; u + 8 < n; u += 4) turn(std::bool_constant<kMasked>{}, u);
-    for (; u <= n; u += 2) {
-      iteration(std::true_type{}, u, u, s0, s1, p1, p0);
-      iteration(std::true_type{}, u + 1, u + 1, s1, s0, p0, p1);
+#pragma unroll
+      for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
+      __syncthreads();   // K(0) has been read: iteration 0 copies K(4) over it
+      // r: u's place in the rings; a literal in the unrolled loop, where LDS addresses are then a lane's constants
+      auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8],
+                           uint32_t(&p_cur)[8]) __attribute__((always_inline)) {
+        constexpr bool kBias = decltype(bias)::value, kAhead = !kMasked && !kBias;
+        if constexpr (!kAhead) units.look(u, unit, bits);
+        forward_phase<kBias, kKeep>(w, s_cur, s_next, p_prev, p_cur, k_slot(r + 1), v_slot(r - 1), k_slot(r + 2), bits[1],
+                                    [&](int slot) {
+                                      if (slot == 1) kc.start<kAhead>(k_lds(r), kAhead ? units.first + u + 4 : unit[4]);
+                                      if (slot == 3) vc.start<kAhead>(v_lds(r + 1), kAhead ? units.first + u + 1 : unit[1]);
+                                    });
+        landed<2>();
+        if constexpr (kBias) {
+          clear_rows(k_slot(r + 3), bits[3]);
+          clear_rows(v_slot(r), bits[0]);
+        }
+        barrier();
+        if constexpr (kMasked) units.shift(unit, bits);
+      };
+      auto turn = [&](auto bias, int u) __attribute__((always_inline)) {
+        iteration(bias, u, 0, s0, s1, p1, p0);
+        iteration(bias, u + 1, 1, s1, s0, p0, p1);
+        iteration(bias, u + 2, 2, s0, s1, p1, p0);
+        iteration(bias, u + 3, 3, s1, s0, p0, p1);
+      };
+      int u = 0;
+      // the last unit is out of reach of what a turn copies, clears and starts from
+      for (; u + 8 < n; u += 4) turn(std::bool_constant<kMasked>{}, u);
+      for (; u <= n; u += 2) {
+        iteration(std::true_type{}, u, u, s0, s1, p1, p0);
+        iteration(std::true_type{}, u + 1, u + 1, s1, s0, p0, p1);
+      }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy writes LDS that the block has left
+  }
+  if (piece.cut >= 0) {
+    const int end = min(A.queries - first, kQueries);
+    store_part(w.acc, A.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int r = q0 - first + g * 16 + (lane & 15);
+      const f32x4 x = {w.top[g], __shfl(w.l[g][0], lane & 15), across(w.sum[g]), 0.0f};
+      if (h4 == 0 && r < end) reinterpret_cast<f32x4*>(A.part_top)[(int64_t)piece.cut * kQueries + r] = x;
+    }
+    return;
   }
   float scale[2];
 #pragma unroll
@@ -577,9 +642,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
   __shared__ __attribute__((aligned(1024))) uint8_t smem[(kDqKRing + kDqVRing) * kUnitBytes];
   const int lane = threadIdx.x & 63, h4 = lane >> 4;
   const int blocks = (A.queries + kQueries - 1) / kQueries;
-  const int block = block_of(), bh = block / blocks, b = bh / A.heads, h = bh - b * A.heads;
-  const int q0 = (block - bh * blocks) * kQueries + (threadIdx.x >> 6) * 32;
-  Units<kMasked> units(A, b);
+  const Piece piece(A);
+  const int block = piece.block, bh = block / blocks, b = bh / A.heads, h = bh - b * A.heads;
+  const int first = (block - bh * blocks) * kQueries, q0 = first + (threadIdx.x >> 6) * 32;
+  Units<kMasked> units(A, b, piece);
   const int n = units.n;
   Dq<T> w;
   load_rows<T>(w.g, A.dO.at<T>(b, h), A.dO.row, q0, A.queries);
@@ -600,7 +666,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
       sum = across(sum);
       w.lse[g] = x == -INFINITY ? -INFINITY : x * -kLog2e;
       w.delta[g] = x == -INFINITY ? 0.0f : -sum;
-      if (h4 == 0 && r < A.q_units * kUnit) {
+      if (piece.split == 0 && h4 == 0 && r < A.q_units * kUnit) {
         float* st = A.stats + ((int64_t)bh * A.q_units + r / kUnit) * 2 * kUnit + r % kUnit;
         st[0] = -w.lse[g];
         st[kUnit] = w.delta[g];
@@ -663,8 +729,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
       if constexpr (!kAhead) units.look(u, unit, bits);
       dq_phase<kBias>(w, s_cur, d_cur, s_next, d_next, p_prev, p_cur, k_slot(r + 1), v_slot(r + 1), k_slot(r + 5),
                       k_slot(r + 2), bits[1], [&](int slot) {
-                        if (slot == 1) kc.start<kAhead>(k_lds(r + 4), kAhead ? u + 4 : unit[4]);
-                        if (slot == 3) vc.start<kAhead>(v_lds(r), kAhead ? u + 3 : unit[3]);
+                        if (slot == 1) kc.start<kAhead>(k_lds(r + 4), kAhead ? units.first + u + 4 : unit[4]);
+                        if (slot == 3) vc.start<kAhead>(v_lds(r), kAhead ? units.first + u + 3 : unit[3]);
                       });
       landed<2>();
       if constexpr (kBias) {
@@ -689,6 +755,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
       r = r + 2 == kDqKRing ? 0 : r + 2;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  if (piece.cut >= 0) {
+    store_part(w.acc, A.part + (int64_t)piece.cut * kQueries * kD, q0 - first, min(A.queries - first, kQueries));
+    return;
   }
   const float one[2] = {1.0f, 1.0f};
   store_rows<T>(w.acc, one, A.dq.at<T>(b, h), A.dq.row, q0, A.queries);
@@ -784,13 +854,13 @@ struct Queries {
   const char* at;        // the next unit
   int64_t step, wrap;    // bytes to the one after it, and from a head's last unit to the next head's first
   int units, unit, left; // its index in its head; heads from its on
-  __device__ __forceinline__ Queries(const Tensor& t, int b, int h, int units, int heads)
-      : at(reinterpret_cast<const char*>(t.at<uint16_t>(b, h))),
-        step(t.row * kUnit * 2),
-        wrap((t.head - (units - 1) * (t.row * kUnit)) * 2),
-        units(units),
-        unit(0),
-        left(heads) {}
+  __device__ __forceinline__ Queries(const Tensor& t, int b, int h, int units, int heads, int first)
+      : step(t.row * kUnit * 2), wrap((t.head - (units - 1) * (t.row * kUnit)) * 2), units(units) {
+    const int skipped = first / units;
+    unit = first - skipped * units;
+    left = heads - skipped;
+    at = reinterpret_cast<const char*>(t.at<uint16_t>(b, h + skipped)) + unit * step;
+  }
   // Whether a head's last unit is none of the next kCount.
   template <int kCount>
   __device__ __forceinline__ bool inside() const {
@@ -811,7 +881,8 @@ struct Queries {
 };
 
 template <bool kSecond, typename T>
-__device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, int b, int h, int k0, bool any) {
+__device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Piece& piece, int b, int h, int first, int k0,
+                                         bool any) {
   const int lane = threadIdx.x & 63, pair = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
   Dkv<T> w;
   const Tensor& own = kSecond ? A.v : A.k;
@@ -827,7 +898,7 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, int b, in
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
   }
   if (any) {
-    const int n = A.q_units * A.group;
+    const int from = piece.first(A.q_units * A.group), n = piece.count(A.q_units * A.group);
     auto q_slot = [&](int i) { return smem + (i & (kQRing - 1)) * kUnitBytes; };
     auto o_slot = [&](int i) { return smem + (kQRing + (i & (kORing - 1))) * kUnitBytes; };
     auto stat_slot = [&](int i) { return smem + kDkvStats + (i & (kStatRing - 1)) * kStatBytes; };
@@ -837,9 +908,9 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, int b, in
     auto o_lds = [&](int i) { return lds + (kQRing + (i & (kORing - 1))) * kUnitBytes; };
     const unsigned stat_lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)smem) + kDkvStats;
     const Copies qc(nullptr, A.q.row, A.queries), oc(nullptr, A.dO.row, A.queries);
-    Queries qs(A.q, b, h * A.group, A.q_units, A.group), os(A.dO, b, h * A.group, A.q_units, A.group);
+    Queries qs(A.q, b, h * A.group, A.q_units, A.group, from), os(A.dO, b, h * A.group, A.q_units, A.group, from);
     const char* stats =
-        reinterpret_cast<const char*>(A.stats + ((int64_t)b * A.heads + h * A.group) * A.q_units * 2 * kUnit);
+        reinterpret_cast<const char*>(A.stats + (((int64_t)b * A.heads + h * A.group) * A.q_units + from) * 2 * kUnit);
     const char* none = reinterpret_cast<const char*>(A.stats + (int64_t)A.batch * A.heads * A.q_units * 2 * kUnit);
     auto copy = [&](auto inside, const Copies& c, Queries& from, unsigned to) __attribute__((always_inline)) {
       constexpr bool kInside = decltype(inside)::value;
@@ -918,6 +989,11 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, int b, in
   for (int g = 0; g < 2; ++g)
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = on[g] ? w.acc[dt][g] : f32x4{};
+  if (piece.cut >= 0) {   // dv's 128 rows, then dk's
+    float* part = A.part + ((int64_t)piece.cut * 2 + kSecond) * kKeys * kD;
+    store_part(w.acc, part, k0 - first, min(A.keys - first, kKeys));
+    return;
+  }
   const float one[2] = {1.0f, 1.0f};
   const Tensor& out = kSecond ? A.dk : A.dv;
   store_rows<T>(w.acc, one, out.at<T>(b, h), out.row, k0, A.keys);
@@ -927,14 +1003,61 @@ template <typename T>
 __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kDkvBytes];
   const int blocks = (A.keys + kKeys - 1) / kKeys;
-  const int block = block_of(), bh = block / blocks, b = bh / A.kv_heads, h = bh - b * A.kv_heads;
+  const Piece piece(A);
+  const int block = piece.block, bh = block / blocks, b = bh / A.kv_heads, h = bh - b * A.kv_heads;
   const int first = (block - bh * blocks) * kKeys;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   bool any = false;
   for (int u = first / kUnit; u < min(A.k_units, (first + kKeys) / kUnit); ++u) any |= kept(A, b, u) != 0;
   const int k0 = first + (wave & 3) * 32;
-  if (wave < 4) dkv_wave<false, T>(A, smem, b, h, k0, any);
-  else dkv_wave<true, T>(A, smem, b, h, k0, any);
+  if (wave < 4) dkv_wave<false, T>(A, smem, piece, b, h, first, k0, any);
+  else dkv_wave<true, T>(A, smem, piece, b, h, first, k0, any);
+}
+
+// Adds the cuts' partial sums in order: 32 lanes a row, 8 rows of a cut block a block.
+enum Joined { kJoinO, kJoinDq, kJoinDkv };
+template <typename T, Joined kOf, bool kKeep>
+__global__ __launch_bounds__(256) void attention_join_kernel(const Args A) {
+  const int lane = threadIdx.x & 31;
+  const int cut_block = blockIdx.x / (kQueries / 8), r = blockIdx.x % (kQueries / 8) * 8 + (threadIdx.x >> 5);
+  const int block = A.whole + cut_block, rows = kOf == kJoinDkv ? A.keys : A.queries;
+  const int per = kOf == kJoinDkv ? kKeys : kQueries, heads = kOf == kJoinDkv ? A.kv_heads : A.heads;
+  const int blocks = (rows + per - 1) / per, bh = block / blocks, b = bh / heads, h = bh - b * heads;
+  const int row = (block - bh * blocks) * per + (kOf == kJoinDkv ? r % kKeys : r);
+  if (row >= rows) return;
+  const int64_t first = ((int64_t)cut_block * A.splits * kQueries + r) * kD;
+  f32x4 x{};
+  if constexpr (kOf == kJoinO) {
+    const f32x4* tops = reinterpret_cast<const f32x4*>(A.part_top) + (int64_t)cut_block * A.splits * kQueries + r;
+    float top = -1e30f, l = 0.0f, sum = 0.0f;
+    for (int i = 0; i < A.splits; ++i) top = fmaxf(top, tops[i * kQueries][0]);
+    for (int i = 0; i < A.splits; ++i) {
+      const f32x4 t = tops[i * kQueries];
+      const float f = __builtin_amdgcn_exp2f((t[0] - top) * kLog2e);
+      x += *reinterpret_cast<const f32x4*>(A.part + first + (int64_t)i * kQueries * kD + lane * 4) * f;
+      l += t[1] * f;
+      sum += t[2] * f;
+    }
+    x *= l > 0.0f ? 1.0f / l : 0.0f;
+    if constexpr (kKeep) {
+      if (lane == 0) A.lse[(int64_t)bh * A.queries + row] = l > 0.0f ? top + __builtin_amdgcn_logf(sum) * kLn2 : -INFINITY;
+      T* low = static_cast<T*>(A.low);
+      if (low) {
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = x[i] - (float)(T)x[i];
+        low += (((int64_t)b * A.queries + row) * A.heads + h) * kD + lane * 4;
+        *reinterpret_cast<uint2*>(low) = make_uint2(pack<T>(y[0], y[1]), pack<T>(y[2], y[3]));
+      }
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < A.splits; ++i)
+      x += *reinterpret_cast<const f32x4*>(A.part + first + (int64_t)i * kQueries * kD + lane * 4);
+  }
+  const Tensor& out = kOf == kJoinO ? A.o : kOf == kJoinDq ? A.dq : r < kKeys ? A.dv : A.dk;
+  *reinterpret_cast<uint2*>(out.at<T>(b, h) + (int64_t)row * out.row + lane * 4) =
+      make_uint2(pack<T>(x[0], x[1]), pack<T>(x[2], x[3]));
 }
 
 // The mask's words and live units, one batch entry a block, a thread a unit, 1024 units a turn.
@@ -990,6 +1113,53 @@ int plan_mask(const void* mask, int64_t batch_stride, Args& A, uint8_t* workspac
   return flk_launch_status();
 }
 
+// How a launch of `blocks` equal blocks, each walking n units, is cut: whole rounds of the 256 CUs, and what is left in
+// pieces, where that is estimated to be faster.
+struct Cut {
+  int whole, splits;
+  int64_t blocks;
+  int64_t grid() const { return whole + (blocks - whole) * splits; }
+  int64_t cuts() const { return splits > 1 ? (blocks - whole) * splits : 0; }
+  int64_t bytes() const { return cuts() * kQueries * (kD + 4) * 4; }
+};
+constexpr int kCUs = 256, kMaxSplits = 64;
+// us of a unit, and of a block's first loads and last stores, and of the join's launch and its bytes
+Cut plan_cut(int64_t blocks, int64_t n, double unit, int rows) {
+  constexpr double kFixed = 6.0, kJoin = 5.0, kBytes = 4e6;
+  auto rounds = [&](int64_t grid) { return (double)((grid + kCUs - 1) / kCUs); };
+  Cut best{(int)blocks, 1, blocks};
+  double least = rounds(blocks) * (n * unit + kFixed);
+  const int64_t whole = blocks / kCUs * kCUs, rest = blocks - whole;
+  if (rest == 0 || blocks > 16 * kCUs) return best;
+  for (int s = 2; s <= kMaxSplits && 4 * s <= n; ++s) {
+    const double time = rounds(whole) * (n * unit + kFixed) + rounds(rest * s) * ((n + s - 1) / s * unit + kFixed) + kJoin +
+                        rest * s * (double)rows * kD * 8 / kBytes;
+    if (time < least) {
+      least = time;
+      best = Cut{(int)whole, s, blocks};
+    }
+  }
+  return best;
+}
+Cut forward_cut(const Args& A) {
+  const int64_t blocks = (int64_t)A.batch * A.heads * ((A.queries + kQueries - 1) / kQueries);
+  return plan_cut(blocks, A.k_units, 0.95, std::min(A.queries, kQueries));
+}
+Cut dq_cut(const Args& A) {
+  const int64_t blocks = (int64_t)A.batch * A.heads * ((A.queries + kQueries - 1) / kQueries);
+  return plan_cut(blocks, A.k_units, 1.2, std::min(A.queries, kQueries));
+}
+Cut dkv_cut(const Args& A) {
+  const int64_t blocks = (int64_t)A.batch * A.kv_heads * ((A.keys + kKeys - 1) / kKeys);
+  return plan_cut(blocks, (int64_t)A.q_units * A.group, 0.85, 2 * std::min(A.keys, kKeys));
+}
+void use_cut(Args& A, const Cut& cut, uint8_t* workspace) {
+  A.whole = cut.whole;
+  A.splits = cut.splits;
+  A.part = reinterpret_cast<float*>(workspace);
+  A.part_top = A.part + cut.cuts() * kQueries * kD;
+}
+
 bool sizes_ok(int batch, int heads, int kv_heads, int queries, int keys) {
   if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || queries < 0 || keys < 0) return false;
   if (queries > 1 << 28 || keys > 1 << 28 || batch > 1 << 20) return false;
@@ -1018,17 +1188,40 @@ Args sizes(int batch, int heads, int kv_heads, int queries, int keys) {
   return A;
 }
 
-template <typename T, typename Launch>
-void forward(const Args& A, Launch&& launch) {
-  if (A.mask.bits) A.lse ? launch(attention_kernel<T, true, true>) : launch(attention_kernel<T, true, false>);
-  else A.lse ? launch(attention_kernel<T, false, true>) : launch(attention_kernel<T, false, false>);
+int64_t join_grid(const Cut& cut) { return (cut.blocks - cut.whole) * (kQueries / 8); }
+
+template <typename T>
+void forward(const Args& A, const Cut& cut, hipStream_t s) {
+  const dim3 grid((unsigned)cut.grid());
+  if (A.mask.bits) {
+    if (A.lse) attention_kernel<T, true, true><<<grid, kThreads, 0, s>>>(A);
+    else attention_kernel<T, true, false><<<grid, kThreads, 0, s>>>(A);
+  } else {
+    if (A.lse) attention_kernel<T, false, true><<<grid, kThreads, 0, s>>>(A);
+    else attention_kernel<T, false, false><<<grid, kThreads, 0, s>>>(A);
+  }
+  if (cut.splits == 1) return;
+  if (A.lse) attention_join_kernel<T, kJoinO, true><<<(unsigned)join_grid(cut), 256, 0, s>>>(A);
+  else attention_join_kernel<T, kJoinO, false><<<(unsigned)join_grid(cut), 256, 0, s>>>(A);
 }
 
 template <typename T>
-void backward(const Args& A, dim3 of_q, dim3 of_k, hipStream_t s) {
-  if (A.mask.bits) attention_dq_kernel<T, true><<<of_q, kThreads, 0, s>>>(A);
-  else attention_dq_kernel<T, false><<<of_q, kThreads, 0, s>>>(A);
-  attention_dkv_kernel<T><<<of_k, kThreads, 0, s>>>(A);
+void backward(Args& A, uint8_t* workspace, hipStream_t s) {
+  const Cut q = dq_cut(A), k = dkv_cut(A);
+  use_cut(A, q, workspace);
+  if (A.mask.bits) attention_dq_kernel<T, true><<<(unsigned)q.grid(), kThreads, 0, s>>>(A);
+  else attention_dq_kernel<T, false><<<(unsigned)q.grid(), kThreads, 0, s>>>(A);
+  if (q.splits > 1) attention_join_kernel<T, kJoinDq, false><<<(unsigned)join_grid(q), 256, 0, s>>>(A);
+  use_cut(A, k, workspace);   // the kernels run one after the other: dq's partial sums have been read
+  attention_dkv_kernel<T><<<(unsigned)k.grid(), kThreads, 0, s>>>(A);
+  if (k.splits > 1) attention_join_kernel<T, kJoinDkv, false><<<(unsigned)join_grid(k), 256, 0, s>>>(A);
+}
+
+int64_t workspace_of(const Args& A, bool masked, bool backward) {
+  if (A.batch == 0 || A.queries == 0 || (A.keys == 0 && backward)) return 0;
+  const int64_t mask = masked ? mask_bytes(A.batch, A.keys) : 0;
+  if (!backward) return mask + forward_cut(A).bytes();
+  return mask + stats_bytes(A.batch, A.heads, A.queries) + std::max(dq_cut(A).bytes(), dkv_cut(A).bytes());
 }
 
 }  // namespace
@@ -1036,7 +1229,8 @@ void backward(const Args& A, dim3 of_q, dim3 of_k, hipStream_t s) {
 extern "C" int flk_attention_plan(int batch, int heads, int kv_heads, int queries, int keys, int masked, int backward,
                                   int64_t* workspace_bytes) {
   if (!workspace_bytes || !sizes_ok(batch, heads, kv_heads, queries, keys)) return FLK_E_INVALID;
-  *workspace_bytes = (masked ? mask_bytes(batch, keys) : 0) + (backward ? stats_bytes(batch, heads, queries) : 0);
+  const Args A = sizes(batch, heads, kv_heads, queries, keys);
+  *workspace_bytes = workspace_of(A, masked, backward);
   return FLK_OK;
 }
 
@@ -1059,7 +1253,7 @@ extern "C" int flk_attention(const void* q, const int64_t* q_strides, const void
     A.v = tensor(v, v_strides);
   }
   if (!flk_host_aligned(low, 16) || !flk_host_aligned(lse, 4)) return FLK_E_ALIGN;
-  const int64_t need = key_mask ? mask_bytes(batch, keys) : 0;
+  const int64_t need = workspace_of(A, key_mask, false);
   if (need && (!workspace || workspace_bytes < need)) return FLK_E_SCRATCH;
   if (!flk_host_aligned(workspace, 256)) return FLK_E_ALIGN;
   A.q = tensor(q, q_strides);
@@ -1068,11 +1262,10 @@ extern "C" int flk_attention(const void* q, const int64_t* q_strides, const void
   A.lse = lse;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (const int st = plan_mask(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace), s)) return st;
-  if (keys == 0) A.k_units = 0;
-  const dim3 grid((unsigned)((int64_t)batch * heads * ((queries + kQueries - 1) / kQueries)));
-  auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(A); };
-  if (dtype == FLK_BF16) forward<__bf16>(A, launch);
-  else forward<_Float16>(A, launch);
+  const Cut cut = forward_cut(A);
+  use_cut(A, cut, static_cast<uint8_t*>(workspace) + (key_mask ? mask_bytes(batch, keys) : 0));
+  if (dtype == FLK_BF16) forward<__bf16>(A, cut, s);
+  else forward<_Float16>(A, cut, s);
   return flk_launch_status();
 }
 
@@ -1096,10 +1289,10 @@ extern "C" int flk_attention_backward(const void* d_o, const int64_t* d_o_stride
     if (const int st = check_tensor(t.p, t.strides)) return st;
   if (!low || !lse) return FLK_E_INVALID;
   if (!flk_host_aligned(low, 16) || !flk_host_aligned(lse, 4)) return FLK_E_ALIGN;
-  const int64_t of_mask = key_mask ? mask_bytes(batch, keys) : 0;
-  if (!workspace || workspace_bytes < of_mask + stats_bytes(batch, heads, queries)) return FLK_E_SCRATCH;
-  if (!flk_host_aligned(workspace, 256)) return FLK_E_ALIGN;
   Args A = sizes(batch, heads, kv_heads, queries, keys);
+  if (!workspace || workspace_bytes < workspace_of(A, key_mask, true)) return FLK_E_SCRATCH;
+  if (!flk_host_aligned(workspace, 256)) return FLK_E_ALIGN;
+  const int64_t of_mask = key_mask ? mask_bytes(batch, keys) : 0;
   A.dO = tensor(d_o, d_o_strides);
   A.q = tensor(q, q_strides);
   A.k = tensor(k, k_strides);
@@ -1113,9 +1306,8 @@ extern "C" int flk_attention_backward(const void* d_o, const int64_t* d_o_stride
   A.stats = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + of_mask);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (const int st = plan_mask(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace), s)) return st;
-  const dim3 of_q((unsigned)((int64_t)batch * heads * ((queries + kQueries - 1) / kQueries)));
-  const dim3 of_k((unsigned)((int64_t)batch * kv_heads * ((keys + kKeys - 1) / kKeys)));
-  if (dtype == FLK_BF16) backward<__bf16>(A, of_q, of_k, s);
-  else backward<_Float16>(A, of_q, of_k, s);
+  uint8_t* parts = reinterpret_cast<uint8_t*>(A.stats) + stats_bytes(batch, heads, queries);
+  if (dtype == FLK_BF16) backward<__bf16>(A, parts, s);
+  else backward<_Float16>(A, parts, s);
   return flk_launch_status();
 }

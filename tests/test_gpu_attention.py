@@ -167,3 +167,17 @@ def test_logit_sizes(device, scale):
 @pytest.mark.parametrize("queries,keys", [(700, 900), (1030, 517)])
 def test_longer(device, queries, keys):
     check(3, 1, 1, 1, queries, keys, "bf16", "middle")
+
+
+@pytest.mark.parametrize("heads,kv_heads,queries,keys,mask", [
+    (2, 2, 3, 5000, None), (2, 1, 40, 3000, "middle"), (3, 3, 260, 2100, "random"), (1, 1, 1500, 100, None),
+    (4, 1, 900, 70, "random"), (6, 2, 33, 1999, "empty")])
+def test_cut_blocks(device, heads, kv_heads, queries, keys, mask):
+    """Too few blocks for the GPU: each is cut along the units it walks, and the partial sums are added."""
+    check(keys, 2, heads, kv_heads, queries, keys, "bf16", mask)
+
+
+@pytest.mark.parametrize("queries,keys", [(270, 1500), (1500, 200)])
+def test_whole_and_cut_blocks(device, queries, keys):
+    """A few blocks more than the GPU's CUs: those are cut, the others are not."""
+    check(keys, 2, 66, 66, queries, keys, "fp16", "middle" if keys == 200 else None)
