@@ -23,7 +23,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .kernels import HEAD_DIM, _on_gpu
+from .kernels import HEAD_DIM, _native, _on_gpu
 from .norm import _CODES
 
 _MAX_ROW = 1 << 25   # elements between two rows
@@ -110,6 +110,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: to
     strides -> (B, Lq, H * D).  ``key_mask`` (B, Lk) bool is True where a key is kept; a query that keeps none gets zeros,
     and what masked keys and values hold is never read into a result.  With ``keep`` also returns the ``Kept`` that
     attention_backward takes.  ``out`` may be a (B, Lq, H * D) view with strided rows that overlaps no operand."""
+    if out is None:
+        done = _native.attention(q, k, v, key_mask, keep)
+        if done is not None:
+            return (done[0], Kept(*done)) if keep else done[0]
     q, k, v, key_mask, sizes = _operands(q, k, v, key_mask)
     batch, heads, _, queries, keys = sizes
     dim = q.shape[3]
@@ -135,6 +139,9 @@ def attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
                        key_mask: torch.Tensor | None = None):
     """(dq, dk, dv) of ``attention(q, k, v, key_mask=key_mask, keep=True)`` for the incoming gradient do (B, Lq, H * D) and
     the ``kept`` that call returned; masked keys get zeros."""
+    done = _native.attention_backward(do, q, k, v, *kept, key_mask)
+    if done is not None:
+        return done
     grads = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     q, k, v, key_mask, sizes = _operands(q, k, v, key_mask)
     batch, heads, _, queries, keys = sizes

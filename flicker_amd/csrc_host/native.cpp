@@ -396,6 +396,88 @@ PyObject* norm_backward(PyObject* dy_, PyObject* x_, PyObject* factor, PyObject*
   return swap ? tuple_of({dx, dc, df}) : tuple_of({dx, df, dc});   // an undefined tensor becomes None
 }
 
+// The operands of residual_modulate: x and branch (B, L, width), and a row of gate, shift and scale per batch entry.
+struct Residual {
+  Blocks x, branch;
+  Params p;   // scale and shift
+  const at::Tensor* gate;
+};
+
+bool like_x(PyObject* o, int device, const Blocks& x, Blocks& b) {
+  return blocks_from(o, device, b) && b.t->sizes() == x.t->sizes() && b.t->scalar_type() == x.t->scalar_type();
+}
+
+bool residual_from(PyObject* const* a, int device, Residual& r) {   // x, branch, gate, shift, scale
+  Params gate;
+  if (!blocks_from(a[0], device, r.x) || r.x.t->dim() != 3 || !like_x(a[1], device, r.x, r.branch) ||
+      !params_from(a[4], a[3], true, r.x, device, r.p) || !params_from(a[2], a[2], true, r.x, device, gate) ||
+      gate.dtype != r.p.dtype)
+    return false;
+  r.gate = gate.factor;
+  return true;
+}
+
+// residual_modulate(x, branch, gate, shift, scale, eps) -> (r, y) or None
+PyObject* residual_modulate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const int device = n == 6 ? device_of(a[0]) : -1;
+  Residual o;
+  float eps;
+  if (device < 0 || !gain_of(a[5], eps) || !residual_from(a, device, o)) return none();
+  at::Tensor r, y;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    const Blocks &x = o.x, &b = o.branch;
+    r = empty(x.t->sizes(), x.t->scalar_type(), device);
+    y = empty(x.t->sizes(), x.t->scalar_type(), device);
+    const int64_t entry = (int64_t)x.length * x.width;
+    st = flk_residual_norm(x.t->data_ptr(), x.batch_stride, x.row_stride, b.t->data_ptr(), b.batch_stride, b.row_stride,
+                           code_of(x.t->scalar_type()), o.gate->data_ptr(), o.p.factor->data_ptr(), o.p.offset->data_ptr(),
+                           code_of(o.p.dtype), x.width, 1, eps, x.batch, x.length, x.width, r.data_ptr(), entry, x.width,
+                           y.data_ptr(), entry, x.width, stream_of(device));
+  }
+  return st == FLK_OK ? tuple_of({r, y}) : failed(st, "flk_residual_norm");
+  END_HANDLE_TH_ERRORS
+}
+
+// residual_modulate_backward(dr, dy, x, branch, gate, shift, scale, eps) -> (dx, dbranch, dgate, dshift, dscale) or None
+PyObject* residual_modulate_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const int device = n == 8 ? device_of(a[2]) : -1;
+  Residual o;
+  Blocks dr, dy;
+  float eps;
+  if (device < 0 || !gain_of(a[7], eps) || !residual_from(a + 2, device, o) || !like_x(a[0], device, o.x, dr) ||
+      !like_x(a[1], device, o.x, dy))
+    return none();
+  at::Tensor dx, db, dg, dc, df;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    const Blocks &x = o.x, &b = o.branch;
+    int64_t bytes = 0;
+    st = flk_residual_norm_backward_plan(x.batch, x.length, x.width, 0, &bytes);
+    if (st == FLK_OK) {
+      const at::Tensor ws = empty({bytes}, at::kByte, device);
+      dx = empty(x.t->sizes(), x.t->scalar_type(), device);
+      db = empty(x.t->sizes(), x.t->scalar_type(), device);
+      dg = empty(o.gate->sizes(), o.p.dtype, device);
+      dc = empty(o.p.offset->sizes(), o.p.dtype, device);
+      df = empty(o.p.factor->sizes(), o.p.dtype, device);
+      const int64_t entry = (int64_t)x.length * x.width;
+      st = flk_residual_norm_backward(
+          dr.t->data_ptr(), dr.batch_stride, dr.row_stride, dy.t->data_ptr(), dy.batch_stride, dy.row_stride,
+          x.t->data_ptr(), x.batch_stride, x.row_stride, b.t->data_ptr(), b.batch_stride, b.row_stride,
+          code_of(x.t->scalar_type()), o.gate->data_ptr(), o.p.factor->data_ptr(), code_of(o.p.dtype), x.width, 1, eps,
+          x.batch, x.length, x.width, dx.data_ptr(), entry, x.width, db.data_ptr(), entry, x.width, dg.data_ptr(),
+          df.data_ptr(), dc.data_ptr(), ws.data_ptr(), bytes, stream_of(device));
+    }
+  }
+  return st == FLK_OK ? tuple_of({dx, db, dg, dc, df}) : failed(st, "flk_residual_norm_backward");
+  END_HANDLE_TH_ERRORS
+}
+
 // layer_norm(x, weight, bias, eps), modulate(x, shift, scale, eps)
 PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -596,11 +678,188 @@ PyObject* gated_mlp_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A (B, H, L, 128) tensor whose rows are 16-byte aligned, with the strides that the library takes (0 along an axis of one).
+struct Heads {
+  const at::Tensor* t;
+  int64_t strides[3];
+};
+
+bool heads_from(PyObject* o, int device, Heads& h) {
+  h.t = gpu_tensor(o, device);
+  if (!h.t || h.t->dim() != 4 || h.t->size(3) != kDim || h.t->stride(3) != 1 || h.t->numel() == 0 || !aligned16(*h.t))
+    return false;
+  for (int i = 0; i < 3; ++i) {
+    h.strides[i] = h.t->size(i) > 1 ? h.t->stride(i) : 0;
+    if (h.strides[i] % 8 || h.t->size(i) > INT32_MAX) return false;
+  }
+  return true;
+}
+
+// qk_prep_backward(dq, dk, dv, qkv, q_scale, k_scale, cos, sin, q_gain, heads, offset) -> (dqkv, dq_scale, dk_scale) or None
+PyObject* qk_prep_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const int device = n == 11 ? device_of(a[3]) : -1;
+  int64_t heads;
+  float gain;
+  Stream s;
+  if (device < 0 || !heads_of(a[9], heads) || !gain_of(a[8], gain) || !stream_from(a[3], a[4], a[5], heads, device, s))
+    return none();
+  const at::Tensor* cos = dense(a[6], device, at::kFloat, {s.length, kDim});
+  const at::Tensor* sin = dense(a[7], device, at::kFloat, {s.length, kDim});
+  const int64_t offset = PyLong_Check(a[10]) ? PyLong_AsLongLong(a[10]) : -1;
+  if (PyErr_Occurred()) PyErr_Clear();
+  Heads g[3];
+  for (int i = 0; i < 3; ++i)
+    if (!heads_from(a[i], device, g[i]) || g[i].t->scalar_type() != at::kBFloat16 || g[i].t->size(0) != s.batch ||
+        g[i].t->size(1) != heads || g[i].t->sizes() != g[0].t->sizes())
+      return none();
+  if (!cos || !sin || offset < 0 || offset > g[0].t->size(2) - s.length) return none();
+  at::Tensor out, dq_scale, dk_scale;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    int64_t bytes = 0;
+    st = flk_qk_prep_backward_plan((int)s.batch, (int)s.length, (int)heads, &bytes);
+    if (st == FLK_OK) {
+      const at::Tensor ws = empty({bytes}, at::kByte, device);
+      out = empty(s.qkv->sizes(), at::kBFloat16, device);
+      dq_scale = empty(s.q_scale->sizes(), s.q_scale->scalar_type(), device);
+      dk_scale = empty(s.k_scale->sizes(), s.k_scale->scalar_type(), device);
+      const int64_t width = 3 * heads * kDim;
+      const void* at[3];
+      for (int i = 0; i < 3; ++i) at[i] = static_cast<const uint16_t*>(g[i].t->data_ptr()) + offset * g[i].strides[2];
+      st = flk_qk_prep_backward(at[0], g[0].strides, at[1], g[1].strides, at[2], g[2].strides, s.qkv->data_ptr(),
+                                s.qkv->stride(0), s.qkv->stride(1), cos->data_ptr<float>(), sin->data_ptr<float>(), kDim,
+                                s.q_scale->data_ptr(), s.k_scale->data_ptr(), s.q_scale->scalar_type() == at::kFloat, gain,
+                                (int)s.batch, (int)s.length, (int)heads, (int)kDim, out.data_ptr(), s.length * width, width,
+                                dq_scale.data_ptr(), dk_scale.data_ptr(), ws.data_ptr(), bytes, stream_of(device));
+    }
+  }
+  return st == FLK_OK ? tuple_of({out, dq_scale, dk_scale}) : failed(st, "flk_qk_prep_backward");
+  END_HANDLE_TH_ERRORS
+}
+
+// The operands of attention: q, k, v of one 16-bit type, and the mask over the keys or none.
+struct Attention {
+  Heads q, k, v;
+  const uint8_t* mask;
+  int64_t mask_stride;
+  int dtype, batch, heads, kv_heads, queries, keys;
+  int64_t merged() const { return (int64_t)heads * kDim; }
+};
+
+bool attention_from(PyObject* const* a, PyObject* mask, int device, Attention& o) {
+  if (!heads_from(a[0], device, o.q) || !heads_from(a[1], device, o.k) || !heads_from(a[2], device, o.v)) return false;
+  const at::ScalarType dt = o.q.t->scalar_type();
+  if ((dt != at::kBFloat16 && dt != at::kHalf) || o.k.t->scalar_type() != dt || o.v.t->scalar_type() != dt ||
+      o.k.t->sizes() != o.v.t->sizes() || o.k.t->size(0) != o.q.t->size(0) || o.q.t->size(1) % o.k.t->size(1))
+    return false;
+  o.dtype = code_of(dt);
+  o.batch = (int)o.q.t->size(0);
+  o.heads = (int)o.q.t->size(1);
+  o.kv_heads = (int)o.k.t->size(1);
+  o.queries = (int)o.q.t->size(2);
+  o.keys = (int)o.k.t->size(2);
+  o.mask = nullptr;
+  o.mask_stride = 0;
+  if (mask == Py_None) return true;
+  const at::Tensor* m = gpu_tensor(mask, device);
+  if (!m || m->scalar_type() != at::kBool || m->dim() != 2 || m->size(0) != o.batch || m->size(1) != o.keys ||
+      (o.keys > 1 && m->stride(1) != 1))
+    return false;
+  o.mask = static_cast<const uint8_t*>(m->data_ptr());
+  o.mask_stride = m->stride(0);
+  return true;
+}
+
+// Workspace of a call; undefined where it needs none.
+int attention_workspace(const Attention& o, bool backward, int device, at::Tensor& ws, int64_t& bytes) {
+  bytes = 0;
+  const int st = flk_attention_plan(o.batch, o.heads, o.kv_heads, o.queries, o.keys, o.mask != nullptr, backward, &bytes);
+  if (st == FLK_OK && bytes) ws = empty({bytes}, at::kByte, device);
+  return st;
+}
+
+// attention(q, k, v, key_mask, keep) -> (o, low, lse), low and lse None without keep; or None
+PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const int device = n == 5 && PyBool_Check(a[4]) ? device_of(a[0]) : -1;
+  Attention o;
+  if (device < 0 || !attention_from(a, a[3], device, o)) return none();
+  at::Tensor out, low, lse;
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    const at::ScalarType dt = o.q.t->scalar_type();
+    at::Tensor ws;
+    int64_t bytes;
+    st = attention_workspace(o, false, device, ws, bytes);
+    if (st == FLK_OK) {
+      const int64_t strides[3] = {o.queries * o.merged(), kDim, o.merged()};
+      out = empty({o.batch, o.queries, o.merged()}, dt, device);
+      if (a[4] == Py_True) {
+        low = empty({o.batch, o.queries, o.merged()}, dt, device);
+        lse = empty({o.batch, o.heads, o.queries}, at::kFloat, device);
+      }
+      st = flk_attention(o.q.t->data_ptr(), o.q.strides, o.k.t->data_ptr(), o.k.strides, o.v.t->data_ptr(), o.v.strides,
+                         o.dtype, o.mask, o.mask_stride, o.batch, o.heads, o.kv_heads, o.queries, o.keys, (int)kDim,
+                         out.data_ptr(), strides, ptr(low), static_cast<float*>(ptr(lse)), ptr(ws), bytes,
+                         stream_of(device));
+    }
+  }
+  return st == FLK_OK ? tuple_of({out, low, lse}) : failed(st, "flk_attention");
+  END_HANDLE_TH_ERRORS
+}
+
+// attention_backward(do, q, k, v, o, low, lse, key_mask) -> (dq, dk, dv) or None
+PyObject* attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const int device = n == 8 ? device_of(a[1]) : -1;
+  Attention o;
+  if (device < 0 || !attention_from(a + 1, a[7], device, o)) return none();
+  const at::ScalarType dt = o.q.t->scalar_type();
+  const int64_t shape[3] = {o.batch, o.queries, o.merged()};
+  const at::Tensor* d_o = dense(a[0], device, dt, shape);
+  const at::Tensor* out = dense(a[4], device, dt, shape);
+  const at::Tensor* low = dense(a[5], device, dt, shape);
+  const at::Tensor* lse = dense(a[6], device, at::kFloat, {o.batch, o.heads, o.queries});
+  if (!d_o || !out || !low || !lse) return none();
+  at::Tensor grads[3];
+  int st;
+  {
+    pybind11::gil_scoped_release release;
+    at::Tensor ws;
+    int64_t bytes;
+    st = attention_workspace(o, true, device, ws, bytes);
+    if (st == FLK_OK) {
+      const int64_t merged[3] = {o.queries * o.merged(), kDim, o.merged()};
+      int64_t strides[3][3];
+      const Heads* of[3] = {&o.q, &o.k, &o.v};
+      for (int i = 0; i < 3; ++i) {
+        const at::Tensor& t = *of[i]->t;
+        grads[i] = empty(t.sizes(), dt, device);
+        strides[i][2] = kDim;
+        strides[i][1] = kDim * t.size(2);
+        strides[i][0] = strides[i][1] * t.size(1);
+      }
+      st = flk_attention_backward(
+          d_o->data_ptr(), merged, o.q.t->data_ptr(), o.q.strides, o.k.t->data_ptr(), o.k.strides, o.v.t->data_ptr(),
+          o.v.strides, out->data_ptr(), merged, low->data_ptr(), lse->data_ptr<float>(), o.dtype, o.mask, o.mask_stride,
+          o.batch, o.heads, o.kv_heads, o.queries, o.keys, (int)kDim, grads[0].data_ptr(), strides[0], grads[1].data_ptr(),
+          strides[1], grads[2].data_ptr(), strides[2], ptr(ws), bytes, stream_of(device));
+    }
+  }
+  return st == FLK_OK ? tuple_of({grads[0], grads[1], grads[2]}) : failed(st, "flk_attention_backward");
+  END_HANDLE_TH_ERRORS
+}
+
 #define FLK_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FLK_METHOD(qk_prep), FLK_METHOD(attend_merged), FLK_METHOD(double_attention),
                          FLK_METHOD(linear), FLK_METHOD(layer_norm), FLK_METHOD(layer_norm_backward),
                          FLK_METHOD(modulate), FLK_METHOD(modulate_backward), FLK_METHOD(swiglu),
                          FLK_METHOD(swiglu_backward), FLK_METHOD(gated_mlp), FLK_METHOD(gated_mlp_backward),
+                         FLK_METHOD(residual_modulate), FLK_METHOD(residual_modulate_backward),
+                         FLK_METHOD(qk_prep_backward), FLK_METHOD(attention), FLK_METHOD(attention_backward),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

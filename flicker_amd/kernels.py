@@ -283,6 +283,11 @@ def qk_prep_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, qkv: 
     dk and dv (B, H, L_out, D) bf16 of its outputs, of which it takes the rows from ``offset`` (a stream's place in the joint
     sequence, as ``out_offset``).  Any L; the roundings inside qk_prep pass gradients through.  ``out`` may be a
     (B, L, 3*H*D) bf16 view with 16-byte aligned rows (columns of linear1's gradient) that overlaps no operand."""
+    if out is None and type(freqs) is Freqs:
+        done = _native.qk_prep_backward(dq, dk, dv, qkv, q_scale, k_scale, freqs.cos, freqs.sin, freqs.q_gain, num_heads,
+                                        offset)
+        if done is not None:
+            return done
     _on_gpu("qkv", qkv)
     if qkv.dim() != 3:
         raise ValueError(f"qkv must be (B, L, 3*H*D), got {tuple(qkv.shape)}")

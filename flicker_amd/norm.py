@@ -267,6 +267,9 @@ def residual_modulate(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor,
                       scale: torch.Tensor, *, eps: float = EPS) -> tuple[torch.Tensor, torch.Tensor]:
     """(r, y) with r = x + gate * branch and y = (1 + scale) * layer_norm(r) + shift: x and branch (B, L, width), one row
     of gate, shift and scale per batch entry, (B, width) or (B, 1, width).  y is of the unrounded sum."""
+    done = _native.residual_modulate(x, branch, gate, shift, scale, eps)
+    if done is not None:
+        return done
     gate, shift, scale = _residual(x, branch, gate, shift, scale)
     r, y = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
     if x.numel() == 0:
@@ -283,6 +286,9 @@ def residual_modulate_backward(dr: torch.Tensor, dy: torch.Tensor, x: torch.Tens
                                gate: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *, eps: float = EPS):
     """(dx, dbranch, dgate, dshift, dscale) of ``residual_modulate`` for the incoming gradients dr of r and dy of y, the
     last three shaped as gate, shift and scale."""
+    done = _native.residual_modulate_backward(dr, dy, x, branch, gate, shift, scale, eps)
+    if done is not None:
+        return done
     shapes = gate, shift, scale
     gate, shift, scale = _residual(x, branch, gate, shift, scale)
     _same("dr", dr, x)
