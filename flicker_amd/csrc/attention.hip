@@ -90,7 +90,7 @@ struct Args {
   int batch, heads, kv_heads, group, queries, keys, q_units, k_units;
   // The blocks from `whole` on are cut into `splits` along the units they walk: partial sums of 256 rows, in order, each
   // with its rows' (top, l, sum) in the forward pass, which attention_join_kernel adds up.
-  int whole, splits;
+  int whole, splits, tile;   // tile: queries of a block
   float* part;      // (cut, 256, 128)
   float* part_top;  // (cut, 256, 4)
 };
@@ -132,6 +132,23 @@ struct Piece {
   __device__ __forceinline__ int count(int n) const { return n / splits + (split < n % splits); }
 };
 
+// A wave's queries in a block of A.tile: 256, 32 a wave, or 192, of which the waves 4-7 take 16 each, so that every SIMD holds
+// 48.
+struct Rows {
+  int b, h, first, end, q0;
+  bool wide;
+  __device__ __forceinline__ Rows(const Args& A, const Piece& piece) {
+    const int blocks = (A.queries + A.tile - 1) / A.tile, bh = piece.block / blocks;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    b = bh / A.heads;
+    h = bh - b * A.heads;
+    first = (piece.block - bh * blocks) * A.tile;
+    end = min(A.queries, first + A.tile);
+    wide = A.tile == kQueries || wave < 4;
+    q0 = first + (wide ? wave * 32 : 64 + wave * 16);
+  }
+};
+
 __device__ __forceinline__ int swz(int row) { return ((row & 7) << 1) | ((row >> 3) & 1); }
 
 // LDS holds units of 32 rows of 256 bytes, whose 16-byte chunk c of row r sits in place c ^ swz(r).
@@ -171,8 +188,8 @@ __device__ __forceinline__ vec8<T> col_operand(const uint8_t* unit, const Places
   return __builtin_bit_cast(vec8<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 // P^T or dS^T of group g as the right operand of a product over a unit's rows: the packed words of its two accumulators.
-template <typename T>
-__device__ __forceinline__ vec8<T> packed(const uint32_t (&p)[8], int g) {
+template <typename T, int N>
+__device__ __forceinline__ vec8<T> packed(const uint32_t (&p)[N], int g) {
   return __builtin_bit_cast(vec8<T>, make_uint4(p[4 * g], p[4 * g + 1], p[4 * g + 2], p[4 * g + 3]));
 }
 
@@ -261,12 +278,12 @@ struct Units {
   }
 };
 
-// The wave's two groups of 16 rows from row0 as the right operand: row lane % 16 of group g, d step st; zeros past `end`.
-template <typename T>
-__device__ __forceinline__ void load_rows(vec8<T> (&x)[4][2], const T* src, int64_t stride, int row0, int end) {
+// The wave's G groups of 16 rows from row0 as the right operand: row lane % 16 of group g, d step st; zeros past `end`.
+template <typename T, int G>
+__device__ __forceinline__ void load_rows(vec8<T> (&x)[4][G], const T* src, int64_t stride, int row0, int end) {
   const int lane = threadIdx.x & 63, h = lane >> 4, hperm = ((h & 1) << 1) | (h >> 1);
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
+  for (int g = 0; g < G; ++g) {
     const int r = row0 + g * 16 + (lane & 15);
 #pragma unroll
     for (int st = 0; st < 4; ++st)
@@ -275,12 +292,12 @@ __device__ __forceinline__ void load_rows(vec8<T> (&x)[4][2], const T* src, int6
 }
 
 // acc (d tile, group) of the wave's rows, times scale[g], as rows of 128: 4 d values a store.
-template <typename T>
-__device__ __forceinline__ void store_rows(const f32x4 (&acc)[8][2], const float (&scale)[2], T* dst, int64_t stride,
+template <typename T, int G>
+__device__ __forceinline__ void store_rows(const f32x4 (&acc)[8][G], const float (&scale)[G], T* dst, int64_t stride,
                                            int row0, int end, T* low = nullptr, int64_t low_stride = 0) {
   const int lane = threadIdx.x & 63, h = lane >> 4;
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
+  for (int g = 0; g < G; ++g) {
     const int r = row0 + g * 16 + (lane & 15);
     if (r >= end) continue;
 #pragma unroll
@@ -301,10 +318,11 @@ __device__ __forceinline__ void store_rows(const f32x4 (&acc)[8][2], const float
 }
 
 // The same unscaled as float32 rows of a cut's partial sums, for rows below `end`.
-__device__ __forceinline__ void store_part(const f32x4 (&acc)[8][2], float* dst, int row0, int end) {
+template <int G>
+__device__ __forceinline__ void store_part(const f32x4 (&acc)[8][G], float* dst, int row0, int end) {
   const int lane = threadIdx.x & 63, h = lane >> 4;
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
+  for (int g = 0; g < G; ++g) {
     const int r = row0 + g * 16 + (lane & 15);
     if (r >= end) continue;
 #pragma unroll
@@ -325,29 +343,48 @@ __device__ __forceinline__ void landed() {
 }
 __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
-template <typename T>
+template <typename T, int G>   // of G groups of 16 queries
 struct Forward {
-  vec8<T> x[4][2];         // Q^T
-  f32x4 acc[8][2];         // O^T
+  vec8<T> x[4][G];         // Q^T
+  f32x4 acc[8][G];         // O^T
   vec8<T> ops[2 * kLead];  // operand of slot n in ops[n % (2 kLead)]
-  f32x4 l[2];              // sums of the rounded P (register 0 of lanes 0-15)
+  f32x4 l[G];              // sums of the rounded P (register 0 of lanes 0-15)
   vec8<T> ones;            // row 0 ones, rows 1-15 zeros
-  float sum[2];            // with kKeep: of the unrounded P, this lane's
-  float top[2], base[2];   // the maximum that P is taken against, and -log2(e) times it
+  float sum[G];            // with kKeep: of the unrounded P, this lane's
+  float top[G], base[G];   // the maximum that P is taken against, and -log2(e) times it
   Places at;
 };
 
 constexpr float kSlack = 9.0f;   // P stays below 2^9
 
+// Slot n's share of the 8 G elements that a phase of 16 slots turns into P: one multiplied, the one before it
+// exponentiated, and the two before that packed.
+template <int G, typename Scaled, typename Exp, typename Put>
+__device__ __forceinline__ void elements(int n, Scaled&& scaled, Exp&& exp, Put&& put) {
+  if constexpr (G == 2) {
+    if (n + 2 < 16) scaled(n + 2);
+    if (n + 1 < 16) exp(n + 1);
+    if (n < 16 && n & 1) put(n - 1);
+  } else {
+    const int m = n >> 1;
+    if ((n & 1) == 0) {
+      if (m + 2 < 8) scaled(m + 2);
+      if (m + 1 < 8) exp(m + 1);
+    } else if (m < 8 && m & 1) {
+      put(m - 1);
+    }
+  }
+}
+
 // Phase u: S(u+1) = K(u+1) Q^T and O^T += V(u-1)^T P(u-1)^T on the matrix pipe while the vector units turn S(u) into P(u).
-template <bool kBias, bool kKeep, typename T, typename Hook>
-__device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur)[4], f32x4 (&s_next)[4],
-                                              const uint32_t (&p_prev)[8], uint32_t (&p_cur)[8], const uint8_t* k_unit,
+template <bool kBias, bool kKeep, typename T, int G, typename Hook>
+__device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_cur)[2 * G], f32x4 (&s_next)[2 * G],
+                                              const uint32_t (&p_prev)[4 * G], uint32_t (&p_cur)[4 * G], const uint8_t* k_unit,
                                               const uint8_t* v_unit, const uint8_t* k_after, uint32_t bits_next,
                                               Hook&& hook) {
-  f32x4 sv[4];
+  f32x4 sv[2 * G];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2 * G; ++i) {
     sv[i] = s_cur[i];
     asm volatile("" : "+v"(sv[i]));
   }
@@ -358,7 +395,8 @@ __device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur
       start[1] = bias_of(bits_next, 1);
     }
   }
-  float t[16], e[16], high = -INFINITY, sum[2] = {};
+  constexpr int kElems = 8 * G;   // of a lane: one a slot, every other slot with one group
+  float t[kElems], e[kElems], high = -INFINITY, sum[G] = {};
   auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, w.base[n >> 3]); };
   auto exp = [&](int n) { e[n] = __builtin_amdgcn_exp2f(t[n]); };
   auto put = [&](int n) {
@@ -367,7 +405,9 @@ __device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur
     high = fmaxf(fmaxf(high, t[n]), t[n + 1]);
     if constexpr (kKeep) sum[n >> 3] += e[n] + e[n + 1];
   };
-  const vec8<T> pb[2] = {packed<T>(p_prev, 0), packed<T>(p_prev, 1)};
+  vec8<T> pb[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) pb[g] = packed<T>(p_prev, g);
   scaled(0);
   scaled(1);
   exp(0);
@@ -378,14 +418,14 @@ __device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur
     if (n < 8) {
       const int st = n >> 1, kt = n & 1;
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
+      for (int g = 0; g < G; ++g)
         s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : kBias ? start[kt] : f32x4{});
     } else {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) w.acc[n - 8][g] = mfma(a, pb[g], w.acc[n - 8][g]);
+      for (int g = 0; g < G; ++g) w.acc[n - 8][g] = mfma(a, pb[g], w.acc[n - 8][g]);
       if (n == 15) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g) w.l[g] = mfma(w.ones, pb[g], w.l[g]);
+        for (int g = 0; g < G; ++g) w.l[g] = mfma(w.ones, pb[g], w.l[g]);
       }
     }
     const int m = n + kLead;
@@ -393,9 +433,7 @@ __device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur
     if (m < 8) to = row_operand<T>(k_unit, w.at, m >> 1, m & 1);
     else if (m < 16) to = col_operand<T>(v_unit, w.at, m - 8);
     else to = row_operand<T>(k_after, w.at, (m - 16) >> 1, m & 1);
-    if (n + 2 < 16) scaled(n + 2);
-    if (n + 1 < 16) exp(n + 1);
-    if (n & 1) put(n - 1);
+    elements<G>(n, scaled, exp, put);
     hook(n);
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -403,7 +441,7 @@ __device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur
   // maximum, what has been summed is scaled, and this unit's P are formed again.
   if (__any(high > kSlack)) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < G; ++g) {
       float x = sv[2 * g][0];
 #pragma unroll
       for (int n = 1; n < 8; ++n) x = fmaxf(x, sv[2 * g + (n >> 2)][n & 3]);
@@ -426,26 +464,23 @@ __device__ __forceinline__ void forward_phase(Forward<T>& w, const f32x4 (&s_cur
     }
   }
   if constexpr (kKeep) {
-    w.sum[0] += sum[0];
-    w.sum[1] += sum[1];
+#pragma unroll
+    for (int g = 0; g < G; ++g) w.sum[g] += sum[g];
   }
 }
 
 constexpr int kKRing = 4, kVRing = 4;   // forward: units of K and of V in LDS
 
-template <typename T, bool kMasked, bool kKeep>
-__global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[(kKRing + kVRing) * kUnitBytes];
-  const int lane = threadIdx.x & 63, h4 = lane >> 4;
-  const int blocks = (A.queries + kQueries - 1) / kQueries;
-  const Piece piece(A);
-  const int block = piece.block, bh = block / blocks, b = bh / A.heads, h = bh - b * A.heads;
-  const int first = (block - bh * blocks) * kQueries, q0 = first + (threadIdx.x >> 6) * 32;
+// One wave's 16 G queries from q0, of a block's `first` .. `end` - 1.
+template <typename T, bool kMasked, bool kKeep, int G>
+__device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const Piece& piece, int b, int h, int first, int end,
+                                             int q0) {
+  const int lane = threadIdx.x & 63, h4 = lane >> 4, bh = b * A.heads + h;
   Units<kMasked> units(A, b, piece);
   const int n = units.n;
-  Forward<T> w;
+  Forward<T, G> w;
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
+  for (int g = 0; g < G; ++g) {
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
     w.l[g] = f32x4{};
@@ -467,32 +502,32 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
       units.get(i, unit[i], bits[i]);
       kc.start<false>(k_lds(i), unit[i]);
     }
-    vc.start<false>(v_lds(0), unit[0]);
-    load_rows<T>(w.x, A.q.at<T>(b, h), A.q.row, q0, A.queries);
+    for (int i = 0; i < 2; ++i) vc.start<false>(v_lds(i), unit[i]);
+    load_rows<T>(w.x, A.q.at<T>(b, h), A.q.row, q0, end);
     w.at = places();
     const T one = (T)((lane & 15) == 0 ? 1.0f : 0.0f);
     w.ones = vec8<T>{one, one, one, one, one, one, one, one};
     reinterpret_cast<uint4*>(v_slot(-1))[threadIdx.x] = make_uint4(0, 0, 0, 0);   // V(-1), times P(-1) = 0
     landed<0>();
     for (int i = 0; i < 4; ++i) clear_rows(k_slot(i), bits[i]);
-    clear_rows(v_slot(0), bits[0]);
+    for (int i = 0; i < 2; ++i) clear_rows(v_slot(i), bits[i]);
     __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(q0) >= A.queries) {   // no queries: this wave's share of the copies
+    if (__builtin_amdgcn_readfirstlane(q0) >= end) {   // no queries: this wave's share of the copies
       __syncthreads();
       const int turns = n > 8 ? (n - 5) / 4 * 4 : 0, all = turns + (n - turns + 2) / 2 * 2;   // as the loops below
       for (int u = 0; u < all; ++u) {
         units.look(u, unit, bits);
         kc.start<false>(k_lds(u), unit[4]);
-        vc.start<false>(v_lds(u + 1), unit[1]);
+        vc.start<false>(v_lds(u + 2), unit[2]);
         landed<2>();
         clear_rows(k_slot(u + 3), bits[3]);
-        clear_rows(v_slot(u), bits[0]);
+        clear_rows(v_slot(u + 1), bits[1]);
         barrier();
         if constexpr (kMasked) units.shift(unit, bits);
       }
     } else {
-      f32x4 s0[4], s1[4];
-      uint32_t p0[8], p1[8] = {};
+      f32x4 s0[2 * G], s1[2 * G];
+      uint32_t p0[4 * G], p1[4 * G] = {};
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         const f32x4 start = bias_of(bits[0], kt);
@@ -500,26 +535,26 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
         for (int st = 0; st < 4; ++st) {
           const vec8<T> a = row_operand<T>(k_slot(0), w.at, st, kt);
 #pragma unroll
-          for (int g = 0; g < 2; ++g) s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : start);
+          for (int g = 0; g < G; ++g) s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : start);
         }
       }
 #pragma unroll
       for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
       __syncthreads();   // K(0) has been read: iteration 0 copies K(4) over it
       // r: u's place in the rings; a literal in the unrolled loop, where LDS addresses are then a lane's constants
-      auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[4], f32x4(&s_next)[4], const uint32_t(&p_prev)[8],
-                           uint32_t(&p_cur)[8]) __attribute__((always_inline)) {
+      auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[2 * G], f32x4(&s_next)[2 * G], const uint32_t(&p_prev)[4 * G],
+                           uint32_t(&p_cur)[4 * G]) __attribute__((always_inline)) {
         constexpr bool kBias = decltype(bias)::value, kAhead = !kMasked && !kBias;
         if constexpr (!kAhead) units.look(u, unit, bits);
         forward_phase<kBias, kKeep>(w, s_cur, s_next, p_prev, p_cur, k_slot(r + 1), v_slot(r - 1), k_slot(r + 2), bits[1],
                                     [&](int slot) {
                                       if (slot == 1) kc.start<kAhead>(k_lds(r), kAhead ? units.first + u + 4 : unit[4]);
-                                      if (slot == 3) vc.start<kAhead>(v_lds(r + 1), kAhead ? units.first + u + 1 : unit[1]);
+                                      if (slot == 3) vc.start<kAhead>(v_lds(r + 2), kAhead ? units.first + u + 2 : unit[2]);
                                     });
         landed<2>();
         if constexpr (kBias) {
           clear_rows(k_slot(r + 3), bits[3]);
-          clear_rows(v_slot(r), bits[0]);
+          clear_rows(v_slot(r + 1), bits[1]);
         }
         barrier();
         if constexpr (kMasked) units.shift(unit, bits);
@@ -541,52 +576,63 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy writes LDS that the block has left
   }
   if (piece.cut >= 0) {
-    const int end = min(A.queries - first, kQueries);
-    store_part(w.acc, A.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end);
+    store_part(w.acc, A.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < G; ++g) {
       const int r = q0 - first + g * 16 + (lane & 15);
       const f32x4 x = {w.top[g], __shfl(w.l[g][0], lane & 15), across(w.sum[g]), 0.0f};
-      if (h4 == 0 && r < end) reinterpret_cast<f32x4*>(A.part_top)[(int64_t)piece.cut * kQueries + r] = x;
+      if (h4 == 0 && r < end - first) reinterpret_cast<f32x4*>(A.part_top)[(int64_t)piece.cut * kQueries + r] = x;
     }
     return;
   }
-  float scale[2];
+  float scale[G];
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
+  for (int g = 0; g < G; ++g) {
     const float l = __shfl(w.l[g][0], lane & 15);
     scale[g] = l > 0.0f ? 1.0f / l : 0.0f;
     if constexpr (kKeep) {
       const float sum = across(w.sum[g]);
       const int r = q0 + g * 16 + (lane & 15);
-      if (h4 == 0 && r < A.queries)
+      if (h4 == 0 && r < end)
         A.lse[(int64_t)bh * A.queries + r] = l > 0.0f ? w.top[g] + __builtin_amdgcn_logf(sum) * kLn2 : -INFINITY;
     }
   }
   T* low = kKeep ? static_cast<T*>(A.low) : nullptr;
   if (low) low += ((int64_t)b * A.queries * A.heads + h) * kD;
-  store_rows<T>(w.acc, scale, A.o.at<T>(b, h), A.o.row, q0, A.queries, low, (int64_t)A.heads * kD);
+  store_rows<T>(w.acc, scale, A.o.at<T>(b, h), A.o.row, q0, end, low, (int64_t)A.heads * kD);
+}
+
+template <typename T, bool kMasked, bool kKeep>
+__global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[(kKRing + kVRing) * kUnitBytes];
+  const Piece piece(A);
+  const Rows rows(A, piece);
+  if (rows.wide)
+    forward_wave<T, kMasked, kKeep, 2>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
+  else
+    forward_wave<T, kMasked, kKeep, 1>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
 }
 
 // dq, and the stats that attention_dkv_kernel reads.
-template <typename T>
+template <typename T, int G>
 struct Dq {
-  vec8<T> x[4][2], g[4][2];   // Q^T, dO^T
-  f32x4 acc[8][2];            // dQ^T
+  vec8<T> x[4][G], g[4][G];   // Q^T, dO^T
+  f32x4 acc[8][G];            // dQ^T
   vec8<T> ops[2 * kLead];
-  float lse[2], delta[2];     // -log2(e) lse, -delta
+  float lse[G], delta[G];     // -log2(e) lse, -delta
   Places at;
 };
 
 // Phase u: S(u+1) = K(u+1) Q^T, dP(u+1) = V(u+1) dO^T and dQ^T += K(u-1)^T dS(u-1)^T, while dS(u) is formed.
-template <bool kBias, typename T, typename Hook>
-__device__ __forceinline__ void dq_phase(Dq<T>& w, const f32x4 (&s_cur)[4], const f32x4 (&d_cur)[4], f32x4 (&s_next)[4],
-                                         f32x4 (&d_next)[4], const uint32_t (&p_prev)[8], uint32_t (&p_cur)[8],
-                                         const uint8_t* k_unit, const uint8_t* v_unit, const uint8_t* k_before,
-                                         const uint8_t* k_after, uint32_t bits_next, Hook&& hook) {
-  f32x4 sv[4], dv[4];
+template <bool kBias, typename T, int G, typename Hook>
+__device__ __forceinline__ void dq_phase(Dq<T, G>& w, const f32x4 (&s_cur)[2 * G], const f32x4 (&d_cur)[2 * G],
+                                         f32x4 (&s_next)[2 * G], f32x4 (&d_next)[2 * G], const uint32_t (&p_prev)[4 * G],
+                                         uint32_t (&p_cur)[4 * G], const uint8_t* k_unit, const uint8_t* v_unit,
+                                         const uint8_t* k_before, const uint8_t* k_after, uint32_t bits_next,
+                                         Hook&& hook) {
+  f32x4 sv[2 * G], dv[2 * G];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2 * G; ++i) {
     sv[i] = s_cur[i];
     dv[i] = d_cur[i];
     asm volatile("" : "+v"(sv[i]), "+v"(dv[i]));
@@ -598,7 +644,7 @@ __device__ __forceinline__ void dq_phase(Dq<T>& w, const f32x4 (&s_cur)[4], cons
       start[1] = bias_of(bits_next, 1);
     }
   }
-  float t[16], e[16];
+  float t[8 * G], e[8 * G];
   auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, w.lse[n >> 3]); };
   auto exp = [&](int n) { e[n] = __builtin_amdgcn_exp2f(t[n]); };
   auto put = [&](int n) {
@@ -606,7 +652,9 @@ __device__ __forceinline__ void dq_phase(Dq<T>& w, const f32x4 (&s_cur)[4], cons
     p_cur[n >> 1] = pack<T>(x, y);
     asm volatile("" : "+v"(p_cur[n >> 1]));
   };
-  const vec8<T> pb[2] = {packed<T>(p_prev, 0), packed<T>(p_prev, 1)};
+  vec8<T> pb[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) pb[g] = packed<T>(p_prev, g);
   scaled(0);
   scaled(1);
   exp(0);
@@ -616,7 +664,7 @@ __device__ __forceinline__ void dq_phase(Dq<T>& w, const f32x4 (&s_cur)[4], cons
     const vec8<T>& a = w.ops[n % (2 * kLead)];
     const int st = (n & 7) >> 1, kt = n & 1;
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < G; ++g) {
       if (n < 8) s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : kBias ? start[kt] : f32x4{});
       else if (n < 16) d_next[2 * g + kt] = mfma(a, w.g[st][g], st ? d_next[2 * g + kt] : f32x4{});
       else w.acc[n - 16][g] = mfma(a, pb[g], w.acc[n - 16][g]);
@@ -627,9 +675,7 @@ __device__ __forceinline__ void dq_phase(Dq<T>& w, const f32x4 (&s_cur)[4], cons
     else if (m < 16) to = row_operand<T>(v_unit, w.at, (m - 8) >> 1, m & 1);
     else if (m < 24) to = col_operand<T>(k_before, w.at, m - 16);
     else to = row_operand<T>(k_after, w.at, (m - 24) >> 1, m & 1);
-    if (n + 2 < 16) scaled(n + 2);
-    if (n + 1 < 16) exp(n + 1);
-    if (n < 16 && n & 1) put(n - 1);
+    elements<G>(n, scaled, exp, put);
     hook(n);
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -637,27 +683,23 @@ __device__ __forceinline__ void dq_phase(Dq<T>& w, const f32x4 (&s_cur)[4], cons
 
 constexpr int kDqKRing = 6, kDqVRing = 3;
 
-template <typename T, bool kMasked>
-__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[(kDqKRing + kDqVRing) * kUnitBytes];
-  const int lane = threadIdx.x & 63, h4 = lane >> 4;
-  const int blocks = (A.queries + kQueries - 1) / kQueries;
-  const Piece piece(A);
-  const int block = piece.block, bh = block / blocks, b = bh / A.heads, h = bh - b * A.heads;
-  const int first = (block - bh * blocks) * kQueries, q0 = first + (threadIdx.x >> 6) * 32;
+template <typename T, bool kMasked, int G>
+__device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piece& piece, int b, int h, int first, int end,
+                                        int q0) {
+  const int lane = threadIdx.x & 63, h4 = lane >> 4, bh = b * A.heads + h;
   Units<kMasked> units(A, b, piece);
   const int n = units.n;
-  Dq<T> w;
-  load_rows<T>(w.g, A.dO.at<T>(b, h), A.dO.row, q0, A.queries);
+  Dq<T, G> w;
+  load_rows<T>(w.g, A.dO.at<T>(b, h), A.dO.row, q0, end);
   {
-    vec8<T> o[4][2], low[4][2];
-    load_rows<T>(o, A.o.at<T>(b, h), A.o.row, q0, A.queries);
+    vec8<T> o[4][G], low[4][G];
+    load_rows<T>(o, A.o.at<T>(b, h), A.o.row, q0, end);
     load_rows<T>(low, static_cast<const T*>(A.low) + ((int64_t)b * A.queries * A.heads + h) * kD, (int64_t)A.heads * kD, q0,
-                 A.queries);
+                 end);
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < G; ++g) {
       const int r = q0 + g * 16 + (lane & 15);
-      const float x = r < A.queries ? A.lse[(int64_t)bh * A.queries + r] : -INFINITY;
+      const float x = r < end ? A.lse[(int64_t)bh * A.queries + r] : -INFINITY;
       float sum = 0.0f;
 #pragma unroll
       for (int st = 0; st < 4; ++st)
@@ -676,7 +718,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
       A.stats[(int64_t)A.batch * A.heads * A.q_units * 2 * kUnit + threadIdx.x] = threadIdx.x < kUnit ? INFINITY : 0.0f;
   }
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
+  for (int g = 0; g < G; ++g)
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
   if (n) {
@@ -695,7 +737,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
       kc.start<false>(k_lds(i), unit[i]);
       if (i < 3) vc.start<false>(v_lds(i), unit[i]);
     }
-    load_rows<T>(w.x, A.q.at<T>(b, h), A.q.row, q0, A.queries);
+    load_rows<T>(w.x, A.q.at<T>(b, h), A.q.row, q0, end);
     w.at = places();
     reinterpret_cast<uint4*>(k_slot(kDqKRing - 1))[threadIdx.x] = make_uint4(0, 0, 0, 0);   // K(-1), times dS(-1) = 0
     landed<0>();
@@ -704,8 +746,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
       if (i < 3) clear_rows(v_slot(i), bits[i]);
     }
     __syncthreads();
-    f32x4 s0[4], s1[4], d0[4], d1[4];
-    uint32_t p0[8], p1[8] = {};
+    f32x4 s0[2 * G], s1[2 * G], d0[2 * G], d1[2 * G];
+    uint32_t p0[4 * G], p1[4 * G] = {};
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       const f32x4 start = bias_of(bits[0], kt);
@@ -713,7 +755,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
       for (int st = 0; st < 4; ++st) {
         const vec8<T> a = row_operand<T>(k_slot(0), w.at, st, kt), c = row_operand<T>(v_slot(0), w.at, st, kt);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < G; ++g) {
           s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : start);
           d0[2 * g + kt] = mfma(c, w.g[st][g], st ? d0[2 * g + kt] : f32x4{});
         }
@@ -723,8 +765,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
     for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
     __syncthreads();   // V(0) has been read: iteration 0 copies V(3) over it
     // r: u's place in K's ring
-    auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[4], const f32x4(&d_cur)[4], f32x4(&s_next)[4],
-                         f32x4(&d_next)[4], const uint32_t(&p_prev)[8], uint32_t(&p_cur)[8]) __attribute__((always_inline)) {
+    auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[2 * G], const f32x4(&d_cur)[2 * G],
+                         f32x4(&s_next)[2 * G],
+                         f32x4(&d_next)[2 * G], const uint32_t(&p_prev)[4 * G], uint32_t(&p_cur)[4 * G]) __attribute__((always_inline)) {
       constexpr bool kBias = decltype(bias)::value, kAhead = !kMasked && !kBias;
       if constexpr (!kAhead) units.look(u, unit, bits);
       dq_phase<kBias>(w, s_cur, d_cur, s_next, d_next, p_prev, p_cur, k_slot(r + 1), v_slot(r + 1), k_slot(r + 5),
@@ -757,11 +800,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   if (piece.cut >= 0) {
-    store_part(w.acc, A.part + (int64_t)piece.cut * kQueries * kD, q0 - first, min(A.queries - first, kQueries));
+    store_part(w.acc, A.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
     return;
   }
-  const float one[2] = {1.0f, 1.0f};
-  store_rows<T>(w.acc, one, A.dq.at<T>(b, h), A.dq.row, q0, A.queries);
+  float one[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) one[g] = 1.0f;
+  store_rows<T>(w.acc, one, A.dq.at<T>(b, h), A.dq.row, q0, end);
+}
+
+template <typename T, bool kMasked>
+__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[(kDqKRing + kDqVRing) * kUnitBytes];
+  const Piece piece(A);
+  const Rows rows(A, piece);
+  if (rows.wide) dq_wave<T, kMasked, 2>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
+  else dq_wave<T, kMasked, 1>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
 }
 
 // dk and dv of 128 keys, 32 a pair of waves: the first holds K^T and dV^T, forms S and P and hands P on through LDS, the second holds
@@ -1021,23 +1075,40 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A) {
   const int lane = threadIdx.x & 31;
   const int cut_block = blockIdx.x / (kQueries / 8), r = blockIdx.x % (kQueries / 8) * 8 + (threadIdx.x >> 5);
   const int block = A.whole + cut_block, rows = kOf == kJoinDkv ? A.keys : A.queries;
-  const int per = kOf == kJoinDkv ? kKeys : kQueries, heads = kOf == kJoinDkv ? A.kv_heads : A.heads;
+  const int per = kOf == kJoinDkv ? kKeys : A.tile, heads = kOf == kJoinDkv ? A.kv_heads : A.heads;
   const int blocks = (rows + per - 1) / per, bh = block / blocks, b = bh / heads, h = bh - b * heads;
   const int row = (block - bh * blocks) * per + (kOf == kJoinDkv ? r % kKeys : r);
-  if (row >= rows) return;
+  if (row >= rows || (kOf != kJoinDkv && r >= per)) return;
   const int64_t first = ((int64_t)cut_block * A.splits * kQueries + r) * kD;
   f32x4 x{};
   if constexpr (kOf == kJoinO) {
+    // lane i of the row's 32 holds the factors of the cuts i and i + 32
     const f32x4* tops = reinterpret_cast<const f32x4*>(A.part_top) + (int64_t)cut_block * A.splits * kQueries + r;
-    float top = -1e30f, l = 0.0f, sum = 0.0f;
-    for (int i = 0; i < A.splits; ++i) top = fmaxf(top, tops[i * kQueries][0]);
-    for (int i = 0; i < A.splits; ++i) {
-      const f32x4 t = tops[i * kQueries];
-      const float f = __builtin_amdgcn_exp2f((t[0] - top) * kLog2e);
-      x += *reinterpret_cast<const f32x4*>(A.part + first + (int64_t)i * kQueries * kD + lane * 4) * f;
-      l += t[1] * f;
-      sum += t[2] * f;
+    f32x4 t[2];
+    float top = -1e30f, l = 0.0f, sum = 0.0f, f[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = lane + 32 * i;
+      t[i] = at < A.splits ? tops[(int64_t)at * kQueries] : f32x4{-1e30f, 0.0f, 0.0f, 0.0f};
+      top = fmaxf(top, t[i][0]);
     }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 32));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f[i] = __builtin_amdgcn_exp2f((t[i][0] - top) * kLog2e);
+      l += t[i][1] * f[i];
+      sum += t[i][2] * f[i];
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      l += __shfl_xor(l, d, 32);
+      sum += __shfl_xor(sum, d, 32);
+    }
+    const float* at = A.part + first + lane * 4;
+#pragma unroll 8
+    for (int i = 0; i < A.splits; ++i)
+      x += *reinterpret_cast<const f32x4*>(at + (int64_t)i * kQueries * kD) * __shfl(i < 32 ? f[0] : f[1], i & 31, 32);
     x *= l > 0.0f ? 1.0f / l : 0.0f;
     if constexpr (kKeep) {
       if (lane == 0) A.lse[(int64_t)bh * A.queries + row] = l > 0.0f ? top + __builtin_amdgcn_logf(sum) * kLn2 : -INFINITY;
@@ -1113,49 +1184,51 @@ int plan_mask(const void* mask, int64_t batch_stride, Args& A, uint8_t* workspac
   return flk_launch_status();
 }
 
-// How a launch of `blocks` equal blocks, each walking n units, is cut: whole rounds of the 256 CUs, and what is left in
+// How a launch of equal blocks of `tile` rows, each walking n units, is cut: whole rounds of the 256 CUs, and what is left in
 // pieces, where that is estimated to be faster.
 struct Cut {
-  int whole, splits;
+  int whole, splits, tile;
   int64_t blocks;
+  double time;
   int64_t grid() const { return whole + (blocks - whole) * splits; }
   int64_t cuts() const { return splits > 1 ? (blocks - whole) * splits : 0; }
   int64_t bytes() const { return cuts() * kQueries * (kD + 4) * 4; }
 };
 constexpr int kCUs = 256, kMaxSplits = 64;
-// us of a unit, and of a block's first loads and last stores, and of the join's launch and its bytes
-Cut plan_cut(int64_t blocks, int64_t n, double unit, int rows) {
+// us of a unit, of a block's first loads and last stores, of the join's launch, and bytes of partial sums written and read a us
+Cut plan_cut(int64_t blocks, int64_t n, double unit, int rows, int tile) {
   constexpr double kFixed = 6.0, kJoin = 5.0, kBytes = 4e6;
   auto rounds = [&](int64_t grid) { return (double)((grid + kCUs - 1) / kCUs); };
-  Cut best{(int)blocks, 1, blocks};
-  double least = rounds(blocks) * (n * unit + kFixed);
+  Cut best{(int)blocks, 1, tile, blocks, rounds(blocks) * (n * unit + kFixed)};
   const int64_t whole = blocks / kCUs * kCUs, rest = blocks - whole;
   if (rest == 0 || blocks > 16 * kCUs) return best;
   for (int s = 2; s <= kMaxSplits && 4 * s <= n; ++s) {
     const double time = rounds(whole) * (n * unit + kFixed) + rounds(rest * s) * ((n + s - 1) / s * unit + kFixed) + kJoin +
                         rest * s * (double)rows * kD * 8 / kBytes;
-    if (time < least) {
-      least = time;
-      best = Cut{(int)whole, s, blocks};
-    }
+    if (time < best.time) best = Cut{(int)whole, s, tile, blocks, time};
   }
   return best;
 }
-Cut forward_cut(const Args& A) {
-  const int64_t blocks = (int64_t)A.batch * A.heads * ((A.queries + kQueries - 1) / kQueries);
-  return plan_cut(blocks, A.k_units, 0.95, std::min(A.queries, kQueries));
+// Blocks of 192 queries take less of a round each, and more in all.
+Cut plan_queries(const Args& A, double unit, double unit192) {
+  Cut best{};
+  for (const int tile : {kQueries, 192}) {
+    const int64_t blocks = (int64_t)A.batch * A.heads * ((A.queries + tile - 1) / tile);
+    const Cut cut = plan_cut(blocks, A.k_units, tile == 192 ? unit192 : unit, std::min(A.queries, tile), tile);
+    if (tile == kQueries || cut.time < best.time) best = cut;
+  }
+  return best;
 }
-Cut dq_cut(const Args& A) {
-  const int64_t blocks = (int64_t)A.batch * A.heads * ((A.queries + kQueries - 1) / kQueries);
-  return plan_cut(blocks, A.k_units, 1.2, std::min(A.queries, kQueries));
-}
+Cut forward_cut(const Args& A) { return plan_queries(A, 0.95, 0.76); }
+Cut dq_cut(const Args& A) { return plan_queries(A, 1.2, 0.95); }
 Cut dkv_cut(const Args& A) {
   const int64_t blocks = (int64_t)A.batch * A.kv_heads * ((A.keys + kKeys - 1) / kKeys);
-  return plan_cut(blocks, (int64_t)A.q_units * A.group, 0.85, 2 * std::min(A.keys, kKeys));
+  return plan_cut(blocks, (int64_t)A.q_units * A.group, 0.85, 2 * std::min(A.keys, kKeys), kKeys);
 }
 void use_cut(Args& A, const Cut& cut, uint8_t* workspace) {
   A.whole = cut.whole;
   A.splits = cut.splits;
+  A.tile = cut.tile;
   A.part = reinterpret_cast<float*>(workspace);
   A.part_top = A.part + cut.cuts() * kQueries * kD;
 }
