@@ -351,11 +351,16 @@ struct Forward {
   f32x4 l[G];              // sums of the rounded P (register 0 of lanes 0-15)
   vec8<T> ones;            // row 0 ones, rows 1-15 zeros
   float sum[G];            // with kKeep: of the unrounded P, this lane's
-  float top[G], base[G];   // the maximum that P is taken against, and -log2(e) times it
+  float top[G], base[G];   // the maximum that P is taken against, and -log2(e) times it less kShift
   Places at;
 };
 
-constexpr float kSlack = 9.0f;   // P stays below 2^9
+// P is held as exp2(log2(e) (S - top) - kShift<T>), where top is the maximum of an earlier unit's row; it has to rise where
+// a P passes 2.  bfloat16 has float32's range: P 2^-60 leaves 2^61 for S to rise by, and no precision is lost at the
+// bottom.  That P passes 2 is then one bit of its packed form.  float16 has neither: exponents are compared with kSlack.
+template <typename T>
+constexpr float kShift = sizeof(T) == 2 && __is_same(T, __bf16) ? 60.0f : 0.0f;
+constexpr float kSlack = 9.0f;
 
 // Slot n's share of the 8 G elements that a phase of 16 slots turns into P: one multiplied, the one before it
 // exponentiated, and the two before that packed.
@@ -396,13 +401,16 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
     }
   }
   constexpr int kElems = 8 * G;   // of a lane: one a slot, every other slot with one group
+  constexpr bool kBits = kShift<T> != 0.0f;
   float t[kElems], e[kElems], high = -INFINITY, sum[G] = {};
+  uint32_t any = 0;
   auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, w.base[n >> 3]); };
   auto exp = [&](int n) { e[n] = __builtin_amdgcn_exp2f(t[n]); };
   auto put = [&](int n) {
     p_cur[n >> 1] = pack<T>(e[n], e[n + 1]);
     asm volatile("" : "+v"(p_cur[n >> 1]));   // keeps the pack in its slot
-    high = fmaxf(fmaxf(high, t[n]), t[n + 1]);
+    if constexpr (!kBits) high = fmaxf(fmaxf(high, t[n]), t[n + 1]);
+    else if (n & 2) any |= p_cur[n >> 1] | p_cur[(n >> 1) - 1];
     if constexpr (kKeep) sum[n >> 3] += e[n] + e[n + 1];
   };
   vec8<T> pb[G];
@@ -437,9 +445,8 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
     hook(n);
     __builtin_amdgcn_sched_barrier(0);
   }
-  // A row's P are exp(S - top) with the top of an earlier unit, until an exponent passes kSlack: then top rises to the row's
-  // maximum, what has been summed is scaled, and this unit's P are formed again.
-  if (__any(high > kSlack)) {
+  // top rises to the row's maximum, what has been summed is scaled, and this unit's P are formed again
+  if (__any(kBits ? (any & 0x40004000u) != 0 : high > kSlack)) {
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       float x = sv[2 * g][0];
@@ -449,7 +456,7 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
       x = fmaxf(fmaxf(x, __shfl_xor(x, 32)), w.top[g]);
       const float factor = __builtin_amdgcn_exp2f((w.top[g] - x) * kLog2e);
       w.top[g] = x;
-      w.base[g] = x * -kLog2e;
+      w.base[g] = x * -kLog2e - kShift<T>;
       sum[g] = 0.0f;
       w.sum[g] *= factor;
       w.l[g] *= factor;   // row 0 of l sits in the lanes 0-15, whose columns are these queries
@@ -486,7 +493,7 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
     w.l[g] = f32x4{};
     w.sum[g] = 0.0f;
     w.top[g] = -1e30f;
-    w.base[g] = 1e30f * kLog2e;
+    w.base[g] = 1e30f * kLog2e - kShift<T>;
   }
   if (n) {
     auto k_slot = [&](int i) { return smem + (i & (kKRing - 1)) * kUnitBytes; };
@@ -594,7 +601,8 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
       const float sum = across(w.sum[g]);
       const int r = q0 + g * 16 + (lane & 15);
       if (h4 == 0 && r < end)
-        A.lse[(int64_t)bh * A.queries + r] = l > 0.0f ? w.top[g] + __builtin_amdgcn_logf(sum) * kLn2 : -INFINITY;
+        A.lse[(int64_t)bh * A.queries + r] =
+            l > 0.0f ? w.top[g] + (__builtin_amdgcn_logf(sum) + kShift<T>) * kLn2 : -INFINITY;
     }
   }
   T* low = kKeep ? static_cast<T*>(A.low) : nullptr;
@@ -1111,7 +1119,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A) {
       x += *reinterpret_cast<const f32x4*>(at + (int64_t)i * kQueries * kD) * __shfl(i < 32 ? f[0] : f[1], i & 31, 32);
     x *= l > 0.0f ? 1.0f / l : 0.0f;
     if constexpr (kKeep) {
-      if (lane == 0) A.lse[(int64_t)bh * A.queries + row] = l > 0.0f ? top + __builtin_amdgcn_logf(sum) * kLn2 : -INFINITY;
+      if (lane == 0)
+        A.lse[(int64_t)bh * A.queries + row] =
+            l > 0.0f ? top + (__builtin_amdgcn_logf(sum) + kShift<T>) * kLn2 : -INFINITY;
       T* low = static_cast<T*>(A.low);
       if (low) {
         float y[4];
@@ -1209,18 +1219,18 @@ Cut plan_cut(int64_t blocks, int64_t n, double unit, int rows, int tile) {
   }
   return best;
 }
-// Blocks of 192 queries take less of a round each, and more in all.
+// Blocks of 192 queries are considered where they fit one round: there each takes less time than one of 256, while over more
+// rounds the chip's power limit lets go of what they would save.
 Cut plan_queries(const Args& A, double unit, double unit192) {
-  Cut best{};
-  for (const int tile : {kQueries, 192}) {
+  auto plan = [&](int tile, double us) {
     const int64_t blocks = (int64_t)A.batch * A.heads * ((A.queries + tile - 1) / tile);
-    const Cut cut = plan_cut(blocks, A.k_units, tile == 192 ? unit192 : unit, std::min(A.queries, tile), tile);
-    if (tile == kQueries || cut.time < best.time) best = cut;
-  }
-  return best;
+    return plan_cut(blocks, A.k_units, us, std::min(A.queries, tile), tile);
+  };
+  const Cut wide = plan(kQueries, unit), narrow = plan(192, unit192);
+  return narrow.blocks <= kCUs && narrow.time < wide.time ? narrow : wide;
 }
-Cut forward_cut(const Args& A) { return plan_queries(A, 0.95, 0.76); }
-Cut dq_cut(const Args& A) { return plan_queries(A, 1.2, 0.95); }
+Cut forward_cut(const Args& A) { return plan_queries(A, 0.82, 0.69); }
+Cut dq_cut(const Args& A) { return plan_queries(A, 1.1, 0.9); }
 Cut dkv_cut(const Args& A) {
   const int64_t blocks = (int64_t)A.batch * A.kv_heads * ((A.keys + kKeys - 1) / kKeys);
   return plan_cut(blocks, (int64_t)A.q_units * A.group, 0.85, 2 * std::min(A.keys, kKeys), kKeys);
