@@ -32,6 +32,11 @@
 // the caches 25.0), 47.5 with such a reader (42.4); 4608 rows 22.1 (22.4).  The rows read are not (13.3 -> 16.7: the last
 // cache often has them), nor the partial rows, read again at once.
 //
+// The residual form of 16-bit rows reads past the caches and stores through them: r and y are read next, and they stay in
+// the last cache where the two operands would have pushed them out.  4 x 4096 rows 65 us (as the norm alone does it 82;
+// both past the caches 80), gradients of 4608 rows 41 (45; 45).  Rows off 16 bytes share words between lanes, which are
+// then fetched twice: 3 x 1157 x 1111 float32 gradients 34 us, past the caches 40.
+//
 // Measured (bf16, width 3 * 1024, among other passes): forward 4 x 4096 rows in 41.7 us, 4.8 TB/s (a large copy's
 // rate is 5.2), backward 4608 rows in 24.9 us (85 MB of operands, and 13 MB of partial rows written and read); 512
 // rows in 4.1 and 11 us: a launch and three latencies one after the other, the factor's, the offset's and the first
@@ -101,10 +106,10 @@ struct Chunks {
       skip[c] = kNarrow ? 0 : min(first - at[c], 8);
     }
   }
-  template <typename T>
+  template <bool kStream = false, typename T>
   __device__ __forceinline__ flk::Raw8<T> load(const T* row, int c, int width) const {
     if constexpr (kNarrow) return flk::load8(row + at[c], width - at[c]);
-    return flk::load8(row + at[c], 8);
+    return flk::load8<kStream>(row + at[c], 8);
   }
   template <bool kStream, typename T>
   __device__ __forceinline__ void store(T* row, int c, int width, const float (&x)[8]) const {
@@ -177,11 +182,14 @@ struct Walk {
   }
 };
 
-// kOne: a wave takes a row alone, kSlots rows a block; otherwise all of the block's waves take one.  kStream: y and
-// dx leave the caches to others (nontemporal).
-template <typename T, typename P, int kV, bool kOne, bool kNarrow, bool kBackward, bool kStream, bool kResidual>
+// Which accesses leave the caches to others (nontemporal): none, the stores of y and dx, or the loads of all rows.
+enum Access { kCached, kStorePast, kLoadPast };
+
+// kOne: a wave takes a row alone, kSlots rows a block; otherwise all of the block's waves take one.
+template <typename T, typename P, int kV, bool kOne, bool kNarrow, bool kBackward, Access kAccess, bool kResidual>
 __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const NormArgs A) {
   constexpr int kSlots = kOne ? 4 : 1, kSums = kResidual ? 3 : 2;
+  constexpr bool kStream = kAccess == kStorePast, kPast = kAccess == kLoadPast;
   __shared__ Exchange ex;
   __shared__ float sums[kOne && kBackward ? kSums * kV * 8 * 64 : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -236,10 +244,10 @@ __global__ __launch_bounds__(kOne ? 256 : 64 * kMaxWaves) void norm_kernel(const
     const T* pr = kResidual && kBackward ? walk.template row<T>(A, A.dr, r) : nullptr;
 #pragma unroll
     for (int c = 0; c < kV; ++c) {
-      x[d][c] = chunks.load(px, c, width);
-      if constexpr (kResidual) br[d][c] = chunks.load(pb, c, width);
-      if constexpr (kBackward) g[d][c] = chunks.load(pg, c, width);
-      if constexpr (kBackward && kResidual) gr[d][c] = chunks.load(pr, c, width);
+      x[d][c] = chunks.template load<kPast>(px, c, width);
+      if constexpr (kResidual) br[d][c] = chunks.template load<kPast>(pb, c, width);
+      if constexpr (kBackward) g[d][c] = chunks.template load<kPast>(pg, c, width);
+      if constexpr (kBackward && kResidual) gr[d][c] = chunks.template load<kPast>(pr, c, width);
     }
   };
 #pragma unroll
@@ -448,7 +456,7 @@ NormArgs from_group(NormArgs a, int64_t g) {
   return a;
 }
 
-template <typename T, typename P, bool kBackward, bool kStream, bool kResidual>
+template <typename T, typename P, bool kBackward, Access kAccess, bool kResidual>
 int launch(const NormArgs& all, int64_t groups, hipStream_t s) {
   const int threads = threads_of(all.width);
   const int64_t most = kMaxItems / threads / all.blocks_per_group;   // groups of one launch
@@ -456,23 +464,36 @@ int launch(const NormArgs& all, int64_t groups, hipStream_t s) {
     const NormArgs a = from_group<T, P>(all, first);
     const dim3 grid((unsigned)(std::min(most, groups - first) * a.blocks_per_group));
     if (a.width < 8)
-      norm_kernel<T, P, 1, true, true, kBackward, kStream, kResidual><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 1, true, true, kBackward, kAccess, kResidual><<<grid, threads, 0, s>>>(a);
     else if (a.width <= 512)
-      norm_kernel<T, P, 1, true, false, kBackward, kStream, kResidual><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 1, true, false, kBackward, kAccess, kResidual><<<grid, threads, 0, s>>>(a);
     else if (a.width <= 512 * kMaxWaves)
-      norm_kernel<T, P, 1, false, false, kBackward, kStream, kResidual><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 1, false, false, kBackward, kAccess, kResidual><<<grid, threads, 0, s>>>(a);
     else
-      norm_kernel<T, P, 2, false, false, kBackward, kStream, kResidual><<<grid, threads, 0, s>>>(a);
+      norm_kernel<T, P, 2, false, false, kBackward, kAccess, kResidual><<<grid, threads, 0, s>>>(a);
     if (const int st = flk_launch_status()) return st;
   }
   return FLK_OK;
 }
 
+// Whether every chunk of a row is a 16-byte word of its own.
+template <typename T>
+bool rows_aligned(const NormArgs& a) {
+  for (const Rows* r : {&a.x, &a.branch, &a.dy, &a.dr}) {
+    const int64_t bytes = (int64_t)(reinterpret_cast<uintptr_t>(r->p) | r->row_stride * sizeof(T) | r->batch_stride * sizeof(T));
+    if (r->p && bytes % 16) return false;
+  }
+  return a.width % 8 == 0;
+}
+
 template <typename T, typename P, bool kBackward, bool kResidual>
 int dispatch(const NormArgs& a, int64_t groups, hipStream_t s) {
-  if constexpr (sizeof(T) == 4)
-    if (a.group_rows * groups * a.width * 4 > kStreamBytes) return launch<T, P, kBackward, false, kResidual>(a, groups, s);
-  return launch<T, P, kBackward, true, kResidual>(a, groups, s);
+  if constexpr (sizeof(T) == 4) {
+    if (a.group_rows * groups * a.width * 4 > kStreamBytes) return launch<T, P, kBackward, kCached, kResidual>(a, groups, s);
+  } else if constexpr (kResidual) {
+    if (rows_aligned<T>(a)) return launch<T, P, kBackward, kLoadPast, true>(a, groups, s);
+  }
+  return launch<T, P, kBackward, kStorePast, kResidual>(a, groups, s);
 }
 
 template <typename P>
