@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from .kernels import HEAD_DIM, _native, _on_gpu
-from .norm import _CODES
+from .norm import _CODES, _refuse_overlap, _rows_apart
 
 _MAX_ROW = 1 << 25   # elements between two rows
 
@@ -125,6 +125,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: to
                 or out.stride(1) % 8 or out.data_ptr() % 16):
             raise ValueError(f"out must be a {q.dtype} ({batch}, {queries}, {heads * dim}) view with contiguous, "
                              "16-byte aligned rows")
+        if out.numel():
+            if not _rows_apart(out):
+                raise ValueError(f"out needs rows that do not overlap, got strides {out.stride()}")
+            for name, t in (("q", q), ("k", k), ("v", v)):
+                if t.numel():
+                    _refuse_overlap(name, out, t)
     low = torch.empty((batch, queries, heads * dim), dtype=q.dtype, device=q.device) if keep else None
     lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=q.device) if keep else None
     if out.numel():

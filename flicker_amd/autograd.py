@@ -1,10 +1,9 @@
-"""``norm`` and ``mlp`` under torch's autograd: the same functions, differentiable.
+"""``norm``, ``mlp``, ``attention`` and ``kernels.qk_prep`` under torch's autograd: the same functions, differentiable.
 
 Each call records the matching ``*_backward`` call; first derivatives only, and no forward mode (an operand
 with a tangent raises NotImplementedError).  They are not captured into a HIP graph with gradients: autograd
 accumulates into a leaf on the stream of whichever graph of that leaf is alive, which need not be the captured
-one, so such a call is refused -- capture the explicit forward and backward calls of ``norm`` and ``mlp``
-instead, which touch no leaves.
+one, so such a call is refused -- capture the explicit forward and backward calls instead, which touch no leaves.
 """
 
 from __future__ import annotations
@@ -13,6 +12,8 @@ import functools
 
 import torch
 
+from . import attention as _attention
+from . import kernels as _kernels
 from . import mlp as _mlp
 from . import norm as _norm
 from .kernels import EPS
@@ -21,7 +22,7 @@ from .kernels import EPS
 def _not_captured() -> None:
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("flicker_amd.autograd is not captured into a graph with gradients: capture the explicit "
-                           "forward and backward calls of flicker_amd.norm and flicker_amd.mlp")
+                           "forward and backward calls of flicker_amd.norm, mlp, attention and kernels")
 
 
 def _recorded(*tensors) -> bool:
@@ -99,6 +100,48 @@ class _GatedMLP(torch.autograd.Function):
         return *_mlp.gated_mlp_backward(dy, x, w_in, w_out, _mlp.Kept(h, gu), wanted=ctx.needs_input_grad[:3]), None
 
 
+class _ResidualModulate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, gate, shift, scale, eps):
+        ctx.save_for_backward(x, branch, gate, shift, scale)
+        ctx.eps = eps
+        return _norm.residual_modulate(x, branch, gate, shift, scale, eps=eps)
+
+    @staticmethod
+    @_first_only
+    def backward(ctx, dr, dy):
+        return *_norm.residual_modulate_backward(dr, dy, *ctx.saved_tensors, eps=ctx.eps), None
+
+
+class _QkPrep(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, q_scale, k_scale, freqs, num_heads):
+        ctx.save_for_backward(qkv, q_scale, k_scale)
+        ctx.freqs, ctx.num_heads = freqs, num_heads
+        return _kernels._launch_qk_prep(qkv, q_scale, k_scale, freqs, num_heads, None, 0)
+
+    @staticmethod
+    @_first_only
+    def backward(ctx, dq, dk, dv):
+        return *_kernels.qk_prep_backward(dq, dk, dv, *ctx.saved_tensors, ctx.freqs, ctx.num_heads), None, None
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_mask, keep):
+        if not keep:
+            return _attention.attention(q, k, v, key_mask=key_mask)
+        o, kept = _attention.attention(q, k, v, key_mask=key_mask, keep=True)
+        ctx.save_for_backward(q, k, v, key_mask, *kept)
+        return o
+
+    @staticmethod
+    @_first_only
+    def backward(ctx, do):
+        q, k, v, key_mask, *kept = ctx.saved_tensors
+        return *_attention.attention_backward(do, q, k, v, _attention.Kept(*kept), key_mask=key_mask), None, None
+
+
 def layer_norm(x, weight=None, bias=None, *, eps: float = EPS) -> torch.Tensor:
     """norm.layer_norm, differentiable in x, weight and bias."""
     _recorded(x, weight, bias)
@@ -121,3 +164,25 @@ def gated_mlp(x, w_in, w_out) -> torch.Tensor:
     """mlp.gated_mlp, differentiable in x, w_in and w_out; keeps what the backward pass needs only where one
     of them requires a gradient."""
     return _GatedMLP.apply(x, w_in, w_out, _recorded(x, w_in, w_out))
+
+
+def residual_modulate(x, branch, gate, shift, scale, *, eps: float = EPS) -> tuple[torch.Tensor, torch.Tensor]:
+    """norm.residual_modulate, differentiable in all five operands."""
+    _recorded(x, branch, gate, shift, scale)
+    return _ResidualModulate.apply(x, branch, gate, shift, scale, eps)
+
+
+def qk_prep(qkv, q_scale, k_scale, freqs, num_heads: int):
+    """kernels.qk_prep of any L, differentiable in qkv and both scales.  freqs' tables are kept as they are: they must not
+    change before the backward pass."""
+    _kernels._on_gpu("qkv", qkv)
+    if qkv.dim() != 3:
+        raise ValueError(f"qkv must be (B, L, 3*H*D), got {tuple(qkv.shape)}")
+    _recorded(qkv, q_scale, k_scale)
+    return _QkPrep.apply(qkv, q_scale, k_scale, freqs, num_heads)
+
+
+def attention(q, k, v, *, key_mask=None) -> torch.Tensor:
+    """attention.attention, differentiable in q, k and v; keeps what the backward pass needs only where one of them
+    requires a gradient."""
+    return _Attention.apply(q, k, v, key_mask, _recorded(q, k, v))

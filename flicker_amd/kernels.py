@@ -319,6 +319,12 @@ def qk_prep_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, qkv: 
         if (out.shape != qkv.shape or out.dtype != qkv.dtype or out.stride(2) != 1 or out.stride(0) % 8
                 or out.stride(1) % 8 or out.data_ptr() % 16):
             raise ValueError(f"out must be a bf16 {tuple(qkv.shape)} view with contiguous, 16-byte aligned rows")
+        if out.numel():
+            from .norm import _refuse_overlap, _rows_apart
+            if not _rows_apart(out):
+                raise ValueError(f"out needs rows that do not overlap, got strides {out.stride()}")
+            for name, t in (("qkv", qkv), ("dq", grads[0]), ("dk", grads[1]), ("dv", grads[2])):
+                _refuse_overlap(name, out, t)
     make = torch.empty if out.numel() else torch.zeros   # sums over no rows
     dscales = tuple(make(shape, dtype=q_scale.dtype, device=qkv.device) for shape in scale_shapes)
     if out.numel() == 0:

@@ -181,3 +181,173 @@ def test_cut_blocks(device, heads, kv_heads, queries, keys, mask):
 def test_whole_and_cut_blocks(device, queries, keys):
     """A few blocks more than the GPU's CUs: those are cut, the others are not."""
     check(keys, 2, 66, 66, queries, keys, "fp16", "middle" if keys == 200 else None)
+
+
+def test_repeats_bit_for_bit(device):
+    """Sums are in a fixed order: two calls give the same bits, cut blocks and shared heads among them."""
+    for args in ((1, 6, 2, 300, 2100), (2, 4, 1, 900, 500)):
+        q, k, v, do, keep = make(5, *args, "bf16", "random")
+        one, two = ((o, *A.attention_backward(do, q, k, v, kept, key_mask=keep))
+                    for o, kept in (A.attention(q, k, v, key_mask=keep, keep=True) for _ in range(2)))
+        assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
+def test_strided_operands(device):
+    """Columns of a wider projection, a row stride that is not 16 bytes (copied), keys and values shared by the batch, and
+    a mask that is a view."""
+    q, k, v, do, keep = make(11, 2, 3, 3, 70, 70, "bf16", "random")
+    o, kept = A.attention(q, k, v, key_mask=keep, keep=True)
+    want = A.attention_backward(do, q, k, v, kept, key_mask=keep)
+    wide = torch.full((2, 70, 3 * 3 * D + 24), float("nan"), dtype=q.dtype, device=device)
+    views = []
+    for i, t in enumerate((q, k, v)):
+        view = wide[..., i * 3 * D:(i + 1) * 3 * D]
+        view.copy_(t.transpose(1, 2).reshape(2, 70, 3 * D))
+        views.append(view.view(2, 70, 3, D).transpose(1, 2))
+    masks = torch.ones(2, 3, 90, dtype=torch.bool, device=device)
+    masks[:, 1, :70] = keep
+    got, kept2 = A.attention(*views, key_mask=masks[:, 1, :70], keep=True)
+    assert torch.equal(got, o)
+    assert all(torch.equal(a, b) for a, b in zip(A.attention_backward(do, *views, kept2, key_mask=masks[:, 1, :70]), want))
+    odd = torch.empty(2, 3, 70, D + 3, dtype=q.dtype, device=device)[..., :D].copy_(q)
+    assert torch.equal(A.attention(odd, k, v, key_mask=keep), o)
+    every = do.repeat(1, 1, 2)[..., ::2]
+    assert all(torch.equal(a, b) for a, b in zip(A.attention_backward(every, q, k, v, kept, key_mask=keep),
+                                                 A.attention_backward(every.contiguous(), q, k, v, kept, key_mask=keep)))
+    shared = A.attention(q, k[:1].expand(2, -1, -1, -1), v[:1].expand(2, -1, -1, -1), key_mask=keep[:1].expand(2, -1))
+    assert torch.equal(shared[1], A.attention(q[1:], k[:1], v[:1], key_mask=keep[:1])[0])
+
+
+def test_out(device):
+    """A result inside wider rows, whose other columns and rows stay as they were; an overlap is refused."""
+    q, k, v, do, _ = make(12, 2, 2, 2, 45, 60, "fp16")
+    buffer = torch.full((2, 50, 2 * D + 64), 7.0, dtype=q.dtype, device=device)
+    out = buffer[:, :45, 32:32 + 2 * D]
+    got, kept = A.attention(q, k, v, out=out, keep=True)
+    want, plain = A.attention(q, k, v, keep=True)
+    assert got is out and torch.equal(out, want)
+    assert (buffer[:, 45:] == 7).all() and (buffer[..., :32] == 7).all() and (buffer[..., 32 + 2 * D:] == 7).all()
+    assert all(torch.equal(a, b) for a, b in zip(A.attention_backward(do, q, k, v, kept),
+                                                 A.attention_backward(do, q, k, v, plain)))
+    with pytest.raises(ValueError, match="shares memory with q"):
+        A.attention(q, k, v, out=q.view(-1)[:2 * 45 * 2 * D].view(2, 45, 2 * D))
+    with pytest.raises(ValueError, match="do not overlap"):
+        A.attention(q, k, v, out=buffer[:1, :45, :2 * D].expand(2, -1, -1))
+    with pytest.raises(ValueError, match="out must be"):
+        A.attention(q, k, v, out=buffer[:, :45, :2 * D - 8])
+
+
+def test_empty(device):
+    q, k, v, do, _ = make(13, 2, 2, 1, 5, 7, "bf16")
+    none = k[:, :, :0]
+    o, kept = A.attention(q, none, none, keep=True)
+    assert not o.any() and torch.isneginf(kept.lse).all()
+    dq, dk, dv = A.attention_backward(do, q, none, none, kept)
+    assert not dq.any() and dk.shape == none.shape
+    assert not A.attention(q, none, none, key_mask=torch.ones(2, 0, dtype=torch.bool, device=device)).any()
+    o, kept = A.attention(q[:, :, :0], k, v, keep=True)
+    dq, dk, dv = A.attention_backward(do[:, :0], q[:, :, :0], k, v, kept)
+    assert o.shape == (2, 0, 2 * D) and not dk.any() and not dv.any()
+    assert A.attention(q[:0], k[:0], v[:0]).shape == (0, 5, 2 * D)
+
+
+def test_captured_and_replayed(device):
+    """Masks are read when a graph is replayed, not when it is captured; two graphs replayed in turn do not disturb each
+    other."""
+    cases = [make(14, 2, 4, 2, 200, 300, "bf16", "random"), make(15, 1, 2, 2, 33, 2000, "bf16", "middle")]
+
+    def step(q, k, v, do, keep):
+        o, kept = A.attention(q, k, v, key_mask=keep, keep=True)
+        return o, *A.attention_backward(do, q, k, v, kept, key_mask=keep)
+    graphs = []
+    for case in cases:
+        step(*case)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*case)
+        graphs.append((graph, out))
+    for i in range(3):
+        wants = []
+        for q, k, v, do, keep in cases:
+            q.mul_(1.25)
+            k.nan_to_num_(0.0, 0.0, 0.0)
+            v.nan_to_num_(0.0, 0.0, 0.0)
+            keep.copy_(torch.rand(keep.shape, generator=torch.Generator().manual_seed(i)).to(device) < 0.5)
+            wants.append(step(q, k, v, do, keep))
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, out), want in zip(graphs, wants):
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def test_two_streams_at_once(device):
+    cases = [make(16 + i, 1, 3, 3, 400, 900, "bf16", "middle") for i in range(2)]
+
+    def step(q, k, v, do, keep):
+        o, kept = A.attention(q, k, v, key_mask=keep, keep=True)
+        return o, *A.attention_backward(do, q, k, v, kept, key_mask=keep)
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(4):
+        for i, (s, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                got[i].append(step(*c))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, w))
+
+
+def test_offsets_past_32_bits(device):
+    """A cache of more than 2^31 elements whose last units alone are kept, and rows 2^21 elements apart."""
+    keys = 2 ** 24 + 2 ** 10
+    q, part_k, part_v, do, _ = make(18, 1, 1, 1, 40, 96, "bf16")
+    k, v = (torch.zeros(1, 1, keys, D, dtype=q.dtype, device=device) for _ in range(2))
+    k[:, :, -96:], v[:, :, -96:] = part_k, part_v
+    keep = torch.zeros(1, keys, dtype=torch.bool, device=device)
+    keep[:, -96:] = True
+    want = expected(q, part_k, part_v, do, None)
+    o, kept = A.attention(q, k, v, key_mask=keep, keep=True)
+    _close("o", o, *want[0])
+    dq, dk, dv = A.attention_backward(do, q, k, v, kept, key_mask=keep)
+    _close("dq", dq, *want[2])
+    _close("dk", dk[:, :, -96:], *want[3])
+    _close("dv", dv[:, :, -96:], *want[4])
+    assert not dk[:, :, :-96].any() and not dv[:, :, :-96].any()
+    del k, v, dk, dv
+    rows = torch.zeros(1100, 2 ** 21, dtype=q.dtype, device=device)
+    q, k, v, do, _ = make(19, 1, 1, 1, 1090, 1100, "bf16")
+    far = rows[:, :D].view(1, 1, 1100, D)
+    far.copy_(k)
+    assert torch.equal(A.attention(q, far, v), A.attention(q, k, v))
+
+
+def test_refusals(device):
+    q, k, v, do, keep = make(20, 2, 4, 2, 9, 11, "bf16", "random")
+    o, kept = A.attention(q, k, v, keep=True)
+    with pytest.raises(TypeError, match="bfloat16 or float16"):
+        A.attention(q.float(), k.float(), v.float())
+    with pytest.raises(TypeError, match="like q"):
+        A.attention(q, k.half(), v)
+    with pytest.raises(ValueError, match="of one shape"):
+        A.attention(q, k, v[:, :, :10])
+    with pytest.raises(ValueError, match="share"):
+        A.attention(q[:, :3], k, v)
+    with pytest.raises(ValueError, match="head_dim 64"):
+        A.attention(q[..., :64], k[..., :64], v[..., :64])
+    with pytest.raises(ValueError, match=r"\(B, H, L, D\)"):
+        A.attention(q[0], k, v)
+    with pytest.raises(TypeError, match="must be bool"):
+        A.attention(q, k, v, key_mask=keep.float())
+    with pytest.raises(ValueError, match="key_mask must be"):
+        A.attention(q, k, v, key_mask=keep[:, :10])
+    with pytest.raises(ValueError, match="GPU only"):
+        A.attention(q, k.cpu(), v)
+    with pytest.raises(ValueError, match="do must be"):
+        A.attention_backward(do[:, :8], q, k, v, kept)
+    with pytest.raises(ValueError, match="kept.lse"):
+        A.attention_backward(do, q, k, v, kept._replace(lse=kept.lse[:, :3]))
+    with pytest.raises(ValueError, match="kept.low"):
+        A.attention_backward(do, q, k, v, kept._replace(low=kept.low.float()))

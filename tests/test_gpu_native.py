@@ -135,3 +135,59 @@ def test_runtime_errors_are_raised(device, monkeypatch, call):
         return str(error.value).split("failed")[1]
 
     assert pending() == python_path(monkeypatch, pending)
+
+
+def _python_too(monkeypatch, f):
+    from flicker_amd import attention, norm
+    with monkeypatch.context() as m:
+        for mod in (kernels, attention, norm):
+            m.setattr(mod, "_native", Declines())
+        return f()
+
+
+def test_training_calls(device, monkeypatch):
+    """attention, residual_modulate, qk_prep_backward and their gradients: the Python path's bits, through views as well."""
+    from flicker_amd import attention, norm
+    n = kernels._native
+    g = torch.Generator().manual_seed(4)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g).to(torch.bfloat16).to(device)
+    q, kv = randn(2, 70, 4, D).transpose(1, 2), randn(2, 2, 90, 2 * D)
+    k, v = kv[..., :D], kv[..., D:]
+    keep = torch.rand(2, 90, generator=g).to(device) < 0.5
+    do = randn(2, 70, 4 * D)
+    assert n.attention(q, k, v, keep, True) is not None
+    o, kept = attention.attention(q, k, v, key_mask=keep, keep=True)
+    assert n.attention_backward(do, q, k, v, *kept, keep) is not None
+    f = lambda: attention.attention(q, k, v, key_mask=keep)   # noqa: E731
+    same(f(), _python_too(monkeypatch, f))
+    f = lambda: attention.attention(q, k, v, keep=True)[1][:2]   # noqa: E731
+    same(tuple(f()), tuple(_python_too(monkeypatch, f)))
+    f = lambda: attention.attention_backward(do, q, k, v, kept, key_mask=keep)   # noqa: E731
+    same(f(), _python_too(monkeypatch, f))
+    x, b, dr, dy = (randn(2, 33, 264)[..., :256] for _ in range(4))
+    rows = [randn(2, 1, 256) for _ in range(3)]
+    assert n.residual_modulate(x, b, *rows, 1e-6) is not None
+    assert n.residual_modulate_backward(dr, dy, x, b, *rows, 1e-6) is not None
+    f = lambda: norm.residual_modulate(x, b, *rows)   # noqa: E731
+    same(f(), _python_too(monkeypatch, f))
+    f = lambda: norm.residual_modulate_backward(dr, dy, x, b, *rows)   # noqa: E731
+    same(f(), _python_too(monkeypatch, f))
+    qkv, scales = stream(device, 2, 50, 3, torch.bfloat16, 5)
+    freqs = tables(device, 50)
+    grads = [randn(2, 3, 80, D) for _ in range(3)]
+    assert n.qk_prep_backward(*grads, qkv, *scales, freqs.cos, freqs.sin, freqs.q_gain, 3, 30) is not None
+    assert n.qk_prep_backward(*grads, qkv, *scales, freqs.cos, freqs.sin, freqs.q_gain, 3, 31) is None
+    assert n.qk_prep_backward(*grads, qkv, *scales, freqs.cos, freqs.sin, freqs.q_gain, 3, -1) is None
+    f = lambda: kernels.qk_prep_backward(*grads, qkv, *scales, freqs, 3, offset=30)   # noqa: E731
+    same(f(), _python_too(monkeypatch, f))
+    for i, bad in ((0, q.cpu()), (0, q.float()), (1, k.half()), (1, k[:, :1]), (2, v[:, :, :9]), (3, keep.float()), (3, keep[:1]),
+                   (4, 1)):
+        args = [q, k, v, keep, False]
+        args[i] = bad
+        assert n.attention(*args) is None, (i, bad)
+    for i, bad in ((0, x[0]), (1, b[:, 1:]), (2, rows[0].float()), (2, rows[0][:1]), (3, None), (5, 1)):
+        args = [x, b, *rows, 1e-6]
+        args[i] = bad
+        assert n.residual_modulate(*args) is None, (i, bad)
