@@ -1035,7 +1035,8 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
       barrier();
     };
     int u = 0;
-    for (; qs.template inside<kQRing>() && u + kQRing <= n; u += kQRing)
+    // a turn copies the stats of up to u + kQRing + 2, which have to be of units below n: the others' are `none`
+    for (; qs.template inside<kQRing>() && u + kQRing + 2 < n; u += kQRing)
 #pragma unroll
       for (int r = 0; r < kQRing; r += 2) {
         iteration(std::true_type{}, u + r, r, s0, s1, p1, p0);

@@ -351,3 +351,9 @@ def test_refusals(device):
         A.attention_backward(do, q, k, v, kept._replace(lse=kept.lse[:, :3]))
     with pytest.raises(ValueError, match="kept.low"):
         A.attention_backward(do, q, k, v, kept._replace(low=kept.low.float()))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(50, 50), (100, 50)])
+def test_long_cuts_of_the_queries(device, heads, kv_heads):
+    """dk and dv in cuts of two dozen units and more: each adds the units of its own range and no others."""
+    check(21, 2, heads, kv_heads, 1500 * kv_heads // heads, 100, "bf16")
