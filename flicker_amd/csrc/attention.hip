@@ -923,11 +923,6 @@ struct Queries {
     left = heads - skipped;
     at = reinterpret_cast<const char*>(t.at<uint16_t>(b, h + skipped)) + unit * step;
   }
-  // Whether a head's last unit is none of the next kCount.
-  template <int kCount>
-  __device__ __forceinline__ bool inside() const {
-    return unit + kCount < units;
-  }
   template <bool kInside>
   __device__ __forceinline__ void next() {   // past the last unit of all: the last; selects, not branches, inside a phase
     if constexpr (kInside) {
@@ -1035,8 +1030,10 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
       barrier();
     };
     int u = 0;
-    // a turn copies the stats of up to u + kQRing + 2, which have to be of units below n: the others' are `none`
-    for (; qs.template inside<kQRing>() && u + kQRing + 2 < n; u += kQRing)
+    // a turn copies kQRing units from qs.unit and os.unit on, none a head's last (qs may be in the next head already), and the
+    // stats of up to u + kQRing + 2, all below n: the stats of units from n on are `none`
+    const int inside = min(A.q_units - max(qs.unit, os.unit), n - 2) - kQRing, end = inside > 0 ? inside : 0;
+    for (; u < end; u += kQRing)
 #pragma unroll
       for (int r = 0; r < kQRing; r += 2) {
         iteration(std::true_type{}, u + r, r, s0, s1, p1, p0);

@@ -357,3 +357,8 @@ def test_refusals(device):
 def test_long_cuts_of_the_queries(device, heads, kv_heads):
     """dk and dv in cuts of two dozen units and more: each adds the units of its own range and no others."""
     check(21, 2, heads, kv_heads, 1500 * kv_heads // heads, 100, "bf16")
+
+
+def test_cuts_that_begin_near_a_head_s_end(device):
+    """Four query heads of ten units a key head, in cuts of 14, 13 and 13: the last begins three units before a head ends."""
+    check(22, 1, 280, 70, 320, 100, "bf16")
