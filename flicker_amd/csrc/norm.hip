@@ -32,10 +32,11 @@
 // the caches 25.0), 47.5 with such a reader (42.4); 4608 rows 22.1 (22.4).  The rows read are not (13.3 -> 16.7: the last
 // cache often has them), nor the partial rows, read again at once.
 //
-// The residual form of 16-bit rows reads past the caches and stores through them: r and y are read next, and they stay in
-// the last cache where the two operands would have pushed them out.  4 x 4096 rows 65 us (as the norm alone does it 82;
-// both past the caches 80), gradients of 4608 rows 41 (45; 45).  Rows off 16 bytes share words between lanes, which are
-// then fetched twice: 3 x 1157 x 1111 float32 gradients 34 us, past the caches 40.
+// The residual form of 16-bit rows reads past the caches and stores through them: both outputs are read next, and they
+// stay in the last cache where the operands would have pushed them out.  us alone, and with what adds the two outputs up
+// behind it (as the norm alone does it; both past the caches): 4608 rows 25.0 and 37.7 (25.1, 42.0; 24.3, 41.5), their
+// gradients 44.5 and 57.4 (45.7, 64.7; 45.3, 60.4), 4 x 4096 rows 83.5 and 126 (81.6, 137; 80.0, 133).  Rows off 16 bytes
+// share words between lanes, which are then fetched twice: 3 x 1157 x 1111 float32 gradients 28.7 us, past the caches 34.
 //
 // Measured (bf16, width 3 * 1024, among other passes): forward 4 x 4096 rows in 41.7 us, 4.8 TB/s (a large copy's
 // rate is 5.2), backward 4608 rows in 24.9 us (85 MB of operands, and 13 MB of partial rows written and read); 512

@@ -13,9 +13,9 @@
 // so the scales' gradients gather in 16 registers while a block walks its tokens and heads; blocks write them as
 // partial rows, which a second kernel adds in a fixed order.
 //
-// Measured (24 heads): 2 x 4096 tokens 71 us, 5.7 TB/s, past a large copy's 5.1 (read through the caches 86; stored past them
-// 82); 512 tokens 11 us, two launches of 7 and 4.  Blocks a CU, 2 x 4096 tokens: 2 78.9, 3 71.8, 4 71.0, 6 75.6, 8 73.8 us;
-// heads a group: 1 81.8, 2 71.0, 3 80.3, 4 72.6.
+// Measured (24 heads): 2 x 4096 tokens 79.5 us, 5.1 TB/s, a large copy's rate (stored through the caches 85, read through
+// them too 87-92; 3 blocks a CU 78.9, 6 84.5, 8 82; of one, three or four heads a group two are fastest); 512 tokens 11 us,
+// two launches of 7 and 4.
 
 #include <algorithm>
 
@@ -49,11 +49,16 @@ struct Args {
   float* partial;   // (block, 2, 128)
 };
 
-// Every operand row is read once and past the caches (nontemporal).
+// Operands are read once, and what is written is read next by matrix products, which wait for no memory: both go past the
+// caches (nontemporal).
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint4 load16(const uint16_t* p) {
-  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
   const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
   return make_uint4(v.x, v.y, v.z, v.w);
+}
+__device__ __forceinline__ void store16(uint16_t* p, uint4 v) {
+  const u32x4 w = {v.x, v.y, v.z, v.w};
+  __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
 }
 
 __device__ __forceinline__ void widen(uint4 raw, float (&x)[8]) {
@@ -132,9 +137,9 @@ __global__ __launch_bounds__(kThreads) void qk_prep_backward_kernel(const Args A
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       const int h = h0 + i;
-      *reinterpret_cast<uint4*>(out + (int64_t)h * kD) = row_gradient(gq[i], xq[i], qs, c, s, A.gain, dqs);
-      *reinterpret_cast<uint4*>(out + (int64_t)(A.heads + h) * kD) = row_gradient(gk[i], xk[i], ks, c, s, 1.0f, dks);
-      *reinterpret_cast<uint4*>(out + (int64_t)(2 * A.heads + h) * kD) = gv[i];
+      store16(out + (int64_t)h * kD, row_gradient(gq[i], xq[i], qs, c, s, A.gain, dqs));
+      store16(out + (int64_t)(A.heads + h) * kD, row_gradient(gk[i], xk[i], ks, c, s, 1.0f, dks));
+      store16(out + (int64_t)(2 * A.heads + h) * kD, gv[i]);
     }
   }
 #pragma unroll
