@@ -80,6 +80,13 @@ struct Mask {
   const int* counts;
 };
 
+// The blocks from `whole` on are cut into `splits` along the units they walk: partial sums of 256 rows, in order, which
+// attention_join_kernel adds up.
+struct Cuts {
+  int whole, splits, tile;   // tile: rows of a block
+  float* part;               // (cut, 256, 128)
+};
+
 struct Args {
   Tensor q, k, v, o, dO, dq, dk, dv;
   void* low;        // (batch, queries, heads, 128): what o's rounding left, in the same type
@@ -88,11 +95,10 @@ struct Args {
                     // end and in the last unit
   Mask mask;
   int batch, heads, kv_heads, group, queries, keys, q_units, k_units;
-  // The blocks from `whole` on are cut into `splits` along the units they walk: partial sums of 256 rows, in order, each
-  // with its rows' (top, l, sum) in the forward pass, which attention_join_kernel adds up.
-  int whole, splits, tile;   // tile: queries of a block
-  float* part;      // (cut, 256, 128)
-  float* part_top;  // (cut, 256, 4)
+  Cuts of_q, of_k;  // of the blocks of queries, and of keys (backwards)
+  float* part_top;  // (cut, 256, 4): in the forward pass each row's (top, l, sum)
+  int q_grid;       // backwards: hardware blocks that take queries, the first ones or, with k_first, the last
+  bool k_first;
 };
 
 // Which keys of unit u are kept.
@@ -112,17 +118,17 @@ __device__ __forceinline__ int by_xcd(int p, int total) {
 // What a hardware block takes: a block, or one of its cuts.
 struct Piece {
   int block, cut, split, splits;   // cut: its place among the partial sums, -1 for a whole block
-  __device__ __forceinline__ explicit Piece(const Args& A) {
-    const int p = blockIdx.x;
-    if (p < A.whole) {
-      block = by_xcd(p, A.whole);
+  // p: which of `total` pieces.
+  __device__ __forceinline__ Piece(const Cuts& c, int p, int total) {
+    if (p < c.whole) {
+      block = by_xcd(p, c.whole);
       cut = -1;
       split = 0;
       splits = 1;
     } else {
-      const int i = by_xcd(p - A.whole, gridDim.x - A.whole);
-      splits = A.splits;
-      block = A.whole + i / splits;
+      const int i = by_xcd(p - c.whole, total - c.whole);
+      splits = c.splits;
+      block = c.whole + i / splits;
       split = i % splits;
       cut = splits > 1 ? i : -1;
     }
@@ -132,19 +138,19 @@ struct Piece {
   __device__ __forceinline__ int count(int n) const { return n / splits + (split < n % splits); }
 };
 
-// A wave's queries in a block of A.tile: 256, 32 a wave, or 192, of which the waves 4-7 take 16 each, so that every SIMD holds
+// A wave's queries in a block of of_q.tile: 256, 32 a wave, or 192, of which the waves 4-7 take 16 each, so that every SIMD holds
 // 48.
 struct Rows {
   int b, h, first, end, q0;
   bool wide;
   __device__ __forceinline__ Rows(const Args& A, const Piece& piece) {
-    const int blocks = (A.queries + A.tile - 1) / A.tile, bh = piece.block / blocks;
+    const int tile = A.of_q.tile, blocks = (A.queries + tile - 1) / tile, bh = piece.block / blocks;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     b = bh / A.heads;
     h = bh - b * A.heads;
-    first = (piece.block - bh * blocks) * A.tile;
-    end = min(A.queries, first + A.tile);
-    wide = A.tile == kQueries || wave < 4;
+    first = (piece.block - bh * blocks) * tile;
+    end = min(A.queries, first + tile);
+    wide = tile == kQueries || wave < 4;
     q0 = first + (wide ? wave * 32 : 64 + wave * 16);
   }
 };
@@ -583,7 +589,7 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy writes LDS that the block has left
   }
   if (piece.cut >= 0) {
-    store_part(w.acc, A.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
+    store_part(w.acc, A.of_q.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const int r = q0 - first + g * 16 + (lane & 15);
@@ -613,7 +619,7 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
 template <typename T, bool kMasked, bool kKeep>
 __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[(kKRing + kVRing) * kUnitBytes];
-  const Piece piece(A);
+  const Piece piece(A.of_q, blockIdx.x, gridDim.x);
   const Rows rows(A, piece);
   if (rows.wide)
     forward_wave<T, kMasked, kKeep, 2>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
@@ -621,7 +627,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
     forward_wave<T, kMasked, kKeep, 1>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
 }
 
-// dq, and the stats that attention_dkv_kernel reads.
 template <typename T, int G>
 struct Dq {
   vec8<T> x[4][G], g[4][G];   // Q^T, dO^T
@@ -694,36 +699,17 @@ constexpr int kDqKRing = 6, kDqVRing = 3;
 template <typename T, bool kMasked, int G>
 __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piece& piece, int b, int h, int first, int end,
                                         int q0) {
-  const int lane = threadIdx.x & 63, h4 = lane >> 4, bh = b * A.heads + h;
+  const int lane = threadIdx.x & 63, bh = b * A.heads + h;
   Units<kMasked> units(A, b, piece);
   const int n = units.n;
   Dq<T, G> w;
   load_rows<T>(w.g, A.dO.at<T>(b, h), A.dO.row, q0, end);
-  {
-    vec8<T> o[4][G], low[4][G];
-    load_rows<T>(o, A.o.at<T>(b, h), A.o.row, q0, end);
-    load_rows<T>(low, static_cast<const T*>(A.low) + ((int64_t)b * A.queries * A.heads + h) * kD, (int64_t)A.heads * kD, q0,
-                 end);
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int r = q0 + g * 16 + (lane & 15);
-      const float x = r < end ? A.lse[(int64_t)bh * A.queries + r] : -INFINITY;
-      float sum = 0.0f;
-#pragma unroll
-      for (int st = 0; st < 4; ++st)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum += (float)w.g[st][g][e] * ((float)o[st][g][e] + (float)low[st][g][e]);
-      sum = across(sum);
-      w.lse[g] = x == -INFINITY ? -INFINITY : x * -kLog2e;
-      w.delta[g] = x == -INFINITY ? 0.0f : -sum;
-      if (piece.split == 0 && h4 == 0 && r < A.q_units * kUnit) {
-        float* st = A.stats + ((int64_t)bh * A.q_units + r / kUnit) * 2 * kUnit + r % kUnit;
-        st[0] = -w.lse[g];
-        st[kUnit] = w.delta[g];
-      }
-    }
-    if (blockIdx.x == 0 && threadIdx.x < 2 * kUnit)
-      A.stats[(int64_t)A.batch * A.heads * A.q_units * 2 * kUnit + threadIdx.x] = threadIdx.x < kUnit ? INFINITY : 0.0f;
+  for (int g = 0; g < G; ++g) {
+    const int r = q0 + g * 16 + (lane & 15);
+    const float* st = A.stats + ((int64_t)bh * A.q_units + r / kUnit) * 2 * kUnit + r % kUnit;
+    w.lse[g] = r < end ? -st[0] : -INFINITY;
+    w.delta[g] = r < end ? st[kUnit] : 0.0f;
   }
 #pragma unroll
   for (int g = 0; g < G; ++g)
@@ -808,22 +794,13 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   if (piece.cut >= 0) {
-    store_part(w.acc, A.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
+    store_part(w.acc, A.of_q.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
     return;
   }
   float one[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) one[g] = 1.0f;
   store_rows<T>(w.acc, one, A.dq.at<T>(b, h), A.dq.row, q0, end);
-}
-
-template <typename T, bool kMasked>
-__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(const Args A) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[(kDqKRing + kDqVRing) * kUnitBytes];
-  const Piece piece(A);
-  const Rows rows(A, piece);
-  if (rows.wide) dq_wave<T, kMasked, 2>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
-  else dq_wave<T, kMasked, 1>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
 }
 
 // dk and dv of 128 keys, 32 a pair of waves: the first holds K^T and dV^T, forms S and P and hands P on through LDS, the second holds
@@ -1050,7 +1027,7 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = on[g] ? w.acc[dt][g] : f32x4{};
   if (piece.cut >= 0) {   // dv's 128 rows, then dk's
-    float* part = A.part + ((int64_t)piece.cut * 2 + kSecond) * kKeys * kD;
+    float* part = A.of_k.part + ((int64_t)piece.cut * 2 + kSecond) * kKeys * kD;
     store_part(w.acc, part, k0 - first, min(A.keys - first, kKeys));
     return;
   }
@@ -1059,13 +1036,24 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
   store_rows<T>(w.acc, one, out.at<T>(b, h), out.row, k0, A.keys);
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(const Args A) {
+// All gradients: blocks of queries and blocks of keys in one launch, so that neither kind's last round leaves CUs idle.
+template <typename T, bool kMasked>
+__global__ __launch_bounds__(kThreads, 2) void attention_backward_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kDkvBytes];
+  static_assert(kDkvBytes >= (kDqKRing + kDqVRing) * kUnitBytes);
+  const int k_grid = gridDim.x - A.q_grid, p = blockIdx.x;
+  const int q_p = A.k_first ? p - k_grid : p, k_p = A.k_first ? p : p - A.q_grid;
+  if (A.k_first ? q_p >= 0 : k_p < 0) {
+    const Piece piece(A.of_q, q_p, A.q_grid);
+    const Rows rows(A, piece);
+    if (rows.wide) dq_wave<T, kMasked, 2>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
+    else dq_wave<T, kMasked, 1>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
+    return;
+  }
   const int blocks = (A.keys + kKeys - 1) / kKeys;
-  const Piece piece(A);
-  const int block = piece.block, bh = block / blocks, b = bh / A.kv_heads, h = bh - b * A.kv_heads;
-  const int first = (block - bh * blocks) * kKeys;
+  const Piece piece(A.of_k, k_p, k_grid);
+  const int bh = piece.block / blocks, b = bh / A.kv_heads, h = bh - b * A.kv_heads;
+  const int first = (piece.block - bh * blocks) * kKeys;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   bool any = false;
   for (int u = first / kUnit; u < min(A.k_units, (first + kKeys) / kUnit); ++u) any |= kept(A, b, u) != 0;
@@ -1074,28 +1062,31 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(const Args A
   else dkv_wave<true, T>(A, smem, piece, b, h, first, k0, any);
 }
 
-// Adds the cuts' partial sums in order: 32 lanes a row, 8 rows of a cut block a block.
-enum Joined { kJoinO, kJoinDq, kJoinDkv };
-template <typename T, Joined kOf, bool kKeep>
-__global__ __launch_bounds__(256) void attention_join_kernel(const Args A) {
-  const int lane = threadIdx.x & 31;
-  const int cut_block = blockIdx.x / (kQueries / 8), r = blockIdx.x % (kQueries / 8) * 8 + (threadIdx.x >> 5);
-  const int block = A.whole + cut_block, rows = kOf == kJoinDkv ? A.keys : A.queries;
-  const int per = kOf == kJoinDkv ? kKeys : A.tile, heads = kOf == kJoinDkv ? A.kv_heads : A.heads;
+// Adds the cuts' partial sums in order: 32 lanes a row, 8 rows of a cut block a block.  kOf: of o, or of the gradients, the
+// queries' cut blocks first.
+template <typename T, bool kForward, bool kKeep>
+__global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q_blocks) {
+  const int lane = threadIdx.x & 31, r = blockIdx.x % (kQueries / 8) * 8 + (threadIdx.x >> 5);
+  int cut_block = blockIdx.x / (kQueries / 8);
+  const bool of_keys = !kForward && cut_block >= q_blocks;
+  if (of_keys) cut_block -= q_blocks;
+  const Cuts& cuts = of_keys ? A.of_k : A.of_q;
+  const int block = cuts.whole + cut_block, rows = of_keys ? A.keys : A.queries;
+  const int per = cuts.tile, heads = of_keys ? A.kv_heads : A.heads;
   const int blocks = (rows + per - 1) / per, bh = block / blocks, b = bh / heads, h = bh - b * heads;
-  const int row = (block - bh * blocks) * per + (kOf == kJoinDkv ? r % kKeys : r);
-  if (row >= rows || (kOf != kJoinDkv && r >= per)) return;
-  const int64_t first = ((int64_t)cut_block * A.splits * kQueries + r) * kD;
+  const int row = (block - bh * blocks) * per + (of_keys ? r % kKeys : r);
+  if (row >= rows || (!of_keys && r >= per)) return;
+  const int64_t first = ((int64_t)cut_block * cuts.splits * kQueries + r) * kD;
   f32x4 x{};
-  if constexpr (kOf == kJoinO) {
+  if constexpr (kForward) {
     // lane i of the row's 32 holds the factors of the cuts i and i + 32
-    const f32x4* tops = reinterpret_cast<const f32x4*>(A.part_top) + (int64_t)cut_block * A.splits * kQueries + r;
+    const f32x4* tops = reinterpret_cast<const f32x4*>(A.part_top) + (int64_t)cut_block * cuts.splits * kQueries + r;
     f32x4 t[2];
     float top = -1e30f, l = 0.0f, sum = 0.0f, f[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int at = lane + 32 * i;
-      t[i] = at < A.splits ? tops[(int64_t)at * kQueries] : f32x4{-1e30f, 0.0f, 0.0f, 0.0f};
+      t[i] = at < cuts.splits ? tops[(int64_t)at * kQueries] : f32x4{-1e30f, 0.0f, 0.0f, 0.0f};
       top = fmaxf(top, t[i][0]);
     }
 #pragma unroll
@@ -1111,9 +1102,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A) {
       l += __shfl_xor(l, d, 32);
       sum += __shfl_xor(sum, d, 32);
     }
-    const float* at = A.part + first + lane * 4;
+    const float* at = cuts.part + first + lane * 4;
 #pragma unroll 8
-    for (int i = 0; i < A.splits; ++i)
+    for (int i = 0; i < cuts.splits; ++i)
       x += *reinterpret_cast<const f32x4*>(at + (int64_t)i * kQueries * kD) * __shfl(i < 32 ? f[0] : f[1], i & 31, 32);
     x *= l > 0.0f ? 1.0f / l : 0.0f;
     if constexpr (kKeep) {
@@ -1131,24 +1122,28 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A) {
     }
   } else {
 #pragma unroll 4
-    for (int i = 0; i < A.splits; ++i)
-      x += *reinterpret_cast<const f32x4*>(A.part + first + (int64_t)i * kQueries * kD + lane * 4);
+    for (int i = 0; i < cuts.splits; ++i)
+      x += *reinterpret_cast<const f32x4*>(cuts.part + first + (int64_t)i * kQueries * kD + lane * 4);
   }
-  const Tensor& out = kOf == kJoinO ? A.o : kOf == kJoinDq ? A.dq : r < kKeys ? A.dv : A.dk;
+  const Tensor& out = kForward ? A.o : !of_keys ? A.dq : r < kKeys ? A.dv : A.dk;
   *reinterpret_cast<uint2*>(out.at<T>(b, h) + (int64_t)row * out.row + lane * 4) =
       make_uint2(pack<T>(x[0], x[1]), pack<T>(x[2], x[3]));
 }
 
-// The mask's words and live units, one batch entry a block, a thread a unit, 1024 units a turn.
+// The mask's words and live units, one batch entry a block of 16 waves, a thread a unit, 1024 units a turn.
 constexpr int kPlanWaves = 16;
-__global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const uint8_t* mask, int64_t batch_stride, int keys,
-                                                                         int units, uint32_t* words, uint2* live,
-                                                                         int* counts) {
-  __shared__ int found[kPlanWaves];
+struct MaskBytes {
+  const uint8_t* mask;   // NULL: none
+  int64_t batch_stride;
+  uint32_t* bits;
+  uint2* live;
+  int* counts;
+};
+__device__ __forceinline__ void plan_entry(const MaskBytes& m, int entry, int keys, int units, int (&found)[kPlanWaves]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint8_t* row = mask + blockIdx.x * batch_stride;
-  words += (int64_t)blockIdx.x * units;
-  live += (int64_t)blockIdx.x * units;
+  const uint8_t* row = m.mask + entry * m.batch_stride;
+  uint32_t* bits = m.bits + (int64_t)entry * units;
+  uint2* live = m.live + (int64_t)entry * units;
   int count = 0;
   for (int u0 = 0; u0 < units; u0 += 64 * kPlanWaves) {
     uint32_t mine = 0;   // of unit u0 + threadIdx.x
@@ -1160,7 +1155,7 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const u
     }
     const int u = u0 + threadIdx.x;
     const uint64_t any = __ballot(mine != 0);
-    if (u < units) words[u] = mine;
+    if (u < units) bits[u] = mine;
     if (lane == 0) found[wave] = __popcll(any);
     __syncthreads();
     int at = count;
@@ -1171,7 +1166,58 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const u
     if (mine) live[at + __popcll(any & ((1ull << lane) - 1))] = make_uint2(u, mine);
     __syncthreads();
   }
-  if (threadIdx.x == 0) counts[blockIdx.x] = count;
+  if (threadIdx.x == 0) m.counts[entry] = count;
+}
+
+__global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const MaskBytes m, int keys, int units) {
+  __shared__ int found[kPlanWaves];
+  plan_entry(m, blockIdx.x, keys, units, found);
+}
+
+// What the gradients need first: the mask's words and lists, in the first A.batch blocks where there is a mask, and every
+// row's stats, 16 lanes a row and 128 rows (four units) a block, which reads do, o and low once.
+template <typename T>
+__global__ __launch_bounds__(64 * kPlanWaves) void attention_prepare_kernel(const MaskBytes m, const Args A) {
+  __shared__ int found[kPlanWaves];
+  const int masks = m.mask ? A.batch : 0;
+  if ((int)blockIdx.x < masks) {
+    plan_entry(m, blockIdx.x, A.keys, A.k_units, found);
+    return;
+  }
+  const int64_t all = (int64_t)A.batch * A.heads * A.q_units;
+  const int64_t unit = (int64_t)(blockIdx.x - masks) * 4 + (threadIdx.x >> 8);   // `all` itself: the unit of no rows
+  if (unit > all) return;
+  const int lane = threadIdx.x & 15, bh = (int)(unit / A.q_units), b = bh / A.heads, h = bh - b * A.heads;
+  const int first = (int)(unit - (int64_t)bh * A.q_units) * kUnit + (threadIdx.x >> 4 & 15);
+  float* st = A.stats + unit * 2 * kUnit + (threadIdx.x >> 4 & 15);
+  vec8<T> x[2][3];
+  float lse[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = first + 16 * i;
+    const bool live = unit < all && r < A.queries;
+    lse[i] = -INFINITY;
+    if (live) {
+      x[i][0] = *reinterpret_cast<const vec8<T>*>(A.dO.at<T>(b, h) + (int64_t)r * A.dO.row + lane * 8);
+      x[i][1] = *reinterpret_cast<const vec8<T>*>(A.o.at<T>(b, h) + (int64_t)r * A.o.row + lane * 8);
+      x[i][2] = *reinterpret_cast<const vec8<T>*>(static_cast<const T*>(A.low) +
+                                                  (((int64_t)b * A.queries + r) * A.heads + h) * kD + lane * 8);
+      lse[i] = A.lse[(int64_t)bh * A.queries + r];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float sum = 0.0f;
+    const bool live = lse[i] != -INFINITY;   // a row that keeps no key has no gradient, whatever do holds
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      sum += live ? (float)x[i][0][e] * ((float)x[i][1][e] + (float)x[i][2][e]) : 0.0f;
+    sum = flk::row16_sum(sum);
+    if (lane == 0) {
+      st[16 * i] = live ? lse[i] * kLog2e : INFINITY;
+      st[16 * i + kUnit] = -sum;
+    }
+  }
 }
 
 int units_of(int rows) { return (rows + kUnit - 1) / kUnit; }
@@ -1180,16 +1226,15 @@ int64_t stats_bytes(int batch, int heads, int queries) {
   return ((int64_t)batch * heads * units_of(queries) + 1) * 2 * kUnit * 4;
 }
 
-// Lays the mask's words and lists out in `workspace` and starts the kernel that fills them.
-int plan_mask(const void* mask, int64_t batch_stride, Args& A, uint8_t* workspace, hipStream_t s) {
-  if (!mask) return FLK_OK;
-  uint2* live = reinterpret_cast<uint2*>(workspace);
-  uint32_t* bits = reinterpret_cast<uint32_t*>(live + (int64_t)A.batch * A.k_units);
-  int* counts = reinterpret_cast<int*>(bits + (int64_t)A.batch * A.k_units);
-  A.mask = Mask{bits, live, counts};
-  attention_mask_kernel<<<A.batch, 64 * kPlanWaves, 0, s>>>(static_cast<const uint8_t*>(mask), batch_stride, A.keys,
-                                                            A.k_units, bits, live, counts);
-  return flk_launch_status();
+// Where the mask's words and lists lie in `workspace`.
+MaskBytes mask_in(const void* mask, int64_t batch_stride, Args& A, uint8_t* workspace) {
+  MaskBytes m{static_cast<const uint8_t*>(mask), batch_stride, nullptr, nullptr, nullptr};
+  if (!mask) return m;
+  m.live = reinterpret_cast<uint2*>(workspace);
+  m.bits = reinterpret_cast<uint32_t*>(m.live + (int64_t)A.batch * A.k_units);
+  m.counts = reinterpret_cast<int*>(m.bits + (int64_t)A.batch * A.k_units);
+  A.mask = Mask{m.bits, m.live, m.counts};
+  return m;
 }
 
 // How a launch of equal blocks of `tile` rows, each walking n units, is cut: whole rounds of the 256 CUs, and what is left in
@@ -1201,18 +1246,21 @@ struct Cut {
   int64_t grid() const { return whole + (blocks - whole) * splits; }
   int64_t cuts() const { return splits > 1 ? (blocks - whole) * splits : 0; }
   int64_t bytes() const { return cuts() * kQueries * (kD + 4) * 4; }
+  Cuts in(uint8_t* workspace) const { return Cuts{whole, splits, tile, reinterpret_cast<float*>(workspace)}; }
 };
 constexpr int kCUs = 256, kMaxSplits = 64;
-// us of a unit, of a block's first loads and last stores, of the join's launch, and bytes of partial sums written and read a us
+// us of a block's first loads and last stores, of the join's launch, and bytes of partial sums written and read a us
+constexpr double kFixed = 6.0, kJoin = 5.0, kBytes = 4e6;
+double join_time(int64_t cuts, int rows) { return cuts ? cuts * (double)rows * kD * 8 / kBytes : 0.0; }
+// unit: us of one.
 Cut plan_cut(int64_t blocks, int64_t n, double unit, int rows, int tile) {
-  constexpr double kFixed = 6.0, kJoin = 5.0, kBytes = 4e6;
   auto rounds = [&](int64_t grid) { return (double)((grid + kCUs - 1) / kCUs); };
   Cut best{(int)blocks, 1, tile, blocks, rounds(blocks) * (n * unit + kFixed)};
   const int64_t whole = blocks / kCUs * kCUs, rest = blocks - whole;
   if (rest == 0 || blocks > 16 * kCUs) return best;
   for (int s = 2; s <= kMaxSplits && 4 * s <= n; ++s) {
     const double time = rounds(whole) * (n * unit + kFixed) + rounds(rest * s) * ((n + s - 1) / s * unit + kFixed) + kJoin +
-                        rest * s * (double)rows * kD * 8 / kBytes;
+                        join_time(rest * s, rows);
     if (time < best.time) best = Cut{(int)whole, s, tile, blocks, time};
   }
   return best;
@@ -1228,17 +1276,108 @@ Cut plan_queries(const Args& A, double unit, double unit192) {
   return narrow.blocks <= kCUs && narrow.time < wide.time ? narrow : wide;
 }
 Cut forward_cut(const Args& A) { return plan_queries(A, 0.82, 0.69); }
-Cut dq_cut(const Args& A) { return plan_queries(A, 1.1, 0.9); }
-Cut dkv_cut(const Args& A) {
-  const int64_t blocks = (int64_t)A.batch * A.kv_heads * ((A.keys + kKeys - 1) / kKeys);
-  return plan_cut(blocks, (int64_t)A.q_units * A.group, 0.85, 2 * std::min(A.keys, kKeys), kKeys);
+
+// When the CUs, each taking the next block as it ends one, have done runs of equal blocks.
+class Schedule {
+  struct Some {
+    double at;
+    int64_t count;
+  } some_[kCUs + 1];   // CUs that are free at the same time, soonest first
+  int n_ = 1;
+
+ public:
+  Schedule() { some_[0] = Some{0.0, kCUs}; }
+  void run(int64_t blocks, double time) {
+    while (blocks > 0) {
+      const int64_t take = std::min(some_[0].count, blocks);
+      const double at = some_[0].at + time;
+      blocks -= take;
+      if ((some_[0].count -= take) == 0) {
+        --n_;
+        for (int i = 0; i < n_; ++i) some_[i] = some_[i + 1];
+      }
+      int i = 0;
+      while (i < n_ && some_[i].at < at) ++i;
+      if (i < n_ && some_[i].at == at) {
+        some_[i].count += take;
+      } else {
+        for (int j = n_; j > i; --j) some_[j] = some_[j - 1];
+        some_[i] = Some{at, take};
+        ++n_;
+      }
+    }
+  }
+  double end() const { return some_[n_ - 1].at; }
+};
+
+// The gradients' launch: how its blocks of queries and of keys are cut, and which come first.
+struct Gradients {
+  Cut q, k;
+  bool k_first;
+  double time;
+  int64_t bytes() const { return q.bytes() + k.bytes(); }
+};
+// us of a unit of 32 keys for 256 and for 192 queries, and of 32 queries for 128 keys
+constexpr double kDqUnit = 1.1, kDqUnit192 = 0.9, kDkvUnit = 0.85;
+
+Gradients search_gradients(const Args& A) {
+  const int64_t k_n = (int64_t)A.q_units * A.group, q_n = A.k_units;
+  const int64_t k_blocks = (int64_t)A.batch * A.kv_heads * ((A.keys + kKeys - 1) / kKeys);
+  auto q_blocks = [&](int tile) { return (int64_t)A.batch * A.heads * ((A.queries + tile - 1) / tile); };
+  const double k_time = k_n * kDkvUnit + kFixed;
+  Gradients best{Cut{(int)q_blocks(kQueries), 1, kQueries, q_blocks(kQueries), 0.0}, Cut{(int)k_blocks, 1, kKeys, k_blocks, 0.0},
+                 k_time > q_n * kDqUnit + kFixed, 1e300};
+  if (best.q.blocks + k_blocks > 32 * kCUs) return best;   // the last round is little of it
+  auto consider = [&](const Cut& q, const Cut& k) {
+    const double unit = q.tile == kQueries ? kDqUnit : kDqUnit192;
+    const double join = q.cuts() + k.cuts() == 0 ? 0.0
+                                                 : kJoin + join_time(q.cuts(), std::min(A.queries, q.tile)) +
+                                                       join_time(k.cuts(), 2 * std::min(A.keys, kKeys));
+    const double q_time = (q_n + q.splits - 1) / q.splits * unit + kFixed, cut_time = (k_n + k.splits - 1) / k.splits * kDkvUnit + kFixed;
+    const double work = q.grid() * q_time + k.whole * k_time + k.cuts() * cut_time;
+    if (std::max(work / kCUs, std::max(q_time, k.whole ? k_time : cut_time)) + join >= best.time) return;
+    for (const bool k_first : {false, true}) {
+      Schedule s;
+      if (!k_first) s.run(q.grid(), q_time);
+      s.run(k.whole, k_time);
+      s.run(k.cuts(), cut_time);
+      if (k_first) s.run(q.grid(), q_time);
+      if (s.end() + join < best.time) best = Gradients{q, k, k_first, s.end() + join};
+    }
+  };
+  for (const int tile : {kQueries, 192})
+    for (const int sq : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      const int64_t blocks = q_blocks(tile);
+      if (sq > 1 && (4 * sq > q_n || blocks * sq > 2 * kCUs)) break;
+      const Cut q{sq == 1 ? (int)blocks : 0, sq, tile, blocks, 0.0};
+      consider(q, Cut{(int)k_blocks, 1, kKeys, k_blocks, 0.0});
+      for (const int sk : {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+        if (4 * sk > k_n) break;
+        if (k_blocks * sk <= 4 * kCUs) consider(q, Cut{0, sk, kKeys, k_blocks, 0.0});
+        for (const int rest : {16, 32, 64, 96, 128, 192, 256})
+          if (rest < k_blocks) consider(q, Cut{(int)k_blocks - rest, sk, kKeys, k_blocks, 0.0});
+      }
+    }
+  return best;
 }
-void use_cut(Args& A, const Cut& cut, uint8_t* workspace) {
-  A.whole = cut.whole;
-  A.splits = cut.splits;
-  A.tile = cut.tile;
-  A.part = reinterpret_cast<float*>(workspace);
-  A.part_top = A.part + cut.cuts() * kQueries * kD;
+
+// The search takes up to 25 us, and a call plans twice; a thread keeps what it found for the last shapes.
+Gradients plan_gradients(const Args& A) {
+  struct Found {
+    int sizes[5];
+    Gradients plan;
+  };
+  constexpr int kFound = 32;
+  static thread_local Found found[kFound];   // batch 0: none
+  const int sizes[5] = {A.batch, A.heads, A.kv_heads, A.queries, A.keys};
+  uint32_t hash = 0;
+  for (const int x : sizes) hash = hash * 2654435761u + (uint32_t)x;
+  Found& f = found[(hash >> 16) % kFound];
+  if (!std::equal(sizes, sizes + 5, f.sizes)) {
+    f.plan = search_gradients(A);
+    std::copy(sizes, sizes + 5, f.sizes);
+  }
+  return f.plan;
 }
 
 bool sizes_ok(int batch, int heads, int kv_heads, int queries, int keys) {
@@ -1269,7 +1408,7 @@ Args sizes(int batch, int heads, int kv_heads, int queries, int keys) {
   return A;
 }
 
-int64_t join_grid(const Cut& cut) { return (cut.blocks - cut.whole) * (kQueries / 8); }
+int64_t join_blocks(const Cut& cut) { return cut.splits > 1 ? cut.blocks - cut.whole : 0; }
 
 template <typename T>
 void forward(const Args& A, const Cut& cut, hipStream_t s) {
@@ -1281,28 +1420,30 @@ void forward(const Args& A, const Cut& cut, hipStream_t s) {
     if (A.lse) attention_kernel<T, false, true><<<grid, kThreads, 0, s>>>(A);
     else attention_kernel<T, false, false><<<grid, kThreads, 0, s>>>(A);
   }
-  if (cut.splits == 1) return;
-  if (A.lse) attention_join_kernel<T, kJoinO, true><<<(unsigned)join_grid(cut), 256, 0, s>>>(A);
-  else attention_join_kernel<T, kJoinO, false><<<(unsigned)join_grid(cut), 256, 0, s>>>(A);
+  const int joined = (int)join_blocks(cut);
+  if (!joined) return;
+  const dim3 join((unsigned)(joined * (kQueries / 8)));
+  if (A.lse) attention_join_kernel<T, true, true><<<join, 256, 0, s>>>(A, joined);
+  else attention_join_kernel<T, true, false><<<join, 256, 0, s>>>(A, joined);
 }
 
 template <typename T>
-void backward(Args& A, uint8_t* workspace, hipStream_t s) {
-  const Cut q = dq_cut(A), k = dkv_cut(A);
-  use_cut(A, q, workspace);
-  if (A.mask.bits) attention_dq_kernel<T, true><<<(unsigned)q.grid(), kThreads, 0, s>>>(A);
-  else attention_dq_kernel<T, false><<<(unsigned)q.grid(), kThreads, 0, s>>>(A);
-  if (q.splits > 1) attention_join_kernel<T, kJoinDq, false><<<(unsigned)join_grid(q), 256, 0, s>>>(A);
-  use_cut(A, k, workspace);   // the kernels run one after the other: dq's partial sums have been read
-  attention_dkv_kernel<T><<<(unsigned)k.grid(), kThreads, 0, s>>>(A);
-  if (k.splits > 1) attention_join_kernel<T, kJoinDkv, false><<<(unsigned)join_grid(k), 256, 0, s>>>(A);
+void backward(const MaskBytes& mask, const Args& A, const Gradients& plan, hipStream_t s) {
+  const int64_t units = (int64_t)A.batch * A.heads * A.q_units + 1;
+  const dim3 prepare((unsigned)((mask.mask ? A.batch : 0) + (units + 3) / 4));
+  attention_prepare_kernel<T><<<prepare, 64 * kPlanWaves, 0, s>>>(mask, A);
+  const dim3 grid((unsigned)(plan.q.grid() + plan.k.grid()));
+  if (A.mask.bits) attention_backward_kernel<T, true><<<grid, kThreads, 0, s>>>(A);
+  else attention_backward_kernel<T, false><<<grid, kThreads, 0, s>>>(A);
+  const int q = (int)join_blocks(plan.q), k = (int)join_blocks(plan.k);
+  if (q + k) attention_join_kernel<T, false, false><<<(unsigned)((q + k) * (kQueries / 8)), 256, 0, s>>>(A, q);
 }
 
 int64_t workspace_of(const Args& A, bool masked, bool backward) {
   if (A.batch == 0 || A.queries == 0 || (A.keys == 0 && backward)) return 0;
   const int64_t mask = masked ? mask_bytes(A.batch, A.keys) : 0;
   if (!backward) return mask + forward_cut(A).bytes();
-  return mask + stats_bytes(A.batch, A.heads, A.queries) + std::max(dq_cut(A).bytes(), dkv_cut(A).bytes());
+  return mask + stats_bytes(A.batch, A.heads, A.queries) + plan_gradients(A).bytes();
 }
 
 }  // namespace
@@ -1342,9 +1483,11 @@ extern "C" int flk_attention(const void* q, const int64_t* q_strides, const void
   A.low = low;
   A.lse = lse;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (const int st = plan_mask(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace), s)) return st;
+  const MaskBytes mask = mask_in(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace));
+  if (mask.mask) attention_mask_kernel<<<batch, 64 * kPlanWaves, 0, s>>>(mask, keys, A.k_units);
   const Cut cut = forward_cut(A);
-  use_cut(A, cut, static_cast<uint8_t*>(workspace) + (key_mask ? mask_bytes(batch, keys) : 0));
+  A.of_q = cut.in(static_cast<uint8_t*>(workspace) + (key_mask ? mask_bytes(batch, keys) : 0));
+  A.part_top = A.of_q.part + cut.cuts() * kQueries * kD;
   if (dtype == FLK_BF16) forward<__bf16>(A, cut, s);
   else forward<_Float16>(A, cut, s);
   return flk_launch_status();
@@ -1386,9 +1529,14 @@ extern "C" int flk_attention_backward(const void* d_o, const int64_t* d_o_stride
   A.lse = const_cast<float*>(lse);
   A.stats = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + of_mask);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (const int st = plan_mask(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace), s)) return st;
+  const MaskBytes mask = mask_in(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace));
+  const Gradients plan = plan_gradients(A);
   uint8_t* parts = reinterpret_cast<uint8_t*>(A.stats) + stats_bytes(batch, heads, queries);
-  if (dtype == FLK_BF16) backward<__bf16>(A, parts, s);
-  else backward<_Float16>(A, parts, s);
+  A.of_q = plan.q.in(parts);
+  A.of_k = plan.k.in(parts + plan.q.bytes());
+  A.q_grid = (int)plan.q.grid();
+  A.k_first = plan.k_first;
+  if (dtype == FLK_BF16) backward<__bf16>(mask, A, plan, s);
+  else backward<_Float16>(mask, A, plan, s);
   return flk_launch_status();
 }
