@@ -236,13 +236,17 @@ __device__ __forceinline__ void clear_rows(uint8_t* slot, uint32_t bits) {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// What the accumulators of a unit's S start from: 0, -inf for the rows (keys) that `bits` leaves out.
-__device__ __forceinline__ f32x4 bias_of(uint32_t bits, int kt) {
-  const uint32_t mine = bits >> (16 * kt + (threadIdx.x >> 4 & 3) * 4);
-  f32x4 x;
+// S of the keys that `bits` leaves out of a unit's accumulators (group, 16-key tile): -inf.
+template <int N>
+__device__ __forceinline__ void leave_out(f32x4 (&s)[N], uint32_t bits) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = mine >> i & 1 ? 0.0f : -INFINITY;
-  return x;
+  for (int kt = 0; kt < 2; ++kt) {
+    const uint32_t mine = bits >> (16 * kt + (threadIdx.x >> 4 & 3) * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int g = 0; g < N / 2; ++g) s[2 * g + kt][i] = mine >> i & 1 ? s[2 * g + kt][i] : -INFINITY;
+  }
 }
 
 // The key units of a batch entry that have kept keys, asked for one after the other from 0; past the last: the last one with
@@ -388,10 +392,10 @@ __device__ __forceinline__ void elements(int n, Scaled&& scaled, Exp&& exp, Put&
 }
 
 // Phase u: S(u+1) = K(u+1) Q^T and O^T += V(u-1)^T P(u-1)^T on the matrix pipe while the vector units turn S(u) into P(u).
-template <bool kBias, bool kKeep, typename T, int G, typename Hook>
+template <bool kPartial, bool kKeep, typename T, int G, typename Hook>
 __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_cur)[2 * G], f32x4 (&s_next)[2 * G],
                                               const uint32_t (&p_prev)[4 * G], uint32_t (&p_cur)[4 * G], const uint8_t* k_unit,
-                                              const uint8_t* v_unit, const uint8_t* k_after, uint32_t bits_next,
+                                              const uint8_t* v_unit, const uint8_t* k_after, uint32_t bits,
                                               Hook&& hook) {
   f32x4 sv[2 * G];
 #pragma unroll
@@ -399,13 +403,8 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
     sv[i] = s_cur[i];
     asm volatile("" : "+v"(sv[i]));
   }
-  f32x4 start[2] = {};
-  if constexpr (kBias) {
-    if (bits_next != ~0u) {
-      start[0] = bias_of(bits_next, 0);
-      start[1] = bias_of(bits_next, 1);
-    }
-  }
+  if constexpr (kPartial)
+    if (bits != ~0u) leave_out(sv, bits);
   constexpr int kElems = 8 * G;   // of a lane: one a slot, every other slot with one group
   constexpr bool kBits = kShift<T> != 0.0f;
   float t[kElems], e[kElems], high = -INFINITY, sum[G] = {};
@@ -433,7 +432,7 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
       const int st = n >> 1, kt = n & 1;
 #pragma unroll
       for (int g = 0; g < G; ++g)
-        s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : kBias ? start[kt] : f32x4{});
+        s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : f32x4{});
     } else {
 #pragma unroll
       for (int g = 0; g < G; ++g) w.acc[n - 8][g] = mfma(a, pb[g], w.acc[n - 8][g]);
@@ -543,40 +542,39 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
       uint32_t p0[4 * G], p1[4 * G] = {};
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const f32x4 start = bias_of(bits[0], kt);
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
           const vec8<T> a = row_operand<T>(k_slot(0), w.at, st, kt);
 #pragma unroll
-          for (int g = 0; g < G; ++g) s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : start);
+          for (int g = 0; g < G; ++g) s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : f32x4{});
         }
       }
 #pragma unroll
       for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
       __syncthreads();   // K(0) has been read: iteration 0 copies K(4) over it
       // r: u's place in the rings; a literal in the unrolled loop, where LDS addresses are then a lane's constants
-      auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[2 * G], f32x4(&s_next)[2 * G], const uint32_t(&p_prev)[4 * G],
+      auto iteration = [&](auto partial, int u, int r, const f32x4(&s_cur)[2 * G], f32x4(&s_next)[2 * G], const uint32_t(&p_prev)[4 * G],
                            uint32_t(&p_cur)[4 * G]) __attribute__((always_inline)) {
-        constexpr bool kBias = decltype(bias)::value, kAhead = !kMasked && !kBias;
+        constexpr bool kPartial = decltype(partial)::value, kAhead = !kMasked && !kPartial;
         if constexpr (!kAhead) units.look(u, unit, bits);
-        forward_phase<kBias, kKeep>(w, s_cur, s_next, p_prev, p_cur, k_slot(r + 1), v_slot(r - 1), k_slot(r + 2), bits[1],
+        forward_phase<kPartial, kKeep>(w, s_cur, s_next, p_prev, p_cur, k_slot(r + 1), v_slot(r - 1), k_slot(r + 2), bits[0],
                                     [&](int slot) {
                                       if (slot == 1) kc.start<kAhead>(k_lds(r), kAhead ? units.first + u + 4 : unit[4]);
                                       if (slot == 3) vc.start<kAhead>(v_lds(r + 2), kAhead ? units.first + u + 2 : unit[2]);
                                     });
         landed<2>();
-        if constexpr (kBias) {
+        if constexpr (kPartial) {
           clear_rows(k_slot(r + 3), bits[3]);
           clear_rows(v_slot(r + 1), bits[1]);
         }
         barrier();
         if constexpr (kMasked) units.shift(unit, bits);
       };
-      auto turn = [&](auto bias, int u) __attribute__((always_inline)) {
-        iteration(bias, u, 0, s0, s1, p1, p0);
-        iteration(bias, u + 1, 1, s1, s0, p0, p1);
-        iteration(bias, u + 2, 2, s0, s1, p1, p0);
-        iteration(bias, u + 3, 3, s1, s0, p0, p1);
+      auto turn = [&](auto partial, int u) __attribute__((always_inline)) {
+        iteration(partial, u, 0, s0, s1, p1, p0);
+        iteration(partial, u + 1, 1, s1, s0, p0, p1);
+        iteration(partial, u + 2, 2, s0, s1, p1, p0);
+        iteration(partial, u + 3, 3, s1, s0, p0, p1);
       };
       int u = 0;
       // the last unit is out of reach of what a turn copies, clears and starts from
@@ -611,8 +609,8 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
             l > 0.0f ? w.top[g] + (__builtin_amdgcn_logf(sum) + kShift<T>) * kLn2 : -INFINITY;
     }
   }
-  T* low = kKeep ? static_cast<T*>(A.low) : nullptr;
-  if (low) low += ((int64_t)b * A.queries * A.heads + h) * kD;
+  T* low = nullptr;
+  if constexpr (kKeep) low = static_cast<T*>(A.low) + ((int64_t)b * A.queries * A.heads + h) * kD;
   store_rows<T>(w.acc, scale, A.o.at<T>(b, h), A.o.row, q0, end, low, (int64_t)A.heads * kD);
 }
 
@@ -637,11 +635,11 @@ struct Dq {
 };
 
 // Phase u: S(u+1) = K(u+1) Q^T, dP(u+1) = V(u+1) dO^T and dQ^T += K(u-1)^T dS(u-1)^T, while dS(u) is formed.
-template <bool kBias, typename T, int G, typename Hook>
+template <bool kPartial, typename T, int G, typename Hook>
 __device__ __forceinline__ void dq_phase(Dq<T, G>& w, const f32x4 (&s_cur)[2 * G], const f32x4 (&d_cur)[2 * G],
                                          f32x4 (&s_next)[2 * G], f32x4 (&d_next)[2 * G], const uint32_t (&p_prev)[4 * G],
                                          uint32_t (&p_cur)[4 * G], const uint8_t* k_unit, const uint8_t* v_unit,
-                                         const uint8_t* k_before, const uint8_t* k_after, uint32_t bits_next,
+                                         const uint8_t* k_before, const uint8_t* k_after, uint32_t bits,
                                          Hook&& hook) {
   f32x4 sv[2 * G], dv[2 * G];
 #pragma unroll
@@ -650,13 +648,8 @@ __device__ __forceinline__ void dq_phase(Dq<T, G>& w, const f32x4 (&s_cur)[2 * G
     dv[i] = d_cur[i];
     asm volatile("" : "+v"(sv[i]), "+v"(dv[i]));
   }
-  f32x4 start[2] = {};
-  if constexpr (kBias) {
-    if (bits_next != ~0u) {
-      start[0] = bias_of(bits_next, 0);
-      start[1] = bias_of(bits_next, 1);
-    }
-  }
+  if constexpr (kPartial)
+    if (bits != ~0u) leave_out(sv, bits);
   float t[8 * G], e[8 * G];
   auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, w.lse[n >> 3]); };
   auto exp = [&](int n) { e[n] = __builtin_amdgcn_exp2f(t[n]); };
@@ -678,7 +671,7 @@ __device__ __forceinline__ void dq_phase(Dq<T, G>& w, const f32x4 (&s_cur)[2 * G
     const int st = (n & 7) >> 1, kt = n & 1;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      if (n < 8) s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : kBias ? start[kt] : f32x4{});
+      if (n < 8) s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : f32x4{});
       else if (n < 16) d_next[2 * g + kt] = mfma(a, w.g[st][g], st ? d_next[2 * g + kt] : f32x4{});
       else w.acc[n - 16][g] = mfma(a, pb[g], w.acc[n - 16][g]);
     }
@@ -744,13 +737,12 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
     uint32_t p0[4 * G], p1[4 * G] = {};
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const f32x4 start = bias_of(bits[0], kt);
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         const vec8<T> a = row_operand<T>(k_slot(0), w.at, st, kt), c = row_operand<T>(v_slot(0), w.at, st, kt);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : start);
+          s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : f32x4{});
           d0[2 * g + kt] = mfma(c, w.g[st][g], st ? d0[2 * g + kt] : f32x4{});
         }
       }
@@ -759,29 +751,29 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
     for (int m = 0; m < kLead; ++m) w.ops[m] = row_operand<T>(k_slot(1), w.at, m >> 1, m & 1);
     __syncthreads();   // V(0) has been read: iteration 0 copies V(3) over it
     // r: u's place in K's ring
-    auto iteration = [&](auto bias, int u, int r, const f32x4(&s_cur)[2 * G], const f32x4(&d_cur)[2 * G],
+    auto iteration = [&](auto partial, int u, int r, const f32x4(&s_cur)[2 * G], const f32x4(&d_cur)[2 * G],
                          f32x4(&s_next)[2 * G],
                          f32x4(&d_next)[2 * G], const uint32_t(&p_prev)[4 * G], uint32_t(&p_cur)[4 * G]) __attribute__((always_inline)) {
-      constexpr bool kBias = decltype(bias)::value, kAhead = !kMasked && !kBias;
+      constexpr bool kPartial = decltype(partial)::value, kAhead = !kMasked && !kPartial;
       if constexpr (!kAhead) units.look(u, unit, bits);
-      dq_phase<kBias>(w, s_cur, d_cur, s_next, d_next, p_prev, p_cur, k_slot(r + 1), v_slot(r + 1), k_slot(r + 5),
-                      k_slot(r + 2), bits[1], [&](int slot) {
+      dq_phase<kPartial>(w, s_cur, d_cur, s_next, d_next, p_prev, p_cur, k_slot(r + 1), v_slot(r + 1), k_slot(r + 5),
+                      k_slot(r + 2), bits[0], [&](int slot) {
                         if (slot == 1) kc.start<kAhead>(k_lds(r + 4), kAhead ? units.first + u + 4 : unit[4]);
                         if (slot == 3) vc.start<kAhead>(v_lds(r), kAhead ? units.first + u + 3 : unit[3]);
                       });
       landed<2>();
-      if constexpr (kBias) {
+      if constexpr (kPartial) {
         clear_rows(k_slot(r + 3), bits[3]);
         clear_rows(v_slot(r + 2), bits[2]);
       }
       barrier();
       if constexpr (kMasked) units.shift(unit, bits);
     };
-    auto turn = [&](auto bias, int u) __attribute__((always_inline)) {
+    auto turn = [&](auto partial, int u) __attribute__((always_inline)) {
 #pragma unroll
       for (int r = 0; r < kDqKRing; r += 2) {
-        iteration(bias, u + r, r, s0, d0, s1, d1, p1, p0);
-        iteration(bias, u + r + 1, r + 1, s1, d1, s0, d0, p0, p1);
+        iteration(partial, u + r, r, s0, d0, s1, d1, p1, p0);
+        iteration(partial, u + r + 1, r + 1, s1, d1, s0, d0, p0, p1);
       }
     };
     int u = 0, r = 0;
@@ -1111,14 +1103,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q
       if (lane == 0)
         A.lse[(int64_t)bh * A.queries + row] =
             l > 0.0f ? top + (__builtin_amdgcn_logf(sum) + kShift<T>) * kLn2 : -INFINITY;
-      T* low = static_cast<T*>(A.low);
-      if (low) {
-        float y[4];
+      float y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = x[i] - (float)(T)x[i];
-        low += (((int64_t)b * A.queries + row) * A.heads + h) * kD + lane * 4;
-        *reinterpret_cast<uint2*>(low) = make_uint2(pack<T>(y[0], y[1]), pack<T>(y[2], y[3]));
-      }
+      for (int i = 0; i < 4; ++i) y[i] = x[i] - (float)(T)x[i];
+      T* low = static_cast<T*>(A.low) + (((int64_t)b * A.queries + row) * A.heads + h) * kD + lane * 4;
+      *reinterpret_cast<uint2*>(low) = make_uint2(pack<T>(y[0], y[1]), pack<T>(y[2], y[3]));
     }
   } else {
 #pragma unroll 4
@@ -1474,6 +1463,7 @@ extern "C" int flk_attention(const void* q, const int64_t* q_strides, const void
     A.k = tensor(k, k_strides);
     A.v = tensor(v, v_strides);
   }
+  if (!low != !lse) return FLK_E_INVALID;
   if (!flk_host_aligned(low, 16) || !flk_host_aligned(lse, 4)) return FLK_E_ALIGN;
   const int64_t need = workspace_of(A, key_mask, false);
   if (need && (!workspace || workspace_bytes < need)) return FLK_E_SCRATCH;

@@ -536,8 +536,9 @@ int flk_mlp_matmul(const void* a, int64_t a_row_stride, int a_transposed, const 
  *   key_mask (batch, keys) bytes, not zero where the key is kept, or NULL: all are.  What k and v hold
  *            elsewhere is not read into any result, whatever it is
  *   o        (batch, heads, queries, head_dim); 0 for a query that keeps no key
- *   low      o's rounding error in its own type, (batch, queries, heads, head_dim), dense, or NULL
- *   lse      (batch, heads, queries) float32, log sum exp of each row (-inf for one without keys), or NULL
+ *   low      o's rounding error in its own type, (batch, queries, heads, head_dim), dense, and
+ *   lse      (batch, heads, queries) float32, log sum exp of each row (-inf for one without keys): for the
+ *            gradients, both or (NULL) neither
  * head_dim is 128 (else FLK_E_UNSUPPORTED); queries and keys at most 2^28, and batch * heads * queries and
  * batch * kv_heads * keys (lengths rounded up to 32) at most 2^27 (else FLK_E_INVALID).  `workspace` (256-byte
  * aligned; the plan's bytes for the same sizes, `masked` whether there is a mask) is free again when the

@@ -90,7 +90,8 @@ def test_forward_validation(lib):
                dict(o=None), dict(qs=None), dict(ks=_strides(0, 0, 2 ** 25 + 8)), dict(vs=_strides(0, 0, -128))):
         assert _forward(lib, **kw) == INVALID, kw
     assert _forward(lib, d=64) == UNSUPPORTED
-    for kw in (dict(q=P + 8), dict(k=P + 2), dict(o=P + 4), dict(low=P + 8), dict(lse=P + 2), dict(qs=_strides(0, 1280, 132)),
+    assert _forward(lib, low=P) == INVALID and _forward(lib, lse=P) == INVALID
+    for kw in (dict(q=P + 8), dict(k=P + 2), dict(o=P + 4), dict(low=P + 8, lse=P), dict(low=P, lse=P + 2), dict(qs=_strides(0, 1280, 132)),
                dict(os=_strides(4, 128, 256))):
         assert _forward(lib, **kw) == ALIGN, kw
     assert _forward(lib, mask=P) == SCRATCH

@@ -211,6 +211,9 @@ def test_strided_operands(device):
     assert all(torch.equal(a, b) for a, b in zip(A.attention_backward(do, *views, kept2, key_mask=masks[:, 1, :70]), want))
     odd = torch.empty(2, 3, 70, D + 3, dtype=q.dtype, device=device)[..., :D].copy_(q)
     assert torch.equal(A.attention(odd, k, v, key_mask=keep), o)
+    far = torch.zeros(70, 2 ** 25 + 8, dtype=q.dtype, device=device)[:, :D].view(1, 1, 70, D).copy_(q[:1, :1])   # copied
+    assert torch.equal(A.attention(far, k[:1, :1], v[:1, :1], key_mask=keep[:1]),
+                       A.attention(q[:1, :1], k[:1, :1], v[:1, :1], key_mask=keep[:1]))
     every = do.repeat(1, 1, 2)[..., ::2]
     assert all(torch.equal(a, b) for a, b in zip(A.attention_backward(every, q, k, v, kept, key_mask=keep),
                                                  A.attention_backward(every.contiguous(), q, k, v, kept, key_mask=keep)))
