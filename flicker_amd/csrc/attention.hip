@@ -906,7 +906,7 @@ struct Queries {
   }
 };
 
-template <bool kSecond, typename T>
+template <bool kSecond, bool kGrouped, typename T>
 __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Piece& piece, int b, int h, int first, int k0,
                                          bool any) {
   const int lane = threadIdx.x & 63, pair = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
@@ -999,14 +999,15 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
       barrier();
     };
     int u = 0;
-    // a turn copies kQRing units from qs.unit and os.unit on, none a head's last (qs may be in the next head already), and the
-    // stats of up to u + kQRing + 2, all below n: the stats of units from n on are `none`
-    const int inside = min(A.q_units - max(qs.unit, os.unit), n - 2) - kQRing, end = inside > 0 ? inside : 0;
+    // A turn copies kQRing units from qs.unit and os.unit on, none a head's last, and the stats of up to u + kQRing + 2, all
+    // below n (those of units from n on are `none`); where heads share the keys a turn may pass from one to the next.
+    const int inside = kGrouped ? n + 3 - kQRing : min(A.q_units - max(qs.unit, os.unit), n - 2) - kQRing;
+    const int end = inside > 0 ? inside : 0;
     for (; u < end; u += kQRing)
 #pragma unroll
       for (int r = 0; r < kQRing; r += 2) {
-        iteration(std::true_type{}, u + r, r, s0, s1, p1, p0);
-        iteration(std::true_type{}, u + r + 1, r + 1, s1, s0, p0, p1);
+        iteration(std::bool_constant<!kGrouped>{}, u + r, r, s0, s1, p1, p0);
+        iteration(std::bool_constant<!kGrouped>{}, u + r + 1, r + 1, s1, s0, p0, p1);
       }
     for (; u < n + 2; u += 2) {   // the second wave's last unit goes into dK at u = n + 1
       iteration(std::false_type{}, u, u, s0, s1, p1, p0);
@@ -1029,7 +1030,7 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
 }
 
 // All gradients: blocks of queries and blocks of keys in one launch, so that neither kind's last round leaves CUs idle.
-template <typename T, bool kMasked>
+template <typename T, bool kMasked, bool kGrouped>   // kGrouped: query heads share key heads
 __global__ __launch_bounds__(kThreads, 2) void attention_backward_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kDkvBytes];
   static_assert(kDkvBytes >= (kDqKRing + kDqVRing) * kUnitBytes);
@@ -1050,8 +1051,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_kernel(const A
   bool any = false;
   for (int u = first / kUnit; u < min(A.k_units, (first + kKeys) / kUnit); ++u) any |= kept(A, b, u) != 0;
   const int k0 = first + (wave & 3) * 32;
-  if (wave < 4) dkv_wave<false, T>(A, smem, piece, b, h, first, k0, any);
-  else dkv_wave<true, T>(A, smem, piece, b, h, first, k0, any);
+  if (wave < 4) dkv_wave<false, kGrouped, T>(A, smem, piece, b, h, first, k0, any);
+  else dkv_wave<true, kGrouped, T>(A, smem, piece, b, h, first, k0, any);
 }
 
 // Adds the cuts' partial sums in order: 32 lanes a row, 8 rows of a cut block a block.  kOf: of o, or of the gradients, the
@@ -1422,8 +1423,13 @@ void backward(const MaskBytes& mask, const Args& A, const Gradients& plan, hipSt
   const dim3 prepare((unsigned)((mask.mask ? A.batch : 0) + (units + 3) / 4));
   attention_prepare_kernel<T><<<prepare, 64 * kPlanWaves, 0, s>>>(mask, A);
   const dim3 grid((unsigned)(plan.q.grid() + plan.k.grid()));
-  if (A.mask.bits) attention_backward_kernel<T, true><<<grid, kThreads, 0, s>>>(A);
-  else attention_backward_kernel<T, false><<<grid, kThreads, 0, s>>>(A);
+  if (A.mask.bits) {
+    if (A.group > 1) attention_backward_kernel<T, true, true><<<grid, kThreads, 0, s>>>(A);
+    else attention_backward_kernel<T, true, false><<<grid, kThreads, 0, s>>>(A);
+  } else {
+    if (A.group > 1) attention_backward_kernel<T, false, true><<<grid, kThreads, 0, s>>>(A);
+    else attention_backward_kernel<T, false, false><<<grid, kThreads, 0, s>>>(A);
+  }
   const int q = (int)join_blocks(plan.q), k = (int)join_blocks(plan.k);
   if (q + k) attention_join_kernel<T, false, false><<<(unsigned)((q + k) * (kQueries / 8)), 256, 0, s>>>(A, q);
 }
