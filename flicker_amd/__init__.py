@@ -3,9 +3,10 @@
   kernels   Freqs, row_tile, lane_pair, qk_prep, logit_bound, attend   (src/flicker/kernels.py)
   rope      img_ids, txt_ids, embed_nd, rope_freqs, rope_lanes           (src/flicker/rope.py)
   modules   heads, merge_heads, qkv_prep, double/single block attention (src/flicker/modules.py)
-  norm      layer_norm, modulate and their gradients                     (src/flicker/nn.py, modules.py)
+  attention any logits, lengths and masks over the keys, with gradients  (src/flicker/kernels.py, modules.py)
+  norm      layer_norm, modulate, residual_modulate and their gradients  (src/flicker/nn.py, modules.py)
   mlp       swiglu, gated_mlp and their gradients                        (src/flicker/modules.py)
-  autograd  norm's and mlp's functions under torch's autograd
+  autograd  norm's, mlp's and attention's functions and qk_prep under torch's autograd
   loader    check_logit_bound                                            (src/flicker/loader.py)
   workloads seeded synthetic Klein attention inputs
 

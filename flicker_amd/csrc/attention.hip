@@ -1,4 +1,4 @@
-// attention: softmax(q k^T) v of any lengths, with the keys that a mask keeps, and its gradients.
+// attention: softmax(q k^T) v of any lengths, over the keys that a mask keeps, and its gradients.
 //
 // Per (b, h) and query i, over the kept keys j of key head h / (heads / kv_heads); q comes scaled:
 //   S_ij = q_i . k_j,  lse_i = log sum_j exp S_ij,  P_ij = exp(S_ij - lse_i),  o_i = sum_j P_ij v_j
@@ -7,6 +7,45 @@
 //   dq_i = sum_j dS_ij k_j,  dk_j = sum_i dS_ij q_i,  dv_j = sum_i P_ij g_i
 // (dk and dv also over the query heads that share the key head).  A query that keeps no key has o = 0, lse = -inf and
 // no gradient.
+//
+// The products run on the 16x16x32 matrix instructions, whose accumulators hold a lane's four rows of one column.  Every
+// product is laid out so that what one leaves is what the next takes: with keys as rows, S^T = K Q^T leaves a lane P of one
+// query and 4 + 4 keys of a 32-key unit, packed the right operand of O^T += V^T P^T; with queries as rows, S = Q K^T leaves
+// it P of one key and 4 + 4 queries, the right operand of dV^T += dO^T P.  So P and dS never pass through LDS to be
+// turned, and a wave keeps its own 32 rows (Q and dO; or K, or V) as right operands in registers.  Left operands come from
+// LDS: rows as they are (b128), columns through the transposing b64 read, both conflict-free by the swizzle below.
+//
+// LDS holds rings of 32-row units, filled by copies straight from memory that were started phases earlier.  A phase is 16
+// or 24 slots of two matrix instructions on one left operand, read four slots before; between them, one element a slot,
+// the vector units turn the last unit's S into P.  Loops are unrolled over the rings, which makes LDS addresses constants
+// of a lane (4608 tokens: 249 -> 240 us forwards, 880 -> 790 backwards).
+//
+// The running maximum is one that lags: P are taken against the maximum of an earlier unit until one passes a limit, and
+// only then is what has been summed scaled and the unit's P formed again, after the fact (a check before each unit's
+// exponents sat ahead of its matrix work: 265 -> 249).  l, the sum that divides o, is of the rounded P (two more matrix
+// instructions with a row of ones); lse is of the unrounded, added up in float32.
+//
+// Gradients take 7 products where 5 would do: dq has blocks of queries, dk and dv blocks of keys, and both form S and dP.
+// Sharing them would mean 4 bytes of dq added to memory per key block and query and d, 2 GB at 4608 tokens and 24 heads,
+// in an order that timing decides; the two products cost 0.2 ms there.  In a block of 128 keys pairs of waves share 32: one
+// holds K and dV, forms S and P and leaves P (float32) in LDS for the other, which holds V and dK and forms dP and dS a unit
+// later.  One wave with all four would need 320 registers at two waves a SIMD.  delta needs o closer
+// than its type holds it where few keys carry a row (at two keys its rounding would cost dq, by estimate, twice all else),
+// so the forward pass keeps what o's rounding left.
+//
+// Masks: bytes become one word of bits a unit and a list of the units that keep any (attention_mask_kernel), and blocks
+// walk that list.  In a unit that keeps part, the rows left out are cleared in LDS before anyone reads them (0 * inf), and
+// their S set to -inf.
+//
+// Blocks that would leave CUs idle are cut along the units they walk, and a second kernel adds the float32 partial sums up in
+// order; which and how many is estimated from a unit's time (plan_cut, search_gradients).  The gradients' two kinds of
+// blocks share a launch, so that neither's last round leaves CUs idle (1536 tokens, forward and gradients: 172 -> 153 us).
+//
+// Bound: the matrix pipe, and over whole rounds of blocks the chip's power: random operands hold it there, where a large
+// library product reaches 1.24 PFLOP/s.  Measured at 24 heads in bfloat16, PFLOP/s over all products that run: forward
+// 4608 tokens 230 us (1.13), 16896 2.66 ms (1.32), with what the gradients need 250 us and 2.82 ms; gradients 730 us
+// (1.25) and 9.4 ms (1.30), of which 14 and 63 us are the rows' stats.  1536 tokens are 144 blocks of queries for 256 CUs:
+// 50 us and 120.  One query on 4608 keys: 15 us for 57 MB, and 5 for the join.
 
 #include <algorithm>
 #include <type_traits>
@@ -22,7 +61,7 @@ constexpr int kUnitBytes = kUnit * kRowBytes;
 constexpr int kWaves = 8;              // two a SIMD
 constexpr int kThreads = 64 * kWaves;
 constexpr int kQueries = 32 * kWaves;  // queries of a block, 32 a wave
-constexpr int kKeys = 16 * kWaves;     // keys of a block of attention_dkv_kernel, 32 a pair of waves
+constexpr int kKeys = 16 * kWaves;     // keys of a block, 32 a pair of waves
 constexpr int kLead = 4;               // slots between an operand's LDS read and its MFMAs
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int64_t kMaxItems = 1LL << 31;
@@ -138,8 +177,8 @@ struct Piece {
   __device__ __forceinline__ int count(int n) const { return n / splits + (split < n % splits); }
 };
 
-// A wave's queries in a block of of_q.tile: 256, 32 a wave, or 192, of which the waves 4-7 take 16 each, so that every SIMD holds
-// 48.
+// A wave's queries in a block of of_q.tile: 256, 32 a wave, or 192, of which the waves 4-7 take 16 each, so that every
+// SIMD holds 48.
 struct Rows {
   int b, h, first, end, q0;
   bool wide;
@@ -485,8 +524,8 @@ constexpr int kKRing = 4, kVRing = 4;   // forward: units of K and of V in LDS
 
 // One wave's 16 G queries from q0, of a block's `first` .. `end` - 1.
 template <typename T, bool kMasked, bool kKeep, int G>
-__device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const Piece& piece, int b, int h, int first, int end,
-                                             int q0) {
+__device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const Piece& piece, int b, int h, int first,
+                                             int end, int q0) {
   const int lane = threadIdx.x & 63, h4 = lane >> 4, bh = b * A.heads + h;
   Units<kMasked> units(A, b, piece);
   const int n = units.n;
@@ -614,6 +653,9 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
   store_rows<T>(w.acc, scale, A.o.at<T>(b, h), A.o.row, q0, end, low, (int64_t)A.heads * kD);
 }
 
+// o of 256 or 192 queries: 32 a wave rather than 64, which leaves a SIMD two waves, whose phases fill each other's gaps; all
+// eight read the same K and V units, so LDS is read once per 256 queries x 32 keys.  What kKeep adds: 16 additions a lane and
+// phase for lse, and o's second store (4608 tokens: 230 -> 250 us).
 template <typename T, bool kMasked, bool kKeep>
 __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[(kKRing + kVRing) * kUnitBytes];
@@ -795,8 +837,8 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
   store_rows<T>(w.acc, one, A.dq.at<T>(b, h), A.dq.row, q0, end);
 }
 
-// dk and dv of 128 keys, 32 a pair of waves: the first holds K^T and dV^T, forms S and P and hands P on through LDS, the second holds
-// V^T and dK^T, forms dP and dS one unit later.
+// dk and dv of 128 keys, 32 a pair of waves: the first holds K^T and dV^T, forms S and P and hands P on through LDS, the
+// second holds V^T and dK^T, forms dP and dS one unit later.
 template <typename T>
 struct Dkv {
   vec8<T> x[4][2];         // K^T (V^T)
@@ -1029,7 +1071,9 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
   store_rows<T>(w.acc, one, out.at<T>(b, h), out.row, k0, A.keys);
 }
 
-// All gradients: blocks of queries and blocks of keys in one launch, so that neither kind's last round leaves CUs idle.
+// All gradients: blocks of queries and blocks of keys in one launch, so that neither kind's last round leaves CUs idle (a
+// launch each, with the stats in the first: 1536 tokens with their forward pass 172 us, now 153; 4608: 1026 and 997).
+// 4608 tokens, 24 heads: 715 us, 1.28 PFLOP/s over the 7 products.
 template <typename T, bool kMasked, bool kGrouped>   // kGrouped: query heads share key heads
 __global__ __launch_bounds__(kThreads, 2) void attention_backward_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kDkvBytes];
@@ -1055,8 +1099,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_kernel(const A
   else dkv_wave<true, kGrouped, T>(A, smem, piece, b, h, first, k0, any);
 }
 
-// Adds the cuts' partial sums in order: 32 lanes a row, 8 rows of a cut block a block.  kOf: of o, or of the gradients, the
-// queries' cut blocks first.
+// Adds the cuts' partial sums in order: 32 lanes a row, 8 rows of a cut block a block.  kForward: of o, or of the
+// gradients, the queries' cut blocks first.  5 us, most of it the launch and the first loads' way to memory.
 template <typename T, bool kForward, bool kKeep>
 __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q_blocks) {
   const int lane = threadIdx.x & 31, r = blockIdx.x % (kQueries / 8) * 8 + (threadIdx.x >> 5);
@@ -1120,7 +1164,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q
       make_uint2(pack<T>(x[0], x[1]), pack<T>(x[2], x[3]));
 }
 
-// The mask's words and live units, one batch entry a block of 16 waves, a thread a unit, 1024 units a turn.
+// The mask's words and live units, one batch entry a block of 16 waves, a thread a unit, 1024 units a turn: one place
+// knows the order of an entry's live units without a second launch.  5 us at 4608 keys, a launch's latency.
 constexpr int kPlanWaves = 16;
 struct MaskBytes {
   const uint8_t* mask;   // NULL: none
@@ -1165,7 +1210,8 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const M
 }
 
 // What the gradients need first: the mask's words and lists, in the first A.batch blocks where there is a mask, and every
-// row's stats, 16 lanes a row and 128 rows (four units) a block, which reads do, o and low once.
+// row's stats, 16 lanes a row and 128 rows (four units) a block, which reads do, o and low once.  Bound by memory: 4608
+// tokens of 24 heads 14 us for 85 MB, which the caches partly hold; 16896 64 us, 4.9 TB/s.
 template <typename T>
 __global__ __launch_bounds__(64 * kPlanWaves) void attention_prepare_kernel(const MaskBytes m, const Args A) {
   __shared__ int found[kPlanWaves];
@@ -1227,8 +1273,9 @@ MaskBytes mask_in(const void* mask, int64_t batch_stride, Args& A, uint8_t* work
   return m;
 }
 
-// How a launch of equal blocks of `tile` rows, each walking n units, is cut: whole rounds of the 256 CUs, and what is left in
-// pieces, where that is estimated to be faster.
+// How a launch of equal blocks of `tile` rows, each walking n units, is cut: whole rounds of the 256 CUs, and what is left
+// in pieces, where that is estimated to be faster.  One query of 24 heads on 4608 keys: 62 us uncut, 21 cut;
+// forward and gradients of 1536 tokens: 166 and 163; of 4608: 1071 and 1046.
 struct Cut {
   int whole, splits, tile;
   int64_t blocks;
@@ -1255,8 +1302,9 @@ Cut plan_cut(int64_t blocks, int64_t n, double unit, int rows, int tile) {
   }
   return best;
 }
-// Blocks of 192 queries are considered where they fit one round: there each takes less time than one of 256, while over more
-// rounds the chip's power limit lets go of what they would save.
+// Blocks of 192 queries are considered where they fit one round: there each takes less time than one of 256 (1536 tokens,
+// forward and gradients: 163 us, with 256 alone 179; 987 of 36 heads: 147 and 158), while over more rounds the chip's power
+// limit lets go of what they would save.
 Cut plan_queries(const Args& A, double unit, double unit192) {
   auto plan = [&](int tile, double us) {
     const int64_t blocks = (int64_t)A.batch * A.heads * ((A.queries + tile - 1) / tile);
@@ -1315,15 +1363,16 @@ Gradients search_gradients(const Args& A) {
   const int64_t k_blocks = (int64_t)A.batch * A.kv_heads * ((A.keys + kKeys - 1) / kKeys);
   auto q_blocks = [&](int tile) { return (int64_t)A.batch * A.heads * ((A.queries + tile - 1) / tile); };
   const double k_time = k_n * kDkvUnit + kFixed;
-  Gradients best{Cut{(int)q_blocks(kQueries), 1, kQueries, q_blocks(kQueries), 0.0}, Cut{(int)k_blocks, 1, kKeys, k_blocks, 0.0},
-                 k_time > q_n * kDqUnit + kFixed, 1e300};
+  Gradients best{Cut{(int)q_blocks(kQueries), 1, kQueries, q_blocks(kQueries), 0.0},
+                 Cut{(int)k_blocks, 1, kKeys, k_blocks, 0.0}, k_time > q_n * kDqUnit + kFixed, 1e300};
   if (best.q.blocks + k_blocks > 32 * kCUs) return best;   // the last round is little of it
   auto consider = [&](const Cut& q, const Cut& k) {
     const double unit = q.tile == kQueries ? kDqUnit : kDqUnit192;
     const double join = q.cuts() + k.cuts() == 0 ? 0.0
                                                  : kJoin + join_time(q.cuts(), std::min(A.queries, q.tile)) +
                                                        join_time(k.cuts(), 2 * std::min(A.keys, kKeys));
-    const double q_time = (q_n + q.splits - 1) / q.splits * unit + kFixed, cut_time = (k_n + k.splits - 1) / k.splits * kDkvUnit + kFixed;
+    const double q_time = (q_n + q.splits - 1) / q.splits * unit + kFixed;
+    const double cut_time = (k_n + k.splits - 1) / k.splits * kDkvUnit + kFixed;
     const double work = q.grid() * q_time + k.whole * k_time + k.cuts() * cut_time;
     if (std::max(work / kCUs, std::max(q_time, k.whole ? k_time : cut_time)) + join >= best.time) return;
     for (const bool k_first : {false, true}) {
