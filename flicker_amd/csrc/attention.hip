@@ -45,7 +45,7 @@
 // library product reaches 1.24 PFLOP/s.  Measured at 24 heads in bfloat16, PFLOP/s over all products that run: forward
 // 4608 tokens 230 us (1.13), 16896 2.66 ms (1.32), with what the gradients need 250 us and 2.82 ms; gradients 730 us
 // (1.25) and 9.4 ms (1.30), of which 14 and 63 us are the rows' stats.  1536 tokens are 144 blocks of queries for 256 CUs:
-// 50 us and 120.  One query on 4608 keys: 15 us for 57 MB, and 5 for the join.
+// 50 us and 120.  Few rows are bound by memory, and have a kernel of their own: one query on 4608 keys 17-19 us.
 
 #include <algorithm>
 #include <type_traits>
@@ -62,6 +62,7 @@ constexpr int kWaves = 8;              // two a SIMD
 constexpr int kThreads = 64 * kWaves;
 constexpr int kQueries = 32 * kWaves;  // queries of a block, 32 a wave
 constexpr int kKeys = 16 * kWaves;     // keys of a block, 32 a pair of waves
+constexpr int kFewRows = 16;           // rows of a block of attention_few_kernel
 constexpr int kLead = 4;               // slots between an operand's LDS read and its MFMAs
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int64_t kMaxItems = 1LL << 31;
@@ -119,12 +120,13 @@ struct Mask {
   const int* counts;
 };
 
-// The blocks from `whole` on are cut into `splits` along the units they walk: partial sums of 256 rows, in order, which
+// The blocks from `whole` on are cut into `splits` along the units they walk: partial sums of `pitch` rows, in order, which
 // attention_join_kernel adds up.
 struct Cuts {
   int whole, splits, tile;   // tile: rows of a block
-  float* part;               // (cut, 256, 128)
+  float* part;               // (cut, pitch, 128)
 };
+constexpr int pitch_of(int tile) { return tile == kFewRows ? kFewRows : kQueries; }
 
 struct Args {
   Tensor q, k, v, o, dO, dq, dk, dv;
@@ -135,7 +137,7 @@ struct Args {
   Mask mask;
   int batch, heads, kv_heads, group, queries, keys, q_units, k_units;
   Cuts of_q, of_k;  // of the blocks of queries, and of keys (backwards)
-  float* part_top;  // (cut, 256, 4): in the forward pass each row's (top, l, sum)
+  float* part_top;  // (cut, pitch, 4): in the forward pass each row's (top, l, sum)
   int q_grid;       // backwards: hardware blocks that take queries, the first ones or, with k_first, the last
   bool k_first;
 };
@@ -667,6 +669,191 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
     forward_wave<T, kMasked, kKeep, 1>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
 }
 
+// o of few rows: the queries of all heads that share a key head, at most 16 rows, so that each key is read once.  Bound by
+// memory, and where few blocks walk many units by its latency.  The four waves walk units of their own (every fourth of the
+// block's), each copied into the wave's own LDS two ahead: no barrier, and 64 to 128 KB on their way to a CU.  The waves'
+// sums are joined at the end.  One query of 24 heads: 4608 keys 19 us with the join (57 MB, 14 of them this kernel), 16896
+// keys 46 us (4.5 TB/s), 8 x 4608 85 us (5.3 TB/s).  Two blocks of two waves a CU: 22.3, 50.6, 89.6.
+constexpr int kFewWaves = 4, kFewRing = 2;
+constexpr int kFewBytes = (2 * kFewRing * kUnit + kFewRows) * kRowBytes;   // of a wave: K ring, V ring, Q
+
+// Starts the copy of a unit's 32 rows by one wave; rows past the last of `rows` repeat it.
+__device__ __forceinline__ void start_unit(const Tensor& t, const uint16_t* head, int rows, int unit, unsigned lds) {
+  const int lane = threadIdx.x & 63, end = min(rows - 1 - unit * kUnit, kUnit - 1);
+  const uint32_t row = (uint32_t)t.row * 2;
+  const char* base = reinterpret_cast<const char*>(head) + (uint64_t)(uint32_t)unit * (row * kUnit);
+#pragma unroll
+  for (int i = 0; i < kUnit / 4; ++i) {
+    const int r = 4 * i + (lane >> 4);
+    flk::dma16_lds(base, min(r, end) * row + (((lane & 15) ^ swz(r)) << 4), lds + i * 4 * kRowBytes);
+  }
+}
+
+template <typename T, bool kMasked>
+__global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Args A) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kFewWaves * kFewBytes];
+  const int lane = threadIdx.x & 63, h4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int p = by_xcd(blockIdx.x, gridDim.x), splits = A.of_q.splits, split = p % splits, block = p / splits;
+  const int b = block / A.kv_heads, hk = block - b * A.kv_heads, rows = A.group * A.queries;
+  const int all = kMasked ? __builtin_amdgcn_readfirstlane(A.mask.counts[b]) : A.k_units;
+  const int first = split * (all / splits) + min(split, all % splits), count = all / splits + (split < all % splits);
+  const int n = count > wave ? (count - wave + kFewWaves - 1) / kFewWaves : 0;
+  uint8_t* mine = smem + wave * kFewBytes;
+  const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)mine);
+  uint8_t* const q_rows = mine + 2 * kFewRing * kUnitBytes;
+
+  f32x4 acc[8], l{};
+  float sum = 0.0f, top = -1e30f;
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{};
+  if (n) {
+    const uint16_t *k = A.k.at<uint16_t>(b, hk), *v = A.v.at<uint16_t>(b, hk);
+    uint2 some;   // of a masked entry: 64 of the wave's units, one a lane
+    int unit[3];  // of the iterations i, i + 1 and i + 2
+    uint32_t bits[3];
+    auto get = [&](int i, int& unit, uint32_t& bits) {
+      if constexpr (kMasked) {
+        if ((i & 63) == 0)
+          some = A.mask.live[(int64_t)b * A.k_units + first + min(wave + kFewWaves * (i + lane), count - 1)];
+        unit = __builtin_amdgcn_readlane(some.x, i & 63);
+        bits = __builtin_amdgcn_readlane(some.y, i & 63);
+      } else {
+        unit = first + min(wave + kFewWaves * i, count - 1);
+        bits = kept(A, b, unit);
+      }
+    };
+    auto k_at = [&](int i) { return (i & (kFewRing - 1)) * kUnitBytes; };
+    auto v_at = [&](int i) { return (kFewRing + (i & (kFewRing - 1))) * kUnitBytes; };
+    get(0, unit[0], bits[0]);
+    get(1, unit[1], bits[1]);
+#pragma unroll
+    for (int i = 0; i < kFewRows / 4; ++i) {   // row gi * queries + qi is query qi of the key head's query head gi
+      const int r = 4 * i + h4, at = min(r, rows - 1), gi = at / A.queries;
+      const uint16_t* src = A.q.at<uint16_t>(b, hk * A.group + gi) + (at - gi * A.queries) * A.q.row;
+      flk::dma16(src + (((lane & 15) ^ swz(r)) << 3), q_rows + i * 4 * kRowBytes);
+    }
+    for (int i = 0; i < min(n, 2); ++i) {
+      start_unit(A.k, k, A.keys, unit[i], lds + k_at(i));
+      start_unit(A.v, v, A.keys, unit[i], lds + v_at(i));
+    }
+    const Places at = places();
+    const T one = (T)((lane & 15) == 0 ? 1.0f : 0.0f);
+    const vec8<T> ones = {one, one, one, one, one, one, one, one};
+    vec8<T> x[4];
+    for (int i = 0; i < n; ++i) {
+      get(i + 2, unit[2], bits[2]);
+      // a unit is 16 copies, K's before V's; those of later units may still be on their way
+      if (i + 1 < n) landed<24>();
+      else landed<8>();
+      if (i == 0)
+#pragma unroll
+        for (int st = 0; st < 4; ++st) x[st] = row_operand<T>(q_rows, at, st, 0);
+      f32x4 s[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+          s[kt] = mfma(row_operand<T>(mine + k_at(i), at, st, kt), x[st], st ? s[kt] : f32x4{});
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K(i) has been read
+      if (i + 2 < n) start_unit(A.k, k, A.keys, unit[2], lds + k_at(i));
+      if (bits[0] != ~0u) leave_out(s, bits[0]);
+      float most = top;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, s[e >> 2][e & 3]);
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      if (__any(most > top)) {
+        const float f = __builtin_amdgcn_exp2f((top - most) * kLog2e);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) acc[dt] *= f;
+        l *= f;
+        sum *= f;
+        top = most;
+      }
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3] - top, kLog2e, -kShift<T>));
+        sum += e[j];
+      }
+      const uint32_t words[4] = {pack<T>(e[0], e[1]), pack<T>(e[2], e[3]), pack<T>(e[4], e[5]), pack<T>(e[6], e[7])};
+      const vec8<T> w = packed<T>(words, 0);
+      l = mfma(ones, w, l);
+      if (i + 2 < n) landed<24>();
+      else if (i + 1 < n) landed<16>();
+      else landed<0>();
+      if (bits[0] != ~0u) {   // 0 * what the rows left out hold would be NaN for infinities
+#pragma unroll
+        for (int j = 0; j < kUnit / 4; ++j)
+          if (!(bits[0] >> (4 * j + h4) & 1))
+            *reinterpret_cast<uint4*>(mine + v_at(i) + j * 4 * kRowBytes + lane * 16) = make_uint4(0, 0, 0, 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) acc[dt] = mfma(col_operand<T>(mine + v_at(i), at, dt), w, acc[dt]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // V(i) has been read
+      if (i + 2 < n) start_unit(A.v, v, A.keys, unit[2], lds + v_at(i));
+      unit[0] = unit[1];
+      bits[0] = bits[1];
+      unit[1] = unit[2];
+      bits[1] = bits[2];
+    }
+  }
+
+  // the waves' sums, through LDS that the wave itself has done with
+  constexpr int kPitch = kD + 4;   // floats of a row
+  float* sums = reinterpret_cast<float*>(mine);
+  sum = across(sum);
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(sums + (lane & 15) * kPitch + dt * 16 + h4 * 4) = acc[dt];
+  if (h4 == 0) *reinterpret_cast<f32x4*>(sums + kFewRows * kPitch + lane * 4) = f32x4{top, l[0], sum, 0.0f};
+  __syncthreads();
+  const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
+  if (row >= rows) return;
+  f32x4 t[kFewWaves], o[2] = {};
+  top = -1e30f;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) {
+    t[i] = *reinterpret_cast<const f32x4*>(smem + i * kFewBytes + (kFewRows * kPitch + row * 4) * 4);
+    top = fmaxf(top, t[i][0]);
+  }
+  float total = 0.0f;
+  sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) {
+    const float f = __builtin_amdgcn_exp2f((t[i][0] - top) * kLog2e);
+    const f32x4* from = reinterpret_cast<const f32x4*>(smem + i * kFewBytes + (row * kPitch + d) * 4);
+    o[0] += from[0] * f;
+    o[1] += from[1] * f;
+    total += t[i][1] * f;
+    sum += t[i][2] * f;
+  }
+  const int gi = row / A.queries, qi = row - gi * A.queries, h = hk * A.group + gi;
+  if (splits > 1) {
+    const int64_t at = ((int64_t)(b * A.heads + h) * splits + split) * kFewRows + qi;
+    f32x4* part = reinterpret_cast<f32x4*>(A.of_q.part + at * kD + d);
+    part[0] = o[0];
+    part[1] = o[1];
+    if (d == 0) reinterpret_cast<f32x4*>(A.part_top)[at] = f32x4{top, total, sum, 0.0f};
+    return;
+  }
+  const float scale = total > 0.0f ? 1.0f / total : 0.0f;
+  uint32_t high[4], low[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y0 = o[i >> 1][2 * (i & 1)] * scale, y1 = o[i >> 1][2 * (i & 1) + 1] * scale;
+    high[i] = pack<T>(y0, y1);
+    low[i] = pack<T>(y0 - (float)(T)y0, y1 - (float)(T)y1);
+  }
+  *reinterpret_cast<uint4*>(A.o.at<T>(b, h) + (int64_t)qi * A.o.row + d) = make_uint4(high[0], high[1], high[2], high[3]);
+  if (!A.lse) return;
+  *reinterpret_cast<uint4*>(static_cast<T*>(A.low) + (((int64_t)b * A.queries + qi) * A.heads + h) * kD + d) =
+      make_uint4(low[0], low[1], low[2], low[3]);
+  if (d == 0)
+    A.lse[(int64_t)(b * A.heads + h) * A.queries + qi] =
+        total > 0.0f ? top + (__builtin_amdgcn_logf(sum) + kShift<T>) * kLn2 : -INFINITY;
+}
+
 template <typename T, int G>
 struct Dq {
   vec8<T> x[4][G], g[4][G];   // Q^T, dO^T
@@ -1099,12 +1286,24 @@ __global__ __launch_bounds__(kThreads, 2) void attention_backward_kernel(const A
   else dkv_wave<true, kGrouped, T>(A, smem, piece, b, h, first, k0, any);
 }
 
+// Partial sums that are `step` floats apart, the first n of kJoined, all asked for at once: a load after the other is a way to
+// memory each.
+constexpr int kJoined = 8;
+__device__ __forceinline__ void parts(const float* at, int step, int n, f32x4 (&y)[kJoined]) {
+#pragma unroll
+  for (int j = 0; j < kJoined; ++j) {
+    const f32x4 t = *reinterpret_cast<const f32x4*>(at + min(j, n - 1) * step);
+    y[j] = j < n ? t : f32x4{};
+  }
+}
+
 // Adds the cuts' partial sums in order: 32 lanes a row, 8 rows of a cut block a block.  kForward: of o, or of the
-// gradients, the queries' cut blocks first.  5 us, most of it the launch and the first loads' way to memory.
+// gradients, the queries' cut blocks first.  4 us, most of it the launch and the first loads' way to memory.
 template <typename T, bool kForward, bool kKeep>
 __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q_blocks) {
-  const int lane = threadIdx.x & 31, r = blockIdx.x % (kQueries / 8) * 8 + (threadIdx.x >> 5);
-  int cut_block = blockIdx.x / (kQueries / 8);
+  const int pitch = kForward ? pitch_of(A.of_q.tile) : kQueries;
+  const int lane = threadIdx.x & 31, r = blockIdx.x % (pitch / 8) * 8 + (threadIdx.x >> 5);
+  int cut_block = blockIdx.x / (pitch / 8);
   const bool of_keys = !kForward && cut_block >= q_blocks;
   if (of_keys) cut_block -= q_blocks;
   const Cuts& cuts = of_keys ? A.of_k : A.of_q;
@@ -1113,17 +1312,17 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q
   const int blocks = (rows + per - 1) / per, bh = block / blocks, b = bh / heads, h = bh - b * heads;
   const int row = (block - bh * blocks) * per + (of_keys ? r % kKeys : r);
   if (row >= rows || (!of_keys && r >= per)) return;
-  const int64_t first = ((int64_t)cut_block * cuts.splits * kQueries + r) * kD;
+  const int64_t first = ((int64_t)cut_block * cuts.splits * pitch + r) * kD;
   f32x4 x{};
   if constexpr (kForward) {
     // lane i of the row's 32 holds the factors of the cuts i and i + 32
-    const f32x4* tops = reinterpret_cast<const f32x4*>(A.part_top) + (int64_t)cut_block * cuts.splits * kQueries + r;
+    const f32x4* tops = reinterpret_cast<const f32x4*>(A.part_top) + (int64_t)cut_block * cuts.splits * pitch + r;
     f32x4 t[2];
     float top = -1e30f, l = 0.0f, sum = 0.0f, f[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int at = lane + 32 * i;
-      t[i] = at < cuts.splits ? tops[(int64_t)at * kQueries] : f32x4{-1e30f, 0.0f, 0.0f, 0.0f};
+      t[i] = at < cuts.splits ? tops[(int64_t)at * pitch] : f32x4{-1e30f, 0.0f, 0.0f, 0.0f};
       top = fmaxf(top, t[i][0]);
     }
 #pragma unroll
@@ -1140,9 +1339,12 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q
       sum += __shfl_xor(sum, d, 32);
     }
     const float* at = cuts.part + first + lane * 4;
-#pragma unroll 8
-    for (int i = 0; i < cuts.splits; ++i)
-      x += *reinterpret_cast<const f32x4*>(at + (int64_t)i * kQueries * kD) * __shfl(i < 32 ? f[0] : f[1], i & 31, 32);
+    for (int i = 0; i < cuts.splits; i += kJoined) {
+      f32x4 y[kJoined];
+      parts(at + (int64_t)i * pitch * kD, pitch * kD, cuts.splits - i, y);
+#pragma unroll
+      for (int j = 0; j < kJoined; ++j) x += y[j] * __shfl(i + j < 32 ? f[0] : f[1], (i + j) & 31, 32);
+    }
     x *= l > 0.0f ? 1.0f / l : 0.0f;
     if constexpr (kKeep) {
       if (lane == 0)
@@ -1155,9 +1357,12 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q
       *reinterpret_cast<uint2*>(low) = make_uint2(pack<T>(y[0], y[1]), pack<T>(y[2], y[3]));
     }
   } else {
-#pragma unroll 4
-    for (int i = 0; i < cuts.splits; ++i)
-      x += *reinterpret_cast<const f32x4*>(cuts.part + first + (int64_t)i * kQueries * kD + lane * 4);
+    for (int i = 0; i < cuts.splits; i += kJoined) {
+      f32x4 y[kJoined];
+      parts(cuts.part + first + (int64_t)i * pitch * kD + lane * 4, pitch * kD, cuts.splits - i, y);
+#pragma unroll
+      for (int j = 0; j < kJoined; ++j) x += y[j];
+    }
   }
   const Tensor& out = kForward ? A.o : !of_keys ? A.dq : r < kKeys ? A.dv : A.dk;
   *reinterpret_cast<uint2*>(out.at<T>(b, h) + (int64_t)row * out.row + lane * 4) =
@@ -1274,15 +1479,16 @@ MaskBytes mask_in(const void* mask, int64_t batch_stride, Args& A, uint8_t* work
 }
 
 // How a launch of equal blocks of `tile` rows, each walking n units, is cut: whole rounds of the 256 CUs, and what is left
-// in pieces, where that is estimated to be faster.  One query of 24 heads on 4608 keys: 62 us uncut, 21 cut;
-// forward and gradients of 1536 tokens: 166 and 163; of 4608: 1071 and 1046.
+// in pieces, where that is estimated to be faster.  Forward and gradients of 1536 tokens: 166 us uncut, 163 cut; of 4608:
+// 1071 and 1046.
 struct Cut {
   int whole, splits, tile;
   int64_t blocks;
   double time;
   int64_t grid() const { return whole + (blocks - whole) * splits; }
   int64_t cuts() const { return splits > 1 ? (blocks - whole) * splits : 0; }
-  int64_t bytes() const { return cuts() * kQueries * (kD + 4) * 4; }
+  int64_t part_rows() const { return cuts() * pitch_of(tile); }
+  int64_t bytes() const { return part_rows() * (kD + 4) * 4; }
   Cuts in(uint8_t* workspace) const { return Cuts{whole, splits, tile, reinterpret_cast<float*>(workspace)}; }
 };
 constexpr int kCUs = 256, kMaxSplits = 64;
@@ -1313,7 +1519,26 @@ Cut plan_queries(const Args& A, double unit, double unit192) {
   const Cut wide = plan(kQueries, unit), narrow = plan(192, unit192);
   return narrow.blocks <= kCUs && narrow.time < wide.time ? narrow : wide;
 }
-Cut forward_cut(const Args& A) { return plan_queries(A, 0.82, 0.69); }
+// Few rows go through attention_few_kernel, one query of 24 heads on 4608 keys in 19 us (through the blocks above in 22.4), on
+// 512 in 8.5 (12.9), of 8 entries in 85 (101), on 4 key heads in 11.2 (18.9), 16 queries in 20 (23.2).
+bool few(const Args& A) { return A.queries <= kFewRows && A.group <= kFewRows / A.queries; }
+// us of a unit: of a block alone, more for every other block, and of a block on each CU at memory's rate; of launches; of the
+// join's, and its for each cut.
+constexpr double kFewUnit = 0.37, kFewMore = 0.001, kFewFull = 0.72, kFewFixed = 4.0, kFewJoin = 4.0, kFewCut = 0.06;
+Cut plan_few(const Args& A) {
+  const int64_t blocks = (int64_t)A.batch * A.kv_heads, heads = (int64_t)A.batch * A.heads;
+  Cut best{(int)heads, 1, kFewRows, heads, 1e300};
+  for (int s = 1; s <= kMaxSplits && (s == 1 || (kFewWaves * s <= A.k_units && blocks * s <= 4 * kCUs)); ++s) {
+    const int64_t grid = blocks * s, rounds = (grid + kCUs - 1) / kCUs;
+    const int turns = ((A.k_units + s - 1) / s + kFewWaves - 1) / kFewWaves;
+    const double at_once = (double)std::min<int64_t>(grid, kCUs);
+    const double unit = std::max(kFewUnit + kFewMore * at_once, kFewFull * at_once / kCUs);
+    const double time = rounds * (turns * kFewWaves * unit + kFewFixed) + (s > 1 ? kFewJoin + kFewCut * s : 0.0);
+    if (time < best.time) best = Cut{s > 1 ? 0 : (int)heads, s, kFewRows, heads, time};
+  }
+  return best;
+}
+Cut forward_cut(const Args& A) { return few(A) ? plan_few(A) : plan_queries(A, 0.82, 0.69); }
 
 // When the CUs, each taking the next block as it ends one, have done runs of equal blocks.
 class Schedule {
@@ -1452,7 +1677,11 @@ int64_t join_blocks(const Cut& cut) { return cut.splits > 1 ? cut.blocks - cut.w
 template <typename T>
 void forward(const Args& A, const Cut& cut, hipStream_t s) {
   const dim3 grid((unsigned)cut.grid());
-  if (A.mask.bits) {
+  if (few(A)) {
+    const dim3 blocks((unsigned)(A.batch * A.kv_heads * cut.splits));
+    if (A.mask.bits) attention_few_kernel<T, true><<<blocks, 64 * kFewWaves, 0, s>>>(A);
+    else attention_few_kernel<T, false><<<blocks, 64 * kFewWaves, 0, s>>>(A);
+  } else if (A.mask.bits) {
     if (A.lse) attention_kernel<T, true, true><<<grid, kThreads, 0, s>>>(A);
     else attention_kernel<T, true, false><<<grid, kThreads, 0, s>>>(A);
   } else {
@@ -1461,7 +1690,7 @@ void forward(const Args& A, const Cut& cut, hipStream_t s) {
   }
   const int joined = (int)join_blocks(cut);
   if (!joined) return;
-  const dim3 join((unsigned)(joined * (kQueries / 8)));
+  const dim3 join((unsigned)(joined * (pitch_of(cut.tile) / 8)));
   if (A.lse) attention_join_kernel<T, true, true><<<join, 256, 0, s>>>(A, joined);
   else attention_join_kernel<T, true, false><<<join, 256, 0, s>>>(A, joined);
 }
@@ -1532,7 +1761,7 @@ extern "C" int flk_attention(const void* q, const int64_t* q_strides, const void
   if (mask.mask) attention_mask_kernel<<<batch, 64 * kPlanWaves, 0, s>>>(mask, keys, A.k_units);
   const Cut cut = forward_cut(A);
   A.of_q = cut.in(static_cast<uint8_t*>(workspace) + (key_mask ? mask_bytes(batch, keys) : 0));
-  A.part_top = A.of_q.part + cut.cuts() * kQueries * kD;
+  A.part_top = A.of_q.part + cut.part_rows() * kD;
   if (dtype == FLK_BF16) forward<__bf16>(A, cut, s);
   else forward<_Float16>(A, cut, s);
   return flk_launch_status();

@@ -10,6 +10,8 @@ subnormal; float16's P and dS reach it).  Per row of one head:
   * lse is off by r.
   * delta: sum_d |g| times what o is off by before its last rounding, which low holds to e^2, and 130 u sum|g o|.
   * dS = P (dP - delta): off by (e + r + 4 u)|dS| + P (130 u sum|g v| + delta's) + t0.
+    In the gradients a P below float32's smallest normal number, z = 2^-126, is zero: exp2 gives no subnormals.  P is off by
+    z more, dS by z |dP - delta|.  (z is far below every other term unless all P of a key are about as small.)
   * dq, dk: those times |k|, |q|, summed, and (terms + 64) u sum|dS k|; dv: sum of (P (e + r) + t0)|g| likewise.
 Masked keys hold infinities and NaN.
 """
@@ -25,6 +27,7 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+FLUSH = 2.0 ** -126
 D = 128
 
 
@@ -104,9 +107,10 @@ def expected(q, k, v, do, keep):
             tols[0][b, :, h], tols[1][b, h] = o_off, r[:, 0]
             delta_off = (ag * (o_off + (e * e + 130 * U) * np.abs(o[b, :, h]))).sum(-1, keepdims=True)
             dp = gh @ vh.T
-            ds = np.abs(p * (dp - (gh * o[b, :, h]).sum(-1, keepdims=True)))
-            ds_off = (e + r + 4 * U) * ds + p * (130 * U * (ag @ av.T) + delta_off) + t0 * on
-            p_off = p * (e + r) + t0 * on
+            spread = np.abs(dp - (gh * o[b, :, h]).sum(-1, keepdims=True))
+            ds = p * spread
+            ds_off = (e + r + 4 * U) * ds + p * (130 * U * (ag @ av.T) + delta_off) + (t0 + FLUSH * spread) * on
+            p_off = p * (e + r) + (t0 + FLUSH) * on
             tols[2][b, h] += ds_off @ ak + (keys + 64) * U * (ds @ ak)
             tols[3][b, hk] += ds_off.T @ aq + (queries * heads + 64) * U * (ds.T @ aq)
             tols[4][b, hk] += p_off.T @ ag + (queries * heads + 64) * U * (p.T @ ag)
@@ -365,3 +369,54 @@ def test_long_cuts_of_the_queries(device, heads, kv_heads):
 def test_cuts_that_begin_near_a_head_s_end(device):
     """Four query heads of ten units a key head, in cuts of 14, 13 and 13: the last begins three units before a head ends."""
     check(22, 1, 280, 70, 320, 100, "bf16")
+
+
+@pytest.mark.parametrize("heads,kv_heads,queries", [(2, 2, 1), (16, 1, 1), (17, 1, 1), (6, 2, 5), (6, 2, 6), (2, 2, 16), (32, 2, 1)])
+@pytest.mark.parametrize("keys,mask", [(31, None), (129, "random"), (2000, "middle"), (4133, None)])
+def test_few_rows(device, heads, kv_heads, queries, keys, mask):
+    """A key head's rows, at most 16 or just past it, in blocks of their own and cut along the keys."""
+    check(heads * keys, 2, heads, kv_heads, queries, keys, "bf16", mask)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("scale", [0.0, 4.0, 30.0])
+def test_few_rows_logit_sizes(device, scale, dtype):
+    check(11, 3, 8, 2, 2, 700, dtype, "random", scale=scale)
+
+
+def test_few_rows_of_many_entries(device):
+    """Enough entries that none is cut, each with more units than a wave fetches at once."""
+    g = torch.Generator("cuda").manual_seed(0)
+    batch, keys = 520, 8333
+    q = (torch.randn(batch, 1, 1, D, generator=g, device=device) * D ** -0.5).bfloat16()
+    k, v = (torch.randn(1, 1, keys, D, generator=g, device=device).bfloat16().expand(batch, -1, -1, -1) for _ in range(2))
+    keep = torch.rand(batch, keys, generator=g, device=device) < 0.5
+    keep[:5] = True
+    keep[5] = False
+    o, kept = A.attention(q, k, v, key_mask=keep, keep=True)
+    s = (q[:, 0, 0].double() @ k[0, 0].double().T).masked_fill(~keep, -torch.inf)
+    lse = torch.logsumexp(s, -1)
+    p = torch.where(keep, torch.exp(s - lse[:, None]), 0.0)
+    want, size = p @ v[0, 0].double(), p @ v[0, 0].double().abs()
+    r = 400 * U * q[:, 0, 0].double().abs() @ k[0, 0].double().abs().T.amax(1, keepdim=True) + 2 * (keys + 64) * U
+    tol = (2 * 2.0 ** -8 + 2 * r) * size + 2.0 ** -8 * want.abs()
+    assert ((o[:, 0].double() - want).abs() <= tol * 1.01).all()
+    assert torch.isneginf(kept.lse[5]).all() and not o[5].any()
+    rest = torch.arange(batch, device=device) != 5
+    assert ((kept.lse[rest, 0, 0].double() - lse[rest]).abs() <= r[rest, 0] + 2 * U * lse[rest].abs()).all()
+    assert torch.equal(o, A.attention(q, k, v, key_mask=keep))
+
+
+def test_few_rows_leave_the_rest(device):
+    """Strided outputs and operands of a cache longer than its keys: what lies behind them is neither read nor written."""
+    g = torch.Generator("cuda").manual_seed(1)
+    cache = torch.randn(2, 2, 900, 2, D, generator=g, device=device).half()
+    cache[:, :, 500:] = float("nan")
+    k, v = cache[:, :, :500, 0], cache[:, :, :500, 1]
+    q = (torch.randn(2, 4, 2, D, generator=g, device=device) * D ** -0.5).half()
+    wide = torch.full((2, 5, 4 * D + 64), 7.0, dtype=torch.float16, device=device)
+    out = A.attention(q, k, v, out=wide[:, 2:4, 32:32 + 4 * D])
+    want = A.attention(q, k.contiguous(), v.contiguous())
+    assert torch.equal(out, want) and torch.isfinite(out).all()
+    wide[:, 2:4, 32:32 + 4 * D] = 7.0
+    assert (wide == 7.0).all()
