@@ -1647,8 +1647,11 @@ Gradients plan_gradients(const Args& A) {
 bool sizes_ok(int batch, int heads, int kv_heads, int queries, int keys) {
   if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || queries < 0 || keys < 0) return false;
   if (queries > 1 << 28 || keys > 1 << 28 || batch > 1 << 20) return false;
-  const int64_t rows = (int64_t)batch * heads, kv = (int64_t)batch * kv_heads;
-  return rows * ((queries + 31) / 32) <= kMaxItems / 512 && kv * ((keys + 31) / 32) <= kMaxItems / 512;
+  auto fits = [&](int heads, int length) {   // batch * heads stays below 2^51
+    const int64_t units = (length + 31) / 32, most = kMaxItems / 512;
+    return units == 0 || (int64_t)batch * heads <= most / units;
+  };
+  return fits(heads, queries) && fits(kv_heads, keys);
 }
 
 int check_tensor(const void* p, const int64_t* strides) {

@@ -183,8 +183,9 @@ int64_t items_of(int batch, int length, int heads) {
 int blocks_of(int64_t items) { return (int)std::min<int64_t>(items, kMaxBlocks); }
 
 bool sizes_ok(int batch, int length, int heads) {
-  return batch >= 0 && length >= 0 && heads > 0 && length <= INT32_MAX - 256 && heads <= 1 << 20 &&
-         items_of(batch, length, heads) <= INT32_MAX - kMaxBlocks;
+  if (batch < 0 || length < 0 || heads <= 0 || length > INT32_MAX - 256 || heads > 1 << 20) return false;
+  const int64_t of_one = items_of(1, length, heads);
+  return batch == 0 || of_one <= (INT32_MAX - kMaxBlocks) / batch;
 }
 
 int check_grad(const void* p, const int64_t* strides) {

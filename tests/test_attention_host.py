@@ -221,3 +221,13 @@ def test_autograd_refuses_forward_mode(monkeypatch):
         for call in (lambda: autograd.attention(dual, x, x), lambda: autograd.residual_modulate(x, dual, x, x, x)):
             with pytest.raises(NotImplementedError):
                 call()
+
+
+def test_sizes_whose_products_pass_64_bits(lib):
+    """Sizes that each are in range are refused by their product, also where it wraps around to nothing."""
+    size = ctypes.c_int64(0)
+    for heads in (2 ** 24, 2 ** 30):
+        assert lib.flk_attention_plan(2 ** 20, heads, heads, 2 ** 28, 2 ** 28, 0, 1, ctypes.byref(size)) == INVALID
+        assert lib.flk_attention_plan(2 ** 20, heads, 1, 2 ** 28, 1, 0, 1, ctypes.byref(size)) == INVALID
+    for batch, length, heads in ((2 ** 30, 2 ** 30, 2 ** 20), (2 ** 30, 2 ** 28, 2 ** 10)):
+        assert lib.flk_qk_prep_backward_plan(batch, length, heads, ctypes.byref(size)) == INVALID
