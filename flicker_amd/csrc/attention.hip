@@ -33,9 +33,9 @@
 // than its type holds it where few keys carry a row (at two keys its rounding would cost dq, by estimate, twice all else),
 // so the forward pass keeps what o's rounding left.
 //
-// Masks: bytes become one word of bits a unit and a list of the units that keep any (attention_mask_kernel), and blocks
-// walk that list.  In a unit that keeps part, the rows left out are cleared in LDS before anyone reads them (0 * inf), and
-// their S set to -inf.
+// Masks: bytes become one word of bits a unit and a list of the units that keep any, in a launch of their own past 64 units
+// (attention_mask_kernel), and blocks walk that list.  In a unit that keeps part, the rows left out are cleared in LDS
+// before anyone reads them (0 * inf), and their S set to -inf.
 //
 // Blocks that would leave CUs idle are cut along the units they walk, and a second kernel adds the float32 partial sums up in
 // order; which and how many is estimated from a unit's time (plan_cut, search_gradients).  The gradients' two kinds of
@@ -113,11 +113,15 @@ struct Tensor {   // element d of row t of head h of batch entry b at p + b * ba
 };
 
 // What the mask's bytes come to: of batch entry b the words bits[b * units + u], bit i of word u set where key 32 u + i is
-// kept, and the units live[b * units + n].x, n < counts[b], whose words (.y) are not zero, in order.  NULL: all are kept.
+// kept, and the units live[b * units + n].x, n < counts[b], whose words (.y) are not zero, in order.  Where `bytes` is set,
+// each wave finds the list by itself, in rows of at most 64 units.  All NULL: all keys are kept.
 struct Mask {
   const uint32_t* bits;
   const uint2* live;
   const int* counts;
+  const uint8_t* bytes;
+  int64_t batch_stride;
+  __host__ __device__ bool none() const { return !bits && !bytes; }
 };
 
 // The blocks from `whole` on are cut into `splits` along the units they walk: partial sums of `pitch` rows, in order, which
@@ -290,6 +294,36 @@ __device__ __forceinline__ void leave_out(f32x4 (&s)[N], uint32_t bits) {
   }
 }
 
+// The word of unit `lane` of a row's 64 from `first` on.  Bytes past the row's end are not read, and none is waited for before
+// half of the others are asked for.
+__device__ __forceinline__ uint32_t mask_word(const uint8_t* row, int first, int keys) {
+  const int lane = threadIdx.x & 63;
+  uint32_t mine = 0;
+  for (int half = 0; half < 32; half += 16) {
+    const int from = (first + 2 * half) * kUnit + lane;
+    if (from - lane >= keys) break;
+    uint8_t x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = row[min(from + 64 * i, keys - 1)];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint64_t both = __ballot(from + 64 * i < keys && x[i] != 0);
+      if (lane >> 1 == half + i) mine = (uint32_t)(lane & 1 ? both >> 32 : both);
+    }
+  }
+  return mine;
+}
+// A row's units that have kept keys, one a lane, and how many they are; the lanes behind them hold the others.
+__device__ __forceinline__ uint2 find_live(const Args& A, int b, int& count) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t mine = mask_word(A.mask.bytes + b * A.mask.batch_stride, 0, A.keys);
+  const uint64_t any = __ballot(mine != 0);
+  const int before = __popcll(any & ((1ull << lane) - 1));
+  count = __popcll(any);
+  const int to = 4 * (mine ? before : count + lane - before);
+  return make_uint2(__builtin_amdgcn_ds_permute(to, lane), __builtin_amdgcn_ds_permute(to, (int)mine));
+}
+
 // The key units of a batch entry that have kept keys, asked for one after the other from 0; past the last: the last one with
 // no key kept.  A masked entry's list is fetched 64 units at a time, one a lane.
 template <bool kMasked>
@@ -299,15 +333,25 @@ struct Units {
   uint32_t tail;
   uint2 some;
   __device__ __forceinline__ Units(const Args& A, int b, const Piece& piece) {
-    const int all = kMasked ? __builtin_amdgcn_readfirstlane(A.mask.counts[b]) : A.k_units;
+    int all = A.k_units;
+    if constexpr (kMasked) {
+      if (A.mask.bytes) some = find_live(A, b, all);
+      else all = A.mask.counts[b];
+      all = __builtin_amdgcn_readfirstlane(all);
+    }
     first = piece.first(all);
     n = piece.count(all);
-    if constexpr (kMasked) live = A.mask.live + (int64_t)b * A.k_units + first;
-    else tail = first + n == all ? kept(A, b, all - 1) : ~0u;
+    if constexpr (kMasked) {
+      live = A.mask.bytes ? nullptr : A.mask.live + (int64_t)b * A.k_units + first;
+      const int from = first + min((int)(threadIdx.x & 63), n - 1);
+      if (!live) some = make_uint2(__shfl(some.x, from), __shfl(some.y, from));
+    } else {
+      tail = first + n == all ? kept(A, b, all - 1) : ~0u;
+    }
   }
   __device__ __forceinline__ void get(int i, int& unit, uint32_t& bits) {
     if constexpr (kMasked) {
-      if ((i & 63) == 0) some = live[min(i + (int)(threadIdx.x & 63), n - 1)];
+      if ((i & 63) == 0 && live) some = live[min(i + (int)(threadIdx.x & 63), n - 1)];
       unit = __builtin_amdgcn_readlane(some.x, i & 63);
       bits = i < n ? __builtin_amdgcn_readlane(some.y, i & 63) : 0u;
     } else {
@@ -695,7 +739,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
   const int lane = threadIdx.x & 63, h4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int p = by_xcd(blockIdx.x, gridDim.x), splits = A.of_q.splits, split = p % splits, block = p / splits;
   const int b = block / A.kv_heads, hk = block - b * A.kv_heads, rows = A.group * A.queries;
-  const int all = kMasked ? __builtin_amdgcn_readfirstlane(A.mask.counts[b]) : A.k_units;
+  uint2 some;   // of a masked entry: 64 of the wave's units, one a lane
+  int all = A.k_units;
+  if constexpr (kMasked) {
+    if (A.mask.bytes) some = find_live(A, b, all);
+    else all = A.mask.counts[b];
+    all = __builtin_amdgcn_readfirstlane(all);
+  }
   const int first = split * (all / splits) + min(split, all % splits), count = all / splits + (split < all % splits);
   const int n = count > wave ? (count - wave + kFewWaves - 1) / kFewWaves : 0;
   uint8_t* mine = smem + wave * kFewBytes;
@@ -708,12 +758,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
   for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{};
   if (n) {
     const uint16_t *k = A.k.at<uint16_t>(b, hk), *v = A.v.at<uint16_t>(b, hk);
-    uint2 some;   // of a masked entry: 64 of the wave's units, one a lane
+    if (kMasked && A.mask.bytes) {
+      const int from = first + min(wave + kFewWaves * lane, count - 1);
+      some = make_uint2(__shfl(some.x, from), __shfl(some.y, from));
+    }
     int unit[3];  // of the iterations i, i + 1 and i + 2
     uint32_t bits[3];
     auto get = [&](int i, int& unit, uint32_t& bits) {
       if constexpr (kMasked) {
-        if ((i & 63) == 0)
+        if ((i & 63) == 0 && !A.mask.bytes)
           some = A.mask.live[(int64_t)b * A.k_units + first + min(wave + kFewWaves * (i + lane), count - 1)];
         unit = __builtin_amdgcn_readlane(some.x, i & 63);
         bits = __builtin_amdgcn_readlane(some.y, i & 63);
@@ -1370,7 +1423,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q
 }
 
 // The mask's words and live units, one batch entry a block of 16 waves, a thread a unit, 1024 units a turn: one place
-// knows the order of an entry's live units without a second launch.  5 us at 4608 keys, a launch's latency.
+// knows the order of an entry's live units without a second launch.  3 us at 4608 keys, a launch and two latencies (with the
+// loads one after the other 5).
 constexpr int kPlanWaves = 16;
 struct MaskBytes {
   const uint8_t* mask;   // NULL: none
@@ -1386,13 +1440,7 @@ __device__ __forceinline__ void plan_entry(const MaskBytes& m, int entry, int ke
   uint2* live = m.live + (int64_t)entry * units;
   int count = 0;
   for (int u0 = 0; u0 < units; u0 += 64 * kPlanWaves) {
-    uint32_t mine = 0;   // of unit u0 + threadIdx.x
-#pragma unroll 8
-    for (int i = 0; i < 32; ++i) {
-      const int key = (u0 + wave * 64 + 2 * i) * kUnit + lane;   // at most keys + 32767
-      const uint64_t both = __ballot(key < keys && row[key] != 0);
-      if (lane >> 1 == i) mine = (uint32_t)(lane & 1 ? both >> 32 : both);
-    }
+    const uint32_t mine = mask_word(row, u0 + wave * 64, keys);   // keys up to keys + 32767
     const int u = u0 + threadIdx.x;
     const uint64_t any = __ballot(mine != 0);
     if (u < units) bits[u] = mine;
@@ -1474,7 +1522,7 @@ MaskBytes mask_in(const void* mask, int64_t batch_stride, Args& A, uint8_t* work
   m.live = reinterpret_cast<uint2*>(workspace);
   m.bits = reinterpret_cast<uint32_t*>(m.live + (int64_t)A.batch * A.k_units);
   m.counts = reinterpret_cast<int*>(m.bits + (int64_t)A.batch * A.k_units);
-  A.mask = Mask{m.bits, m.live, m.counts};
+  A.mask = Mask{m.bits, m.live, m.counts, nullptr, 0};
   return m;
 }
 
@@ -1679,12 +1727,11 @@ int64_t join_blocks(const Cut& cut) { return cut.splits > 1 ? cut.blocks - cut.w
 
 template <typename T>
 void forward(const Args& A, const Cut& cut, hipStream_t s) {
-  const dim3 grid((unsigned)cut.grid());
+  const dim3 grid((unsigned)(few(A) ? (int64_t)A.batch * A.kv_heads * cut.splits : cut.grid()));
   if (few(A)) {
-    const dim3 blocks((unsigned)(A.batch * A.kv_heads * cut.splits));
-    if (A.mask.bits) attention_few_kernel<T, true><<<blocks, 64 * kFewWaves, 0, s>>>(A);
-    else attention_few_kernel<T, false><<<blocks, 64 * kFewWaves, 0, s>>>(A);
-  } else if (A.mask.bits) {
+    if (!A.mask.none()) attention_few_kernel<T, true><<<grid, 64 * kFewWaves, 0, s>>>(A);
+    else attention_few_kernel<T, false><<<grid, 64 * kFewWaves, 0, s>>>(A);
+  } else if (!A.mask.none()) {
     if (A.lse) attention_kernel<T, true, true><<<grid, kThreads, 0, s>>>(A);
     else attention_kernel<T, true, false><<<grid, kThreads, 0, s>>>(A);
   } else {
@@ -1715,10 +1762,14 @@ void backward(const MaskBytes& mask, const Args& A, const Gradients& plan, hipSt
   if (q + k) attention_join_kernel<T, false, false><<<(unsigned)((q + k) * (kQueries / 8)), 256, 0, s>>>(A, q);
 }
 
+// Whether the forward pass's waves find the live units themselves, one a lane, which spares a launch (3 x 12 heads of 77
+// tokens 9.8 us, with the launch 11.9; 2 x 24 of 512 23.3 and 25.7, 8 x 24 of 2048 406 and 405).
+bool waves_find(const Args& A) { return A.k_units <= 64; }
+
 int64_t workspace_of(const Args& A, bool masked, bool backward) {
   if (A.batch == 0 || A.queries == 0 || (A.keys == 0 && backward)) return 0;
   const int64_t mask = masked ? mask_bytes(A.batch, A.keys) : 0;
-  if (!backward) return mask + forward_cut(A).bytes();
+  if (!backward) return (waves_find(A) ? 0 : mask) + forward_cut(A).bytes();
   return mask + stats_bytes(A.batch, A.heads, A.queries) + plan_gradients(A).bytes();
 }
 
@@ -1760,10 +1811,16 @@ extern "C" int flk_attention(const void* q, const int64_t* q_strides, const void
   A.low = low;
   A.lse = lse;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const MaskBytes mask = mask_in(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace));
-  if (mask.mask) attention_mask_kernel<<<batch, 64 * kPlanWaves, 0, s>>>(mask, keys, A.k_units);
   const Cut cut = forward_cut(A);
-  A.of_q = cut.in(static_cast<uint8_t*>(workspace) + (key_mask ? mask_bytes(batch, keys) : 0));
+  uint8_t* parts = static_cast<uint8_t*>(workspace);
+  if (key_mask && waves_find(A)) {
+    A.mask = Mask{nullptr, nullptr, nullptr, static_cast<const uint8_t*>(key_mask), mask_batch_stride};
+  } else if (key_mask) {
+    const MaskBytes mask = mask_in(key_mask, mask_batch_stride, A, parts);
+    attention_mask_kernel<<<batch, 64 * kPlanWaves, 0, s>>>(mask, keys, A.k_units);
+    parts += mask_bytes(batch, keys);
+  }
+  A.of_q = cut.in(parts);
   A.part_top = A.of_q.part + cut.part_rows() * kD;
   if (dtype == FLK_BF16) forward<__bf16>(A, cut, s);
   else forward<_Float16>(A, cut, s);

@@ -68,7 +68,8 @@ def test_plan(lib):
     assert plan(1, 2, 2, 4, 4, 0, 0, None) == INVALID
     assert _bytes(lib, 0, 2, 2, 4, 4, 1, 1) == 0 and _bytes(lib, 1, 2, 2, 0, 4, 1, 1) == 0
     assert _bytes(lib, 1, 24, 24, 512, 64, 0, 0) == 0               # nothing to cut, no mask
-    assert _bytes(lib, 1, 24, 24, 512, 64, 1, 0) > 0
+    assert _bytes(lib, 1, 24, 24, 512, 64, 1, 0) == 0               # nor a mask that needs room
+    assert _bytes(lib, 1, 24, 24, 512, 2049, 1, 0) > 0
     assert _bytes(lib, 1, 24, 24, 1, 4608, 0, 0) > 0                # cut along the keys
     for b, h, kv, nq, nk in ((1, 24, 24, 4608, 4608), (3, 12, 4, 987, 1203), (2, 6, 1, 1, 2 ** 20), (1, 1, 1, 2 ** 20, 1)):
         for masked in (0, 1):
@@ -94,9 +95,10 @@ def test_forward_validation(lib):
     for kw in (dict(q=P + 8), dict(k=P + 2), dict(o=P + 4), dict(low=P + 8, lse=P), dict(low=P, lse=P + 2), dict(qs=_strides(0, 1280, 132)),
                dict(os=_strides(4, 128, 256))):
         assert _forward(lib, **kw) == ALIGN, kw
-    assert _forward(lib, mask=P) == SCRATCH
-    need = _bytes(lib, 1, 2, 2, 10, 10, 1, 0)
-    assert _forward(lib, mask=P, ws=P, nb=need - 1) == SCRATCH and _forward(lib, mask=P, ws=P + 16, nb=need) == ALIGN
+    assert _forward(lib, mask=P, nk=2049) == SCRATCH
+    need = _bytes(lib, 1, 2, 2, 10, 2049, 1, 0)
+    assert _forward(lib, mask=P, nk=2049, ws=P, nb=need - 1) == SCRATCH
+    assert _forward(lib, mask=P, nk=2049, ws=P + 16, nb=need) == ALIGN
 
 
 def _backward(lib, **kw):

@@ -420,3 +420,24 @@ def test_few_rows_leave_the_rest(device):
     assert torch.equal(out, want) and torch.isfinite(out).all()
     wide[:, 2:4, 32:32 + 4 * D] = 7.0
     assert (wide == 7.0).all()
+
+
+@pytest.mark.parametrize("mask", ["random", "middle", "last", "empty"])
+@pytest.mark.parametrize("queries,keys", [(1, 2047), (3, 2048), (2, 2049), (40, 2048), (40, 2080)])
+def test_masks_of_64_units_and_more(device, queries, keys, mask):
+    """Up to 64 units each wave finds the live ones itself; past them a launch does."""
+    check(keys, 2, 2, 1, queries, keys, "bf16", mask)
+
+
+@pytest.mark.parametrize("keys", [67, 2300])
+def test_mask_views(device, keys):
+    """Rows of a wider mask that start at any byte, one row for every entry, and bytes that are not 1."""
+    q, k, v, _, keep = make(3, 3, 2, 2, 20, keys, "bf16", "random")
+    want = A.attention(q, k, v, key_mask=keep)
+    wide = torch.zeros(3, keys + 9, dtype=torch.bool, device=device)
+    wide[:, 5:5 + keys] = keep
+    assert torch.equal(want, A.attention(q, k, v, key_mask=wide[:, 5:5 + keys]))
+    assert torch.equal(want, A.attention(q, k, v, key_mask=(keep.to(torch.uint8) * 128).view(torch.bool)))
+    row = keep[:1].expand(3, -1)
+    k, v = (torch.where(row[:, None, :, None], torch.randn_like(t), t.new_tensor(float("nan"))) for t in (k, v))
+    assert torch.equal(A.attention(q, k, v, key_mask=row), A.attention(q, k, v, key_mask=row.contiguous()))
