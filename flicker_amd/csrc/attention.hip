@@ -713,11 +713,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
     forward_wave<T, kMasked, kKeep, 1>(A, smem, piece, rows.b, rows.h, rows.first, rows.end, rows.q0);
 }
 
-// o of few rows: the queries of all heads that share a key head, at most 16 rows, so that each key is read once.  Bound by
-// memory, and where few blocks walk many units by its latency.  The four waves walk units of their own (every fourth of the
-// block's), each copied into the wave's own LDS two ahead: no barrier, and 64 to 128 KB on their way to a CU.  The waves'
-// sums are joined at the end.  One query of 24 heads: 4608 keys 19 us with the join (57 MB, 14 of them this kernel), 16896
-// keys 46 us (4.5 TB/s), 8 x 4608 85 us (5.3 TB/s).  Two blocks of two waves a CU: 22.3, 50.6, 89.6.
+// o of 16 rows, among the queries of all heads that share a key head, so that for a single query of each every key is read
+// once.  For few rows: bound by memory, and where few blocks walk many units by its latency.  The four waves walk units of their
+// own (every fourth of the block's), each copied into the wave's own LDS two ahead: no barrier, and 64 to 128 KB on their
+// way to a CU.  The waves' sums are joined at the end.  One query of 24 heads: 4608 keys 19 us with the join (57 MB, 14 of
+// them this kernel), 16896 keys 46 us (4.5 TB/s), 8 x 4608 85 us (5.3 TB/s).  Two blocks of two waves a CU: 22.3, 50.6, 89.6.
 constexpr int kFewWaves = 4, kFewRing = 2;
 constexpr int kFewBytes = (2 * kFewRing * kUnit + kFewRows) * kRowBytes;   // of a wave: K ring, V ring, Q
 
@@ -738,7 +738,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kFewWaves * kFewBytes];
   const int lane = threadIdx.x & 63, h4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int p = by_xcd(blockIdx.x, gridDim.x), splits = A.of_q.splits, split = p % splits, block = p / splits;
-  const int b = block / A.kv_heads, hk = block - b * A.kv_heads, rows = A.group * A.queries;
+  const int rows = A.group * A.queries, tiles = (rows + kFewRows - 1) / kFewRows, bk = block / tiles;
+  const int b = bk / A.kv_heads, hk = bk - b * A.kv_heads, row0 = (block - bk * tiles) * kFewRows;
   uint2 some;   // of a masked entry: 64 of the wave's units, one a lane
   int all = A.k_units;
   if constexpr (kMasked) {
@@ -781,7 +782,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
     get(1, unit[1], bits[1]);
 #pragma unroll
     for (int i = 0; i < kFewRows / 4; ++i) {   // row gi * queries + qi is query qi of the key head's query head gi
-      const int r = 4 * i + h4, at = min(r, rows - 1), gi = at / A.queries;
+      const int r = 4 * i + h4, at = min(row0 + r, rows - 1), gi = at / A.queries;
       const uint16_t* src = A.q.at<uint16_t>(b, hk * A.group + gi) + (at - gi * A.queries) * A.q.row;
       flk::dma16(src + (((lane & 15) ^ swz(r)) << 3), q_rows + i * 4 * kRowBytes);
     }
@@ -862,7 +863,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
   if (h4 == 0) *reinterpret_cast<f32x4*>(sums + kFewRows * kPitch + lane * 4) = f32x4{top, l[0], sum, 0.0f};
   __syncthreads();
   const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
-  if (row >= rows) return;
+  if (row0 + row >= rows) return;
   f32x4 t[kFewWaves], o[2] = {};
   top = -1e30f;
 #pragma unroll
@@ -881,9 +882,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
     total += t[i][1] * f;
     sum += t[i][2] * f;
   }
-  const int gi = row / A.queries, qi = row - gi * A.queries, h = hk * A.group + gi;
-  if (splits > 1) {
-    const int64_t at = ((int64_t)(b * A.heads + h) * splits + split) * kFewRows + qi;
+  const int gi = (row0 + row) / A.queries, qi = row0 + row - gi * A.queries, h = hk * A.group + gi;
+  if (splits > 1) {   // as if a head's queries had blocks of their own
+    const int blocks = (A.queries + kFewRows - 1) / kFewRows;
+    const int64_t of = (int64_t)(b * A.heads + h) * blocks + qi / kFewRows, at = (of * splits + split) * kFewRows + qi % kFewRows;
     f32x4* part = reinterpret_cast<f32x4*>(A.of_q.part + at * kD + d);
     part[0] = o[0];
     part[1] = o[1];
@@ -1567,26 +1569,35 @@ Cut plan_queries(const Args& A, double unit, double unit192) {
   const Cut wide = plan(kQueries, unit), narrow = plan(192, unit192);
   return narrow.blocks <= kCUs && narrow.time < wide.time ? narrow : wide;
 }
-// Few rows go through attention_few_kernel, one query of 24 heads on 4608 keys in 19 us (through the blocks above in 22.4), on
-// 512 in 8.5 (12.9), of 8 entries in 85 (101), on 4 key heads in 11.2 (18.9), 16 queries in 20 (23.2).
-bool few(const Args& A) { return A.queries <= kFewRows && A.group <= kFewRows / A.queries; }
-// us of a unit: of a block alone, more for every other block, and of a block on each CU at memory's rate; of launches; of the
-// join's, and its for each cut.
-constexpr double kFewUnit = 0.37, kFewMore = 0.001, kFewFull = 0.72, kFewFixed = 4.0, kFewJoin = 4.0, kFewCut = 0.06;
+// us of a unit: of a block alone, more for every other that reads other keys, and at memory's rate of a block on each CU that
+// does; of the first round of blocks, with its launch, and of each other; of the join's launch, and its for each cut.
+constexpr double kFewUnit = 0.32, kFewMore = 0.0013, kFewFull = 0.72, kFewFixed = 4.0, kFewRound = 2.8, kFewJoin = 4.0,
+                 kFewCut = 0.06;
+int64_t few_blocks(const Args& A) {
+  return (int64_t)A.batch * A.kv_heads * (((int64_t)A.group * A.queries + kFewRows - 1) / kFewRows);
+}
 Cut plan_few(const Args& A) {
-  const int64_t blocks = (int64_t)A.batch * A.kv_heads, heads = (int64_t)A.batch * A.heads;
-  Cut best{(int)heads, 1, kFewRows, heads, 1e300};
+  const int64_t blocks = few_blocks(A), joined = (int64_t)A.batch * A.heads * ((A.queries + kFewRows - 1) / kFewRows);
+  Cut best{(int)joined, 1, kFewRows, joined, 1e300};
   for (int s = 1; s <= kMaxSplits && (s == 1 || (kFewWaves * s <= A.k_units && blocks * s <= 4 * kCUs)); ++s) {
     const int64_t grid = blocks * s, rounds = (grid + kCUs - 1) / kCUs;
     const int turns = ((A.k_units + s - 1) / s + kFewWaves - 1) / kFewWaves;
-    const double at_once = (double)std::min<int64_t>(grid, kCUs);
-    const double unit = std::max(kFewUnit + kFewMore * at_once, kFewFull * at_once / kCUs);
-    const double time = rounds * (turns * kFewWaves * unit + kFewFixed) + (s > 1 ? kFewJoin + kFewCut * s : 0.0);
-    if (time < best.time) best = Cut{s > 1 ? 0 : (int)heads, s, kFewRows, heads, time};
+    const double others = (double)std::min<int64_t>(grid, kCUs) * A.batch * A.kv_heads / blocks;
+    const double unit = std::max(kFewUnit + kFewMore * others, kFewFull * others / kCUs);
+    const double time = rounds * (turns * kFewWaves * unit + kFewRound) + kFewFixed - kFewRound +
+                        (s > 1 ? kFewJoin + kFewCut * s : 0.0);
+    if (time < best.time) best = Cut{s > 1 ? 0 : (int)joined, s, kFewRows, joined, time};
   }
   return best;
 }
-Cut forward_cut(const Args& A) { return few(A) ? plan_few(A) : plan_queries(A, 0.82, 0.69); }
+// Blocks of 16 rows where they take less, by the estimates and kStart more for blocks of 256.  24 heads, us in blocks of 16
+// and 256: one query of 512 keys 8.5 and 12.9, of 4608 19 and 22.4 (on 4 key heads 11.4 and 18.9, of 8 entries 85 and 101),
+// 64 queries of 4608 33.5 and 23; 128 tokens 5.2 and 11.6, 256 11.1 and 16.6, 384 19.8 and 19.0, 512 24.4 and 21.0.
+constexpr double kStart = 3.0;
+Cut forward_cut(const Args& A) {
+  const Cut few = plan_few(A), many = plan_queries(A, 0.82, 0.69);
+  return few.time < many.time + kStart ? few : many;
+}
 
 // When the CUs, each taking the next block as it ends one, have done runs of equal blocks.
 class Schedule {
@@ -1727,8 +1738,9 @@ int64_t join_blocks(const Cut& cut) { return cut.splits > 1 ? cut.blocks - cut.w
 
 template <typename T>
 void forward(const Args& A, const Cut& cut, hipStream_t s) {
-  const dim3 grid((unsigned)(few(A) ? (int64_t)A.batch * A.kv_heads * cut.splits : cut.grid()));
-  if (few(A)) {
+  const bool few = cut.tile == kFewRows;
+  const dim3 grid((unsigned)(few ? few_blocks(A) * cut.splits : cut.grid()));
+  if (few) {
     if (!A.mask.none()) attention_few_kernel<T, true><<<grid, 64 * kFewWaves, 0, s>>>(A);
     else attention_few_kernel<T, false><<<grid, 64 * kFewWaves, 0, s>>>(A);
   } else if (!A.mask.none()) {

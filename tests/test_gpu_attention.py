@@ -441,3 +441,11 @@ def test_mask_views(device, keys):
     row = keep[:1].expand(3, -1)
     k, v = (torch.where(row[:, None, :, None], torch.randn_like(t), t.new_tensor(float("nan"))) for t in (k, v))
     assert torch.equal(A.attention(q, k, v, key_mask=row), A.attention(q, k, v, key_mask=row.contiguous()))
+
+
+@pytest.mark.parametrize("queries,keys,mask,dtype", [
+    (33, 1, None, "bf16"), (33, 31, None, "fp16"), (47, 64, "random", "bf16"), (63, 129, "middle", "fp16"), (40, 97, "none", "bf16"),
+    (40, 97, "first", "bf16"), (65, 66, "empty", "fp16"), (34, 300, "random", "bf16"), (257, 33, "last", "bf16")])
+def test_many_heads(device, queries, keys, mask, dtype):
+    """Short sequences of enough heads that blocks of 256 queries take them, not blocks of 16."""
+    check(queries, 64, 8, 8, queries, keys, dtype, mask)
