@@ -451,10 +451,10 @@ struct Forward {
 };
 
 // P is held as exp2(log2(e) (S - top) - kShift<T>), where top is the maximum of an earlier unit's row; it has to rise where
-// a P passes 2.  bfloat16 has float32's range: P 2^-60 leaves 2^61 for S to rise by, and no precision is lost at the
-// bottom.  That P passes 2 is then one bit of its packed form.  float16 has neither: exponents are compared with kSlack.
+// a P passes 2.  bfloat16 has float32's range: P 2^-20 leaves 2^21 for S to rise by, and 2^-106 for P v, the sums' smallest
+// terms (2^-60 takes the same time).  That P passes 2 is then one bit of its packed form.  float16 has neither: exponents are compared with kSlack.
 template <typename T>
-constexpr float kShift = sizeof(T) == 2 && __is_same(T, __bf16) ? 60.0f : 0.0f;
+constexpr float kShift = sizeof(T) == 2 && __is_same(T, __bf16) ? 20.0f : 0.0f;
 constexpr float kSlack = 9.0f;
 
 // Slot n's share of the 8 G elements that a phase of 16 slots turns into P: one multiplied, the one before it

@@ -449,3 +449,13 @@ def test_mask_views(device, keys):
 def test_many_heads(device, queries, keys, mask, dtype):
     """Short sequences of enough heads that blocks of 256 queries take them, not blocks of 16."""
     check(queries, 64, 8, 8, queries, keys, dtype, mask)
+
+
+@pytest.mark.parametrize("batch,queries", [(2, 5), (64, 33)])
+@pytest.mark.parametrize("size,scale", [(2.0 ** -80, 1.0), (2.0 ** 100, 1.0), (2.0 ** -80, 30.0)])
+def test_sizes_of_values(device, batch, queries, size, scale):
+    """Values far from 1 in either direction: bfloat16 has float32's range, and sums of P v keep it."""
+    q, k, v, do, keep = make(9, batch, 8, 8, queries, 100, "bf16", "random", scale=scale)
+    v = torch.where(keep[:, None, :, None], v * size, v)
+    want = expected(q, k, v, do, keep)
+    _close("o", A.attention(q, k, v, key_mask=keep), *want[0])
