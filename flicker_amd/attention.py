@@ -11,6 +11,7 @@ lengths, several query heads to a key head, and a mask over each batch entry's k
 
 Statistics and sums are float32; P, and backwards dS, are rounded to the operands' type, which the matrix cores take,
 and every output is rounded once.  In float16 that rounding has the type's range: a dS below 2^-25 is zero.
+In bfloat16 a term P v below 2^-106 is.
 For gradients through torch's autograd see ``flicker_amd.autograd``.
 """
 
