@@ -77,6 +77,7 @@ SIGNATURES = {
     "flk_residual_norm_backward": (_i, [*[_p, _i64, _i64] * 4, _i, _p, _p, _i, _i64, _i, _f, _i, _i, _i,
                                         *[_p, _i64, _i64] * 2, _p, _p, _p, _p, _i64, _p]),
     "flk_attention_plan": (_i, [_i, _i, _i, _i, _i, _i, _i, _sp]),
+    "flk_attention_blocks": (_i, [_i, _i, _i, _i, _i, _i, _ip]),
     "flk_attention": (_i, [_p, _sp, _p, _sp, _p, _sp, _i, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _sp, _p, _p, _p, _i64, _p]),
     "flk_attention_backward": (_i, [*[_p, _sp] * 5, _p, _p, _i, _p, _i64, _i, _i, _i, _i, _i, _i, *[_p, _sp] * 3,
                                     _p, _i64, _p]),

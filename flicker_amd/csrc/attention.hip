@@ -1795,6 +1795,29 @@ extern "C" int flk_attention_plan(int batch, int heads, int kv_heads, int querie
   return FLK_OK;
 }
 
+extern "C" int flk_attention_blocks(int batch, int heads, int kv_heads, int queries, int keys, int backward, int* blocks) {
+  if (!blocks || !sizes_ok(batch, heads, kv_heads, queries, keys)) return FLK_E_INVALID;
+  std::fill(blocks, blocks + 8, 0);
+  if (batch == 0 || queries == 0 || (keys == 0 && backward)) return FLK_OK;
+  const Args A = sizes(batch, heads, kv_heads, queries, keys);
+  auto report = [](const Cut& cut, int64_t all, int* to) {
+    to[0] = cut.tile;
+    to[1] = (int)(all - join_blocks(cut));
+    to[2] = (int)join_blocks(cut);
+    to[3] = cut.splits;
+  };
+  if (backward) {
+    const Gradients plan = plan_gradients(A);
+    report(plan.q, plan.q.blocks, blocks);
+    report(plan.k, plan.k.blocks, blocks + 4);
+    return FLK_OK;
+  }
+  const Cut cut = forward_cut(A);
+  report(cut, cut.blocks, blocks);
+  if (cut.tile == kFewRows) blocks[cut.splits > 1 ? 2 : 1] = (int)few_blocks(A);   // all of them are cut or none
+  return FLK_OK;
+}
+
 extern "C" int flk_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                              const void* v, const int64_t* v_strides, int dtype, const void* key_mask,
                              int64_t mask_batch_stride, int batch, int heads, int kv_heads, int queries, int keys,

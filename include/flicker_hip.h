@@ -545,6 +545,10 @@ int flk_mlp_matmul(const void* a, int64_t a_row_stride, int a_transposed, const 
  * call's kernels have run, and needs no initial value. */
 int flk_attention_plan(int batch, int heads, int kv_heads, int queries, int keys, int masked, int backward,
                        int64_t* workspace_bytes);
+/* How a call's work is split, in `blocks`, eight values: of the blocks of queries their rows (16: of all query heads
+ * that share a key head), how many are whole, how many are cut along the keys, and into how many pieces each; the same of
+ * the gradients' blocks of keys (zeros forwards).  All zeros where there is nothing to compute. */
+int flk_attention_blocks(int batch, int heads, int kv_heads, int queries, int keys, int backward, int* blocks);
 int flk_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                   const int64_t* v_strides, int dtype, const void* key_mask, int64_t mask_batch_stride, int batch,
                   int heads, int kv_heads, int queries, int keys, int head_dim, void* o, const int64_t* o_strides,
