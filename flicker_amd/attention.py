@@ -9,7 +9,8 @@ lengths, several query heads to a key head, and a mask over each batch entry's k
 ``attention_backward`` returns the gradients of q, k and v; it takes what the forward call keeps with
 ``keep=True``.  As for ``attend``, q comes scaled by 1 / sqrt(D) (``Freqs.q_gain``).
 
-Statistics and sums are float32; P, and backwards dS, are rounded to the operands' type, which the matrix cores take,
+Logits may have any size that float32 holds; backwards P = exp(S - lse) is off by lse's rounding, up to 2^-24 |lse| of
+itself.  Statistics and sums are float32; P, and backwards dS, are rounded to the operands' type, which the matrix cores take,
 and every output is rounded once.  In float16 that rounding has the type's range: a dS below 2^-25 is zero.
 In bfloat16 a term P v below 2^-106 is.
 For gradients through torch's autograd see ``flicker_amd.autograd``.

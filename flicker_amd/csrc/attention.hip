@@ -65,6 +65,7 @@ constexpr int kKeys = 16 * kWaves;     // keys of a block, 32 a pair of waves
 constexpr int kFewRows = 16;           // rows of a block of attention_few_kernel
 constexpr int kLead = 4;               // slots between an operand's LDS read and its MFMAs
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLowest = -3.402823466e38f;   // a running maximum of no keys
 constexpr int64_t kMaxItems = 1LL << 31;
 constexpr int64_t kMaxRow = 1LL << 25;   // elements between two rows: a unit's byte offsets stay below 2^31
 
@@ -136,7 +137,7 @@ struct Args {
   Tensor q, k, v, o, dO, dq, dk, dv;
   void* low;        // (batch, queries, heads, 128): what o's rounding left, in the same type
   float* lse;       // (batch, heads, queries)
-  float* stats;     // (batch * heads * q_units + 1, 2, 32): a unit's log2(e) lse and -delta; inf and 0 in rows past the
+  float* stats;     // (batch * heads * q_units + 1, 2, 32): a unit's lse and -delta; inf and 0 in rows past the
                     // end and in the last unit
   Mask mask;
   int batch, heads, kv_heads, group, queries, keys, q_units, k_units;
@@ -447,6 +448,7 @@ struct Forward {
   vec8<T> ones;            // row 0 ones, rows 1-15 zeros
   float sum[G];            // with kKeep: of the unrounded P, this lane's
   float top[G], base[G];   // the maximum that P is taken against, and -log2(e) times it less kShift
+  bool far;                // whether base holds one of them too coarsely, or there is none yet
   Places at;
 };
 
@@ -456,6 +458,10 @@ struct Forward {
 template <typename T>
 constexpr float kShift = sizeof(T) == 2 && __is_same(T, __bf16) ? 20.0f : 0.0f;
 constexpr float kSlack = 9.0f;
+// base is rounded, by up to 2^-12 at this size of top, which takes 2^-12 off the exponents of P, and past 2^28 their range.  Beyond it
+// (and before the first maximum) each unit's P are formed again from the differences S - top, which are exact where it matters.
+// From the differences at once: 4608 tokens 244 us rather than 237.
+constexpr float kFar = 4096.0f;
 
 // Slot n's share of the 8 G elements that a phase of 16 slots turns into P: one multiplied, the one before it
 // exponentiated, and the two before that packed.
@@ -536,7 +542,8 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
     __builtin_amdgcn_sched_barrier(0);
   }
   // top rises to the row's maximum, what has been summed is scaled, and this unit's P are formed again
-  if (__any(kBits ? (any & 0x40004000u) != 0 : high > kSlack)) {
+  if (w.far || __any(kBits ? (any & 0x40004000u) != 0 : high > kSlack)) {
+    bool far = false;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       float x = sv[2 * g][0];
@@ -547,6 +554,7 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
       const float factor = __builtin_amdgcn_exp2f((w.top[g] - x) * kLog2e);
       w.top[g] = x;
       w.base[g] = x * -kLog2e - kShift<T>;
+      far |= fabsf(x) > kFar;
       sum[g] = 0.0f;
       w.sum[g] *= factor;
       w.l[g] *= factor;   // row 0 of l sits in the lanes 0-15, whose columns are these queries
@@ -554,11 +562,12 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
       for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] *= factor;
 #pragma unroll
       for (int n = 8 * g; n < 8 * g + 8; ++n) {
-        scaled(n);
+        t[n] = __builtin_fmaf(sv[n >> 2][n & 3] - x, kLog2e, -kShift<T>);
         exp(n);
         if (n & 1) put(n - 1);
       }
     }
+    w.far = __any(far);
   }
   if constexpr (kKeep) {
 #pragma unroll
@@ -582,9 +591,10 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
     w.l[g] = f32x4{};
     w.sum[g] = 0.0f;
-    w.top[g] = -1e30f;
-    w.base[g] = 1e30f * kLog2e - kShift<T>;
+    w.top[g] = kLowest;
+    w.base[g] = 0.0f;
   }
+  w.far = true;
   if (n) {
     auto k_slot = [&](int i) { return smem + (i & (kKRing - 1)) * kUnitBytes; };
     auto v_slot = [&](int i) { return smem + (kKRing + (i & (kVRing - 1))) * kUnitBytes; };
@@ -754,7 +764,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
   uint8_t* const q_rows = mine + 2 * kFewRing * kUnitBytes;
 
   f32x4 acc[8], l{};
-  float sum = 0.0f, top = -1e30f;
+  float sum = 0.0f, top = kLowest;
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{};
   if (n) {
@@ -865,7 +875,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
   const int row = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
   if (row0 + row >= rows) return;
   f32x4 t[kFewWaves], o[2] = {};
-  top = -1e30f;
+  top = kLowest;
 #pragma unroll
   for (int i = 0; i < kFewWaves; ++i) {
     t[i] = *reinterpret_cast<const f32x4*>(smem + i * kFewBytes + (kFewRows * kPitch + row * 4) * 4);
@@ -914,7 +924,8 @@ struct Dq {
   vec8<T> x[4][G], g[4][G];   // Q^T, dO^T
   f32x4 acc[8][G];            // dQ^T
   vec8<T> ops[2 * kLead];
-  float lse[G], delta[G];     // -log2(e) lse, -delta
+  float lse[G];
+  f32x4 delta[G];             // -delta, from which dP's sums start
   Places at;
 };
 
@@ -935,11 +946,10 @@ __device__ __forceinline__ void dq_phase(Dq<T, G>& w, const f32x4 (&s_cur)[2 * G
   if constexpr (kPartial)
     if (bits != ~0u) leave_out(sv, bits);
   float t[8 * G], e[8 * G];
-  auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, w.lse[n >> 3]); };
+  auto scaled = [&](int n) { t[n] = (sv[n >> 2][n & 3] - w.lse[n >> 3]) * kLog2e; };
   auto exp = [&](int n) { e[n] = __builtin_amdgcn_exp2f(t[n]); };
   auto put = [&](int n) {
-    const float x = e[n] * (dv[n >> 2][n & 3] + w.delta[n >> 3]), y = e[n + 1] * (dv[n >> 2][(n & 3) + 1] + w.delta[n >> 3]);
-    p_cur[n >> 1] = pack<T>(x, y);
+    p_cur[n >> 1] = pack<T>(e[n] * dv[n >> 2][n & 3], e[n + 1] * dv[n >> 2][(n & 3) + 1]);
     asm volatile("" : "+v"(p_cur[n >> 1]));
   };
   vec8<T> pb[G];
@@ -956,7 +966,7 @@ __device__ __forceinline__ void dq_phase(Dq<T, G>& w, const f32x4 (&s_cur)[2 * G
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       if (n < 8) s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : f32x4{});
-      else if (n < 16) d_next[2 * g + kt] = mfma(a, w.g[st][g], st ? d_next[2 * g + kt] : f32x4{});
+      else if (n < 16) d_next[2 * g + kt] = mfma(a, w.g[st][g], st ? d_next[2 * g + kt] : w.delta[g]);
       else w.acc[n - 16][g] = mfma(a, pb[g], w.acc[n - 16][g]);
     }
     const int m = n + kLead;
@@ -985,8 +995,9 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
   for (int g = 0; g < G; ++g) {
     const int r = q0 + g * 16 + (lane & 15);
     const float* st = A.stats + ((int64_t)bh * A.q_units + r / kUnit) * 2 * kUnit + r % kUnit;
-    w.lse[g] = r < end ? -st[0] : -INFINITY;
-    w.delta[g] = r < end ? st[kUnit] : 0.0f;
+    w.lse[g] = r < end ? st[0] : INFINITY;
+    const float delta = r < end ? st[kUnit] : 0.0f;
+    w.delta[g] = f32x4{delta, delta, delta, delta};
   }
 #pragma unroll
   for (int g = 0; g < G; ++g)
@@ -1027,7 +1038,7 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : f32x4{});
-          d0[2 * g + kt] = mfma(c, w.g[st][g], st ? d0[2 * g + kt] : f32x4{});
+          d0[2 * g + kt] = mfma(c, w.g[st][g], st ? d0[2 * g + kt] : w.delta[g]);
         }
       }
     }
@@ -1086,7 +1097,7 @@ struct Dkv {
   vec8<T> x[4][2];         // K^T (V^T)
   f32x4 acc[8][2];         // dV^T (dK^T)
   vec8<T> ops[2 * kLead];
-  f32x4 stat[2];           // this phase's log2(e) lse (-delta) of the rows of each accumulator
+  f32x4 stat[2];           // this phase's lse (-delta) of the rows of each accumulator
   Places at;
 };
 
@@ -1107,7 +1118,7 @@ __device__ __forceinline__ void dkv_phase(Dkv<T>& w, const f32x4 (&s_cur)[4], f3
     if constexpr (kSecond) e4[i] = mine[64 * i];
   }
   float t[16];
-  auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, -w.stat[n >> 2 & 1][n & 3]); };
+  auto scaled = [&](int n) { t[n] = (sv[n >> 2][n & 3] - w.stat[n >> 2 & 1][n & 3]) * kLog2e; };
   auto exp = [&](int n) { e4[n >> 2][n & 3] = __builtin_amdgcn_exp2f(t[n]); };
   auto put = [&](int n) {
     float x = e4[n >> 2][n & 3], y = e4[n >> 2][(n & 3) + 1];
@@ -1373,11 +1384,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q
     // lane i of the row's 32 holds the factors of the cuts i and i + 32
     const f32x4* tops = reinterpret_cast<const f32x4*>(A.part_top) + (int64_t)cut_block * cuts.splits * pitch + r;
     f32x4 t[2];
-    float top = -1e30f, l = 0.0f, sum = 0.0f, f[2];
+    float top = kLowest, l = 0.0f, sum = 0.0f, f[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int at = lane + 32 * i;
-      t[i] = at < cuts.splits ? tops[(int64_t)at * pitch] : f32x4{-1e30f, 0.0f, 0.0f, 0.0f};
+      t[i] = at < cuts.splits ? tops[(int64_t)at * pitch] : f32x4{kLowest, 0.0f, 0.0f, 0.0f};
       top = fmaxf(top, t[i][0]);
     }
 #pragma unroll
@@ -1505,7 +1516,7 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_prepare_kernel(cons
       sum += live ? (float)x[i][0][e] * ((float)x[i][1][e] + (float)x[i][2][e]) : 0.0f;
     sum = flk::row16_sum(sum);
     if (lane == 0) {
-      st[16 * i] = live ? lse[i] * kLog2e : INFINITY;
+      st[16 * i] = live ? lse[i] : INFINITY;
       st[16 * i + kUnit] = -sum;
     }
   }

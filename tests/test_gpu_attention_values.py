@@ -1,0 +1,84 @@
+"""attention and its gradients where values are far from what a norm leaves: logits up to the type's and float32's ends,
+infinities and NaN in operands that are not masked.  Each in every form of the forward pass (attention_forms.FORMS)."""
+
+import pytest
+import torch
+
+from flicker_amd import attention as A
+from tests.attention_forms import FORMS
+from tests.test_gpu_attention import D, TYPES, U
+
+pytestmark = pytest.mark.gpu
+SHORT = ["16", "16 cut", "192", "192 cut", "256", "256 cut", "256 both", "256 shared"]
+
+
+def exact_logits(seed, form, dtype, q_size, k_size, masked, negative, device):
+    """q rows of one value +-q_size, k of whole numbers times k_size: logits that float32 holds exactly, in each row one largest
+    that is far above the others.  (q, k, v, do, keep, index (B, H, Lq) of the largest's key, its logit)."""
+    batch, heads, kv_heads, queries, keys = FORMS[form][0]
+    g = torch.Generator().manual_seed(seed)
+    n = torch.randint(-99, -1 if negative else 100, (batch, kv_heads, keys, D), generator=g).double()
+    keep = torch.rand(batch, keys, generator=g) < 0.7 if masked else torch.ones(batch, keys, dtype=torch.bool)
+    keep[:, keys // 2:keys // 2 + 2] = True
+    high, low = torch.empty(batch, kv_heads, D, dtype=torch.long), torch.empty(batch, kv_heads, D, dtype=torch.long)
+    for b in range(batch):
+        on = keep[b].nonzero().flatten()
+        for h in range(kv_heads):
+            for i, (to, value) in enumerate(((low, -100.0), (high, -1.0 if negative else 100.0))):   # of different keys
+                to[b, h] = on[i::2][torch.randint(len(on) // 2, (D,), generator=g)]
+                n[b, h].scatter_(0, to[b, h][None], value)
+    n[~keep[:, None, :].expand(batch, kv_heads, keys)] = 127.0
+    column = torch.arange(queries) % D
+    sign = torch.ones(batch, heads, queries) if negative else torch.randint(0, 2, (batch, heads, queries), generator=g) * 2.0 - 1
+    q = torch.zeros(batch, heads, queries, D, dtype=torch.float64)
+    q[:, :, torch.arange(queries), column] = sign.double() * q_size
+    group = heads // kv_heads
+    high, low = (t.repeat_interleave(group, 1)[:, :, column] for t in (high, low))
+    index = torch.where(sign > 0, high, low)
+    top = sign * q_size * k_size * n.repeat_interleave(group, 1)[torch.arange(batch)[:, None, None], torch.arange(heads)[:, None], index,
+                                                                column]
+    t = TYPES[dtype]
+    v = torch.randn(batch, kv_heads, keys, D, generator=g).to(t)
+    do = torch.randn(batch, queries, heads * D, generator=g).to(t)
+    return [x.to(device) for x in (q.to(t), (n * k_size).to(t), v, do, keep, index, top)]
+
+
+SIZES = [("fp16", 2.0 ** 6, 2.0 ** 6), ("fp16", 2.0 ** 15, 2.0 ** 9), ("bf16", 2.0 ** 10, 2.0 ** 15), ("bf16", 2.0 ** 40, 2.0 ** 56),
+         ("bf16", 2.0 ** 60, 2.0 ** 60)]
+
+
+@pytest.mark.parametrize("form", SHORT)
+@pytest.mark.parametrize("negative", [False, True])
+@pytest.mark.parametrize("dtype,q_size,k_size", SIZES)
+def test_far_logits(device, form, dtype, q_size, k_size, negative):
+    """The logits' differences are all of q_size * k_size >= 2^12 and more, so the largest's P is 1 and the others' 0: o is that
+    key's v, exactly; lse its logit, off by a rounding and 2^-20 of a logarithm; dv the sums of do, off by their additions, at
+    most queries * group + 64 deep, and by P's error, 8 u |lse|, where |lse| is less than 2^23 (past it lse is that logit).  dS is
+    what dP and delta leave of each other: 2 * 130 u sum|do v| and, from o's rounding being held to e^2, sum|do o| e^2."""
+    print(f"far logits {form} {dtype} {q_size} {k_size} {negative}", flush=True)
+    masked = form != "192"
+    q, k, v, do, keep, index, top = exact_logits(1, form, dtype, q_size, k_size, masked, negative, device)
+    mask = keep if masked else None
+    (batch, heads, queries, _), (_, kv_heads, keys, _) = q.shape, k.shape
+    group = heads // kv_heads
+    o, kept = A.attention(q, k, v, key_mask=mask, keep=True)
+    pick = index[..., None].expand(-1, -1, -1, D)
+    want = v.repeat_interleave(group, 1).gather(2, pick).transpose(1, 2).reshape(o.shape)
+    assert torch.equal(o, want) and torch.equal(A.attention(q, k, v, key_mask=mask), want)
+    assert ((kept.lse.double() - top).abs() <= 2 * U * top.abs() + 2.0 ** -20).all()
+    dq, dk, dv = A.attention_backward(do, q, k, v, kept, key_mask=mask)
+    g4 = do.view(batch, queries, heads, D).transpose(1, 2).double()
+    sums, sizes = (torch.zeros(batch, heads, keys, D, dtype=torch.float64, device=device).scatter_add_(2, pick, t).view(
+        batch, kv_heads, group, keys, D).sum(2) for t in (g4, g4.abs()))
+    e = torch.finfo(q.dtype).eps / 2
+    p_off = 8 * U * min(float(top.abs().max()), 2.0 ** 23)
+    p_off = p_off + e if p_off > 0 else e
+    off = (p_off + (queries * group + 64) * U) * sizes
+    tiny = 2.0 ** -25 if dtype == "fp16" else 0.0
+    assert ((dv.double() - sums).abs() <= e * (sums.abs() + off) + off + tiny).all()
+    o4 = want.view(batch, queries, heads, D).transpose(1, 2).double()
+    ds = ((260 * U + e * e) * (1 + p_off) * (g4.abs() * o4.abs()).sum(-1, keepdim=True))
+    size = k.double().abs().repeat_interleave(group, 1).gather(2, pick)
+    # what lies below float16's range in dS is dropped or kept, off by 2^-25 at most
+    assert (dq.double().abs() <= (ds + tiny) * (1 + e) * size + tiny).all()
+    assert torch.isfinite(dq).all() and torch.isfinite(dk).all()
