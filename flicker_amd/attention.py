@@ -109,8 +109,8 @@ def _split(o: torch.Tensor, heads: int) -> torch.Tensor:
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: torch.Tensor | None = None,
               keep: bool = False, out: torch.Tensor | None = None):
     """softmax(q k^T) v of q (B, H, Lq, D) and k, v (B, Hkv, Lk, D), bfloat16 or float16, Hkv dividing H, views of any
-    strides -> (B, Lq, H * D).  ``key_mask`` (B, Lk) bool is True where a key is kept; a query that keeps none gets zeros,
-    and what masked keys and values hold is never read into a result.  With ``keep`` also returns the ``Kept`` that
+    strides -> (B, Lq, H * D).  ``key_mask`` (B, Lk) bool is True where a key is kept; a query that keeps none (or
+    only such as its logits are -inf for) gets zeros, and what masked keys and values hold is never read into a result.  With ``keep`` also returns the ``Kept`` that
     attention_backward takes.  ``out`` may be a (B, Lq, H * D) view with strided rows that overlaps no operand."""
     if out is None:
         done = _native.attention(q, k, v, key_mask, keep)

@@ -463,6 +463,13 @@ constexpr float kSlack = 9.0f;
 // From the differences at once: 4608 tokens 244 us rather than 237.
 constexpr float kFar = 4096.0f;
 
+// What divides a row's sums, and its lse.  l, the sum of the rounded P, is 0 where no key is kept; a NaN among them stays one.
+__device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+template <typename T>
+__device__ __forceinline__ float lse_of(float top, float l, float sum) {
+  return l == 0.0f ? -INFINITY : top + (__builtin_amdgcn_logf(sum) + kShift<T>) * kLn2;
+}
+
 // Slot n's share of the 8 G elements that a phase of 16 slots turns into P: one multiplied, the one before it
 // exponentiated, and the two before that packed.
 template <int G, typename Scaled, typename Exp, typename Put>
@@ -695,13 +702,11 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const float l = __shfl(w.l[g][0], lane & 15);
-    scale[g] = l > 0.0f ? 1.0f / l : 0.0f;
+    scale[g] = inverse_of(l);
     if constexpr (kKeep) {
       const float sum = across(w.sum[g]);
       const int r = q0 + g * 16 + (lane & 15);
-      if (h4 == 0 && r < end)
-        A.lse[(int64_t)bh * A.queries + r] =
-            l > 0.0f ? w.top[g] + (__builtin_amdgcn_logf(sum) + kShift<T>) * kLn2 : -INFINITY;
+      if (h4 == 0 && r < end) A.lse[(int64_t)bh * A.queries + r] = lse_of<T>(w.top[g], l, sum);
     }
   }
   T* low = nullptr;
@@ -902,7 +907,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
     if (d == 0) reinterpret_cast<f32x4*>(A.part_top)[at] = f32x4{top, total, sum, 0.0f};
     return;
   }
-  const float scale = total > 0.0f ? 1.0f / total : 0.0f;
+  const float scale = inverse_of(total);
   uint32_t high[4], low[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -914,9 +919,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
   if (!A.lse) return;
   *reinterpret_cast<uint4*>(static_cast<T*>(A.low) + (((int64_t)b * A.queries + qi) * A.heads + h) * kD + d) =
       make_uint4(low[0], low[1], low[2], low[3]);
-  if (d == 0)
-    A.lse[(int64_t)(b * A.heads + h) * A.queries + qi] =
-        total > 0.0f ? top + (__builtin_amdgcn_logf(sum) + kShift<T>) * kLn2 : -INFINITY;
+  if (d == 0) A.lse[(int64_t)(b * A.heads + h) * A.queries + qi] = lse_of<T>(top, total, sum);
 }
 
 template <typename T, int G>
@@ -1411,11 +1414,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args A, int q
 #pragma unroll
       for (int j = 0; j < kJoined; ++j) x += y[j] * __shfl(i + j < 32 ? f[0] : f[1], (i + j) & 31, 32);
     }
-    x *= l > 0.0f ? 1.0f / l : 0.0f;
+    x *= inverse_of(l);
     if constexpr (kKeep) {
-      if (lane == 0)
-        A.lse[(int64_t)bh * A.queries + row] =
-            l > 0.0f ? top + (__builtin_amdgcn_logf(sum) + kShift<T>) * kLn2 : -INFINITY;
+      if (lane == 0) A.lse[(int64_t)bh * A.queries + row] = lse_of<T>(top, l, sum);
       float y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = x[i] - (float)(T)x[i];

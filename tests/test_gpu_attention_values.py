@@ -5,8 +5,8 @@ import pytest
 import torch
 
 from flicker_amd import attention as A
-from tests.attention_forms import FORMS
-from tests.test_gpu_attention import D, TYPES, U
+from tests.attention_forms import FORMS, expected
+from tests.test_gpu_attention import D, TINY, TYPES, U, make
 
 pytestmark = pytest.mark.gpu
 SHORT = ["16", "16 cut", "192", "192 cut", "256", "256 cut", "256 both", "256 shared"]
@@ -82,3 +82,63 @@ def test_far_logits(device, form, dtype, q_size, k_size, negative):
     # what lies below float16's range in dS is dropped or kept, off by 2^-25 at most
     assert (dq.double().abs() <= (ds + tiny) * (1 + e) * size + tiny).all()
     assert torch.isfinite(dq).all() and torch.isfinite(dk).all()
+
+
+def _plain(q, k, v, do):
+    """(o, lse, dq, dk, dv) in float64 from the formulas; no mask."""
+    (batch, heads, queries, _), kv_heads = q.shape, k.shape[1]
+    group = heads // kv_heads
+    g = do.view(batch, queries, heads, D).transpose(1, 2).double().contiguous()
+    q, k, v = q.double(), *(t.double().repeat_interleave(group, 1) for t in (k, v))
+    s = q @ k.transpose(2, 3).contiguous()
+    top = s.amax(-1, keepdim=True)
+    p = torch.exp(s - top)
+    total = p.sum(-1, keepdim=True)
+    p = p / total
+    o = p @ v
+    ds = p * (g @ v.transpose(2, 3).contiguous() - (g * o).sum(-1, keepdim=True))
+    shared = (batch, kv_heads, group, *k.shape[2:])
+    dk, dv = (t.transpose(2, 3).contiguous() @ x for t, x in ((ds, q), (p, g)))
+    return o.transpose(1, 2).flatten(2), (top + total.log())[..., 0], ds @ k, dk.view(shared).sum(2), dv.view(shared).sum(2)
+
+
+@pytest.mark.parametrize("form", ["16", "16 cut", "192", "192 cut", "256 shared"])
+@pytest.mark.parametrize("which,value", [("q", "nan"), ("q", "inf"), ("k", "nan"), ("k", "inf"), ("k", "-inf"), ("v", "nan"), ("v", "inf"),
+                                         ("v", "-inf"), ("do", "nan"), ("do", "inf")])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_not_finite(device, form, which, value, dtype):
+    """One value that is not finite reaches every result that the formulas give it to, and no other: those stay within
+    the tolerance of the call without it."""
+    print(f"not finite {form} {which} {value} {dtype}", flush=True)
+    ops = dict(zip(("q", "k", "v", "do", "keep"), make(3, *FORMS[form][0], dtype)))
+    clean = _plain(ops["q"], ops["k"], ops["v"], ops["do"])
+    tols = expected(*ops.values())
+    t = ops[which]
+    ops[which] = t = t.clone()
+    at = (0, t.shape[1] // 2, t.shape[2] // 3) if t.dim() == 3 else (0, t.shape[1] - 1, t.shape[2] // 2, 77)
+    t[at] = float(value)
+    want = _plain(ops["q"], ops["k"], ops["v"], ops["do"])
+    o, kept = A.attention(ops["q"], ops["k"], ops["v"], keep=True)
+    assert torch.equal(o.nan_to_num(1e4), A.attention(ops["q"], ops["k"], ops["v"]).nan_to_num(1e4))
+    got = (o, kept.lse, *A.attention_backward(ops["do"], ops["q"], ops["k"], ops["v"], kept))
+    assert not all(w.isfinite().all() for w in want)
+    for name, g, w, c, (_, off) in zip(("o", "lse", "dq", "dk", "dv"), got, want, clean, tols):
+        finite = w.isfinite()
+        assert torch.equal(g.isfinite(), finite), (name, int((g.isfinite() & ~finite).sum()), int((~g.isfinite() & finite).sum()))
+        same = finite & (w == c)
+        e = torch.finfo(g.dtype).eps / 2
+        off = e * (c.abs() + off) + off + TINY.get(g.dtype, 2 * U)
+        assert ((g.double() - c).abs() <= off)[same].all(), name
+
+
+@pytest.mark.parametrize("form", ["16", "192", "256 shared"])
+def test_every_logit_minus_infinity(device, form):
+    """A row with nothing to weigh is one without keys; the others of its block are not touched."""
+    q, k, v, _, _ = make(4, *FORMS[form][0], "bf16")
+    k[..., 0] = float("-inf")
+    q[..., 0] = 0.5
+    q[:, :, 1::2] = float("nan")
+    o, kept = A.attention(q, k, v, keep=True)
+    o = o.unflatten(2, (q.shape[1], D))
+    assert not o[:, ::2].any() and o[:, 1::2].isnan().all()
+    assert kept.lse[:, :, ::2].isneginf().all() and kept.lse[:, :, 1::2].isnan().all()
