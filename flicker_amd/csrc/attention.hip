@@ -139,6 +139,8 @@ struct Args {
   float* lse;       // (batch, heads, queries)
   float* stats;     // (batch * heads * q_units + 1, 2, 32): a unit's lse and -delta; inf and 0 in rows past the
                     // end and in the last unit
+  float* norms;     // float16's gradients: most |do|^2 of each four of a unit's waves' rows, (batch * heads * q_units, 4), and
+                    // |v|^2 of kept keys, (batch * kv_heads * k_units, 4)
   Mask mask;
   int batch, heads, kv_heads, group, queries, keys, q_units, k_units;
   Cuts of_q, of_k;  // of the blocks of queries, and of keys (backwards)
@@ -413,16 +415,16 @@ __device__ __forceinline__ void store_rows(const f32x4 (&acc)[8][G], const float
   }
 }
 
-// The same unscaled as float32 rows of a cut's partial sums, for rows below `end`.
+// The same as float32 rows of a cut's partial sums, for rows below `end`.
 template <int G>
-__device__ __forceinline__ void store_part(const f32x4 (&acc)[8][G], float* dst, int row0, int end) {
+__device__ __forceinline__ void store_part(const f32x4 (&acc)[8][G], const float (&scale)[G], float* dst, int row0, int end) {
   const int lane = threadIdx.x & 63, h = lane >> 4;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const int r = row0 + g * 16 + (lane & 15);
     if (r >= end) continue;
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(dst + r * kD + dt * 16 + h * 4) = acc[dt][g];
+    for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(dst + r * kD + dt * 16 + h * 4) = acc[dt][g] * scale[g];
   }
 }
 
@@ -689,7 +691,10 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy writes LDS that the block has left
   }
   if (piece.cut >= 0) {
-    store_part(w.acc, A.of_q.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
+    float one[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) one[g] = 1.0f;
+    store_part(w.acc, one, A.of_q.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const int r = q0 - first + g * 16 + (lane & 15);
@@ -922,19 +927,67 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
   if (d == 0) A.lse[(int64_t)(b * A.heads + h) * A.queries + qi] = lse_of<T>(top, total, sum);
 }
 
-template <typename T, int G>
+// float16 holds P and dS backwards times powers of two, undone at the end: P 2^kUp, and dS 2^e where
+//   |dS_ij| <= |g_i| (|v_j| + |o_i|) <= 2 |g_i| max |v|   over the kept keys, o being a mean of their v
+// shows that 2^e may take it to 2^15.  Unscaled, P and dS of 2^-14 and less lose bits and those below 2^-25 all, at 4608 tokens already for
+// gradients of 2^-10.  e is a row's own for dq, and one for all rows of a key head, whose dS are summed, for dk.  The norms
+// cost the stats' launch a pass over v, and the second wave of dk a multiplication an element: 4608 tokens with gradients 1065 us rather
+// than 1038.
+template <typename T>
+constexpr bool kHalf = !__is_same(T, __bf16);
+constexpr int kUp = 14;
+__device__ __forceinline__ int up_of(float g2, float v2) {   // from the squares of both norms
+  return kUp - ((__builtin_amdgcn_frexp_expf(g2 * v2) + 1) >> 1);
+}
+__device__ __forceinline__ float power_of(int e) { return __builtin_ldexpf(1.0f, e); }
+__device__ __forceinline__ float uniform(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
+// The most of `units` x 4 norms.
+__device__ __forceinline__ float most_of(const float* norms, int64_t units) {
+  const f32x4* at = reinterpret_cast<const f32x4*>(norms);
+  float x = 0.0f;
+  for (int64_t i = threadIdx.x & 63; i < units; i += 256) {
+    f32x4 y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = at[min(i + 64 * j, units - 1)];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x = fmaxf(fmaxf(fmaxf(x, y[j][0]), y[j][1]), fmaxf(y[j][2], y[j][3]));
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+  return x;
+}
+__device__ __forceinline__ float most_do(const Args& A, int b, int first_head, int heads) {
+  return most_of(A.norms + ((int64_t)b * A.heads + first_head) * A.q_units * 4, (int64_t)heads * A.q_units);
+}
+__device__ __forceinline__ float most_v(const Args& A, int b, int h) {
+  const int64_t of_q = (int64_t)A.batch * A.heads * A.q_units;
+  return most_of(A.norms + (of_q + ((int64_t)b * A.kv_heads + h) * A.k_units) * 4, A.k_units);
+}
+
+// kFrom: dP's sums start from -delta, which spares an addition an element and takes six registers that a masked pass's loop does
+// not have (16896 tokens with gradients 12.40 ms rather than 12.53).
+template <typename T, int G, bool kFrom>
 struct Dq {
   vec8<T> x[4][G], g[4][G];   // Q^T, dO^T
   f32x4 acc[8][G];            // dQ^T
   vec8<T> ops[2 * kLead];
-  float lse[G];
-  f32x4 delta[G];             // -delta, from which dP's sums start
+  float lse[G];               // in float16 less the logarithm of what dS is held times
+  std::conditional_t<kFrom, f32x4, float> delta[G];   // -delta
   Places at;
 };
 
+template <typename T, int G, bool kFrom>
+__device__ __forceinline__ f32x4 start_of(const Dq<T, G, kFrom>& w, int g) {
+  if constexpr (kFrom) return w.delta[g];
+  return f32x4{};
+}
+
 // Phase u: S(u+1) = K(u+1) Q^T, dP(u+1) = V(u+1) dO^T and dQ^T += K(u-1)^T dS(u-1)^T, while dS(u) is formed.
-template <bool kPartial, typename T, int G, typename Hook>
-__device__ __forceinline__ void dq_phase(Dq<T, G>& w, const f32x4 (&s_cur)[2 * G], const f32x4 (&d_cur)[2 * G],
+template <bool kPartial, typename T, int G, bool kFrom, typename Hook>
+__device__ __forceinline__ void dq_phase(Dq<T, G, kFrom>& w, const f32x4 (&s_cur)[2 * G], const f32x4 (&d_cur)[2 * G],
                                          f32x4 (&s_next)[2 * G], f32x4 (&d_next)[2 * G], const uint32_t (&p_prev)[4 * G],
                                          uint32_t (&p_cur)[4 * G], const uint8_t* k_unit, const uint8_t* v_unit,
                                          const uint8_t* k_before, const uint8_t* k_after, uint32_t bits,
@@ -952,7 +1005,12 @@ __device__ __forceinline__ void dq_phase(Dq<T, G>& w, const f32x4 (&s_cur)[2 * G
   auto scaled = [&](int n) { t[n] = (sv[n >> 2][n & 3] - w.lse[n >> 3]) * kLog2e; };
   auto exp = [&](int n) { e[n] = __builtin_amdgcn_exp2f(t[n]); };
   auto put = [&](int n) {
-    p_cur[n >> 1] = pack<T>(e[n] * dv[n >> 2][n & 3], e[n + 1] * dv[n >> 2][(n & 3) + 1]);
+    float x = dv[n >> 2][n & 3], y = dv[n >> 2][(n & 3) + 1];
+    if constexpr (!kFrom) {
+      x += w.delta[n >> 3];
+      y += w.delta[n >> 3];
+    }
+    p_cur[n >> 1] = pack<T>(e[n] * x, e[n + 1] * y);
     asm volatile("" : "+v"(p_cur[n >> 1]));
   };
   vec8<T> pb[G];
@@ -969,7 +1027,7 @@ __device__ __forceinline__ void dq_phase(Dq<T, G>& w, const f32x4 (&s_cur)[2 * G
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       if (n < 8) s_next[2 * g + kt] = mfma(a, w.x[st][g], st ? s_next[2 * g + kt] : f32x4{});
-      else if (n < 16) d_next[2 * g + kt] = mfma(a, w.g[st][g], st ? d_next[2 * g + kt] : w.delta[g]);
+      else if (n < 16) d_next[2 * g + kt] = mfma(a, w.g[st][g], st ? d_next[2 * g + kt] : start_of(w, g));
       else w.acc[n - 16][g] = mfma(a, pb[g], w.acc[n - 16][g]);
     }
     const int m = n + kLead;
@@ -992,7 +1050,7 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
   const int lane = threadIdx.x & 63, bh = b * A.heads + h;
   Units<kMasked> units(A, b, piece);
   const int n = units.n;
-  Dq<T, G> w;
+  Dq<T, G, !kMasked> w;
   load_rows<T>(w.g, A.dO.at<T>(b, h), A.dO.row, q0, end);
 #pragma unroll
   for (int g = 0; g < G; ++g) {
@@ -1000,7 +1058,8 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
     const float* st = A.stats + ((int64_t)bh * A.q_units + r / kUnit) * 2 * kUnit + r % kUnit;
     w.lse[g] = r < end ? st[0] : INFINITY;
     const float delta = r < end ? st[kUnit] : 0.0f;
-    w.delta[g] = f32x4{delta, delta, delta, delta};
+    if constexpr (kMasked) w.delta[g] = delta;
+    else w.delta[g] = f32x4{delta, delta, delta, delta};
   }
 #pragma unroll
   for (int g = 0; g < G; ++g)
@@ -1025,6 +1084,18 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
     load_rows<T>(w.x, A.q.at<T>(b, h), A.q.row, q0, end);
     w.at = places();
     reinterpret_cast<uint4*>(k_slot(kDqKRing - 1))[threadIdx.x] = make_uint4(0, 0, 0, 0);   // K(-1), times dS(-1) = 0
+    if constexpr (kHalf<T>) {
+      const float v2 = most_v(A, b, h / A.group);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float g2 = 0.0f;
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g2 += (float)w.g[st][g][e] * (float)w.g[st][g][e];
+        w.lse[g] -= (float)up_of(across(g2), v2) * kLn2;
+      }
+    }
     landed<0>();
     for (int i = 0; i < 4; ++i) {
       clear_rows(k_slot(i), bits[i]);
@@ -1041,7 +1112,7 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           s0[2 * g + kt] = mfma(a, w.x[st][g], st ? s0[2 * g + kt] : f32x4{});
-          d0[2 * g + kt] = mfma(c, w.g[st][g], st ? d0[2 * g + kt] : w.delta[g]);
+          d0[2 * g + kt] = mfma(c, w.g[st][g], st ? d0[2 * g + kt] : start_of(w, g));
         }
       }
     }
@@ -1083,14 +1154,21 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
+  float down[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    down[g] = 1.0f;
+    if constexpr (kHalf<T>) {   // what the difference came to: none of it where lse is far past it
+      const int r = q0 + g * 16 + (lane & 15);
+      const float lse = r < end ? A.stats[((int64_t)bh * A.q_units + r / kUnit) * 2 * kUnit + r % kUnit] : INFINITY;
+      if (lse != INFINITY) down[g] = __builtin_amdgcn_exp2f((w.lse[g] - lse) * kLog2e);
+    }
+  }
   if (piece.cut >= 0) {
-    store_part(w.acc, A.of_q.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
+    store_part(w.acc, down, A.of_q.part + (int64_t)piece.cut * kQueries * kD, q0 - first, end - first);
     return;
   }
-  float one[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) one[g] = 1.0f;
-  store_rows<T>(w.acc, one, A.dq.at<T>(b, h), A.dq.row, q0, end);
+  store_rows<T>(w.acc, down, A.dq.at<T>(b, h), A.dq.row, q0, end);
 }
 
 // dk and dv of 128 keys, 32 a pair of waves: the first holds K^T and dV^T, forms S and P and hands P on through LDS, the
@@ -1101,6 +1179,7 @@ struct Dkv {
   f32x4 acc[8][2];         // dV^T (dK^T)
   vec8<T> ops[2 * kLead];
   f32x4 stat[2];           // this phase's lse (-delta) of the rows of each accumulator
+  float more;              // the second wave's: what float16's dS is held times beside P's 2^kUp
   Places at;
 };
 
@@ -1121,11 +1200,18 @@ __device__ __forceinline__ void dkv_phase(Dkv<T>& w, const f32x4 (&s_cur)[4], f3
     if constexpr (kSecond) e4[i] = mine[64 * i];
   }
   float t[16];
-  auto scaled = [&](int n) { t[n] = (sv[n >> 2][n & 3] - w.stat[n >> 2 & 1][n & 3]) * kLog2e; };
+  auto scaled = [&](int n) {
+    const float x = sv[n >> 2][n & 3] - w.stat[n >> 2 & 1][n & 3];
+    t[n] = kHalf<T> ? __builtin_fmaf(x, kLog2e, (float)kUp) : x * kLog2e;
+  };
   auto exp = [&](int n) { e4[n >> 2][n & 3] = __builtin_amdgcn_exp2f(t[n]); };
   auto put = [&](int n) {
     float x = e4[n >> 2][n & 3], y = e4[n >> 2][(n & 3) + 1];
     if constexpr (kSecond) {
+      if constexpr (kHalf<T>) {
+        x *= w.more;
+        y *= w.more;
+      }
       x *= sv[n >> 2][n & 3];
       y *= sv[n >> 2][(n & 3) + 1];
     }
@@ -1221,6 +1307,7 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = f32x4{};
   }
+  float down[2] = {1.0f, 1.0f};
   if (any) {
     const int from = piece.first(A.q_units * A.group), n = piece.count(A.q_units * A.group);
     auto q_slot = [&](int i) { return smem + (i & (kQRing - 1)) * kUnitBytes; };
@@ -1260,6 +1347,14 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
     if (!kSecond)
 #pragma unroll
       for (int i = 0; i < 4; ++i) reinterpret_cast<f32x4*>(hand(1))[64 * i + lane] = f32x4{};
+    if constexpr (kHalf<T>) {
+      int up = kUp;
+      if constexpr (kSecond) {
+        up = up_of(most_do(A, b, h * A.group, A.group), most_v(A, b, h));
+        w.more = uniform(power_of(up - kUp));
+      }
+      down[0] = down[1] = uniform(power_of(-up));
+    }
     landed<0>();
     __syncthreads();
     f32x4 s0[4] = {}, s1[4];
@@ -1319,12 +1414,11 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
     for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] = on[g] ? w.acc[dt][g] : f32x4{};
   if (piece.cut >= 0) {   // dv's 128 rows, then dk's
     float* part = A.of_k.part + ((int64_t)piece.cut * 2 + kSecond) * kKeys * kD;
-    store_part(w.acc, part, k0 - first, min(A.keys - first, kKeys));
+    store_part(w.acc, down, part, k0 - first, min(A.keys - first, kKeys));
     return;
   }
-  const float one[2] = {1.0f, 1.0f};
   const Tensor& out = kSecond ? A.dk : A.dv;
-  store_rows<T>(w.acc, one, out.at<T>(b, h), out.row, k0, A.keys);
+  store_rows<T>(w.acc, down, out.at<T>(b, h), out.row, k0, A.keys);
 }
 
 // All gradients: blocks of queries and blocks of keys in one launch, so that neither kind's last round leaves CUs idle (a
@@ -1476,8 +1570,23 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const M
   plan_entry(m, blockIdx.x, keys, units, found);
 }
 
+// The most |x|^2 of a wave's rows, 16 lanes and 8 values each, into norms[unit][threadIdx.x / 64 % 4].
+template <typename T>
+__device__ __forceinline__ float norm2(const vec8<T>& x) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum += (float)x[e] * (float)x[e];
+  return flk::row16_sum(sum);
+}
+__device__ __forceinline__ void put_norm(float* norms, int64_t unit, float most) {
+  most = fmaxf(most, __shfl_xor(most, 16));
+  most = fmaxf(most, __shfl_xor(most, 32));
+  if ((threadIdx.x & 63) == 0) norms[unit * 4 + (threadIdx.x >> 6 & 3)] = most;
+}
+
 // What the gradients need first: the mask's words and lists, in the first A.batch blocks where there is a mask, and every
-// row's stats, 16 lanes a row and 128 rows (four units) a block, which reads do, o and low once.  Bound by memory: 4608
+// row's stats, 16 lanes a row and 128 rows (four units) a block, which reads do, o and low once; in float16 the norms of do's
+// rows beside them and, in the blocks behind those, of v's.  Bound by memory: 4608
 // tokens of 24 heads 14 us for 85 MB, which the caches partly hold; 16896 64 us, 4.9 TB/s.
 template <typename T>
 __global__ __launch_bounds__(64 * kPlanWaves) void attention_prepare_kernel(const MaskBytes m, const Args A) {
@@ -1489,9 +1598,30 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_prepare_kernel(cons
   }
   const int64_t all = (int64_t)A.batch * A.heads * A.q_units;
   const int64_t unit = (int64_t)(blockIdx.x - masks) * 4 + (threadIdx.x >> 8);   // `all` itself: the unit of no rows
+  const int lane = threadIdx.x & 15;
+  if constexpr (kHalf<T>) {
+    const int64_t of_v = unit - (all + 4) / 4 * 4;
+    if (of_v >= (int64_t)A.batch * A.kv_heads * A.k_units) return;
+    if (of_v >= 0) {
+      const int bh = (int)(of_v / A.k_units), b = bh / A.kv_heads, h = bh - b * A.kv_heads;
+      const int first = (int)(of_v - (int64_t)bh * A.k_units) * kUnit + (threadIdx.x >> 4 & 15);
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = first + 16 * i;
+        vec8<T> x{};
+        if (r < A.keys && (!m.mask || m.mask[b * m.batch_stride + r]))
+          x = *reinterpret_cast<const vec8<T>*>(A.v.at<T>(b, h) + (int64_t)r * A.v.row + lane * 8);
+        most = fmaxf(most, norm2<T>(x));
+      }
+      put_norm(A.norms, all + of_v, most);
+      return;
+    }
+  }
   if (unit > all) return;
-  const int lane = threadIdx.x & 15, bh = (int)(unit / A.q_units), b = bh / A.heads, h = bh - b * A.heads;
+  const int bh = (int)(unit / A.q_units), b = bh / A.heads, h = bh - b * A.heads;
   const int first = (int)(unit - (int64_t)bh * A.q_units) * kUnit + (threadIdx.x >> 4 & 15);
+  float most = 0.0f;
   float* st = A.stats + unit * 2 * kUnit + (threadIdx.x >> 4 & 15);
   vec8<T> x[2][3];
   float lse[2];
@@ -1516,11 +1646,14 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_prepare_kernel(cons
     for (int e = 0; e < 8; ++e)
       sum += live ? (float)x[i][0][e] * ((float)x[i][1][e] + (float)x[i][2][e]) : 0.0f;
     sum = flk::row16_sum(sum);
+    if constexpr (kHalf<T>) most = fmaxf(most, norm2<T>(live ? x[i][0] : vec8<T>{}));
     if (lane == 0) {
       st[16 * i] = live ? lse[i] : INFINITY;
       st[16 * i + kUnit] = -sum;
     }
   }
+  if constexpr (kHalf<T>)
+    if (unit < all) put_norm(A.norms, unit, most);
 }
 
 int units_of(int rows) { return (rows + kUnit - 1) / kUnit; }
@@ -1528,6 +1661,7 @@ int64_t mask_bytes(int batch, int keys) { return ((int64_t)batch * (units_of(key
 int64_t stats_bytes(int batch, int heads, int queries) {
   return ((int64_t)batch * heads * units_of(queries) + 1) * 2 * kUnit * 4;
 }
+int64_t norms_bytes(const Args& A) { return (int64_t)A.batch * (A.heads * (int64_t)A.q_units + A.kv_heads * (int64_t)A.k_units) * 16; }
 
 // Where the mask's words and lists lie in `workspace`.
 MaskBytes mask_in(const void* mask, int64_t batch_stride, Args& A, uint8_t* workspace) {
@@ -1772,7 +1906,8 @@ void forward(const Args& A, const Cut& cut, hipStream_t s) {
 template <typename T>
 void backward(const MaskBytes& mask, const Args& A, const Gradients& plan, hipStream_t s) {
   const int64_t units = (int64_t)A.batch * A.heads * A.q_units + 1;
-  const dim3 prepare((unsigned)((mask.mask ? A.batch : 0) + (units + 3) / 4));
+  const int64_t of_v = kHalf<T> ? (int64_t)A.batch * A.kv_heads * A.k_units : 0;
+  const dim3 prepare((unsigned)((mask.mask ? A.batch : 0) + (units + 3) / 4 + (of_v + 3) / 4));
   attention_prepare_kernel<T><<<prepare, 64 * kPlanWaves, 0, s>>>(mask, A);
   const dim3 grid((unsigned)(plan.q.grid() + plan.k.grid()));
   if (A.mask.bits) {
@@ -1794,7 +1929,7 @@ int64_t workspace_of(const Args& A, bool masked, bool backward) {
   if (A.batch == 0 || A.queries == 0 || (A.keys == 0 && backward)) return 0;
   const int64_t mask = masked ? mask_bytes(A.batch, A.keys) : 0;
   if (!backward) return (waves_find(A) ? 0 : mask) + forward_cut(A).bytes();
-  return mask + stats_bytes(A.batch, A.heads, A.queries) + plan_gradients(A).bytes();
+  return mask + stats_bytes(A.batch, A.heads, A.queries) + norms_bytes(A) + plan_gradients(A).bytes();
 }
 
 }  // namespace
@@ -1912,7 +2047,8 @@ extern "C" int flk_attention_backward(const void* d_o, const int64_t* d_o_stride
   hipStream_t s = static_cast<hipStream_t>(stream);
   const MaskBytes mask = mask_in(key_mask, mask_batch_stride, A, static_cast<uint8_t*>(workspace));
   const Gradients plan = plan_gradients(A);
-  uint8_t* parts = reinterpret_cast<uint8_t*>(A.stats) + stats_bytes(batch, heads, queries);
+  A.norms = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(A.stats) + stats_bytes(batch, heads, queries));
+  uint8_t* parts = reinterpret_cast<uint8_t*>(A.norms) + norms_bytes(A);
   A.of_q = plan.q.in(parts);
   A.of_k = plan.k.in(parts + plan.q.bytes());
   A.q_grid = (int)plan.q.grid();

@@ -557,7 +557,8 @@ int flk_attention(const void* q, const int64_t* q_strides, const void* k, const 
 /* Gradients of flk_attention for d_o, the gradient of o (of o's shape, any strides as above), from the
  * forward call's operands and its o, low and lse: dq, dk and dv, shaped as q, k and v.  P and dS
  * are rounded to dtype between the products.  The gradients of masked keys are zero.  Nothing is written when
- * batch, queries or keys is 0.  Sums are in a fixed order. */
+ * batch, queries or keys is 0.  Sums are in a fixed order.  In FLK_F16 P and dS are scaled by powers of two before they are
+ * rounded, so that small gradients keep their bits and large ones stay finite. */
 int flk_attention_backward(const void* d_o, const int64_t* d_o_strides, const void* q, const int64_t* q_strides,
                            const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
                            const void* o, const int64_t* o_strides, const void* low, const float* lse, int dtype,
