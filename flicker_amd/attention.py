@@ -12,7 +12,8 @@ lengths, several query heads to a key head, and a mask over each batch entry's k
 Logits may have any size that float32 holds; backwards P = exp(S - lse) is off by lse's rounding, up to 2^-24 |lse| of
 itself.  Statistics and sums are float32; P, and backwards dS, are rounded to the operands' type, which the matrix cores take,
 and every output is rounded once.  In float16 the gradients' P and dS are held times powers of two, by do's and v's norms, so
-that they neither overflow nor lose what small gradients leave of them; forwards a P below 2^-25 of its row's largest is zero.
+that they neither overflow nor lose what small gradients leave of them; forwards P has all its bits down to 2^-22 of its row's
+largest, and below 2^-33 is zero.
 In bfloat16 a term P v below 2^-106 is.
 For gradients through torch's autograd see ``flicker_amd.autograd``.
 """

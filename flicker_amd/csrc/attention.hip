@@ -454,12 +454,18 @@ struct Forward {
   Places at;
 };
 
-// P is held as exp2(log2(e) (S - top) - kShift<T>), where top is the maximum of an earlier unit's row; it has to rise where
-// a P passes 2.  bfloat16 has float32's range: P 2^-20 leaves 2^21 for S to rise by, and 2^-106 for P v, the sums' smallest
-// terms (2^-60 takes the same time).  That P passes 2 is then one bit of its packed form.  float16 has neither: exponents are compared with kSlack.
+// P is held as exp2(log2(e) (S - top) - kShift<T>), where top is the maximum of an earlier unit's row, which has to rise where
+// that passes a limit.  bfloat16 has float32's range: P 2^-20 and a limit of 2 leave 2^21 for S to rise by, and 2^-106 for P v, the sums'
+// smallest terms (2^-60 takes the same time); past 2 is one bit of the packed form.  In float16 P 2^8 keeps all bits of P down to
+// 2^-22 and some of them to 2^-33, and exponents are compared with kLimit, its range, which leaves 2^7 for S to rise by (as fast as P
+// itself with 2^9, and zero below 2^-25; P 2^11 and 2^4: 4608 tokens 249 -> 258 us).
 template <typename T>
-constexpr float kShift = sizeof(T) == 2 && __is_same(T, __bf16) ? 20.0f : 0.0f;
-constexpr float kSlack = 9.0f;
+constexpr float kShift = __is_same(T, __bf16) ? 20.0f : -8.0f;
+constexpr float kLimit = 15.0f;
+template <typename T>
+__device__ __forceinline__ float shifted(float x, float y) {   // x y - kShift; in float16 by 4s that take no register from the loop
+  return __is_same(T, __bf16) ? __builtin_fmaf(x, y, -kShift<T>) : __builtin_fmaf(x, y, -0.5f * kShift<T>) - 0.5f * kShift<T>;
+}
 // base is rounded, by up to 2^-12 at this size of top, which takes 2^-12 off the exponents of P, and past 2^28 their range.  Beyond it
 // (and before the first maximum) each unit's P are formed again from the differences S - top, which are exact where it matters.
 // From the differences at once: 4608 tokens 244 us rather than 237.
@@ -506,7 +512,7 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
   if constexpr (kPartial)
     if (bits != ~0u) leave_out(sv, bits);
   constexpr int kElems = 8 * G;   // of a lane: one a slot, every other slot with one group
-  constexpr bool kBits = kShift<T> != 0.0f;
+  constexpr bool kBits = __is_same(T, __bf16);
   float t[kElems], e[kElems], high = -INFINITY, sum[G] = {};
   uint32_t any = 0;
   auto scaled = [&](int n) { t[n] = __builtin_fmaf(sv[n >> 2][n & 3], kLog2e, w.base[n >> 3]); };
@@ -551,7 +557,7 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
     __builtin_amdgcn_sched_barrier(0);
   }
   // top rises to the row's maximum, what has been summed is scaled, and this unit's P are formed again
-  if (w.far || __any(kBits ? (any & 0x40004000u) != 0 : high > kSlack)) {
+  if (w.far || __any(kBits ? (any & 0x40004000u) != 0 : high > kLimit)) {
     bool far = false;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -562,7 +568,7 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
       x = fmaxf(fmaxf(x, __shfl_xor(x, 32)), w.top[g]);
       const float factor = __builtin_amdgcn_exp2f((w.top[g] - x) * kLog2e);
       w.top[g] = x;
-      w.base[g] = x * -kLog2e - kShift<T>;
+      w.base[g] = shifted<T>(x, -kLog2e);
       far |= fabsf(x) > kFar;
       sum[g] = 0.0f;
       w.sum[g] *= factor;
@@ -571,7 +577,7 @@ __device__ __forceinline__ void forward_phase(Forward<T, G>& w, const f32x4 (&s_
       for (int dt = 0; dt < 8; ++dt) w.acc[dt][g] *= factor;
 #pragma unroll
       for (int n = 8 * g; n < 8 * g + 8; ++n) {
-        t[n] = __builtin_fmaf(sv[n >> 2][n & 3] - x, kLog2e, -kShift<T>);
+        t[n] = shifted<T>(sv[n >> 2][n & 3] - x, kLog2e);
         exp(n);
         if (n & 1) put(n - 1);
       }

@@ -127,3 +127,26 @@ def test_zero_gradients_and_values(device):
     o, kept = A.attention(q, k, v * 0, keep=True)
     dq, dk, dv = A.attention_backward(do, q, k, v * 0, kept)
     assert not dq.any() and not dk.any() and dv.any()
+
+
+@pytest.mark.parametrize("form", ["16", "16 cut", "192", "192 cut", "256", "256 both", "256 cut"])
+def test_many_small_weights(device, form):
+    """All keys but one at 2^-25.4 of the largest P, and o theirs alone.  P 2^8 is a subnormal of float16 there, off by 2^-25 at
+    most, which is 2^-33 of the largest P; the sum that divides o is 1 and at most 2e-4 more."""
+    batch, heads, kv_heads, queries, keys = FORMS[form][0]
+    q, k, v = (torch.zeros(batch, h, n, D, dtype=torch.float16, device=device)
+               for h, n in ((heads, queries), (kv_heads, keys), (kv_heads, keys)))
+    q[..., 5] = 1.0
+    k[..., 5] = -17.625
+    v[:] = 64.0
+    for h in range(kv_heads):                       # the largest in another unit of each head
+        k[:, h, (37 * h) % keys, 5] = 0.0
+        v[:, h, (37 * h) % keys] = 0.0
+    p = torch.exp(torch.tensor(-17.625, dtype=torch.float64))
+    want = float(64 * (keys - 1) * p / (1 + (keys - 1) * p))
+    o, kept = A.attention(q, k, v, keep=True)
+    off = 64 * (keys - 1) * 2.0 ** -33 + 2 * E * want + 64 * U * keys * want
+    assert ((o.double() - want).abs() <= off + E * want + 2.0 ** -25).all(), (float(o.min()), float(o.max()), want)
+    assert torch.equal(o, A.attention(q, k, v))
+    total = float(torch.log1p((keys - 1) * p))
+    assert ((kept.lse.double() - total).abs() <= 64 * U * 18).all()
