@@ -77,13 +77,14 @@ def _on_gpu(name: str, t: torch.Tensor) -> None:
 def _dense_rows(t: torch.Tensor) -> torch.Tensor:
     """Keep a view whose last axis is contiguous and whose other strides keep 16-byte rows;
     anything else is compacted on the device first."""
-    if t.data_ptr() % 16:
-        return t.contiguous()
     *outer, inner = t.stride()
-    for s in outer:
-        if s % 8:
-            return t.contiguous()
-    return t if inner == 1 else t.contiguous()
+    if t.data_ptr() % 16 == 0 and inner == 1:
+        for s in outer:
+            if s % 8:
+                break
+        else:
+            return t
+    return t.clone(memory_format=torch.contiguous_format)   # contiguous() keeps what is dense but off 16 bytes
 
 
 def _vector(t: torch.Tensor) -> torch.Tensor:
