@@ -1915,13 +1915,25 @@ void backward(const MaskBytes& mask, const Args& A, const Gradients& plan, hipSt
   const int64_t of_v = kHalf<T> ? (int64_t)A.batch * A.kv_heads * A.k_units : 0;
   const dim3 prepare((unsigned)((mask.mask ? A.batch : 0) + (units + 3) / 4 + (of_v + 3) / 4));
   attention_prepare_kernel<T><<<prepare, 64 * kPlanWaves, 0, s>>>(mask, A);
-  const dim3 grid((unsigned)(plan.q.grid() + plan.k.grid()));
-  if (A.mask.bits) {
-    if (A.group > 1) attention_backward_kernel<T, true, true><<<grid, kThreads, 0, s>>>(A);
-    else attention_backward_kernel<T, true, false><<<grid, kThreads, 0, s>>>(A);
-  } else {
-    if (A.group > 1) attention_backward_kernel<T, false, true><<<grid, kThreads, 0, s>>>(A);
-    else attention_backward_kernel<T, false, false><<<grid, kThreads, 0, s>>>(A);
+  auto launch = [&](const Args& of, int64_t blocks) {
+    const dim3 grid((unsigned)blocks);
+    if (of.mask.bits) {
+      if (of.group > 1) attention_backward_kernel<T, true, true><<<grid, kThreads, 0, s>>>(of);
+      else attention_backward_kernel<T, true, false><<<grid, kThreads, 0, s>>>(of);
+    } else {
+      if (of.group > 1) attention_backward_kernel<T, false, true><<<grid, kThreads, 0, s>>>(of);
+      else attention_backward_kernel<T, false, false><<<grid, kThreads, 0, s>>>(of);
+    }
+  };
+  const int64_t q_grid = plan.q.grid(), k_grid = plan.k.grid();
+  if ((q_grid + k_grid) * kThreads <= kMaxItems) {
+    launch(A, q_grid + k_grid);
+  } else {   // more work-items than a launch counts: each kind fits one, by sizes_ok
+    Args one = A;
+    one.k_first = false;
+    launch(one, q_grid);
+    one.q_grid = 0;
+    launch(one, k_grid);
   }
   const int q = (int)join_blocks(plan.q), k = (int)join_blocks(plan.k);
   if (q + k) attention_join_kernel<T, false, false><<<(unsigned)((q + k) * (kQueries / 8)), 256, 0, s>>>(A, q);

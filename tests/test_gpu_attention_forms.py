@@ -5,6 +5,7 @@ form; tests/test_attention_plan_host.py holds these shapes to theirs.  Tolerance
 import pytest
 import torch
 
+from flicker_amd import _lib
 from flicker_amd import attention as A
 from tests.attention_forms import FORMS, check, close, expected
 from tests.test_gpu_attention import D, U, make
@@ -143,3 +144,25 @@ def test_few_rows_of_long_lists(device, batch, heads, keys, masked):
         r = 2 * 130 * U * size + 8 * U * (s.abs().amax(-1, keepdim=True) + lse.abs()) + (keys + 128) * U
         off = (2 * 2.0 ** -8 + 2 * r + (keys + 64) * U) * (p @ vb.abs())
         close(f"entry {b}", o[b, 0].view(heads, D), p @ vb, off)
+
+
+def test_most_heads(device):
+    """As many heads as a call takes, one query and one key each: the gradients' blocks of queries and of keys together are
+    more work-items than a launch counts.  P = 1: o is v and dv do; dS is what 2 * 130 roundings leave of dP - delta."""
+    g = torch.Generator("cuda").manual_seed(0)
+    batch, heads = 2 ** 20, 4
+    q, k, v, do = (torch.randn(batch, heads, 1, D, generator=g, device=device, dtype=torch.bfloat16) for _ in range(4))
+    q *= D ** -0.5
+    o, kept = A.attention(q, k, v, keep=True)
+    assert torch.equal(o.view(v.shape), v)
+    dq, dk, dv = A.attention_backward(do.view(batch, 1, heads * D), q, k, v, kept)
+    assert torch.equal(dv, do)
+    for first in range(0, batch, 2 ** 17):
+        part = slice(first, first + 2 ** 17)
+        off = 260 * U * (do[part].float() * v[part].float()).abs().sum(-1, keepdim=True) * 1.01
+        for grad, by in ((dq, k), (dk, q)):
+            assert (grad[part].float().abs() <= off * by[part].float().abs()).all()
+    del o, kept, dq, dk, dv
+    with pytest.raises(_lib.HipKernelError, match="flk_attention_plan"):
+        A.attention(torch.empty(batch, heads + 1, 1, D, dtype=torch.bfloat16, device=device), *[torch.empty(
+            batch, heads + 1, 1, D, dtype=torch.bfloat16, device=device)] * 2)
