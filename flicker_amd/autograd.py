@@ -110,7 +110,7 @@ class _ResidualModulate(torch.autograd.Function):
     @staticmethod
     @_first_only
     def backward(ctx, dr, dy):
-        return *_norm.residual_modulate_backward(dr, dy, *ctx.saved_tensors, eps=ctx.eps), None
+        return *_norm.residual_modulate_backward(dr, dy, *ctx.saved_tensors, eps=ctx.eps, wanted=ctx.needs_input_grad[2:5]), None
 
 
 class _QkPrep(torch.autograd.Function):

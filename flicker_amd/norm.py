@@ -283,12 +283,15 @@ def residual_modulate(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor,
 
 
 def residual_modulate_backward(dr: torch.Tensor, dy: torch.Tensor, x: torch.Tensor, branch: torch.Tensor,
-                               gate: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *, eps: float = EPS):
+                               gate: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *, eps: float = EPS,
+                               wanted: tuple[bool, bool, bool] = (True, True, True)):
     """(dx, dbranch, dgate, dshift, dscale) of ``residual_modulate`` for the incoming gradients dr of r and dy of y, the
-    last three shaped as gate, shift and scale."""
-    done = _native.residual_modulate_backward(dr, dy, x, branch, gate, shift, scale, eps)
-    if done is not None:
-        return done
+    last three shaped as gate, shift and scale.  Where ``wanted`` is false (a frozen modulation) one of those is None; its
+    sum is not stored, and without any of them none is formed."""
+    if all(wanted):
+        done = _native.residual_modulate_backward(dr, dy, x, branch, gate, shift, scale, eps)
+        if done is not None:
+            return done
     shapes = gate, shift, scale
     gate, shift, scale = _residual(x, branch, gate, shift, scale)
     _same("dr", dr, x)
@@ -296,16 +299,18 @@ def residual_modulate_backward(dr: torch.Tensor, dy: torch.Tensor, x: torch.Tens
     batch, length, width = x.shape
     dx, dbranch = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
     make = torch.empty if x.numel() else torch.zeros   # sums over no rows
-    dgate, dshift, dscale = (make(t.shape, dtype=t.dtype, device=x.device) for t in shapes)
+    dgate, dshift, dscale = (make(t.shape, dtype=t.dtype, device=x.device) if want else None
+                             for t, want in zip(shapes, wanted, strict=True))
     if x.numel() == 0:
         return dx, dbranch, dgate, dshift, dscale
-    size = ctypes.c_int64(0)
-    _lib.check(_lib.lib().flk_residual_norm_backward_plan(batch, length, width, 0, ctypes.byref(size)),
-               "flk_residual_norm_backward_plan")
-    ws = torch.empty(size.value, dtype=torch.uint8, device=x.device)
+    size, ws = ctypes.c_int64(0), None
+    if any(wanted):
+        _lib.check(_lib.lib().flk_residual_norm_backward_plan(batch, length, width, 0, ctypes.byref(size)),
+                   "flk_residual_norm_backward_plan")
+        ws = torch.empty(size.value, dtype=torch.uint8, device=x.device)
     rb, yb, xb, bb = (_blocks(t) for t in (dr, dy, x, branch))
     _lib.run("flk_residual_norm_backward", (dr, dy, x, branch, gate, scale, dx, dbranch, dgate, dscale, dshift, ws),
              *_rows(rb), *_rows(yb), *_rows(xb), *_rows(bb), _CODES[x.dtype], gate.data_ptr(), scale.data_ptr(),
              _CODES[scale.dtype], width, 1, float(eps), batch, length, width, *_rows(dx), *_rows(dbranch),
-             dgate.data_ptr(), dscale.data_ptr(), dshift.data_ptr(), ws.data_ptr(), size.value, _lib.stream_of(x))
+             *(_lib.ptr(t) for t in (dgate, dscale, dshift, ws)), size.value, _lib.stream_of(x))
     return dx, dbranch, dgate, dshift, dscale
