@@ -139,8 +139,8 @@ struct Args {
   float* lse;       // (batch, heads, queries)
   float* stats;     // (batch * heads * q_units + 1, 2, 32): a unit's lse and -delta; inf and 0 in rows past the
                     // end and in the last unit
-  float* norms;     // float16's gradients: most |do|^2 of each four of a unit's waves' rows, (batch * heads * q_units, 4), and
-                    // |v|^2 of kept keys, (batch * kv_heads * k_units, 4)
+  float* norms;     // float16's gradients, of a quarter of a unit's rows each: the most |do|^2 and delta^2,
+                    // (batch * heads * q_units, 4, 2), and |v|^2 of kept keys, (batch * kv_heads * k_units, 4)
   Mask mask;
   int batch, heads, kv_heads, group, queries, keys, q_units, k_units;
   Cuts of_q, of_k;  // of the blocks of queries, and of keys (backwards)
@@ -934,43 +934,67 @@ __global__ __launch_bounds__(64 * kFewWaves) void attention_few_kernel(const Arg
 }
 
 // float16 holds P and dS backwards times powers of two, undone at the end: P 2^kUp, and dS 2^e where
-//   |dS_ij| <= |g_i| (|v_j| + |o_i|) <= 2 |g_i| max |v|   over the kept keys, o being a mean of their v
+//   |dS_ij| <= |g_i| |v_j| + |delta_i| <= 2 max(|g_i| |v_j|, |delta_i|)
 // shows that 2^e may take it to 2^15.  Unscaled, P and dS of 2^-14 and less lose bits and those below 2^-25 all, at 4608 tokens already for
-// gradients of 2^-10.  e is a row's own for dq, and one for all rows of a key head, whose dS are summed, for dk.  The norms
-// cost the stats' launch a pass over v, and the second wave of dk a multiplication an element: 4608 tokens with gradients 1065 us rather
-// than 1038.
+// gradients of 2^-10.  e is a row's own for dq, by the v that its wave walks, and one for dk's wave of 32 keys, by the rows that
+// it walks: a block reads as many norms as units.  They cost the stats' launch a pass over v, and the second wave of dk a
+// multiplication an element, us of fp16 with gradients, 24 heads: 4608 tokens 1106 rather than 1073, 512 60 and 58, 40 queries of
+// 16896 keys 302 and 271.
 template <typename T>
 constexpr bool kHalf = !__is_same(T, __bf16);
 constexpr int kUp = 14;
-__device__ __forceinline__ int up_of(float g2, float v2) {   // from the squares of both norms
-  return kUp - ((__builtin_amdgcn_frexp_expf(g2 * v2) + 1) >> 1);
+__device__ __forceinline__ int up_of(float x) {   // x: that max, squared
+  return kUp - ((__builtin_amdgcn_frexp_expf(x) + 1) >> 1);
 }
 __device__ __forceinline__ float power_of(int e) { return __builtin_ldexpf(1.0f, e); }
 __device__ __forceinline__ float uniform(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
 }
+template <typename T>
+__device__ __forceinline__ float square_of(const vec8<T>& x) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum += (float)x[e] * (float)x[e];
+  return sum;
+}
+__device__ __forceinline__ float most_lane(float x, int lanes) {   // of `lanes` neighbours
+  for (int d = lanes >> 1; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+  return x;
+}
 
-// The most of `units` x 4 norms.
-__device__ __forceinline__ float most_of(const float* norms, int64_t units) {
-  const f32x4* at = reinterpret_cast<const f32x4*>(norms);
+// The most |v|^2 of the units that a wave walks.
+template <bool kMasked>
+__device__ __forceinline__ float most_v(const Args& A, int b, int h, const Units<kMasked>& units) {
+  const f32x4* at = reinterpret_cast<const f32x4*>(A.norms) + (int64_t)A.batch * A.heads * A.q_units * 2 +
+                    ((int64_t)b * A.kv_heads + h) * A.k_units;
   float x = 0.0f;
-  for (int64_t i = threadIdx.x & 63; i < units; i += 256) {
+  for (int i = threadIdx.x & 63; i < units.n; i += 256) {
     f32x4 y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = at[min(i + 64 * j, units - 1)];
+    for (int j = 0; j < 4; ++j) {
+      const int n = min(i + 64 * j, units.n - 1);
+      y[j] = at[kMasked ? units.live[n].x : units.first + n];
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) x = fmaxf(fmaxf(fmaxf(x, y[j][0]), y[j][1]), fmaxf(y[j][2], y[j][3]));
   }
+  return most_lane(x, 64);
+}
+// The most |do|^2 and delta^2 of n units.
+__device__ __forceinline__ float2 most_do(const Args& A, int64_t first, int n) {
+  const f32x4* at = reinterpret_cast<const f32x4*>(A.norms) + first * 2;
+  float x = 0.0f, y = 0.0f;
+  for (int i = threadIdx.x & 63; i < 2 * n; i += 256) {
+    f32x4 z[4];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-  return x;
-}
-__device__ __forceinline__ float most_do(const Args& A, int b, int first_head, int heads) {
-  return most_of(A.norms + ((int64_t)b * A.heads + first_head) * A.q_units * 4, (int64_t)heads * A.q_units);
-}
-__device__ __forceinline__ float most_v(const Args& A, int b, int h) {
-  const int64_t of_q = (int64_t)A.batch * A.heads * A.q_units;
-  return most_of(A.norms + (of_q + ((int64_t)b * A.kv_heads + h) * A.k_units) * 4, A.k_units);
+    for (int j = 0; j < 4; ++j) z[j] = at[min(i + 64 * j, 2 * n - 1)];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x = fmaxf(fmaxf(x, z[j][0]), z[j][2]);
+      y = fmaxf(fmaxf(y, z[j][1]), z[j][3]);
+    }
+  }
+  return make_float2(most_lane(x, 64), most_lane(y, 64));
 }
 
 // kFrom: dP's sums start from -delta, which spares an addition an element and takes six registers that a masked pass's loop does
@@ -1091,15 +1115,15 @@ __device__ __forceinline__ void dq_wave(const Args& A, uint8_t* smem, const Piec
     w.at = places();
     reinterpret_cast<uint4*>(k_slot(kDqKRing - 1))[threadIdx.x] = make_uint4(0, 0, 0, 0);   // K(-1), times dS(-1) = 0
     if constexpr (kHalf<T>) {
-      const float v2 = most_v(A, b, h / A.group);
+      const float v2 = most_v(A, b, h / A.group, units);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        float g2 = 0.0f;
+        float g2 = 0.0f, delta;
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g2 += (float)w.g[st][g][e] * (float)w.g[st][g][e];
-        w.lse[g] -= (float)up_of(across(g2), v2) * kLn2;
+        for (int st = 0; st < 4; ++st) g2 += square_of<T>(w.g[st][g]);
+        if constexpr (kMasked) delta = w.delta[g];
+        else delta = w.delta[g][0];
+        w.lse[g] -= (float)up_of(fmaxf(across(g2) * v2, delta * delta)) * kLn2;
       }
     }
     landed<0>();
@@ -1356,7 +1380,16 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
     if constexpr (kHalf<T>) {
       int up = kUp;
       if constexpr (kSecond) {
-        up = up_of(most_do(A, b, h * A.group, A.group), most_v(A, b, h));
+        const float2 most = most_do(A, ((int64_t)b * A.heads + h * A.group) * A.q_units + from, n);
+        float v2 = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int st = 0; st < 4; ++st) sum += square_of<T>(w.x[st][g]);
+          v2 = fmaxf(v2, across(sum));
+        }
+        up = up_of(fmaxf(most.x * most_lane(v2, 16), most.y));
         w.more = uniform(power_of(up - kUp));
       }
       down[0] = down[1] = uniform(power_of(-up));
@@ -1576,20 +1609,6 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const M
   plan_entry(m, blockIdx.x, keys, units, found);
 }
 
-// The most |x|^2 of a wave's rows, 16 lanes and 8 values each, into norms[unit][threadIdx.x / 64 % 4].
-template <typename T>
-__device__ __forceinline__ float norm2(const vec8<T>& x) {
-  float sum = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sum += (float)x[e] * (float)x[e];
-  return flk::row16_sum(sum);
-}
-__device__ __forceinline__ void put_norm(float* norms, int64_t unit, float most) {
-  most = fmaxf(most, __shfl_xor(most, 16));
-  most = fmaxf(most, __shfl_xor(most, 32));
-  if ((threadIdx.x & 63) == 0) norms[unit * 4 + (threadIdx.x >> 6 & 3)] = most;
-}
-
 // What the gradients need first: the mask's words and lists, in the first A.batch blocks where there is a mask, and every
 // row's stats, 16 lanes a row and 128 rows (four units) a block, which reads do, o and low once; in float16 the norms of do's
 // rows beside them and, in the blocks behind those, of v's.  Bound by memory: 4608
@@ -1618,16 +1637,18 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_prepare_kernel(cons
         vec8<T> x{};
         if (r < A.keys && (!m.mask || m.mask[b * m.batch_stride + r]))
           x = *reinterpret_cast<const vec8<T>*>(A.v.at<T>(b, h) + (int64_t)r * A.v.row + lane * 8);
-        most = fmaxf(most, norm2<T>(x));
+        most = fmaxf(most, flk::row16_sum(square_of<T>(x)));
       }
-      put_norm(A.norms, all + of_v, most);
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      if ((threadIdx.x & 63) == 0) A.norms[all * 8 + of_v * 4 + (threadIdx.x >> 6 & 3)] = most;
       return;
     }
   }
   if (unit > all) return;
   const int bh = (int)(unit / A.q_units), b = bh / A.heads, h = bh - b * A.heads;
   const int first = (int)(unit - (int64_t)bh * A.q_units) * kUnit + (threadIdx.x >> 4 & 15);
-  float most = 0.0f;
+  float most_g = 0.0f, most_delta = 0.0f;
   float* st = A.stats + unit * 2 * kUnit + (threadIdx.x >> 4 & 15);
   vec8<T> x[2][3];
   float lse[2];
@@ -1652,14 +1673,23 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_prepare_kernel(cons
     for (int e = 0; e < 8; ++e)
       sum += live ? (float)x[i][0][e] * ((float)x[i][1][e] + (float)x[i][2][e]) : 0.0f;
     sum = flk::row16_sum(sum);
-    if constexpr (kHalf<T>) most = fmaxf(most, norm2<T>(live ? x[i][0] : vec8<T>{}));
+    if constexpr (kHalf<T>) {
+      most_g = fmaxf(most_g, flk::row16_sum(live ? square_of<T>(x[i][0]) : 0.0f));
+      most_delta = fmaxf(most_delta, sum * sum);
+    }
     if (lane == 0) {
       st[16 * i] = live ? lse[i] : INFINITY;
       st[16 * i + kUnit] = -sum;
     }
   }
-  if constexpr (kHalf<T>)
-    if (unit < all) put_norm(A.norms, unit, most);
+  if constexpr (kHalf<T>) {
+    for (int d = 16; d <= 32; d <<= 1) {
+      most_g = fmaxf(most_g, __shfl_xor(most_g, d));
+      most_delta = fmaxf(most_delta, __shfl_xor(most_delta, d));
+    }
+    if (unit < all && (threadIdx.x & 63) == 0)
+      *reinterpret_cast<float2*>(A.norms + unit * 8 + (threadIdx.x >> 6 & 3) * 2) = make_float2(most_g, most_delta);
+  }
 }
 
 int units_of(int rows) { return (rows + kUnit - 1) / kUnit; }
@@ -1667,7 +1697,9 @@ int64_t mask_bytes(int batch, int keys) { return ((int64_t)batch * (units_of(key
 int64_t stats_bytes(int batch, int heads, int queries) {
   return ((int64_t)batch * heads * units_of(queries) + 1) * 2 * kUnit * 4;
 }
-int64_t norms_bytes(const Args& A) { return (int64_t)A.batch * (A.heads * (int64_t)A.q_units + A.kv_heads * (int64_t)A.k_units) * 16; }
+int64_t norms_bytes(const Args& A) {
+  return (int64_t)A.batch * (2LL * A.heads * A.q_units + (int64_t)A.kv_heads * A.k_units) * 16;
+}
 
 // Where the mask's words and lists lie in `workspace`.
 MaskBytes mask_in(const void* mask, int64_t batch_stride, Args& A, uint8_t* workspace) {

@@ -150,3 +150,21 @@ def test_many_small_weights(device, form):
     assert torch.equal(o, A.attention(q, k, v))
     total = float(torch.log1p((keys - 1) * p))
     assert ((kept.lse.double() - total).abs() <= 64 * U * 18).all()
+
+
+@pytest.mark.parametrize("queries,keys,masked", [(16, 16896, False), (40, 9000, True), (3000, 20, False), (1, 5000, True)])
+def test_long_and_short(device, queries, keys, masked):
+    """Pieces of long walks each find their own powers of two, by the units of their lists."""
+    q, k, v, do, keep = make(6, 2, 3, 1, queries, keys, "fp16", "random" if masked else None)
+    sizes = 2.0 ** -(torch.arange(keys, device=device) // 500 % 10).to(v.dtype)     # values that differ along the keys
+    v = torch.where(torch.isfinite(v), v * sizes[:, None], v)
+    q, k, do = q / 64, k * 64, do * 2.0 ** -10
+    (dq, dev), (dk, dk_dev), (dv, dv_dev) = bounds(q, k, v, do, keep)
+    o, kept = A.attention(q, k, v, key_mask=keep, keep=True)
+    got = A.attention_backward(do, q, k, v, kept, key_mask=keep)
+    within("dq", got[0], dq, dev, (2, 3))
+    q, k, do = q * 2 ** 12, k / 2 ** 12, do * 2.0 ** 10
+    want = bounds(q, k, v, do, keep)
+    o, kept = A.attention(q, k, v, key_mask=keep, keep=True)
+    for name, g, (w, d) in zip(("dk", "dv"), A.attention_backward(do, q, k, v, kept, key_mask=keep)[1:], want[1:]):
+        within(name, g, w, d, (2, 3))
