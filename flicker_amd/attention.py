@@ -132,8 +132,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_mask: to
         if out.numel():
             if not _rows_apart(out):
                 raise ValueError(f"out needs rows that do not overlap, got strides {out.stride()}")
-            for name, t in (("q", q), ("k", k), ("v", v)):
-                if t.numel():
+            for name, t in (("q", q), ("k", k), ("v", v), ("key_mask", key_mask)):
+                if t is not None and t.numel():
                     _refuse_overlap(name, out, t)
     low = torch.empty((batch, queries, heads * dim), dtype=q.dtype, device=q.device) if keep else None
     lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=q.device) if keep else None

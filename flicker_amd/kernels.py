@@ -324,7 +324,8 @@ def qk_prep_backward(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, qkv: 
             from .norm import _refuse_overlap, _rows_apart
             if not _rows_apart(out):
                 raise ValueError(f"out needs rows that do not overlap, got strides {out.stride()}")
-            for name, t in (("qkv", qkv), ("dq", grads[0]), ("dk", grads[1]), ("dv", grads[2])):
+            for name, t in (("qkv", qkv), ("dq", grads[0]), ("dk", grads[1]), ("dv", grads[2]), ("q_scale", q_scale),
+                            ("k_scale", k_scale), ("cos", cos), ("sin", sin)):
                 _refuse_overlap(name, out, t)
     make = torch.empty if out.numel() else torch.zeros   # sums over no rows
     dscales = tuple(make(shape, dtype=q_scale.dtype, device=qkv.device) for shape in scale_shapes)
