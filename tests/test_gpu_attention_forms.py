@@ -166,3 +166,13 @@ def test_most_heads(device):
     with pytest.raises(_lib.HipKernelError, match="flk_attention_plan"):
         A.attention(torch.empty(batch, heads + 1, 1, D, dtype=torch.bfloat16, device=device), *[torch.empty(
             batch, heads + 1, 1, D, dtype=torch.bfloat16, device=device)] * 2)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("sizes,mask", [((1, 1, 1, 2 ** 20 + 5, 3), None), ((1, 2, 1, 1, 2 ** 21 + 3), "random"), ((1, 1, 1, 70000, 40), "random"),
+                                        ((700, 3, 3, 2, 2), "random"), ((1, 64, 1, 33, 77), "middle")])
+def test_long_sides(device, sizes, mask, dtype):
+    """One side of a million rows beside a few; many entries of two; 64 heads on one."""
+    print(f"sides {sizes} {mask} {dtype}", flush=True)
+    ops = make(17, *sizes, dtype, mask)
+    check(str(sizes), step(*ops), expected(*ops))
