@@ -43,9 +43,9 @@
 //
 // Bound: the matrix pipe, and over whole rounds of blocks the chip's power: random operands hold it there, where a large
 // library product reaches 1.24 PFLOP/s.  Measured at 24 heads in bfloat16, PFLOP/s over all products that run: forward
-// 4608 tokens 230 us (1.13), 16896 2.66 ms (1.32), with what the gradients need 250 us and 2.82 ms; gradients 730 us
-// (1.25) and 9.4 ms (1.30), of which 14 and 63 us are the rows' stats.  1536 tokens are 144 blocks of queries for 256 CUs:
-// 50 us and 120.  Few rows are bound by memory, and have a kernel of their own: one query on 4608 keys 17-19 us.
+// 4608 tokens 237 us (1.10), 16896 2.75 ms (1.28), with what the gradients need 261 us and 2.91 ms; gradients 741 us
+// (1.23) and 9.6 ms (1.28), of which 15 and 66 us are the rows' stats.  1536 tokens are 192 blocks of queries for 256 CUs:
+// 46 us and 113.  Few rows are bound by memory, and have a kernel of their own: one query on 4608 keys 17 us.
 
 #include <algorithm>
 #include <type_traits>
@@ -727,7 +727,7 @@ __device__ __forceinline__ void forward_wave(const Args& A, uint8_t* smem, const
 
 // o of 256 or 192 queries: 32 a wave rather than 64, which leaves a SIMD two waves, whose phases fill each other's gaps; all
 // eight read the same K and V units, so LDS is read once per 256 queries x 32 keys.  What kKeep adds: 16 additions a lane and
-// phase for lse, and o's second store (4608 tokens: 230 -> 250 us).
+// phase for lse, and o's second store (4608 tokens: 237 -> 261 us).
 template <typename T, bool kMasked, bool kKeep>
 __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[(kKRing + kVRing) * kUnitBytes];
@@ -742,8 +742,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(const Args A) {
 // o of 16 rows, among the queries of all heads that share a key head, so that for a single query of each every key is read
 // once.  For few rows: bound by memory, and where few blocks walk many units by its latency.  The four waves walk units of their
 // own (every fourth of the block's), each copied into the wave's own LDS two ahead: no barrier, and 64 to 128 KB on their
-// way to a CU.  The waves' sums are joined at the end.  One query of 24 heads: 4608 keys 19 us with the join (57 MB, 14 of
-// them this kernel), 16896 keys 46 us (4.5 TB/s), 8 x 4608 85 us (5.3 TB/s).  Two blocks of two waves a CU: 22.3, 50.6, 89.6.
+// way to a CU.  The waves' sums are joined at the end.  One query of 24 heads: 4608 keys 17 us with the join (57 MB, 14 of
+// them this kernel), 16896 keys 44 us (4.7 TB/s), 8 x 4608 81 us (5.6 TB/s).  Two blocks of two waves a CU take 5-17% more.
 constexpr int kFewWaves = 4, kFewRing = 2;
 constexpr int kFewBytes = (2 * kFewRing * kUnit + kFewRows) * kRowBytes;   // of a wave: K ring, V ring, Q
 
@@ -1462,7 +1462,7 @@ __device__ __forceinline__ void dkv_wave(const Args& A, uint8_t* smem, const Pie
 
 // All gradients: blocks of queries and blocks of keys in one launch, so that neither kind's last round leaves CUs idle (a
 // launch each, with the stats in the first: 1536 tokens with their forward pass 172 us, now 153; 4608: 1026 and 997).
-// 4608 tokens, 24 heads: 715 us, 1.28 PFLOP/s over the 7 products.
+// 4608 tokens, 24 heads: 726 us without the stats, 1.26 PFLOP/s over the 7 products.
 template <typename T, bool kMasked, bool kGrouped>   // kGrouped: query heads share key heads
 __global__ __launch_bounds__(kThreads, 2) void attention_backward_kernel(const Args A) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kDkvBytes];
@@ -1612,7 +1612,7 @@ __global__ __launch_bounds__(64 * kPlanWaves) void attention_mask_kernel(const M
 // What the gradients need first: the mask's words and lists, in the first A.batch blocks where there is a mask, and every
 // row's stats, 16 lanes a row and 128 rows (four units) a block, which reads do, o and low once; in float16 the norms of do's
 // rows beside them and, in the blocks behind those, of v's.  Bound by memory: 4608
-// tokens of 24 heads 14 us for 85 MB, which the caches partly hold; 16896 64 us, 4.9 TB/s.
+// tokens of 24 heads 15 us for 85 MB, which the caches partly hold; 16896 66 us, 4.7 TB/s.
 template <typename T>
 __global__ __launch_bounds__(64 * kPlanWaves) void attention_prepare_kernel(const MaskBytes m, const Args A) {
   __shared__ int found[kPlanWaves];
@@ -1775,7 +1775,7 @@ Cut plan_few(const Args& A) {
   return best;
 }
 // Blocks of 16 rows where they take less, by the estimates and kStart more for blocks of 256.  24 heads, us in blocks of 16
-// and 256: one query of 512 keys 8.5 and 12.9, of 4608 19 and 22.4 (on 4 key heads 11.4 and 18.9, of 8 entries 85 and 101),
+// and 256: one query of 512 keys 8.5 and 12.9, of 4608 17 and 20.5 (on 4 key heads 11.4 and 18.9, of 8 entries 85 and 101),
 // 64 queries of 4608 33.5 and 23; 128 tokens 5.2 and 11.6, 256 11.1 and 16.6, 384 19.8 and 19.0, 512 24.4 and 21.0.
 constexpr double kStart = 3.0;
 Cut forward_cut(const Args& A) {
