@@ -142,3 +142,33 @@ def test_every_logit_minus_infinity(device, form):
     o = o.unflatten(2, (q.shape[1], D))
     assert not o[:, ::2].any() and o[:, 1::2].isnan().all()
     assert kept.lse[:, :, ::2].isneginf().all() and kept.lse[:, :, 1::2].isnan().all()
+
+
+@pytest.mark.parametrize("form", SHORT)
+@pytest.mark.parametrize("dtype,size", [("fp16", 2.0 ** 10), ("bf16", 2.0 ** 10), ("bf16", 2.0 ** 50)])
+def test_far_logits_of_many_terms(device, form, dtype, size):
+    """Logits of 128 unequal terms each, whose roundings are far more than 1: forwards and backwards form the same ones, so that
+    P of a row's largest is 1 where the next is far below, off by no more than lse's rounding at 2^-1 of its unit."""
+    print(f"far logits of many terms {form} {dtype} {size}", flush=True)
+    batch, heads, kv_heads, queries, keys = FORMS[form][0]
+    group = heads // kv_heads
+    q, k, v, do, _ = make(6, *FORMS[form][0], dtype, scale=D ** 0.5)
+    q, k = q * size, k * size
+    s = q.double() @ k.double().repeat_interleave(group, 1).transpose(2, 3).contiguous()
+    (first, second), at = s.topk(2, -1).values.unbind(-1), s.argmax(-1)
+    clear = first - second > 200 + 4 * 130 * U * (q.double().abs().sum(-1) * k.double().abs().amax())
+    assert clear.float().mean() > 0.9
+    o, kept = A.attention(q, k, v, keep=True)
+    pick = at[..., None].expand(-1, -1, -1, D)
+    want = v.repeat_interleave(group, 1).gather(2, pick)
+    got = o.unflatten(2, (heads, D)).transpose(1, 2)
+    assert torch.equal(got[clear], want[clear])
+    do = torch.where(clear.transpose(1, 2)[..., None], do.unflatten(2, (heads, D)), 0.0).flatten(2)
+    dq, dk, dv = A.attention_backward(do, q, k, v, kept)
+    g4 = do.view(batch, queries, heads, D).transpose(1, 2).double()
+    sums, sizes = (torch.zeros(batch, heads, keys, D, dtype=torch.float64, device=device).scatter_add_(2, pick, t).view(
+        batch, kv_heads, group, keys, D).sum(2) for t in (g4, g4.abs()))
+    e = torch.finfo(q.dtype).eps / 2
+    off = (queries * group + 64) * U * sizes
+    assert ((dv.double() - sums).abs() <= e * (sums.abs() + off) + off + (2.0 ** -25 if dtype == "fp16" else 0.0)).all()
+    assert not dq.isnan().any() and not dk.isnan().any()
